@@ -329,7 +329,8 @@ def _nearest_e4m3(v):
 
 def _exact_scale(v, dim):
     amax = v.abs().amax(dim, keepdim=True)
-    k = torch.ceil(torch.log2(amax / 448)).clamp(min=-126)
+    m, e = torch.frexp(amax / 448)  # (a logarithm may be off by its last bit where this is a power of two)
+    k = torch.where(m == 0.5, e - 1, e).clamp(min=-126).double()
     return torch.where(amax > 0, torch.exp2(k), torch.ones_like(amax))
 
 
