@@ -14,6 +14,12 @@ pub const B200_ERR_UNSUPPORTED: c_int = -5;
 pub const B200_ACT_NONE: i32 = 0;
 pub const B200_ACT_CRELU: i32 = 1;
 pub const B200_ACT_SCRELU: i32 = 2;
+pub const B200_ACT_RELU: i32 = 3;
+
+pub const B200_TYPE_F32: i32 = 0;
+pub const B200_TYPE_BF16: i32 = 1;
+pub const B200_TYPE_F16: i32 = 2;
+pub const B200_TYPE_E4M3: i32 = 3;
 
 pub const B200_KIND_WEIGHT: c_int = 0;
 pub const B200_KIND_MOMENTUM: c_int = 1;
@@ -113,6 +119,134 @@ pub struct b200_ft_op {
     pub idx_nstm: *const u16,
     pub x: *mut f32,
     pub u: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_rms_norm_op {
+    pub rows: i32,
+    pub cols: i32,
+    pub x_type: i32,
+    pub y_type: i32,
+    pub ldx: i64,
+    pub ldr: i64,
+    pub lds: i64,
+    pub ldy: i64,
+    pub x: *const c_void,
+    pub residual: *const c_void,
+    pub weight: *const f32,
+    pub sum: *mut c_void,
+    pub y: *mut c_void,
+    pub scale: *mut f32,
+    pub rstd: *mut f32,
+    pub eps: f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_rms_norm_grad_op {
+    pub rows: i32,
+    pub cols: i32,
+    pub x_type: i32,
+    pub dy_type: i32,
+    pub lddy: i64,
+    pub lds: i64,
+    pub ldds: i64,
+    pub lddx: i64,
+    pub dy: *const c_void,
+    pub sum: *const c_void,
+    pub rstd: *const f32,
+    pub weight: *const f32,
+    pub dsum: *const c_void,
+    pub dx: *mut c_void,
+    pub dweight: *mut f32,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_pack8_op {
+    pub rows: i32,
+    pub cols: i32,
+    pub x_type: i32,
+    pub act: i32,
+    pub by_column: i32,
+    pub ldx: i64,
+    pub ldq: i64,
+    pub x: *const c_void,
+    pub q: *mut c_void,
+    pub scale: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_unpack8_op {
+    pub rows: i32,
+    pub cols: i32,
+    pub y_type: i32,
+    pub by_column: i32,
+    pub ldq: i64,
+    pub ldy: i64,
+    pub q: *const c_void,
+    pub scale: *const f32,
+    pub y: *mut c_void,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_dense_op {
+    pub rows: i32,
+    pub r#in: i32,
+    pub out: i32,
+    pub x_type: i32,
+    pub y_type: i32,
+    pub act: i32,
+    pub ldx: i64,
+    pub ldw: i64,
+    pub ldr: i64,
+    pub ldy: i64,
+    pub x: *const c_void,
+    pub x_scale: *const f32,
+    pub w: *const c_void,
+    pub w_scale: *const f32,
+    pub bias: *const f32,
+    pub residual: *const c_void,
+    pub y: *mut c_void,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_dense_grad_op {
+    pub rows: i32,
+    pub r#in: i32,
+    pub out: i32,
+    pub dy_type: i32,
+    pub x_type: i32,
+    pub y_type: i32,
+    pub dw_type: i32,
+    pub act: i32,
+    pub lddy: i64,
+    pub ldx: i64,
+    pub ldy: i64,
+    pub ldw: i64,
+    pub ldskip: i64,
+    pub lddx: i64,
+    pub lddw: i64,
+    pub dy: *const c_void,
+    pub x: *const c_void,
+    pub x_scale: *const f32,
+    pub y: *const c_void,
+    pub y_scale: *const f32,
+    pub w: *const c_void,
+    pub dskip: *const c_void,
+    pub dx: *mut c_void,
+    pub dw: *mut c_void,
+    pub dbias: *mut f32,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: i64,
 }
 
 /// One entry of an export in the reference's `SavedFormat` scheme
@@ -245,6 +379,15 @@ extern "C" {
 
     pub fn b200_op_ft_forward(device: c_int, stream: *mut c_void, op: *const b200_ft_op) -> c_int;
     pub fn b200_op_ft_forward_noalloc(device: c_int, stream: *mut c_void, op: *const b200_ft_op) -> c_int;
+    pub fn b200_op_rms_norm(device: c_int, stream: *mut c_void, op: *const b200_rms_norm_op) -> c_int;
+    pub fn b200_op_rms_norm_backward_workspace(op: *const b200_rms_norm_grad_op, bytes: *mut i64) -> c_int;
+    pub fn b200_op_rms_norm_backward(device: c_int, stream: *mut c_void, op: *const b200_rms_norm_grad_op) -> c_int;
+    pub fn b200_op_pack8(device: c_int, stream: *mut c_void, op: *const b200_pack8_op) -> c_int;
+    pub fn b200_op_unpack8(device: c_int, stream: *mut c_void, op: *const b200_unpack8_op) -> c_int;
+    pub fn b200_op_dense_workspace(op: *const b200_dense_op, bytes: *mut i64) -> c_int;
+    pub fn b200_op_dense(device: c_int, stream: *mut c_void, op: *const b200_dense_op) -> c_int;
+    pub fn b200_op_dense_backward_workspace(op: *const b200_dense_grad_op, bytes: *mut i64) -> c_int;
+    pub fn b200_op_dense_backward(device: c_int, stream: *mut c_void, op: *const b200_dense_grad_op) -> c_int;
 
     pub fn b200_map_chess768(records: *const c_void, n: i32, stm: *mut i32, nstm: *mut i32, nnz: i32) -> c_int;
     pub fn b200_map_chess_buckets_mirrored(

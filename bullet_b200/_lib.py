@@ -25,6 +25,8 @@ SYMBOLS = (
     "b200_exchange_export", "b200_exchange_import", "b200_update_exchange", "b200_update_exchange_range",
     "b200_grad_zero_range", "b200_batch_upload_records", "b200_set_host_threads", "b200_step_exchange",
     "b200_batch_upload_records_gpu", "b200_slot_read", "b200_probe_bandwidth", "b200_net_set_optimiser",
+    "b200_op_rms_norm", "b200_op_rms_norm_backward_workspace", "b200_op_rms_norm_backward", "b200_op_pack8", "b200_op_unpack8",
+    "b200_op_dense_workspace", "b200_op_dense", "b200_op_dense_backward_workspace", "b200_op_dense_backward",
 )
 
 
@@ -44,6 +46,48 @@ class CFtOp(ctypes.Structure):
 
     _fields_ = [(n, ctypes.c_int32) for n in ("n_inputs", "nnz", "ft_out", "ft_act", "pairwise", "ft_block_rows", "n")] + \
                [(n, ctypes.c_void_p) for n in ("table", "bias", "idx_stm", "idx_nstm", "x", "u")]
+
+
+def _fields(i32, i64, pointers, f32="", last=""):
+    return ([(n, ctypes.c_int32) for n in i32.split()] + [(n, ctypes.c_int64) for n in i64.split()] +
+            [(n, ctypes.c_void_p) for n in pointers.split()] + [(n, ctypes.c_float) for n in f32.split()] + [(n, ctypes.c_int64) for n in last.split()])
+
+
+class CRmsNorm(ctypes.Structure):
+    """b200_rms_norm_op"""
+
+    _fields_ = _fields("rows cols x_type y_type", "ldx ldr lds ldy", "x residual weight sum y scale rstd", f32="eps")
+
+
+class CRmsNormGrad(ctypes.Structure):
+    """b200_rms_norm_grad_op"""
+
+    _fields_ = _fields("rows cols x_type dy_type", "lddy lds ldds lddx", "dy sum rstd weight dsum dx dweight workspace", last="workspace_bytes")
+
+
+class CPack8(ctypes.Structure):
+    """b200_pack8_op"""
+
+    _fields_ = _fields("rows cols x_type act by_column", "ldx ldq", "x q scale")
+
+
+class CUnpack8(ctypes.Structure):
+    """b200_unpack8_op"""
+
+    _fields_ = _fields("rows cols y_type by_column", "ldq ldy", "q scale y")
+
+
+class CDense(ctypes.Structure):
+    """b200_dense_op"""
+
+    _fields_ = _fields("rows in_ out x_type y_type act", "ldx ldw ldr ldy", "x x_scale w w_scale bias residual y workspace", last="workspace_bytes")
+
+
+class CDenseGrad(ctypes.Structure):
+    """b200_dense_grad_op"""
+
+    _fields_ = _fields("rows in_ out dy_type x_type y_type dw_type act", "lddy ldx ldy ldw ldskip lddx lddw",
+                       "dy x x_scale y y_scale w dskip dx dw dbias workspace", last="workspace_bytes")
 
 
 class CSavedFormat(ctypes.Structure):
@@ -134,6 +178,15 @@ def load() -> ctypes.CDLL:
         "b200_net_get_stat": [vp, cp, ctypes.POINTER(i64)],
         "b200_op_ft_forward": [ctypes.c_int, vp, ctypes.POINTER(CFtOp)],
         "b200_op_ft_forward_noalloc": [ctypes.c_int, vp, ctypes.POINTER(CFtOp)],
+        "b200_op_rms_norm": [ctypes.c_int, vp, ctypes.POINTER(CRmsNorm)],
+        "b200_op_rms_norm_backward_workspace": [ctypes.POINTER(CRmsNormGrad), ctypes.POINTER(i64)],
+        "b200_op_rms_norm_backward": [ctypes.c_int, vp, ctypes.POINTER(CRmsNormGrad)],
+        "b200_op_pack8": [ctypes.c_int, vp, ctypes.POINTER(CPack8)],
+        "b200_op_unpack8": [ctypes.c_int, vp, ctypes.POINTER(CUnpack8)],
+        "b200_op_dense_workspace": [ctypes.POINTER(CDense), ctypes.POINTER(i64)],
+        "b200_op_dense": [ctypes.c_int, vp, ctypes.POINTER(CDense)],
+        "b200_op_dense_backward_workspace": [ctypes.POINTER(CDenseGrad), ctypes.POINTER(i64)],
+        "b200_op_dense_backward": [ctypes.c_int, vp, ctypes.POINTER(CDenseGrad)],
         "b200_map_chess768": [vp, i32, vp, vp, i32],
         "b200_map_chess_buckets_mirrored": [vp, i32, vp, vp, vp, i32],
         "b200_map_ataxx147": [vp, i32, vp, vp, i32],

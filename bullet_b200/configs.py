@@ -13,6 +13,7 @@ import dataclasses
 from dataclasses import dataclass, field
 
 ACT_NONE, ACT_CRELU, ACT_SCRELU = 0, 1, 2
+ACT_RELU = 3  # the dense trunk's operators only (ops.py)
 
 #: tensor names in flat-buffer order (name-sorted, as the reference's BTreeMap iterates them,
 #: crates/trainer/src/model/weights.rs:95-110)

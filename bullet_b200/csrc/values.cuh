@@ -1,0 +1,72 @@
+// Values of the dense trunk's operators: types of 32, 16 and 8 bits, the 8-bit scales, and activations with their gradients.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "../../include/bullet_b200.h"
+
+namespace b200 {
+
+using bf16 = __nv_bfloat16;
+using f16 = __half;
+struct e4m3 {
+    uint8_t code;
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(f16 v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(e4m3 v) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(v.code, __NV_E4M3))); }
+template <class T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ bf16 from_float<bf16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ f16 from_float<f16>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u; }
+
+// The scale for a largest finite magnitude given by its bits: the smallest power of two from 2^-126 on with magnitude / scale
+// <= 448 = 1.75 * 2^8.  1 for a magnitude of 0.
+__device__ __forceinline__ uint32_t scale_bits(uint32_t magnitude) {
+    if (magnitude == 0) return 127u << 23;
+    const int e = (int)(magnitude >> 23) - 8 + ((magnitude & 0x7fffffu) > 0x600000u);
+    return (uint32_t)max(e, 1) << 23;
+}
+__device__ __forceinline__ float one_over_scale(uint32_t scale) { return __uint_as_float((254u << 23) - scale); }
+
+// The code of v / scale (`by` = 1 / scale): nearest, halves to even, NaN for what is not finite.
+__device__ __forceinline__ uint8_t code_of(float v, float by) {
+    const uint8_t q = __nv_cvt_float_to_fp8(v * by, __NV_SATFINITE, __NV_E4M3);
+    return finite(v) ? q : 0x7f;
+}
+// The same for outputs of an activation: what is above 0 stays above 0, what is below 1 stays below 1.
+__device__ __forceinline__ uint8_t code_of_output(float v, float by, float scale, int act) {
+    uint8_t q = code_of(v, by);
+    if (act == B200_ACT_NONE || !finite(v)) return q;
+    if (v > 0.f && (q & 0x7f) == 0) q = 1;
+    if (act != B200_ACT_RELU && v > 0.f && v < 1.f && to_float(e4m3{q}) * scale >= 1.f) q--;  // codes above 0 are in the order of their values
+    return q;
+}
+
+// NaN stays NaN in all of them.
+__device__ __forceinline__ float activate(float z, int act) {
+    if (act == B200_ACT_NONE) return z;
+    z = z < 0.f ? 0.f : z;
+    if (act == B200_ACT_RELU) return z;
+    z = z > 1.f ? 1.f : z;
+    return act == B200_ACT_SCRELU ? z * z : z;
+}
+// dy times the activation's derivative, taken from its output; 0 where that is cut off, whatever dy is.
+__device__ __forceinline__ float gradient_from_output(float dy, float y, int act) {
+    if (act == B200_ACT_NONE) return dy;
+    const bool inside = y > 0.f && (act == B200_ACT_RELU || y < 1.f);
+    if (act == B200_ACT_SCRELU) dy *= 2.f * sqrtf(y);
+    return inside ? dy : 0.f;
+}
+
+}  // namespace b200

@@ -371,6 +371,146 @@ int b200_op_ft_forward(int device, void* stream, const b200_ft_op* op);
 #define B200_OP_NOALLOC_MAX_POSITIONS 16384
 int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
 
+/* ---- operators of a wide dense trunk, on caller-owned DEVICE memory, without a b200_net: layers wider than the
+ * output-bucketed ones of a network (dense_out <= 32), with a norm in front and a residual behind, and activations kept
+ * for the backward pass in 8 bits.  (The reference builds such layers from ModelBuilder::new_affine, crates/compiler/src/
+ * model/builder.rs:145-147, its activations and elementwise operations, in fp32; norm and 8 bits have no counterpart.)
+ *
+ * Common to all of them:
+ *   - they only enqueue on `stream` (NULL = the default stream), allocate nothing, leave the thread's current device as it
+ *     was and may be captured into a graph (each once outside a capture before); memory of theirs is the caller's until the stream has passed the call;
+ *   - matrices have rows of consecutive elements; `ld*` is the distance of two rows in elements, at least their length.
+ *     Any ld and any address aligned to the element will do; 16-byte aligned rows are faster.  Indices are 64-bit;
+ *   - no rows: nothing is done (gradients of weights become 0) and B200_OK returned;
+ *   - outputs overlap neither inputs nor one another;
+ *   - all sums are held in 32 bits and taken in the same order by every call of the same shape: equal inputs give equal bits;
+ *   - a B200_TYPE_E4M3 matrix holds codes of 8 bits (four significand bits, largest value 448, no infinities) and goes with
+ *     a scale, a power of two in fp32, per row (or per column, where said): it stands for code * scale. */
+#define B200_ACT_RELU 3 /* these operators only; 0 to 2 as above */
+#define B200_TYPE_F32 0
+#define B200_TYPE_BF16 1
+#define B200_TYPE_F16 2
+#define B200_TYPE_E4M3 3
+
+/* sum = x + residual; rstd = 1 / sqrt(mean(sum^2) + eps); y = sum * rstd * weight, per row.  The norm is taken of the sum
+ * before that is rounded to x_type.  y in 8 bits: each row's scale is the smallest power of two from 2^-126 on that brings
+ * the row's largest magnitude to 448 or below. */
+typedef struct b200_rms_norm_op {
+    int32_t rows, cols;
+    int32_t x_type;        /* B200_TYPE_F32, _BF16 or _F16: of x, residual and sum */
+    int32_t y_type;        /* any B200_TYPE_* */
+    int64_t ldx, ldr, lds, ldy;
+    const void* x;
+    const void* residual;  /* or NULL */
+    const float* weight;   /* [cols], or NULL: 1 */
+    void* sum;             /* out: x + residual; NULL without a residual, or where it is not needed */
+    void* y;               /* out */
+    float* scale;          /* out, y_type E4M3 only: [rows] */
+    float* rstd;           /* out: [rows], or NULL */
+    float eps;
+} b200_rms_norm_op;
+int b200_op_rms_norm(int device, void* stream, const b200_rms_norm_op* op);
+
+/* Its gradient.  With n = sum * rstd and g = dy * weight:  dx = rstd * (g - n * mean(g * n)) + dsum, which is the gradient at
+ * x and at the residual, and dweight = sum over rows of dy * n.  Codes of 8 bits pass their gradient on as if they had not
+ * been rounded. */
+typedef struct b200_rms_norm_grad_op {
+    int32_t rows, cols;
+    int32_t x_type;        /* of sum, dsum and dx */
+    int32_t dy_type;       /* B200_TYPE_F32, _BF16 or _F16 */
+    int64_t lddy, lds, ldds, lddx;
+    const void* dy;
+    const void* sum;       /* what b200_op_rms_norm gave (x where there was no residual) */
+    const float* rstd;
+    const float* weight;   /* or NULL: 1 */
+    const void* dsum;      /* the gradient that reaches the sum by itself, or NULL */
+    void* dx;              /* out, or NULL */
+    float* dweight;        /* out: [cols], or NULL */
+    void* workspace;       /* 16-byte aligned; may be NULL where none is needed */
+    int64_t workspace_bytes;
+} b200_rms_norm_grad_op;
+int b200_op_rms_norm_backward_workspace(const b200_rms_norm_grad_op* op, int64_t* bytes);
+int b200_op_rms_norm_backward(int device, void* stream, const b200_rms_norm_grad_op* op);
+
+/* Activations (or weights) to 8 bits with a scale per row (or column), and back.  The scale is the smallest power of two from 2^-126 on that
+ * brings the largest finite magnitude to 448 or below (1 where there is none but 0); codes are the nearest, halves to the
+ * even one; infinities and NaN become NaN.  `act` names the activation whose outputs these are: for B200_ACT_RELU, _CRELU
+ * and _SCRELU a value above 0 keeps a code above 0, for the latter two a value below 1 one that stands for less than 1, so
+ * that the activation's gradient is cut off where it would have been without the rounding.
+ * A power of two as scale leaves every value exact in bf16 and fp32. */
+typedef struct b200_pack8_op {
+    int32_t rows, cols;
+    int32_t x_type;    /* B200_TYPE_F32, _BF16 or _F16 */
+    int32_t act;       /* B200_ACT_* */
+    int32_t by_column; /* 1: scale [cols], 0: scale [rows] */
+    int64_t ldx, ldq;
+    const void* x;
+    void* q;           /* out: codes */
+    float* scale;      /* out */
+} b200_pack8_op;
+int b200_op_pack8(int device, void* stream, const b200_pack8_op* op);
+typedef struct b200_unpack8_op {
+    int32_t rows, cols;
+    int32_t y_type;    /* B200_TYPE_F32, _BF16 or _F16 */
+    int32_t by_column;
+    int64_t ldq, ldy;
+    const void* q;
+    const float* scale;
+    void* y;           /* out */
+} b200_unpack8_op;
+int b200_op_unpack8(int device, void* stream, const b200_unpack8_op* op);
+
+/* y = act(x W + bias) + residual for rows of `in` inputs.  W is column-major out x in like the weights of a network:
+ * w[i * ldw + o].  x and W are both bf16, both fp16, or both codes of 8 bits, x with a scale per row, W with one per output
+ * (b200_op_pack8 with by_column). */
+typedef struct b200_dense_op {
+    int32_t rows, in, out;
+    int32_t x_type;        /* B200_TYPE_BF16, _F16 or _E4M3: of x and w */
+    int32_t y_type;        /* B200_TYPE_F32, _BF16 or _F16: of residual and y */
+    int32_t act;           /* B200_ACT_* */
+    int64_t ldx, ldw, ldr, ldy;
+    const void* x;
+    const float* x_scale;  /* [rows], x_type E4M3 only */
+    const void* w;
+    const float* w_scale;  /* [out], x_type E4M3 only */
+    const float* bias;     /* [out], or NULL */
+    const void* residual;  /* [rows][out], or NULL */
+    void* y;               /* out */
+    void* workspace;       /* 16-byte aligned; may be NULL where none is needed */
+    int64_t workspace_bytes;
+} b200_dense_op;
+int b200_op_dense_workspace(const b200_dense_op* op, int64_t* bytes);
+int b200_op_dense(int device, void* stream, const b200_dense_op* op);
+
+/* The gradient of act(x W + bias).  dz = act'(y) * dy with act' taken from the output y as in the reference (crates/
+ * compiler/src/tensor/operation/autograd/dfo.rs:47-88; 0 outside, whatever dy is), dx = dz W^T + dskip, dw = x^T dz, dbias =
+ * sum over rows of dz.  dz enters the products rounded to dy_type, which rounds nothing but for SCReLU.  x and y may be the
+ * 8-bit checkpoints that b200_op_pack8 or b200_op_rms_norm left (dy_type bf16 then): the values they stand for are exact in
+ * bf16 and enter the products as they are. */
+typedef struct b200_dense_grad_op {
+    int32_t rows, in, out;
+    int32_t dy_type;       /* B200_TYPE_BF16 or _F16: of dy, w, dskip and dx */
+    int32_t x_type;        /* dy_type, or B200_TYPE_E4M3 with bf16 */
+    int32_t y_type;        /* dy_type, or B200_TYPE_E4M3 with bf16 */
+    int32_t dw_type;       /* B200_TYPE_F32, or dy_type */
+    int32_t act;           /* B200_ACT_* */
+    int64_t lddy, ldx, ldy, ldw, ldskip, lddx, lddw;
+    const void* dy;        /* [rows][out] */
+    const void* x;         /* [rows][in]; may be NULL without dw */
+    const float* x_scale;  /* [rows], x_type E4M3 only */
+    const void* y;         /* [rows][out]; may be NULL with B200_ACT_NONE */
+    const float* y_scale;  /* [rows], y_type E4M3 only */
+    const void* w;         /* [in][out] as above; may be NULL without dx */
+    const void* dskip;     /* [rows][in], or NULL */
+    void* dx;              /* out: [rows][in], or NULL */
+    void* dw;              /* out: [in][out], or NULL */
+    float* dbias;          /* out: [out], or NULL */
+    void* workspace;       /* 16-byte aligned; may be NULL where none is needed */
+    int64_t workspace_bytes;
+} b200_dense_grad_op;
+int b200_op_dense_backward_workspace(const b200_dense_grad_op* op, int64_t* bytes);
+int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* op);
+
 /* ---- bandwidth probes: the measured denominators for kernels whose table stays in L2.  kind 0: every SM
  * reads a buffer of `bytes` bytes `reps` times with 16-byte loads (a buffer well below the L2 size measures L2,
  * one far above it measures HBM); kind 1: 16-byte vector reductions (red.global.add.v4.f32) into it; kinds 2
