@@ -1,4 +1,12 @@
 // Kernels over the rows of a matrix: root-mean-square norm and its gradient, 8-bit packing.
+//
+// All of them are bound by HBM where there are many rows, by latency where there are few.  A row is read once: W warps hold it in
+// registers, NV vectors of eight elements a lane, from its first load to the last store, so that the norm's sum, the largest
+// magnitude for the scale and the codes cost no second pass.  One warp takes up to 2048 columns by itself (no barrier anywhere, 16
+// loads of 16 bytes a lane in flight with a residual); wider rows, and narrower ones when there are too few rows for a warp each to
+// fill the GPU, are shared by the warps of a CTA.  A vector's elements lie side by side where rows start on 16 bytes, else 32 apart, so that
+// loads of single elements are coalesced.  Rows that do not fit in registers are taken by the *_any_ kernels, a CTA per row,
+// in passes over L2.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -7,32 +15,350 @@
 namespace b200 {
 
 constexpr int kRowThreads = 256;
+constexpr int kRowWarpsMost = 8;  // of a row
 
-__device__ __forceinline__ float block_sum(float v, float* shared) {  // the same bits in every thread; `shared`: one float per warp
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// over `warps` warps, which are the CTA unless that is one; the same bits in every thread.  `shared`: one word per warp, and not
+// the one of the call before.
+__device__ __forceinline__ float row_sum(float v, int warps, float* shared) {
+    v = warp_sum(v);
+    if (warps == 1) return v;
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0.f;
-    for (int k = 0; k < (int)blockDim.x / 32; k++) v += shared[k];
-    __syncthreads();
+    for (int k = 0; k < warps; k++) v += shared[k];
     return v;
 }
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* shared) {
+__device__ __forceinline__ uint32_t row_max(uint32_t v, int warps, uint32_t* shared) {
     v = __reduce_max_sync(0xffffffffu, v);
+    if (warps == 1) return v;
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0;
-    for (int k = 0; k < (int)blockDim.x / 32; k++) v = max(v, shared[k]);
+    for (int k = 0; k < warps; k++) v = max(v, shared[k]);
+    return v;
+}
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t finite_magnitude(float v) { return finite(v) ? magnitude_bits(v) : 0u; }
+
+// Eight elements from `first` on (VEC) or from `first` on in steps of 32; those at or past `cols` are 0.
+template <bool VEC, class T>
+struct Eight {
+    static constexpr int kWords = sizeof(T) / 2;  // of 16 bytes
+    uint4 raw[VEC && sizeof(T) > 1 ? kWords : 1];
+    T one[VEC ? 1 : 8];
+    __device__ __forceinline__ void load(const T* row, int first, int cols) {
+        if constexpr (VEC) {
+            if (first < cols) {
+#pragma unroll
+                for (int k = 0; k < kWords; k++) raw[k] = __ldcs(reinterpret_cast<const uint4*>(row + first) + k);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kWords; k++) raw[k] = make_uint4(0, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) one[k] = first + 32 * k < cols ? __ldcs(row + first + 32 * k) : from_float<T>(0.f);
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = to_float(one[k]);
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                v[4 * k] = __uint_as_float(raw[k].x), v[4 * k + 1] = __uint_as_float(raw[k].y), v[4 * k + 2] = __uint_as_float(raw[k].z), v[4 * k + 3] = __uint_as_float(raw[k].w);
+        } else {
+            const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) unpack2<T>(w[k], v[2 * k], v[2 * k + 1]);
+        }
+    }
+};
+template <bool VEC>
+__device__ __forceinline__ void load_weights(const float* w, int first, int cols, float (&v)[8]) {
+    if constexpr (VEC) {
+        const float4 a = first < cols ? __ldg(reinterpret_cast<const float4*>(w + first)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 b = first < cols ? __ldg(reinterpret_cast<const float4*>(w + first) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = first + 32 * k < cols ? __ldg(w + first + 32 * k) : 0.f;
+    }
+}
+template <bool VEC, class T>
+__device__ __forceinline__ void store_eight(T* row, int first, int cols, const float (&v)[8]) {
+    if constexpr (!VEC) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (first + 32 * k < cols) row[first + 32 * k] = from_float<T>(v[k]);
+    } else if (first < cols) {
+        uint4* at = reinterpret_cast<uint4*>(row + first);
+        if constexpr (sizeof(T) == 4) {
+            at[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            at[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+        } else {
+            at[0] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        }
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void store_typed(void* at, int64_t row_at, int type, int first, int cols, const float (&v)[8]) {
+    if (type == B200_TYPE_F32)
+        store_eight<VEC>(static_cast<float*>(at) + row_at, first, cols, v);
+    else if (type == B200_TYPE_BF16)
+        store_eight<VEC>(static_cast<bf16*>(at) + row_at, first, cols, v);
+    else
+        store_eight<VEC>(static_cast<f16*>(at) + row_at, first, cols, v);
+}
+// Eight codes.  `all_finite`: of the row; then no value needs looking at but those that an activation's outputs have to keep.
+template <bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, const float (&v)[8], uint32_t scale, int act, bool all_finite) {
+    const float by = one_over_scale(scale);
+    uint32_t q[4];
+    if (all_finite && act == B200_ACT_NONE && scale != kTopScale) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) q[k] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * k] * by, v[2 * k + 1] * by), __NV_SATFINITE, __NV_E4M3);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            q[k] = code_of_output(v[2 * k], scale, act) | (uint32_t)code_of_output(v[2 * k + 1], scale, act) << 8;
+    }
+    if constexpr (VEC) {
+        if (first < cols) *reinterpret_cast<uint2*>(row + first) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (first + 32 * k < cols) row[first + 32 * k] = (uint8_t)(q[k / 2] >> 8 * (k & 1));
+    }
+}
+
+// This thread's row and first elements.
+struct RowPlace {
+    int64_t row;
+    int lane_at, step, warps;  // columns lane_at + step * j, j < NV, are its vectors' first
+    template <bool VEC>
+    __device__ __forceinline__ static RowPlace here(int warps) {
+        RowPlace p;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        p.warps = warps;
+        p.row = warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
+        p.lane_at = (warps == 1 ? 0 : 256 * warp) + (VEC ? 8 * lane : lane);
+        p.step = 256 * warps;
+        return p;
+    }
+};
+
+template <class TX, int NV, bool VEC>
+static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_norm_op a, int warps) {
+    __shared__ float sums[kRowWarpsMost];
+    __shared__ uint32_t largest[2][kRowWarpsMost];
+    const RowPlace p = RowPlace::here<VEC>(warps);
+    if (p.row >= a.rows) return;  // (whole warps of their own)
+    Eight<VEC, TX> x[NV], r[NV];
+    const TX* xr = static_cast<const TX*>(a.x) + p.row * a.ldx;
+#pragma unroll
+    for (int j = 0; j < NV; j++) x[j].load(xr, p.lane_at + p.step * j, a.cols);
+    if (a.residual) {
+        const TX* rr = static_cast<const TX*>(a.residual) + p.row * a.ldr;
+#pragma unroll
+        for (int j = 0; j < NV; j++) r[j].load(rr, p.lane_at + p.step * j, a.cols);
+    }
+    float v[NV][8], squares = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        x[j].get(v[j]);
+        if (a.residual) {
+            float s[8];
+            r[j].get(s);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[j][k] += s[k];
+        }
+        if (a.sum) store_eight<VEC>(static_cast<TX*>(a.sum) + p.row * a.lds, p.lane_at + p.step * j, a.cols, v[j]);
+#pragma unroll
+        for (int k = 0; k < 8; k++) squares = fmaf(v[j][k], v[j][k], squares);
+    }
+    const float rstd = 1.f / sqrtf(row_sum(squares, warps, sums) / (float)a.cols + a.eps);
+    if (a.rstd && (threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.rstd[p.row] = rstd;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        float w[8];
+        if (a.weight) load_weights<VEC>(a.weight, p.lane_at + p.step * j, a.cols, w);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            v[j][k] *= rstd;
+            if (a.weight) v[j][k] *= w[k];
+            // (past the columns there are zeros, and zeros times an infinite rstd, which no code is to know of)
+            if (VEC ? p.lane_at + p.step * j < a.cols : p.lane_at + p.step * j + 32 * k < a.cols) m = max(m, magnitude_bits(v[j][k]));
+        }
+        if (a.y_type != B200_TYPE_E4M3) store_typed<VEC>(a.y, p.row * a.ldy, a.y_type, p.lane_at + p.step * j, a.cols, v[j]);
+    }
+    if (a.y_type != B200_TYPE_E4M3) return;
+    m = row_max(m, warps, largest[0]);
+    const bool all_finite = m < 0x7f800000u;
+    if (!all_finite) {  // the same in all threads of the row
+        m = 0;
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) m = max(m, finite_magnitude(v[j][k]));
+        m = row_max(m, warps, largest[1]);
+    }
+    const uint32_t scale = scale_bits(m);
+    if ((threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.scale[p.row] = __uint_as_float(scale);
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+        store_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, v[j], scale, B200_ACT_NONE, all_finite);
+}
+
+template <class TX, int NV, bool VEC>
+static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pack8_op a, int warps) {
+    __shared__ uint32_t largest[2][kRowWarpsMost];
+    const RowPlace p = RowPlace::here<VEC>(warps);
+    if (p.row >= a.rows) return;
+    Eight<VEC, TX> x[NV];
+    const TX* xr = static_cast<const TX*>(a.x) + p.row * a.ldx;
+#pragma unroll
+    for (int j = 0; j < NV; j++) x[j].load(xr, p.lane_at + p.step * j, a.cols);
+    float v[NV][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        x[j].get(v[j]);
+#pragma unroll
+        for (int k = 0; k < 8; k++) m = max(m, magnitude_bits(v[j][k]));
+    }
+    m = row_max(m, warps, largest[0]);
+    const bool all_finite = m < 0x7f800000u;
+    if (!all_finite) {
+        m = 0;
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) m = max(m, finite_magnitude(v[j][k]));
+        m = row_max(m, warps, largest[1]);
+    }
+    const uint32_t scale = scale_bits(m);
+    if ((threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.scale[p.row] = __uint_as_float(scale);
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+        store_codes<VEC>(static_cast<uint8_t*>(a.q) + p.row * a.ldq, p.lane_at + p.step * j, a.cols, v[j], scale, a.act, all_finite);
+}
+
+// The gradient.  A group of W warps takes rows group, group + groups, ...; dy * n of its columns is added up in registers over
+// its rows, and the CTA's groups in shared memory at the end: parts[CTA][cols].
+template <class TX, class TD, int NV, bool VEC>
+static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b200_rms_norm_grad_op a, float* parts, int warps) {
+    extern __shared__ float added[];  // [groups of the CTA][cols], where there are several
+    __shared__ float sums[2][kRowWarpsMost];
+    const RowPlace p = RowPlace::here<VEC>(warps);
+    const int groups = warps == 1 ? blockDim.x >> 5 : 1;
+    float dw[NV][8] = {};
+    int turn = 0;
+    for (int64_t row = p.row; row < a.rows; row += (int64_t)gridDim.x * groups, turn ^= 1) {
+        Eight<VEC, TX> s[NV], ds[NV];
+        Eight<VEC, TD> dy[NV];
+        const TX* sr = static_cast<const TX*>(a.sum) + row * a.lds;
+        const TD* dr = static_cast<const TD*>(a.dy) + row * a.lddy;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            s[j].load(sr, p.lane_at + p.step * j, a.cols);
+            dy[j].load(dr, p.lane_at + p.step * j, a.cols);
+        }
+        const bool through = a.dsum && a.dx;
+        if (through) {
+            const TX* dsr = static_cast<const TX*>(a.dsum) + row * a.ldds;
+#pragma unroll
+            for (int j = 0; j < NV; j++) ds[j].load(dsr, p.lane_at + p.step * j, a.cols);
+        }
+        const float rstd = a.rstd[row];
+        float n[NV][8], g[NV][8], dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            float w[8];
+            if (a.weight) load_weights<VEC>(a.weight, p.lane_at + p.step * j, a.cols, w);
+            s[j].get(n[j]);
+            dy[j].get(g[j]);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                // (past the columns both are 0, and stay so where rstd is infinite)
+                n[j][k] = (VEC ? p.lane_at + p.step * j < a.cols : p.lane_at + p.step * j + 32 * k < a.cols) ? n[j][k] * rstd : 0.f;
+                dw[j][k] = fmaf(g[j][k], n[j][k], dw[j][k]);
+                if (a.weight) g[j][k] *= w[k];
+                dot = fmaf(g[j][k], n[j][k], dot);
+            }
+        }
+        if (!a.dx) continue;
+        const float mean = row_sum(dot, warps, sums[turn]) / (float)a.cols;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            float d[8] = {};
+            if (through) ds[j].get(d);
+#pragma unroll
+            for (int k = 0; k < 8; k++) d[k] = fmaf(rstd, fmaf(-n[j][k], mean, g[j][k]), d[k]);
+            store_eight<VEC>(static_cast<TX*>(a.dx) + row * a.lddx, p.lane_at + p.step * j, a.cols, d);
+        }
+    }
+    if (!a.dweight) return;
+    float* part = parts + (int64_t)blockIdx.x * a.cols;
+    float* to = groups == 1 ? part : added + (int64_t)(threadIdx.x >> 5) * a.cols;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int c = p.lane_at + p.step * j + (VEC ? k : 32 * k);
+            if (c < a.cols) to[c] = dw[j][k];
+        }
+    if (groups == 1) return;
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+        float v = 0.f;
+        for (int k = 0; k < groups; k++) v += added[(int64_t)k * a.cols + c];
+        part[c] = v;
+    }
+}
+
+// out[c] = the sum of parts[...][c]: 32 columns a CTA, eight warps that take every eighth part.
+static __global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, int n_parts, int cols, float* out) {
+    __shared__ float sums[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float v = 0.f;
+    if (c < cols) {
+#pragma unroll 8
+        for (int k = warp; k < n_parts; k += 8) v += parts[(int64_t)k * cols + c];
+    }
+    sums[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && c < cols) {
+        v = 0.f;
+        for (int k = 0; k < 8; k++) v += sums[k][lane];
+        out[c] = v;
+    }
+}
+
+// ---- rows of any length: a CTA of eight warps per row, element by element
+
+__device__ __forceinline__ float cta_sum(float v, float* shared) {
+    v = row_sum(v, kRowWarpsMost, shared);
     __syncthreads();
     return v;
 }
-__device__ __forceinline__ uint32_t finite_magnitude(float v) { return finite(v) ? __float_as_uint(v) & 0x7fffffffu : 0u; }
+__device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* shared) {
+    v = row_max(v, kRowWarpsMost, shared);
+    __syncthreads();
+    return v;
+}
 
-// A CTA per row at a time, elements one by one.
-template <class TX, class TY>
-static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_norm_op a) {
-    __shared__ float sums[kRowThreads / 32];
-    __shared__ uint32_t largest[kRowThreads / 32];
+template <class TX>
+static __global__ void __launch_bounds__(kRowThreads) rms_norm_any_kernel(b200_rms_norm_op a) {
+    __shared__ float sums[kRowWarpsMost];
+    __shared__ uint32_t largest[kRowWarpsMost];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* x = static_cast<const TX*>(a.x) + row * a.ldx;
         const TX* r = a.residual ? static_cast<const TX*>(a.residual) + row * a.ldr : nullptr;
@@ -43,24 +369,23 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
             v = fmaf(t, t, v);
             if (a.sum) static_cast<TX*>(a.sum)[row * a.lds + c] = from_float<TX>(t);
         }
-        const float rstd = 1.f / sqrtf(block_sum(v, sums) / (float)a.cols + a.eps);
+        const float rstd = 1.f / sqrtf(cta_sum(v, sums) / (float)a.cols + a.eps);
         if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
         auto normed = [&](int c) { return total(c) * rstd * (a.weight ? a.weight[c] : 1.f); };
-        if constexpr (sizeof(TY) == 1) {
+        if (a.y_type == B200_TYPE_E4M3) {
             uint32_t m = 0;
             for (int c = threadIdx.x; c < a.cols; c += kRowThreads) m = max(m, finite_magnitude(normed(c)));
-            const uint32_t scale = scale_bits(block_max(m, largest));
+            const uint32_t scale = scale_bits(cta_max(m, largest));
             if (threadIdx.x == 0) a.scale[row] = __uint_as_float(scale);
-            for (int c = threadIdx.x; c < a.cols; c += kRowThreads) static_cast<uint8_t*>(a.y)[row * a.ldy + c] = code_of(normed(c), one_over_scale(scale));
+            for (int c = threadIdx.x; c < a.cols; c += kRowThreads) static_cast<uint8_t*>(a.y)[row * a.ldy + c] = code_of_output(normed(c), scale, B200_ACT_NONE);
         } else {
-            for (int c = threadIdx.x; c < a.cols; c += kRowThreads) static_cast<TY*>(a.y)[row * a.ldy + c] = from_float<TY>(normed(c));
+            for (int c = threadIdx.x; c < a.cols; c += kRowThreads) store_value(a.y, row * a.ldy + c, a.y_type, normed(c));
         }
     }
 }
-
 template <class TX, class TD>
-static __global__ void __launch_bounds__(kRowThreads) rms_norm_dx_kernel(b200_rms_norm_grad_op a) {
-    __shared__ float sums[kRowThreads / 32];
+static __global__ void __launch_bounds__(kRowThreads) rms_norm_dx_any_kernel(b200_rms_norm_grad_op a) {
+    __shared__ float sums[kRowWarpsMost];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* s = static_cast<const TX*>(a.sum) + row * a.lds;
         const TD* dy = static_cast<const TD*>(a.dy) + row * a.lddy;
@@ -69,17 +394,16 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_dx_kernel(b200_rm
         auto g = [&](int c) { return to_float(dy[c]) * (a.weight ? a.weight[c] : 1.f); };
         float v = 0.f;
         for (int c = threadIdx.x; c < a.cols; c += kRowThreads) v = fmaf(g(c), to_float(s[c]) * rstd, v);
-        const float mean = block_sum(v, sums) / (float)a.cols;
+        const float mean = cta_sum(v, sums) / (float)a.cols;
         for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
             const float dx = rstd * (g(c) - to_float(s[c]) * rstd * mean);
             static_cast<TX*>(a.dx)[row * a.lddx + c] = from_float<TX>(ds ? dx + to_float(ds[c]) : dx);
         }
     }
 }
-
 // Sums over a piece of the rows, a thread per column: parts[piece][cols].
 template <class TX, class TD>
-static __global__ void __launch_bounds__(kRowThreads) rms_norm_dweight_kernel(b200_rms_norm_grad_op a, float* parts) {
+static __global__ void __launch_bounds__(kRowThreads) rms_norm_dweight_any_kernel(b200_rms_norm_grad_op a, float* parts) {
     const int c = blockIdx.x * kRowThreads + threadIdx.x;
     if (c >= a.cols) return;
     const int64_t first = (int64_t)a.rows * blockIdx.y / gridDim.y, last = (int64_t)a.rows * (blockIdx.y + 1) / gridDim.y;
@@ -88,62 +412,144 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_dweight_kernel(b2
         v = fmaf(to_float(static_cast<const TD*>(a.dy)[row * a.lddy + c]), to_float(static_cast<const TX*>(a.sum)[row * a.lds + c]) * a.rstd[row], v);
     parts[(int64_t)blockIdx.y * a.cols + c] = v;
 }
-static __global__ void __launch_bounds__(kRowThreads) add_parts_kernel(const float* parts, int n_parts, int cols, float* out) {
-    const int c = blockIdx.x * kRowThreads + threadIdx.x;
-    if (c >= cols) return;
-    float v = 0.f;
-    for (int k = 0; k < n_parts; k++) v += parts[(int64_t)k * cols + c];
-    out[c] = v;
-}
-
 template <class TX>
-static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pack8_op a) {
-    __shared__ uint32_t largest[kRowThreads / 32];
+static __global__ void __launch_bounds__(kRowThreads) pack8_rows_any_kernel(b200_pack8_op a) {
+    __shared__ uint32_t largest[kRowWarpsMost];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* x = static_cast<const TX*>(a.x) + row * a.ldx;
         uint32_t m = 0;
         for (int c = threadIdx.x; c < a.cols; c += kRowThreads) m = max(m, finite_magnitude(to_float(x[c])));
-        const uint32_t scale = scale_bits(block_max(m, largest));
+        const uint32_t scale = scale_bits(cta_max(m, largest));
         if (threadIdx.x == 0) a.scale[row] = __uint_as_float(scale);
         for (int c = threadIdx.x; c < a.cols; c += kRowThreads)
-            static_cast<uint8_t*>(a.q)[row * a.ldq + c] = code_of_output(to_float(x[c]), one_over_scale(scale), __uint_as_float(scale), a.act);
+            static_cast<uint8_t*>(a.q)[row * a.ldq + c] = code_of_output(to_float(x[c]), scale, a.act);
     }
 }
 
-// By column: a thread per column and piece of the rows.  Scales are in the order of their bits and none is 0, so the largest of
-// the pieces' is the column's; a column without a finite value but 0 is left at 0, which pack8_columns_kernel takes for 1 and
-// whose first piece writes 1 there: the others take either as 1.
-template <class TX>
-static __global__ void __launch_bounds__(kRowThreads) column_scales_kernel(b200_pack8_op a) {
-    const int c = blockIdx.x * kRowThreads + threadIdx.x;
-    if (c >= a.cols) return;
-    const int64_t first = (int64_t)a.rows * blockIdx.y / gridDim.y, last = (int64_t)a.rows * (blockIdx.y + 1) / gridDim.y;
-    uint32_t m = 0;
-    for (int64_t row = first; row < last; row++) m = max(m, finite_magnitude(to_float(static_cast<const TX*>(a.x)[row * a.ldx + c])));
-    if (m) atomicMax(reinterpret_cast<uint32_t*>(a.scale) + c, scale_bits(m));
-}
-template <class TX>
-static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_pack8_op a) {
-    const int c = blockIdx.x * kRowThreads + threadIdx.x;
-    if (c >= a.cols) return;
-    const int64_t first = (int64_t)a.rows * blockIdx.y / gridDim.y, last = (int64_t)a.rows * (blockIdx.y + 1) / gridDim.y;
-    volatile uint32_t* at = reinterpret_cast<uint32_t*>(a.scale) + c;
-    uint32_t scale = *at;
-    if (scale == 0) {
-        scale = scale_bits(0);
-        if (blockIdx.y == 0) *at = scale;
+// ---- by column
+
+// A thread takes V columns (eight side by side, or one) of the rows of its CTA's piece, the CTA's threads `across` of them side by
+// side and the rest in other rows.  Scales are in the order of their bits and none is 0, so the largest of the pieces' is the
+// column's; a column without a finite value but 0 is left at 0, which pack8_columns_kernel takes for 1 and whose first piece
+// writes 1 there: the others take either as 1.
+struct ColumnPlace {
+    int column;
+    int64_t row, last, step;
+    __device__ __forceinline__ ColumnPlace(int rows, int across, int v) {
+        const int64_t first = (int64_t)rows * blockIdx.y / gridDim.y;
+        last = (int64_t)rows * (blockIdx.y + 1) / gridDim.y;
+        column = (blockIdx.x * across + (int)threadIdx.x % across) * v;
+        step = kRowThreads / across;
+        row = first + (int)threadIdx.x / across;
     }
-    for (int64_t row = first; row < last; row++)
-        static_cast<uint8_t*>(a.q)[row * a.ldq + c] =
-            code_of_output(to_float(static_cast<const TX*>(a.x)[row * a.ldx + c]), one_over_scale(scale), __uint_as_float(scale), a.act);
+};
+constexpr int kColumnRows = 4;  // in flight
+template <class T>
+__device__ __forceinline__ void load_columns(const T* at, float (&v)[8]) {
+    Eight<true, T> e;
+    e.load(at, 0, 8);
+    e.get(v);
+}
+template <class T>
+__device__ __forceinline__ void load_columns(const T* at, float (&v)[1]) {
+    v[0] = to_float(*at);
+}
+template <class TX, int V>
+static __global__ void __launch_bounds__(kRowThreads) column_scales_kernel(b200_pack8_op a, int across) {
+    ColumnPlace p(a.rows, across, V);
+    if (p.column >= a.cols) return;
+    uint32_t m[V] = {};
+    const TX* x = static_cast<const TX*>(a.x) + p.column;
+    for (; p.row < p.last; p.row += p.step * kColumnRows) {
+        float v[kColumnRows][V];
+#pragma unroll
+        for (int r = 0; r < kColumnRows; r++) load_columns(x + min(p.row + r * p.step, p.last - 1) * a.ldx, v[r]);
+#pragma unroll
+        for (int r = 0; r < kColumnRows; r++)
+#pragma unroll
+            for (int k = 0; k < V; k++) m[k] = max(m[k], finite_magnitude(v[r][k]));
+    }
+#pragma unroll
+    for (int k = 0; k < V; k++)
+        if (m[k]) atomicMax(reinterpret_cast<uint32_t*>(a.scale) + p.column + k, scale_bits(m[k]));
+}
+template <class TX, int V>
+static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_pack8_op a, int across) {
+    ColumnPlace p(a.rows, across, V);
+    if (p.column >= a.cols) return;
+    uint32_t scale[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+        volatile uint32_t* at = reinterpret_cast<uint32_t*>(a.scale) + p.column + k;
+        scale[k] = *at;
+        if (scale[k] == 0) {
+            scale[k] = scale_bits(0);
+            if (blockIdx.y == 0) *at = scale[k];
+        }
+    }
+    const TX* x = static_cast<const TX*>(a.x) + p.column;
+    uint8_t* q = static_cast<uint8_t*>(a.q) + p.column;
+    for (; p.row < p.last; p.row += p.step * kColumnRows) {
+        float v[kColumnRows][V];
+#pragma unroll
+        for (int r = 0; r < kColumnRows; r++) load_columns(x + min(p.row + r * p.step, p.last - 1) * a.ldx, v[r]);
+#pragma unroll
+        for (int r = 0; r < kColumnRows; r++) {
+            if (p.row + r * p.step >= p.last) break;
+            uint32_t code[V];
+#pragma unroll
+            for (int k = 0; k < V; k++) code[k] = code_of_output(v[r][k], scale[k], a.act);
+            if constexpr (V == 8)
+                *reinterpret_cast<uint2*>(q + (p.row + r * p.step) * a.ldq) = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
+                                                                                        code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
+            else
+                q[(p.row + r * p.step) * a.ldq] = (uint8_t)code[0];
+        }
+    }
 }
 
-template <class TY>
-static __global__ void __launch_bounds__(kRowThreads) unpack8_kernel(b200_unpack8_op a) {
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x)
-        for (int c = threadIdx.x; c < a.cols; c += kRowThreads)
-            static_cast<TY*>(a.y)[row * a.ldy + c] =
-                from_float<TY>(to_float(static_cast<const e4m3*>(a.q)[row * a.ldq + c]) * a.scale[a.by_column ? c : row]);
+// ---- codes to values: the threads of a CTA `across` side by side, V codes each (eight or one), kUnpackRows rows in flight
+constexpr int kUnpackRows = 4;
+template <class TY, int V>
+static __global__ void __launch_bounds__(kRowThreads) unpack8_kernel(b200_unpack8_op a, int across) {
+    const int rows_at_once = kRowThreads / across, lane = (int)threadIdx.x % across;
+    const int64_t first = (int64_t)blockIdx.x * rows_at_once * kUnpackRows + (int)threadIdx.x / across;
+    const uint8_t* q = static_cast<const uint8_t*>(a.q);
+    for (int c = lane * V; c < a.cols; c += across * V) {
+        uint2 code[kUnpackRows];
+        float scale[kUnpackRows];
+#pragma unroll
+        for (int r = 0; r < kUnpackRows; r++) {
+            const int64_t row = min(first + (int64_t)r * rows_at_once, (int64_t)a.rows - 1);
+            if constexpr (V == 8)
+                code[r] = __ldcs(reinterpret_cast<const uint2*>(q + row * a.ldq + c));
+            else
+                code[r].x = q[row * a.ldq + c];
+            scale[r] = a.by_column ? 1.f : __ldg(a.scale + row);
+        }
+        float by_column[V];
+#pragma unroll
+        for (int k = 0; k < V; k++) by_column[k] = a.by_column ? __ldg(a.scale + c + k) : 1.f;
+#pragma unroll
+        for (int r = 0; r < kUnpackRows; r++) {
+            const int64_t row = first + (int64_t)r * rows_at_once;
+            if (row >= a.rows) break;
+            float v[V];
+#pragma unroll
+            for (int k = 0; k < V; k += V == 8 ? 2 : 1) {
+                const uint32_t pair = (k < 4 ? code[r].x : code[r].y) >> 8 * (k & 3);
+                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(pair & 0xffffu), __NV_E4M3);
+                const float2 f = __half22float2(__half2(h));
+                v[k] = f.x * scale[r] * by_column[k];
+                if constexpr (V == 8) v[k + 1] = f.y * scale[r] * by_column[k + 1];
+            }
+            TY* y = static_cast<TY*>(a.y) + row * a.ldy + c;
+            if constexpr (V == 8)
+                store_eight<true>(y, 0, 8, v);
+            else
+                *y = from_float<TY>(v[0]);
+        }
+    }
 }
 
 }  // namespace b200

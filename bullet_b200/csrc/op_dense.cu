@@ -1,5 +1,6 @@
 // Operator-level entry points of dense layers: b200_op_dense and its gradient.
 #include <algorithm>
+#include <atomic>
 
 #include "kernels_product.cuh"
 #include "kernels_rows.cuh"
@@ -9,14 +10,220 @@ namespace {
 
 using namespace b200;
 
-int launch_product(const Product& p, cudaStream_t s) {
-    if ((p.m + 63) / 64 > 65535) return fail(B200_ERR_UNSUPPORTED, "too many rows");
-    product_kernel<<<dim3((unsigned)((p.n + 63) / 64), (unsigned)((p.m + 63) / 64)), 256, 0, s>>>(p);
-    OP_CK(cudaGetLastError());
+// ---- the host's word for waits that gave up (Waits)
+
+// Memory of the library image that both sides may touch at any time; kernels touch it only if there is something to report.
+static __managed__ int g_gave_up;
+
+// Its address for kernels, or null where the device cannot share such memory while it is running.
+int* gave_up_word(int device) {
+    constexpr int kDevices = 64;
+    static std::atomic<signed char> known[kDevices];  // 0 not asked yet, 1 yes, -1 no
+    if (device < 0 || device >= kDevices) return nullptr;
+    if (known[device] == 0) {
+        int concurrent = 0;
+        if (cudaDeviceGetAttribute(&concurrent, cudaDevAttrConcurrentManagedAccess, device) != cudaSuccess) concurrent = 0;
+        if (concurrent) {  // (hints: the word stays in host memory)
+            cudaMemAdvise(&g_gave_up, sizeof g_gave_up, cudaMemAdviseSetPreferredLocation, cudaCpuDeviceId);
+            cudaMemAdvise(&g_gave_up, sizeof g_gave_up, cudaMemAdviseSetAccessedBy, device);
+        }
+        cudaGetLastError();
+        known[device] = concurrent ? 1 : -1;
+    }
+    return known[device] > 0 ? &g_gave_up : nullptr;
+}
+int check_gave_up(const char* who, int* word) {
+    if (word && *reinterpret_cast<volatile int*>(word)) {
+        *reinterpret_cast<volatile int*>(word) = 0;
+        return fail(B200_ERR_STATE, "%s: a kernel of a call before waited too long for its own copies or products; that call's outputs are not valid", who);
+    }
     return 0;
 }
 
-int pieces(int rows, int cols) { return std::max(1, std::min(rows / 16, 148 * 8 / ((cols + 255) / 256))); }
+// ---- products
+
+struct Operand {  // rows of `cols` consecutive elements
+    const void* at;
+    int64_t ld, rows, cols;
+    int type;
+    int64_t bytes_of_row() const { return ld * type_bytes(type); }
+    bool aligned() const { return (uintptr_t)at % 16 == 0 && bytes_of_row() % 16 == 0; }
+    int64_t copy_ld() const { return (cols * type_bytes(type) + 15) / 16 * 16 / type_bytes(type); }
+    int64_t copy_bytes() const { return aligned() ? 0 : (rows * copy_ld() * type_bytes(type) + 255) / 256 * 256; }
+};
+Operand operand(const void* at, int64_t ld, int64_t rows, int64_t cols, int type) {
+    Operand o{at, ld, rows, cols, type};
+    if (rows == 1) o.ld = o.copy_ld();  // (there is no second row)
+    return o;
+}
+
+struct Call {
+    Operand a, b;
+    bool a_across, b_across, codes;  // codes: a is an 8-bit checkpoint with a scale per k
+    ProductArgs p;
+    bool bytes() const { return a.type == B200_TYPE_E4M3 && !codes; }
+    int block() const { return bytes() ? 128 : 64; }  // of k in a stage
+};
+
+// How a product is cut.  The costs are clocks: of a stage (128 bytes of k) of each tile, of an item besides, of a join and of its
+// bytes per clock.
+struct Plan {
+    int columns;  // of a tile; 256: a pair's
+    int parts, blocks;
+};
+constexpr int kSms = 148;  // that products are cut for
+constexpr int kStage256 = 560, kStage128 = 520, kStage64 = 400, kItem = 1500, kJoin = 6000, kJoinBytes = 2500, kPartsMost = 32;
+Plan plan_of(const Call& c) {
+    const int64_t blocks = (c.p.k + c.block() - 1) / c.block();
+    Plan best{};
+    double least = 1e300;
+    for (int columns : {256, 128, 64}) {
+        if (columns == 64 && c.bytes()) continue;  // (boxes across are 128 columns there)
+        const int64_t rows = columns == 256 ? 256 : 128, units = columns == 256 ? kSms / 2 : kSms;
+        const int64_t tiles = ((c.p.m + rows - 1) / rows) * ((c.p.n + columns - 1) / columns);
+        const double stage = columns == 256 ? kStage256 : columns == 128 ? kStage128 : kStage64;
+        for (int64_t parts = 1; parts <= std::min<int64_t>(kPartsMost, blocks); parts++) {
+            if (parts > 1 && tiles * (parts - 1) >= 2 * units) break;
+            const int64_t each = (blocks + parts - 1) / parts, rounds = (tiles * parts + units - 1) / units;
+            double cost = (double)rounds * (each * stage + kItem);
+            if (parts > 1) cost += kJoin + 8.0 * parts * c.p.m * c.p.n / kJoinBytes;
+            if (cost < least) least = cost, best = {columns, (int)((blocks + each - 1) / each), (int)each};
+        }
+    }
+    return best;
+}
+int64_t parts_bytes(const Call& c, const Plan& plan) { return plan.parts > 1 ? (int64_t)plan.parts * c.p.m * ((c.p.n + 7) / 8 * 8) * 4 : 0; }
+int64_t call_bytes(const Call& c) { return c.a.copy_bytes() + c.b.copy_bytes() + (parts_bytes(c, plan_of(c)) + 255) / 256 * 256; }
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+Encode encoder() {
+    static std::atomic<void*> found;
+    if (!found) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult how;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &how) == cudaSuccess && how == cudaDriverEntryPointSuccess) found = fn;
+    }
+    return reinterpret_cast<Encode>(found.load());
+}
+int make_map(CUtensorMap* map, const Operand& o, int box_cols, int box_rows, bool swizzled) {
+    const Encode encode = encoder();
+    if (!encode) return fail(B200_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t size[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows}, stride[1] = {(cuuint64_t)o.bytes_of_row()};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, each[2] = {1, 1};
+    const CUtensorMapDataType type = o.type == B200_TYPE_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : o.type == B200_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult rc = encode(map, type, 2, const_cast<void*>(o.at), size, stride, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS)
+        return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) on %lld rows of %lld, %lld bytes apart", (int)rc, (long long)o.rows, (long long)o.cols, (long long)o.bytes_of_row());
+    return 0;
+}
+
+template <int BN, bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
+int launch(const Call& c, cudaStream_t stream) {
+    constexpr bool PAIR = BN == 256;
+    using T = Tile<BN, PAIR, BYTES, A_ACROSS, B_ACROSS, CODES>;
+    CUtensorMap a, b;
+    if (int rc = CODES ? make_map(&a, c.a, 128, 64, false) : A_ACROSS ? make_map(&a, c.a, T::kBlock, T::kBlock, true) : make_map(&a, c.a, T::kBlock, 128, true)) return rc;
+    if (int rc = B_ACROSS ? make_map(&b, c.b, T::kBlock, T::kBlock, true) : make_map(&b, c.b, T::kBlock, T::kOwnColumns, true)) return rc;
+    auto kernel = product_kernel<BN, PAIR, BYTES, A_ACROSS, B_ACROSS, CODES>;
+    static std::atomic<uint64_t> allowed;  // a bit per device
+    int device = 0;
+    OP_CK(cudaGetDevice(&device));
+    if (device >= 64 || !(allowed >> device & 1)) {
+        OP_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kShared));
+        if (device < 64) allowed |= (uint64_t)1 << device;
+    }
+    const int64_t items = (int64_t)c.p.tiles_m * c.p.tiles_n * c.p.parts_n, units = PAIR ? kSms / 2 : kSms;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)(std::min(items, units) * (PAIR ? 2 : 1)));
+    config.blockDim = dim3(T::kThreads);
+    config.dynamicSmemBytes = T::kShared;
+    config.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {PAIR ? 2u : 1u, 1, 1};
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    OP_CK(cudaLaunchKernelEx(&config, kernel, a, b, c.p));
+    return 0;
+}
+template <bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
+int launch_columns(const Call& c, int columns, cudaStream_t stream) {
+    if (columns == 256) return launch<256, BYTES, A_ACROSS, B_ACROSS, CODES>(c, stream);
+    if constexpr (!BYTES)
+        if (columns == 64) return launch<64, BYTES, A_ACROSS, B_ACROSS, CODES>(c, stream);
+    return launch<128, BYTES, A_ACROSS, B_ACROSS, CODES>(c, stream);
+}
+
+// An operand whose rows do not start on 16 bytes is copied first: the copy moves less than the product does.
+int align(Operand& o, char*& space, cudaStream_t stream) {
+    if (o.aligned()) return 0;
+    void* to = space;
+    space += o.copy_bytes();
+    const int64_t grid = (o.rows + 7) / 8 * ((o.cols + 255) / 256);
+    if (grid > INT32_MAX) return fail(B200_ERR_UNSUPPORTED, "too many elements in rows that do not start on 16 bytes");
+    if (type_bytes(o.type) == 1)
+        align_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>(static_cast<const uint8_t*>(o.at), o.ld, static_cast<uint8_t*>(to), o.copy_ld(), o.rows, o.cols);
+    else
+        align_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>(static_cast<const uint16_t*>(o.at), o.ld, static_cast<uint16_t*>(to), o.copy_ld(), o.rows, o.cols);
+    OP_CK(cudaGetLastError());
+    o.ld = o.copy_ld();
+    o.at = to;
+    return 0;
+}
+
+int run_product(Call c, char* space, cudaStream_t stream) {
+    const Plan plan = plan_of(c);
+    if (int rc = align(c.a, space, stream)) return rc;
+    if (int rc = align(c.b, space, stream)) return rc;
+    ProductArgs& p = c.p;
+    const int rows = plan.columns == 256 ? 256 : 128;
+    p.tiles_m = (int)((p.m + rows - 1) / rows);
+    p.tiles_n = (int)((p.n + plan.columns - 1) / plan.columns);
+    p.k_blocks = (int)((p.k + c.block() - 1) / c.block());
+    p.blocks_per_item = plan.blocks;
+    p.parts_n = plan.parts;
+    p.ldp = (p.n + 7) / 8 * 8;
+    p.parts = plan.parts > 1 ? reinterpret_cast<float*>(space) : nullptr;
+    p.form_type = c.b.type == B200_TYPE_BF16;
+    const int size = type_bytes(p.d_type);
+    auto start = [&](const void* at, int64_t ld, int to) { return ((uintptr_t)at | (uintptr_t)(ld * size)) % to == 0; };
+    p.wide = start(p.d, p.ldd, 16) && (!p.residual || start(p.residual, p.ldr, 16)) ? (start(p.d, p.ldd, 32) ? 2 : 1) : 0;
+    const int rc = c.bytes()    ? launch_columns<true, false, true, false>(c, plan.columns, stream)
+                   : c.codes    ? launch_columns<false, true, true, true>(c, plan.columns, stream)
+                   : c.a_across ? launch_columns<false, true, true, false>(c, plan.columns, stream)
+                   : c.b_across ? launch_columns<false, false, true, false>(c, plan.columns, stream)
+                                : launch_columns<false, false, false, false>(c, plan.columns, stream);
+    if (rc) return rc;
+    if (p.parts) {
+        join_kernel<<<(unsigned)((p.m * (p.ldp / 4) + 255) / 256), 256, 0, stream>>>(p);
+        OP_CK(cudaGetLastError());
+    }
+    return 0;
+}
+
+// ---- the operators
+
+// How dense_dz_kernel deals a matrix out.
+struct DzShape {
+    bool vec;
+    int across, pieces;
+    dim3 grid;
+};
+DzShape dz_shape(const b200_dense_grad_op* op) {
+    auto on = [](const void* at, int64_t ld, int bytes, int to) { return ((uintptr_t)at | (uintptr_t)(ld * bytes)) % to == 0; };
+    DzShape s;
+    s.vec = op->out % 8 == 0 && on(op->dy, op->lddy, 2, 16) &&
+            (op->act == B200_ACT_NONE || (op->y_type == B200_TYPE_E4M3 ? on(op->y, op->ldy, 1, 8) : on(op->y, op->ldy, 2, 16)));
+    const int vectors = s.vec ? op->out / 8 : op->out;
+    s.across = 1;
+    while (s.across < 256 && s.across < vectors) s.across *= 2;
+    const int ctas = (vectors + s.across - 1) / s.across, at_once = 256 / s.across * 4;
+    s.pieces = std::max(1, std::min(op->rows / at_once, std::max(1, kSms * 4 / ctas)));
+    s.grid = dim3(ctas, s.pieces);
+    return s;
+}
 
 int check_dense(const b200_dense_op* op, const char* who) {
     if (!op) return fail(B200_ERR_ARG, "%s: null operator description", who);
@@ -37,9 +244,50 @@ int check_dense_grad(const b200_dense_grad_op* op, const char* who) {
     return 0;
 }
 
-// Where the parts of a workspace begin, in bytes.
+Call forward_call(const b200_dense_op* op) {
+    Call c{};
+    c.a = operand(op->x, op->ldx, op->rows, op->in, op->x_type);
+    c.b = operand(op->w, op->ldw, op->in, op->out, op->x_type);
+    c.b_across = true;
+    ProductArgs& p = c.p;
+    p.m = op->rows, p.n = op->out, p.k = op->in;
+    if (op->x_type == B200_TYPE_E4M3) p.a_scale = op->x_scale, p.b_scale = op->w_scale;
+    p.bias = op->bias, p.residual = op->residual, p.ldr = op->ldr;
+    p.d = op->y, p.ldd = op->ldy, p.d_type = op->y_type, p.act = op->act;
+    return c;
+}
+int64_t dense_bytes(const b200_dense_op* op) {
+    const int64_t bytes = op->rows ? call_bytes(forward_call(op)) : 0;
+    return bytes ? bytes + 256 : 0;
+}
+// g: dz, or dy where that is dz
+Call dx_call(const b200_dense_grad_op* op, const void* g, int64_t ldg) {
+    Call c{};
+    c.a = operand(g, ldg, op->rows, op->out, op->dy_type);
+    c.b = operand(op->w, op->ldw, op->in, op->out, op->dy_type);
+    ProductArgs& p = c.p;
+    p.m = op->rows, p.n = op->in, p.k = op->out;
+    p.residual = op->dskip, p.ldr = op->ldskip;
+    p.d = op->dx, p.ldd = op->lddx, p.d_type = op->dy_type;
+    return c;
+}
+Call dw_call(const b200_dense_grad_op* op, const void* g, int64_t ldg) {
+    Call c{};
+    c.a = operand(op->x, op->ldx, op->rows, op->in, op->x_type);
+    c.b = operand(g, ldg, op->rows, op->out, op->dy_type);
+    c.a_across = c.b_across = true;
+    c.codes = op->x_type == B200_TYPE_E4M3;
+    ProductArgs& p = c.p;
+    p.m = op->in, p.n = op->out, p.k = op->rows;
+    if (c.codes) p.a_scale = op->x_scale;
+    p.d = op->dw, p.ldd = op->lddw, p.d_type = op->dw_type;
+    return c;
+}
+
+// Where the parts of a gradient's workspace begin, in bytes, behind its first multiple of 256.
 struct GradSpace {
-    int64_t dz, parts, all;
+    bool dz_made;
+    int64_t ldz, dz, sums, products, all;
 };
 GradSpace grad_space(const b200_dense_grad_op* op) {
     GradSpace s{};
@@ -49,10 +297,17 @@ GradSpace grad_space(const b200_dense_grad_op* op) {
         s.all += (bytes + 255) / 256 * 256;
         return at;
     };
-    s.dz = next(op->act != B200_ACT_NONE && (op->dx || op->dw) ? (int64_t)op->rows * op->out * 2 : 0);
-    s.parts = next(op->dbias ? (int64_t)pieces(op->rows, op->out) * op->out * 4 : 0);
+    s.ldz = (op->out + 7) / 8 * 8;
+    s.dz_made = op->act != B200_ACT_NONE && (op->dx || op->dw);
+    s.dz = next(s.dz_made ? op->rows * s.ldz * 2 : 0);
+    s.sums = next(op->dbias ? (int64_t)dz_shape(op).pieces * op->out * 4 : 0);
+    const void* g = s.dz_made ? nullptr : op->dy;  // (dz is aligned, as NULL is)
+    const int64_t ldg = s.dz_made ? s.ldz : op->lddy;
+    s.products = next(std::max(op->dx ? call_bytes(dx_call(op, g, ldg)) : 0, op->dw ? call_bytes(dw_call(op, g, ldg)) : 0));
+    if (s.all) s.all += 256;
     return s;
 }
+char* aligned_space(void* workspace) { return reinterpret_cast<char*>(((uintptr_t)workspace + 255) & ~(uintptr_t)255); }
 
 }  // namespace
 
@@ -61,7 +316,7 @@ extern "C" {
 int b200_op_dense_workspace(const b200_dense_op* op, int64_t* bytes) {
     if (int rc = check_dense(op, "op_dense")) return rc;
     if (!bytes) return fail(B200_ERR_ARG, "op_dense: null result");
-    *bytes = 0;
+    *bytes = dense_bytes(op);
     return 0;
 }
 
@@ -81,16 +336,13 @@ int b200_op_dense(int device, void* stream, const b200_dense_op* op) {
         if (int rc = check_floats(who, "x_scale", op->x_scale)) return rc;
         if (int rc = check_floats(who, "w_scale", op->w_scale)) return rc;
     }
+    if (int rc = check_workspace(who, op->workspace, op->workspace_bytes, dense_bytes(op))) return rc;
     OnDevice on(device);
     OP_CK(on.status);
-    Product p{};
-    p.m = op->rows, p.n = op->out, p.k = op->in;
-    p.a = op->x, p.a_m = op->ldx, p.a_k = 1, p.a_type = op->x_type;
-    p.b = op->w, p.b_k = op->ldw, p.b_n = 1, p.b_type = op->x_type;
-    if (packed) p.a_scale_m = op->x_scale, p.b_scale_n = op->w_scale;
-    p.bias = op->bias, p.residual = op->residual, p.ldr = op->ldr;
-    p.d = op->y, p.ldd = op->ldy, p.d_type = op->y_type, p.act = op->act;
-    return launch_product(p, static_cast<cudaStream_t>(stream));
+    Call c = forward_call(op);
+    c.p.gave_up = gave_up_word(device);
+    if (int rc = check_gave_up(who, c.p.gave_up)) return rc;
+    return run_product(c, aligned_space(op->workspace), static_cast<cudaStream_t>(stream));
 }
 
 int b200_op_dense_backward_workspace(const b200_dense_grad_op* op, int64_t* bytes) {
@@ -137,34 +389,41 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
         if (op->dbias) OP_CK(cudaMemsetAsync(op->dbias, 0, (size_t)op->out * 4, s));
         return 0;
     }
-    char* base = static_cast<char*>(op->workspace);
-    const bool products = op->dx || op->dw;
-    void* dz = acts && products ? base + space.dz : nullptr;
-    float* parts = op->dbias ? reinterpret_cast<float*>(base + space.parts) : nullptr;
-    if (dz || parts) {
-        const int n = pieces(op->rows, op->out), ctas = (op->out + 255) / 256;
-        dense_dz_kernel<<<dim3(ctas, n), 256, 0, s>>>(*op, dz, parts);
-        if (parts) add_parts_kernel<<<ctas, kRowThreads, 0, s>>>(parts, n, op->out, op->dbias);
+    int* word = gave_up_word(device);
+    if (int rc = check_gave_up(who, word)) return rc;
+    char* base = aligned_space(op->workspace);
+    void* dz = space.dz_made ? base + space.dz : nullptr;
+    float* sums = op->dbias ? reinterpret_cast<float*>(base + space.sums) : nullptr;
+    if (dz || sums) {
+        const DzShape g = dz_shape(op);
+        auto go = [&](auto d, auto y) {
+            using TD = decltype(d);
+            using TY = decltype(y);
+            if (g.vec)
+                dense_dz_kernel<TD, TY, 8><<<g.grid, 256, 0, s>>>(*op, static_cast<TD*>(dz), space.ldz, sums, g.across);
+            else
+                dense_dz_kernel<TD, TY, 1><<<g.grid, 256, 0, s>>>(*op, static_cast<TD*>(dz), space.ldz, sums, g.across);
+        };
+        if (op->dy_type == B200_TYPE_F16)
+            go(f16{}, f16{});
+        else if (op->y_type == B200_TYPE_E4M3)
+            go(bf16{}, e4m3{});
+        else
+            go(bf16{}, bf16{});
+        if (sums) add_parts_kernel<<<(op->out + 31) / 32, 256, 0, s>>>(sums, g.pieces, op->out, op->dbias);
+        OP_CK(cudaGetLastError());
     }
-    OP_CK(cudaGetLastError());
     const void* g = dz ? dz : op->dy;
-    const int64_t ldg = dz ? op->out : op->lddy;
+    const int64_t ldg = dz ? space.ldz : op->lddy;
     if (op->dx) {
-        Product p{};
-        p.m = op->rows, p.n = op->in, p.k = op->out;
-        p.a = g, p.a_m = ldg, p.a_k = 1, p.a_type = op->dy_type;
-        p.b = op->w, p.b_k = 1, p.b_n = op->ldw, p.b_type = op->dy_type;
-        p.residual = op->dskip, p.ldr = op->ldskip;
-        p.d = op->dx, p.ldd = op->lddx, p.d_type = op->dy_type;
-        if (int rc = launch_product(p, s)) return rc;
+        Call c = dx_call(op, g, ldg);
+        c.p.gave_up = word;
+        if (int rc = run_product(c, base + space.products, s)) return rc;
     }
     if (op->dw) {
-        Product p{};
-        p.m = op->in, p.n = op->out, p.k = op->rows;
-        p.a = op->x, p.a_m = 1, p.a_k = op->ldx, p.a_type = op->x_type, p.a_scale_k = op->x_type == B200_TYPE_E4M3 ? op->x_scale : nullptr;
-        p.b = g, p.b_k = ldg, p.b_n = 1, p.b_type = op->dy_type;
-        p.d = op->dw, p.ldd = op->lddw, p.d_type = op->dw_type;
-        if (int rc = launch_product(p, s)) return rc;
+        Call c = dw_call(op, g, ldg);
+        c.p.gave_up = word;
+        if (int rc = run_product(c, base + space.products, s)) return rc;
     }
     return 0;
 }

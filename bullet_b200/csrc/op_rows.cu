@@ -1,5 +1,6 @@
 // Operator-level entry points over the rows of a matrix: b200_op_rms_norm and its gradient, b200_op_pack8, b200_op_unpack8.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels_rows.cuh"
 #include "op_call.h"
@@ -14,9 +15,59 @@ auto with_float(int type, F f) {
     return type == B200_TYPE_F32 ? f(float{}) : type == B200_TYPE_BF16 ? f(bf16{}) : f(f16{});
 }
 
-int row_ctas(int rows) { return std::min(rows, 148 * 8); }
-// pieces of the rows for sums over a column
-int pieces(int rows, int cols) { return std::max(1, std::min(rows / 16, 148 * 8 / ((cols + kRowThreads - 1) / kRowThreads))); }
+// How a launch deals rows out: `warps` of a CTA to a row (1: every warp one of its own), `vectors` of eight elements a lane.
+struct RowShape {
+    int warps, vectors, threads;
+    int64_t groups;  // rows of a CTA
+};
+// A warp takes up to 256 * `most` columns; the others, or fewer rows than the GPU has warps to spare (kFewRows), have the row shared out, a
+// vector or two a lane. 
+constexpr int kFewRows = 148 * 4;
+RowShape row_shape(int64_t rows, int cols, int most) {
+    RowShape s;
+    const int needed = (cols + 255) / 256;  // vectors of a warp
+    s.warps = rows <= kFewRows ? std::min(kRowWarpsMost, needed) : (needed + most - 1) / most;
+    s.warps = std::max(1, std::min(kRowWarpsMost, s.warps));
+    s.vectors = (needed + s.warps - 1) / s.warps;
+    s.threads = s.warps == 1 ? 128 : 32 * s.warps;
+    s.groups = s.warps == 1 ? 4 : 1;
+    return s;
+}
+// f(std::integral_constant) for the smallest of 1, 2, 4, ... that holds `vectors`
+template <int Most, class F>
+void with_vectors(int vectors, F f) {
+    if (vectors <= 1)
+        f(std::integral_constant<int, 1>{});
+    else if (vectors <= 2)
+        f(std::integral_constant<int, 2>{});
+    else if (vectors <= 4 || Most == 4)
+        f(std::integral_constant<int, 4>{});
+    else
+        f(std::integral_constant<int, Most == 4 ? 4 : 8>{});
+}
+template <class F>
+void with_bool(bool b, F f) {
+    if (b)
+        f(std::true_type{});
+    else
+        f(std::false_type{});
+}
+constexpr int kRowVectors = 8, kGradVectors = 4;  // most of a lane
+constexpr int kRowCols = 256 * kRowWarpsMost * kRowVectors, kGradCols = 256 * kRowWarpsMost * kGradVectors;
+int any_ctas(int rows) { return std::min(rows, 148 * 8); }
+// pieces of the rows for sums over a column by CTAs that take `width` columns and, of those, `at_once` rows
+int pieces(int64_t rows, int cols, int width, int at_once) {
+    const int64_t across = (cols + width - 1) / width;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({rows / (4 * at_once), 148 * 8 / across, 65535}));
+}
+// threads side by side in a row of `vectors`
+int threads_across(int vectors) {
+    int t = 1;
+    while (t < kRowThreads && t < vectors) t *= 2;
+    return t;
+}
+bool aligned(const void* at, int64_t ld, int type, int to) { return ((uintptr_t)at | (uintptr_t)(ld * type_bytes(type))) % to == 0; }
+bool aligned8(const void* at, int64_t ld, int type) { return aligned(at, ld, type, type == B200_TYPE_E4M3 ? 8 : 16); }  // vectors of eight elements
 
 int check_norm(const b200_rms_norm_op* op, const char* who) {
     if (!op) return fail(B200_ERR_ARG, "%s: null operator description", who);
@@ -46,9 +97,14 @@ int check_norm_grad(const b200_rms_norm_grad_op* op, const char* who) {
     return 0;
 }
 
-int64_t norm_grad_workspace(const b200_rms_norm_grad_op* op) {
-    return op->dweight && op->rows ? (int64_t)pieces(op->rows, op->cols) * op->cols * 4 : 0;
+// CTAs of the gradient, each of which leaves a row of sums: two per SM (a thread holds 24 to 32 values of eight columns), fewer where there are fewer rows.
+int norm_grad_ctas(const b200_rms_norm_grad_op* op) {
+    if (op->cols > kGradCols) return pieces(op->rows, op->cols, kRowThreads, 4);
+    const RowShape g = row_shape(op->rows, op->cols, kGradVectors);
+    const int per_sm = g.warps == 1 ? 4 : std::max(1, 16 / g.warps);
+    return (int)std::min<int64_t>((op->rows + g.groups - 1) / g.groups, 148 * per_sm);
 }
+int64_t norm_grad_workspace(const b200_rms_norm_grad_op* op) { return op->dweight && op->rows ? (int64_t)norm_grad_ctas(op) * op->cols * 4 : 0; }
 
 int check_pack(int rows, int cols, int type, const char* who) {
     if (rows < 0 || cols < 1) return fail(B200_ERR_ARG, "%s: %d rows of %d", who, rows, cols);
@@ -66,13 +122,20 @@ int b200_op_rms_norm(int device, void* stream, const b200_rms_norm_op* op) {
     OnDevice on(device);
     OP_CK(on.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    with_float(op->x_type, [&](auto x) {
-        using TX = decltype(x);
-        if (op->y_type == B200_TYPE_E4M3)
-            rms_norm_kernel<TX, e4m3><<<row_ctas(op->rows), kRowThreads, 0, s>>>(*op);
-        else
-            with_float(op->y_type, [&](auto y) { rms_norm_kernel<TX, decltype(y)><<<row_ctas(op->rows), kRowThreads, 0, s>>>(*op); });
-    });
+    if (op->cols > kRowCols) {
+        with_float(op->x_type, [&](auto x) { rms_norm_any_kernel<decltype(x)><<<any_ctas(op->rows), kRowThreads, 0, s>>>(*op); });
+    } else {
+        const bool vec = op->cols % 8 == 0 && aligned8(op->x, op->ldx, op->x_type) && aligned8(op->y, op->ldy, op->y_type) && (!op->residual || aligned8(op->residual, op->ldr, op->x_type)) &&
+                         (!op->sum || aligned8(op->sum, op->lds, op->x_type)) && (uintptr_t)op->weight % 16 == 0;
+        const RowShape g = row_shape(op->rows, op->cols, kRowVectors);
+        with_float(op->x_type, [&](auto x) {
+            with_bool(vec, [&](auto v) {
+                with_vectors<kRowVectors>(g.vectors, [&](auto nv) {
+                    rms_norm_kernel<decltype(x), nv(), v()><<<(unsigned)((op->rows + g.groups - 1) / g.groups), g.threads, 0, s>>>(*op, g.warps);
+                });
+            });
+        });
+    }
     OP_CK(cudaGetLastError());
     return 0;
 }
@@ -108,15 +171,32 @@ int b200_op_rms_norm_backward(int device, void* stream, const b200_rms_norm_grad
         if (op->dweight) OP_CK(cudaMemsetAsync(op->dweight, 0, (size_t)op->cols * 4, s));
         return 0;
     }
-    const int column_ctas = (op->cols + kRowThreads - 1) / kRowThreads, n = pieces(op->rows, op->cols);
+    const int ctas = norm_grad_ctas(op);
     float* parts = static_cast<float*>(op->workspace);
-    with_float(op->x_type, [&](auto x) {
-        with_float(op->dy_type, [&](auto dy) {
-            if (op->dx) rms_norm_dx_kernel<decltype(x), decltype(dy)><<<row_ctas(op->rows), kRowThreads, 0, s>>>(*op);
-            if (op->dweight) rms_norm_dweight_kernel<decltype(x), decltype(dy)><<<dim3(column_ctas, n), kRowThreads, 0, s>>>(*op, parts);
+    if (op->cols > kGradCols) {
+        with_float(op->x_type, [&](auto x) {
+            with_float(op->dy_type, [&](auto dy) {
+                if (op->dx) rms_norm_dx_any_kernel<decltype(x), decltype(dy)><<<any_ctas(op->rows), kRowThreads, 0, s>>>(*op);
+                if (op->dweight)
+                    rms_norm_dweight_any_kernel<decltype(x), decltype(dy)><<<dim3((op->cols + kRowThreads - 1) / kRowThreads, ctas), kRowThreads, 0, s>>>(*op, parts);
+            });
         });
-    });
-    if (op->dweight) add_parts_kernel<<<column_ctas, kRowThreads, 0, s>>>(parts, n, op->cols, op->dweight);
+    } else if (op->dx || op->dweight) {
+        const bool vec = op->cols % 8 == 0 && aligned8(op->dy, op->lddy, op->dy_type) && aligned8(op->sum, op->lds, op->x_type) && (!op->dx || aligned8(op->dx, op->lddx, op->x_type)) &&
+                         (!op->dsum || aligned8(op->dsum, op->ldds, op->x_type)) && (uintptr_t)op->weight % 16 == 0;
+        const RowShape g = row_shape(op->rows, op->cols, kGradVectors);
+        const size_t shared = op->dweight && g.groups > 1 ? (size_t)g.groups * op->cols * 4 : 0;  // at most 4 x 1024 floats
+        with_float(op->x_type, [&](auto x) {
+            with_float(op->dy_type, [&](auto dy) {
+                with_bool(vec, [&](auto v) {
+                    with_vectors<kGradVectors>(g.vectors, [&](auto nv) {
+                        rms_norm_backward_kernel<decltype(x), decltype(dy), nv(), v()><<<ctas, g.threads, shared, s>>>(*op, parts, g.warps);
+                    });
+                });
+            });
+        });
+    }
+    if (op->dweight) add_parts_kernel<<<(op->cols + 31) / 32, 256, 0, s>>>(parts, ctas, op->cols, op->dweight);
     OP_CK(cudaGetLastError());
     return 0;
 }
@@ -137,14 +217,27 @@ int b200_op_pack8(int device, void* stream, const b200_pack8_op* op) {
     OnDevice on(device);
     OP_CK(on.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (!op->by_column) {
-        with_float(op->x_type, [&](auto x) { pack8_rows_kernel<decltype(x)><<<row_ctas(op->rows), kRowThreads, 0, s>>>(*op); });
-    } else {
-        const dim3 grid((op->cols + kRowThreads - 1) / kRowThreads, pieces(op->rows, op->cols));
+    const bool vec = op->cols % 8 == 0 && aligned8(op->x, op->ldx, op->x_type) && aligned8(op->q, op->ldq, B200_TYPE_E4M3);
+    if (op->by_column) {
+        const int across = threads_across(vec ? op->cols / 8 : op->cols), width = across * (vec ? 8 : 1);
+        const dim3 grid((op->cols + width - 1) / width, pieces(op->rows, op->cols, width, kRowThreads / across));
         OP_CK(cudaMemsetAsync(op->scale, 0, (size_t)op->cols * 4, s));
         with_float(op->x_type, [&](auto x) {
-            column_scales_kernel<decltype(x)><<<grid, kRowThreads, 0, s>>>(*op);
-            pack8_columns_kernel<decltype(x)><<<grid, kRowThreads, 0, s>>>(*op);
+            with_bool(vec, [&](auto v) {
+                column_scales_kernel<decltype(x), v() ? 8 : 1><<<grid, kRowThreads, 0, s>>>(*op, across);
+                pack8_columns_kernel<decltype(x), v() ? 8 : 1><<<grid, kRowThreads, 0, s>>>(*op, across);
+            });
+        });
+    } else if (op->cols > kRowCols) {
+        with_float(op->x_type, [&](auto x) { pack8_rows_any_kernel<decltype(x)><<<any_ctas(op->rows), kRowThreads, 0, s>>>(*op); });
+    } else {
+        const RowShape g = row_shape(op->rows, op->cols, kRowVectors);
+        with_float(op->x_type, [&](auto x) {
+            with_bool(vec, [&](auto v) {
+                with_vectors<kRowVectors>(g.vectors, [&](auto nv) {
+                    pack8_rows_kernel<decltype(x), nv(), v()><<<(unsigned)((op->rows + g.groups - 1) / g.groups), g.threads, 0, s>>>(*op, g.warps);
+                });
+            });
         });
     }
     OP_CK(cudaGetLastError());
@@ -161,7 +254,13 @@ int b200_op_unpack8(int device, void* stream, const b200_unpack8_op* op) {
     if (int rc = check_floats(who, "scale", op->scale)) return rc;
     OnDevice on(device);
     OP_CK(on.status);
-    with_float(op->y_type, [&](auto y) { unpack8_kernel<decltype(y)><<<row_ctas(op->rows), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op); });
+    const bool vec = op->cols % 8 == 0 && aligned8(op->q, op->ldq, B200_TYPE_E4M3) && aligned8(op->y, op->ldy, op->y_type);
+    const int across = threads_across(vec ? op->cols / 8 : op->cols), rows = kRowThreads / across * kUnpackRows;
+    with_float(op->y_type, [&](auto y) {
+        with_bool(vec, [&](auto v) {
+            unpack8_kernel<decltype(y), v() ? 8 : 1><<<(unsigned)(((int64_t)op->rows + rows - 1) / rows), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, across);
+        });
+    });
     OP_CK(cudaGetLastError());
     return 0;
 }

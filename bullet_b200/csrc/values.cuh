@@ -28,6 +28,48 @@ __device__ __forceinline__ bf16 from_float<bf16>(float v) { return __float2bfloa
 template <>
 __device__ __forceinline__ f16 from_float<f16>(float v) { return __float2half_rn(v); }
 
+// two neighbours of 16 bits in a word
+template <class T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& low, float& high);
+template <>
+__device__ __forceinline__ void unpack2<bf16>(uint32_t w, float& low, float& high) {
+    low = __uint_as_float(w << 16), high = __uint_as_float(w & 0xffff0000u);
+}
+template <>
+__device__ __forceinline__ void unpack2<f16>(uint32_t w, float& low, float& high) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    low = f.x, high = f.y;
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float low, float high);
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16>(float low, float high) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<f16>(float low, float high) {
+    const __half2 v = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// elements of a type that the launch names
+__device__ __forceinline__ float load_value(const void* at, int64_t i, int type) {
+    switch (type) {
+        case B200_TYPE_F32: return static_cast<const float*>(at)[i];
+        case B200_TYPE_BF16: return to_float(static_cast<const bf16*>(at)[i]);
+        case B200_TYPE_F16: return to_float(static_cast<const f16*>(at)[i]);
+        default: return to_float(static_cast<const e4m3*>(at)[i]);
+    }
+}
+__device__ __forceinline__ void store_value(void* at, int64_t i, int type, float v) {
+    switch (type) {
+        case B200_TYPE_F32: static_cast<float*>(at)[i] = v; break;
+        case B200_TYPE_BF16: static_cast<bf16*>(at)[i] = from_float<bf16>(v); break;
+        default: static_cast<f16*>(at)[i] = from_float<f16>(v);
+    }
+}
+
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u; }
 
 // The scale for a largest finite magnitude given by its bits: the smallest power of two from 2^-126 on with magnitude / scale
@@ -39,17 +81,16 @@ __device__ __forceinline__ uint32_t scale_bits(uint32_t magnitude) {
 }
 __device__ __forceinline__ float one_over_scale(uint32_t scale) { return __uint_as_float((254u << 23) - scale); }
 
-// The code of v / scale (`by` = 1 / scale): nearest, halves to even, NaN for what is not finite.
-__device__ __forceinline__ uint8_t code_of(float v, float by) {
-    const uint8_t q = __nv_cvt_float_to_fp8(v * by, __NV_SATFINITE, __NV_E4M3);
-    return finite(v) ? q : 0x7f;
-}
-// The same for outputs of an activation: what is above 0 stays above 0, what is below 1 stays below 1.
-__device__ __forceinline__ uint8_t code_of_output(float v, float by, float scale, int act) {
-    uint8_t q = code_of(v, by);
-    if (act == B200_ACT_NONE || !finite(v)) return q;
-    if (v > 0.f && (q & 0x7f) == 0) q = 1;
-    if (act != B200_ACT_RELU && v > 0.f && v < 1.f && to_float(e4m3{q}) * scale >= 1.f) q--;  // codes above 0 are in the order of their values
+// The code of v / scale: nearest, halves to even, NaN for what is not finite; what would round up out of fp32 (kTopScale) rounds down.
+// For outputs of an activation: what is above 0 stays above 0, what is below 1 stays below 1.
+constexpr uint32_t kTopScale = 247u << 23;  // the largest there is: 256 times that is past fp32
+__device__ __forceinline__ uint8_t code_of_output(float v, uint32_t scale, int act) {
+    uint8_t q = __nv_cvt_float_to_fp8(v * one_over_scale(scale), __NV_SATFINITE, __NV_E4M3);
+    if (!finite(v)) return 0x7f;
+    if (scale == kTopScale && (q & 0x7f) >= 0x78) q = (q & 0x80) | 0x77;
+    if (act == B200_ACT_NONE) return q;
+    if (v > 0.f && q == 0) q = 1;
+    if (act != B200_ACT_RELU && v > 0.f && v < 1.f && to_float(e4m3{q}) * __uint_as_float(scale) >= 1.f) q--;  // codes above 0 are in the order of their values
     return q;
 }
 

@@ -446,36 +446,38 @@ def test_calls_run_on_the_current_stream_and_in_graphs(rows):
 
 
 def test_long_matrices_pass_32_bit_offsets():
-    """More than 2^31 elements: the last rows come out as they do alone."""
-    rows, cols = (1 << 20) + 37, 2056
+    """More than 2^31 elements: the last rows are those of the plain forms, by the bounds of the tests above."""
+    rows, cols, n = (1 << 20) + 37, 2056, 40
+    sums = cols * 2.0 ** -23 + FEW
     x = torch.zeros(rows, cols, device="cuda", dtype=BF16)
-    x[-40:] = normal(111, 40, cols).to(BF16)
-    tail = x[-40:].clone()
+    x[-n:] = normal(111, n, cols).to(BF16)
+    tail = x[-n:].double()
     w = normal(112, cols, 16).to(BF16)
-    assert torch.equal(ops.dense(x, w)[-40:], ops.dense(tail, w))
-    y, _, _ = ops.rms_norm(x, out_dtype=E4M3)
-    z, _, _ = ops.rms_norm(tail, out_dtype=E4M3)
-    assert torch.equal(y.codes[-40:].view(torch.uint8), z.codes.view(torch.uint8)) and torch.equal(y.scale[-40:], z.scale)
-    v = ops.unpack8(y)[-40:]
-    assert torch.equal(v, ops.unpack8(z))
-    del y, v
+    near(ops.dense(x, w)[-n:], tail @ w.double(), ROUND[BF16], 2 * sums * (tail.abs() @ w.double().abs()))
+    y, _, rstd = ops.rms_norm(x, out_dtype=E4M3)
+    s = 1 / torch.sqrt(tail.square().mean(1) + 1e-5)
+    near(rstd[-n:], s, sums)
+    want, last = tail * s[:, None], ops.Packed8(y.codes[-n:], y.scale[-n:])
+    near(ops.unpack8(y, F32)[-n:], want, sums, half_step(want, exact_scale(want, 1)) * (1 + FEW))
+    assert (last.scale.double() == exact_scale(want, 1)[:, 0]).all()
+    del y, last
     p = ops.pack8(x)
-    assert torch.equal(p.codes[-40:].view(torch.uint8), ops.pack8(tail).codes.view(torch.uint8))
+    near(ops.unpack8(p)[-n:], tail, 0, half_step(tail, exact_scale(tail, 1)))
     dy = torch.zeros(rows, 16, device="cuda", dtype=BF16)
-    dy[-40:] = whole(113, -1, 1, 40, 16)
-    dx, dw, _ = ops.dense_backward(dy, p, w)
-    want = ops.dense_backward(dy[-40:].contiguous(), ops.pack8(tail), w)
-    assert torch.equal(dx[-40:], want[0])
-    near(dw, want[1], 2.0 ** -20, 1e-5)
-    del dx, p
-    total = x
+    dy[-n:] = whole(113, -1, 1, n, 16)
+    g, xv = dy[-n:].double(), ops.unpack8(p)[-n:].double()
+    dx, dw, db = ops.dense_backward(dy, p, w)
+    near(dx[-n:], g @ w.double().t(), ROUND[BF16], (g.abs() @ w.double().abs().t()) * (16 * 2.0 ** -23 + FEW))
+    near(dw, xv.t() @ g, 0, (xv.abs().t() @ g.abs()) * (n * 2.0 ** -23 + FEW))
+    assert torch.equal(db.double(), g.sum(0))
+    del dx, p, dy
     dn = torch.zeros_like(x)
-    dn[-40:] = normal(114, 40, cols).to(BF16)
-    rstd = torch.ones(rows, device="cuda")
-    dx, dweight = ops.rms_norm_backward(dn, total, rstd, torch.ones(cols, device="cuda"))
-    want = ops.rms_norm_backward(dn[-40:].contiguous(), tail, rstd[-40:].contiguous(), torch.ones(cols, device="cuda"))
-    assert torch.equal(dx[-40:], want[0])
-    near(dweight, want[1], 2.0 ** -18, 1e-4)
+    dn[-n:] = normal(114, n, cols).to(BF16)
+    g = dn[-n:].double()
+    dx, dweight = ops.rms_norm_backward(dn, x, torch.ones(rows, device="cuda"), torch.ones(cols, device="cuda"))
+    mean = (g * tail).mean(1, keepdim=True)
+    near(dx[-n:], g - tail * mean, ROUND[BF16], (g.abs() + tail.abs() * (g * tail).abs().mean(1, keepdim=True)) * sums)
+    near(dweight, (g * tail).sum(0), 0, (g * tail).abs().sum(0) * (n * 2.0 ** -23 + FEW))
 
 
 def test_the_threads_device_stays(monkeypatch):
