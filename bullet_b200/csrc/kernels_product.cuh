@@ -8,9 +8,9 @@
 //
 // A CTA (or, PAIR, a pair of two SMs that share a tile of 256 rows and each fetch half of its columns) takes items, a tile of
 // the result times a piece of k, one after another.  One thread has TMA fetch boxes of 128 bytes by rows, with the 128-byte
-// swizzle, into a ring of stages; one issues the products of a stage as it arrives, with sums in tensor memory; four warps take
-// finished sums out, a thread a row, while the products of the next item go to the other half of tensor memory.  Their stores are whole
-// 32-byte sectors.  With k cut (`parts`) the pieces' sums go to memory in fp32 and join_kernel adds them up in order.
+// swizzle, into a ring of stages; one issues the products of a stage as it arrives, with sums in tensor memory; eight warps take
+// finished sums out, a thread a row, while the products of the next item go to the other half of tensor memory, and hand them to
+// TMA in boxes of 32 rows of 128 bytes, in which the residual lies already.  With k cut (`parts`) the pieces' sums go to memory in fp32 and join_kernel adds them up in order.
 //
 // CODES: a is an 8-bit checkpoint with a scale per k.  Four more warps turn its codes into bf16 on the way from one place in
 // shared memory to another: a power of two as scale makes that exact, so there is no product of other values than those
@@ -33,7 +33,7 @@ struct ProductArgs {
     void* d;
     int64_t ldd;
     int d_type, act;
-    int wide;      // rows of d and of the residual start on 16 bytes; 2: of d on 32
+    int boxes;     // rows of d and of the residual start on 16 bytes: TMA takes them; else element by element
     float* parts;  // [parts_n][m][ldp], ldp = n up to a multiple of 8; null: none
     int64_t ldp;
     int* gave_up;
@@ -42,141 +42,115 @@ struct ProductArgs {
 template <int BN, bool PAIR, bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
 struct Tile {
     static constexpr int kColumns = BN, kRows = PAIR ? 256 : 128;
-    static constexpr int kOwnColumns = PAIR ? BN / 2 : BN;   // of b, that this CTA fetches
+    static constexpr int kWide = BN == 512 ? 2 : 1;          // products of 256 columns side by side
+    static constexpr int kOwnColumns = PAIR ? 128 : BN;      // of b, that this CTA fetches for each
     static constexpr int kBlock = BYTES ? 128 : 64;          // of k in a stage: 128 bytes
-    static constexpr uint32_t kA = 128 * 128, kB = kOwnColumns * 128, kRaw = CODES ? 64 * 128 : 0, kStage = kA + kB + kRaw;
-    static constexpr int kStages = PAIR || BN == 128 ? 196608 / kStage : 98304 / kStage;  // (two CTAs of the narrowest tile fit on an SM)
-    static constexpr int kThreads = CODES ? 320 : 192;
-    static constexpr size_t kShared = 1024 + (size_t)kStages * kStage;
-    static constexpr uint32_t kMemory = 2 * BN;  // columns of tensor memory
+    static constexpr uint32_t kA = 128 * 128, kBOne = kOwnColumns * 128, kB = kWide * kBOne, kRaw = CODES ? 64 * 128 : 0, kStage = kA + kB;
+    static constexpr int kTakers = BN == 64 || CODES ? 4 : 8;  // warps that take sums out
+    static constexpr int kOwn = BN * 4 / kTakers;              // columns of each of them
+    static constexpr bool kColumnValues = B_ACROSS && !A_ACROSS;  // a bias, and scales of 8-bit weights
+    static constexpr int kGroups = CODES ? 3 : 0;              // of four warps that turn codes into bf16, a stage by turns
+    static constexpr int kRaws = BN == 64 || BN == 512 ? kGroups : 2 * kGroups;  // codes on their way: a ring of their own
+    static constexpr int kThreads = 64 + 32 * (kTakers + 4 * kGroups + (CODES ? 1 : 0));
+    static constexpr size_t kBoxes = kTakers * 4096;           // a box of the result on its way out for each
+    static constexpr size_t kValues = kColumnValues ? (size_t)kTakers * 2 * kOwn * 4 : 0;
+    static constexpr size_t kRest = 1024 + kBoxes + kValues + kRaws * kRaw;
+    static constexpr int kFit = (int)((232448 - 1024 - kRest) / kStage), kStages = kFit < 8 ? kFit : 8;  // (1 KB for barriers)
+    static constexpr size_t kShared = kRest + (size_t)kStages * kStage;
+    static constexpr int kSums = BN == 512 ? 1 : 2;            // items whose sums there is room for
+    static constexpr uint32_t kMemory = kSums * BN;            // columns of tensor memory
     static_assert(!(BYTES && B_ACROSS) || kOwnColumns % 128 == 0, "boxes across are 128 bytes wide");
     static_assert(!CODES || (A_ACROSS && !BYTES), "");
+    // A group has places of the ring of codes to itself, so that it is never more than one use of a place behind or ahead; and the
+    // products that were before the last ones in the place of the stage it writes next have been waited for.
+    static_assert(kGroups <= kStages && kStages >= 3, "");
 };
 
-// Four codes to bf16, times f (powers of two; `more`: and g).  A code's bits, moved to bf16's, are its value times 2^-120.
-__device__ __forceinline__ void codes_to_bf16(uint32_t w, __nv_bfloat162 f, bool more, __nv_bfloat162 g, uint32_t& low, uint32_t& high) {
+// Four codes to bf16, times f.  A code's bits, moved to bf16's, are its value times 2^-120 (but NaN's, which would be 480).
+__device__ __forceinline__ void codes_to_bf16(uint32_t w, __nv_bfloat162 f, uint32_t& low, uint32_t& high) {
     uint32_t t[2] = {__byte_perm(w, 0, 0x1404), __byte_perm(w, 0, 0x3424)};
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const uint32_t v = (t[h] & 0x80008000u) | ((t[h] & 0x7f007f00u) >> 4);
-        __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), f);
-        if (more) x = __hmul2(x, g);
+        const uint32_t v = (t[h] & 0x80008000u) | (t[h] >> 4 & 0x07f007f0u);
+        const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), f);
         t[h] = *reinterpret_cast<const uint32_t*>(&x);
     }
     low = t[0], high = t[1];
 }
 __device__ __forceinline__ uint32_t has_nan_code(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }  // & 0x80808080
+// Four codes one by one into memory, for NaN and scales past 2^7.
+static __device__ __noinline__ void codes_to_bf16_slowly(uint32_t w, float scale, uint32_t* to) {
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) reinterpret_cast<bf16*>(to)[q] = __float2bfloat16_rn(to_float(e4m3{(uint8_t)(w >> 8 * q)}) * scale);
+}
 
-// What becomes of eight sums of a row, all inside the result: d and the residual on 16 bytes.
-template <class T>
-__device__ __forceinline__ void finish_eight(const float (&v)[32], int g, T* d, const T* residual, bool two_sectors) {
-    float x[8];
+// 32 sums of a row as whole sums end: scales, bias (of these columns, in shared memory), activation.
+template <bool BYTES, bool VALUES>
+__device__ __forceinline__ void finish_sums(const ProductArgs& p, float (&v)[32], float a_scale, const float* bias, const float* b_scale) {
+    if constexpr (BYTES) {
 #pragma unroll
-    for (int k = 0; k < 8; k++) x[k] = v[8 * g + k];
-    if (residual) {
+        for (int g = 0; g < 8; g++) {
+            const float4 b = reinterpret_cast<const float4*>(b_scale)[g];
+            v[4 * g] *= a_scale * b.x, v[4 * g + 1] *= a_scale * b.y, v[4 * g + 2] *= a_scale * b.z, v[4 * g + 3] *= a_scale * b.w;
+        }
+    }
+    if constexpr (VALUES) {
+#pragma unroll
+        for (int g = 0; g < 8; g++) {
+            const float4 b = reinterpret_cast<const float4*>(bias)[g];
+            v[4 * g] += b.x, v[4 * g + 1] += b.y, v[4 * g + 2] += b.z, v[4 * g + 3] += b.w;
+        }
+        if (p.act != B200_ACT_NONE)
+#pragma unroll
+            for (int k = 0; k < 32; k++) v[k] = activate(v[k], p.act);
+    }
+}
+// Half of a row of a box (16 bits: 32 columns of 64; fp32: 32 columns, the whole), the residual there added, in place.  Rows of 128 bytes
+// in the 128-byte swizzle; `row`: its start, r its number.
+template <class T>
+__device__ __forceinline__ void box_out(unsigned char* row, int r, int first_piece, const float (&v)[32], bool residual) {
+    constexpr int kPieces = sizeof(T) == 4 ? 8 : 4;
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+        uint4* at = reinterpret_cast<uint4*>(row + (((first_piece + k) ^ (r & 7)) << 4));
+        uint32_t w[4];
         if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const float4 r = __ldg(reinterpret_cast<const float4*>(residual) + k);
-                x[4 * k] += r.x, x[4 * k + 1] += r.y, x[4 * k + 2] += r.z, x[4 * k + 3] += r.w;
+            float x[4] = {v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+            if (residual) {
+                const float4 o = *reinterpret_cast<const float4*>(at);
+                x[0] += o.x, x[1] += o.y, x[2] += o.z, x[3] += o.w;
             }
+#pragma unroll
+            for (int q = 0; q < 4; q++) w[q] = __float_as_uint(x[q]);
         } else {
-            const uint4 r = __ldg(reinterpret_cast<const uint4*>(residual));
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+            float x[8];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                float low, high;
-                unpack2<T>(w[k], low, high);
-                x[2 * k] += low, x[2 * k + 1] += high;
-            }
-        }
-    }
-    if constexpr (sizeof(T) == 4) {
-        uint32_t w[8];
+            for (int q = 0; q < 8; q++) x[q] = v[8 * k + q];
+            if (residual) {
+                const uint4 o = *at;
+                const uint32_t u[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-        for (int k = 0; k < 8; k++) w[k] = __float_as_uint(x[k]);
-        if (two_sectors) {
-            store_32_bytes(d, w);
-        } else {
-            reinterpret_cast<uint4*>(d)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            reinterpret_cast<uint4*>(d)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        }
-    } else {
-        *reinterpret_cast<uint4*>(d) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-    }
-}
-template <class T>
-__device__ __forceinline__ void finish_typed(const ProductArgs& p, const float (&v)[32], int count, T* d, const T* residual) {
-    if (p.wide) {
-        if constexpr (sizeof(T) == 2) {
-            if (count == 32 && p.wide == 2) {  // whole sectors
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t w[8], r[8] = {};
-                    if (residual) {
-                        const uint4 r0 = __ldg(reinterpret_cast<const uint4*>(residual + 16 * h)), r1 = __ldg(reinterpret_cast<const uint4*>(residual + 16 * h) + 1);
-                        r[0] = r0.x, r[1] = r0.y, r[2] = r0.z, r[3] = r0.w, r[4] = r1.x, r[5] = r1.y, r[6] = r1.z, r[7] = r1.w;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        float low, high;
-                        unpack2<T>(r[k], low, high);
-                        w[k] = residual ? pack2<T>(v[16 * h + 2 * k] + low, v[16 * h + 2 * k + 1] + high) : pack2<T>(v[16 * h + 2 * k], v[16 * h + 2 * k + 1]);
-                    }
-                    store_32_bytes(d + 16 * h, w);
+                for (int q = 0; q < 4; q++) {
+                    float low, high;
+                    unpack2<T>(u[q], low, high);
+                    x[2 * q] += low, x[2 * q + 1] += high;
                 }
-                return;
             }
+#pragma unroll
+            for (int q = 0; q < 4; q++) w[q] = pack2<T>(x[2 * q], x[2 * q + 1]);
         }
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-            if (8 * g + 8 <= count) finish_eight<T>(v, g, d + 8 * g, residual ? residual + 8 * g : nullptr, p.wide == 2);
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    const int from = p.wide ? count & ~7 : 0;
-#pragma unroll
-    for (int k = 0; k < 32; k++)
-        if (k >= from && k < count) d[k] = from_float<T>(residual ? v[k] + to_float(residual[k]) : v[k]);
-}
-// What becomes of 32 sums of a row, from column n on.
-__device__ __forceinline__ void finish_sums(const ProductArgs& p, int part, int64_t m, int64_t n, float (&v)[32], float a_scale) {
-    const int count = (int)min((int64_t)32, p.n - n);
-    if (p.parts) {
-        float* at = p.parts + (part * p.m + m) * p.ldp + n;
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-            if (8 * g < count) {  // (rows have room for eights)
-                uint32_t w[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++) w[k] = __float_as_uint(v[8 * g + k]);
-                store_32_bytes(at + 8 * g, w);
-            }
-        return;
-    }
-    if (p.b_scale)
-#pragma unroll
-        for (int k = 0; k < 32; k++) v[k] *= a_scale * (k < count ? __ldg(p.b_scale + n + k) : 0.f);
-    if (p.bias)
-#pragma unroll
-        for (int k = 0; k < 32; k++) v[k] += k < count ? __ldg(p.bias + n + k) : 0.f;
-    if (p.act != B200_ACT_NONE)
-#pragma unroll
-        for (int k = 0; k < 32; k++) v[k] = activate(v[k], p.act);
-    const int64_t d_at = m * p.ldd + n, r_at = m * p.ldr + n;
-    if (p.d_type == B200_TYPE_F32)
-        finish_typed(p, v, count, static_cast<float*>(p.d) + d_at, p.residual ? static_cast<const float*>(p.residual) + r_at : nullptr);
-    else if (p.d_type == B200_TYPE_BF16)
-        finish_typed(p, v, count, static_cast<bf16*>(p.d) + d_at, p.residual ? static_cast<const bf16*>(p.residual) + r_at : nullptr);
-    else
-        finish_typed(p, v, count, static_cast<f16*>(p.d) + d_at, p.residual ? static_cast<const f16*>(p.residual) + r_at : nullptr);
 }
 
 template <int BN, bool PAIR, bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
 static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACROSS, CODES>::kThreads), 1)
-    product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const ProductArgs p) {
+    product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap d_map,
+                   const __grid_constant__ CUtensorMap r_map, const ProductArgs p) {
     using T = Tile<BN, PAIR, BYTES, A_ACROSS, B_ACROSS, CODES>;
     constexpr int kStages = T::kStages, kCtas = PAIR ? 2 : 1;
     extern __shared__ unsigned char raw_smem[];
-    __shared__ uint64_t full[kStages], empty[kStages], codes_in[kStages], ready[kStages], sums_done[2], sums_free[2];
+    __shared__ uint64_t full[kStages], empty[kStages], ready[kStages], sums_done[2], sums_free[2], codes_in[T::kRaws + 1], codes_out[T::kRaws + 1], residual_in[T::kTakers];
     __shared__ uint32_t memory_at;
     __shared__ int dead;
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
@@ -188,12 +162,16 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
         for (int s = 0; s < kStages; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
-            mbar_init(&codes_in[s], 1);
             mbar_init(&ready[s], 4 * kCtas);
         }
+        for (int s = 0; s < T::kRaws; s++) {
+            mbar_init(&codes_in[s], 1);
+            mbar_init(&codes_out[s], 4);
+        }
+        for (int k = 0; k < T::kTakers; k++) mbar_init(&residual_in[k], 1);
         for (int k = 0; k < 2; k++) {
             mbar_init(&sums_done[k], 1);
-            mbar_init(&sums_free[k], 4 * kCtas);
+            mbar_init(&sums_free[k], T::kTakers * kCtas);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
@@ -225,27 +203,29 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
             for (int64_t item = first; item < items && !dead; item += step) {
                 item_of(item, m0, n0, k0, k1, part);
                 m0 += 128 * rank;
-                n0 += T::kOwnColumns * rank;
+                n0 += PAIR ? 128 * rank : 0;
                 for (int kb = k0; kb < k1; kb++) {
                     if (!wait(&empty[s], phase)) break;
-                    const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA, raw_at = b_at + T::kB;
+                    const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA;
                     const uint32_t bar = PAIR ? of_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
                     const int k = kb * T::kBlock;
                     if (rank == 0) mbar_expect_tx(&full[s], kCtas * (CODES ? T::kB : T::kA + T::kB));
-                    if constexpr (CODES) {
-                        mbar_expect_tx(&codes_in[s], T::kRaw);
-                        load_box<false>(raw_at, &a_map, (int)m0, k, smem_u32(&codes_in[s]));
+                    if constexpr (CODES) {  // (others fetch and write a)
                     } else if constexpr (A_ACROSS) {
 #pragma unroll
                         for (int c = 0; c < 128 / T::kBlock; c++) load_box<PAIR>(a_at + c * T::kBlock * 128, &a_map, (int)m0 + c * T::kBlock, k, bar);
                     } else {
                         load_box<PAIR>(a_at, &a_map, k, (int)m0, bar);
                     }
-                    if constexpr (B_ACROSS) {
 #pragma unroll
-                        for (int c = 0; c < T::kOwnColumns / T::kBlock; c++) load_box<PAIR>(b_at + c * T::kBlock * 128, &b_map, (int)n0 + c * T::kBlock, k, bar);
-                    } else {
-                        load_box<PAIR>(b_at, &b_map, k, (int)n0, bar);
+                    for (int h = 0; h < T::kWide; h++) {
+                        if constexpr (B_ACROSS) {
+#pragma unroll
+                            for (int c = 0; c < T::kOwnColumns / T::kBlock; c++)
+                                load_box<PAIR>(b_at + h * T::kBOne + c * T::kBlock * 128, &b_map, (int)n0 + 256 * h + c * T::kBlock, k, bar);
+                        } else {
+                            load_box<PAIR>(b_at + h * T::kBOne, &b_map, k, (int)n0 + 256 * h, bar);
+                        }
                     }
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
@@ -255,14 +235,14 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
         if (lane == 0 && rank == 0) {  // multiplies
             constexpr uint32_t column = T::kBlock * 128;                                    // bytes from 128 bytes across to the next
             constexpr uint32_t a_step = A_ACROSS ? T::kBlock * 32 : 32, b_step = B_ACROSS ? T::kBlock * 32 : 32;  // a quarter of a stage's k
-            const uint32_t form = product_form(p.form_type, A_ACROSS, B_ACROSS, T::kRows, BN);
+            const uint32_t form = product_form(p.form_type, A_ACROSS, B_ACROSS, T::kRows, BN / T::kWide);
             int s = 0, done = 0;
             uint32_t phase = 0;
             for (int64_t item = first; item < items && !dead; item += step, done++) {
                 item_of(item, m0, n0, k0, k1, part);
-                const int half = done & 1;
+                const int half = done % T::kSums;
                 const uint32_t sums = memory + half * BN;
-                if (!wait(&sums_free[half], (done >> 1 & 1) ^ 1)) break;
+                if (!wait(&sums_free[half], (done / T::kSums & 1) ^ 1)) break;
                 tensor_fence_after();
                 bool fine = true;
                 for (int kb = k0; kb < k1 && fine; kb++) {
@@ -272,39 +252,122 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
                     const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA;
 #pragma unroll
                     for (int q = 0; q < 4; q++)
-                        multiply<PAIR, BYTES>(sums, tile_descriptor(a_at + q * a_step, A_ACROSS ? column : 16), tile_descriptor(b_at + q * b_step, B_ACROSS ? column : 16), form,
-                                              kb > k0 || q > 0);
+#pragma unroll
+                        for (int h = 0; h < T::kWide; h++)
+                            multiply<PAIR, BYTES>(sums + 256 * h, tile_descriptor(a_at + q * a_step, A_ACROSS ? column : 16),
+                                                  tile_descriptor(b_at + h * T::kBOne + q * b_step, B_ACROSS ? column : 16), form, kb > k0 || q > 0);
                     when_multiplied<PAIR>(&empty[s]);
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
                 when_multiplied<PAIR>(&sums_done[half]);
             }
         }
-    } else if (warp < 6) {  // takes sums out
-        const int quarter = warp & 3;
+    } else if (warp < 2 + T::kTakers) {  // takes sums out, kOwn columns of 32 rows
+        const int quarter = warp & 3, taker = warp - 2, c0 = taker / 4 * T::kOwn;
+        unsigned char* box = base + kStages * T::kStage + T::kRaws * T::kRaw + taker * 4096;
+        float* bias = reinterpret_cast<float*>(base + kStages * T::kStage + T::kRaws * T::kRaw + T::kBoxes) + taker * 2 * T::kOwn;
+        float* b_scale = bias + T::kOwn;
+        const bool wide = p.boxes && (p.d_type == B200_TYPE_F32 || p.parts), adds = p.residual && !p.parts;
+        const int width = wide ? 32 : 64;  // columns of a box
+        uint32_t residuals = 0;
         int done = 0;
         for (int64_t item = first; item < items; item += step, done++) {
             item_of(item, m0, n0, k0, k1, part);
-            const int half = done & 1;
-            const int64_t m = m0 + 128 * rank + 32 * quarter + lane;
+            const int half = done % T::kSums;
+            const int64_t rows0 = m0 + 128 * rank + 32 * quarter, m = rows0 + lane, own0 = n0 + c0;
+            const int own = rows0 < p.m ? (int)min((int64_t)T::kOwn, p.n - own0) : 0;  // columns there are, 0 or less: nothing here
             const bool here = m < p.m;
-            const float a_scale = BYTES && here && !p.parts ? __ldg(p.a_scale + m) : 1.f;
-            const bool fine = __all_sync(0xffffffffu, wait(&sums_done[half], done >> 1 & 1));
+            const float a_scale = BYTES && here ? __ldg(p.a_scale + m) : 1.f;
+            auto fetch_residual = [&](int c) {
+                if (lane == 0) {
+                    bulk_wait_read<0>();
+                    mbar_expect_tx(&residual_in[taker], 4096);
+                    load_box3(smem_u32(box), &r_map, (int)own0 + c, (int)rows0, 0, smem_u32(&residual_in[taker]));
+                }
+            };
+            if (adds && p.boxes && own > 0) fetch_residual(0);
+            if constexpr (T::kColumnValues) {
+                __syncwarp();
+                for (int c = lane; c < T::kOwn; c += 32) {
+                    bias[c] = p.bias && c < own ? __ldg(p.bias + own0 + c) : 0.f;
+                    if constexpr (BYTES) b_scale[c] = c < own ? __ldg(p.b_scale + own0 + c) : 0.f;
+                }
+                __syncwarp();
+            }
+            const bool fine = __all_sync(0xffffffffu, wait(&sums_done[half], done / T::kSums & 1));
             if (!fine) break;
             tensor_fence_after();
-            for (int c = 0; c < BN / 32 && n0 + 32 * c < p.n; c++) {
+            const uint32_t sums = memory + ((uint32_t)quarter << 21) + half * BN + c0;
+            for (int c = 0; c < own; c += 32) {
                 float v[32];
-                load_sums32(memory + ((uint32_t)quarter << 21) + half * BN + 32 * c, v);
-                if (here) finish_sums(p, part, m, n0 + 32 * c, v, a_scale);
+                load_sums32(sums + c, v);
+                if (!p.parts) finish_sums<BYTES, T::kColumnValues>(p, v, a_scale, bias + c, b_scale + c);
+                if (p.boxes) {
+                    const bool starts = c % width == 0, ends = (c + 32) % width == 0 || c + 32 >= own;
+                    if (starts) {
+                        if (adds) {
+                            if (c > 0) fetch_residual(c);
+                            if (!__all_sync(0xffffffffu, wait(&residual_in[taker], residuals & 1))) break;
+                            residuals++;
+                        } else {
+                            if (lane == 0) bulk_wait_read<0>();
+                            __syncwarp();
+                        }
+                    }
+                    unsigned char* row = box + lane * 128;
+                    if (wide)
+                        box_out<float>(row, lane, 0, v, adds);
+                    else if (p.d_type == B200_TYPE_BF16)
+                        box_out<bf16>(row, lane, starts ? 0 : 4, v, adds);
+                    else
+                        box_out<f16>(row, lane, starts ? 0 : 4, v, adds);
+                    if (ends) {
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            store_box3(&d_map, smem_u32(box), (int)own0 + c / width * width, (int)rows0, part);
+                            bulk_commit();
+                        }
+                        __syncwarp();
+                    }
+                } else if (here) {
+                    for (int k = 0; k < 32; k++) {
+                        if (c + k >= own) break;
+                        float x = v[0];
+#pragma unroll
+                        for (int q = 1; q < 32; q++) x = q == k ? v[q] : x;
+                        if (adds) x += load_value(p.residual, m * p.ldr + own0 + c + k, p.d_type);
+                        store_value(p.d, m * p.ldd + own0 + c + k, p.d_type, x);
+                    }
+                }
             }
             tensor_fence_before();
             __syncwarp();
             if (lane == 0) arrive_at(PAIR ? of_rank(smem_u32(&sums_free[half]), 0) : smem_u32(&sums_free[half]));
         }
+        if (lane == 0) bulk_wait_all();
+    } else if (CODES && warp == T::kThreads / 32 - 1) {
+        if (lane == 0) {  // fetches codes
+            int s = 0;
+            uint32_t phase = 1;
+            for (int64_t item = first; item < items && !dead; item += step) {
+                item_of(item, m0, n0, k0, k1, part);
+                for (int kb = k0; kb < k1; kb++) {
+                    if (!wait(&codes_out[s], phase)) break;
+                    mbar_expect_tx(&codes_in[s], T::kRaw);
+                    load_box<false>(smem_u32(base + kStages * T::kStage + s * T::kRaw), &a_map, (int)(m0 + 128 * rank), kb * T::kBlock, smem_u32(&codes_in[s]));
+                    if (++s == T::kRaws) s = 0, phase ^= 1;
+                }
+            }
+        }
     } else if constexpr (CODES) {  // 8 threads a row of 128 codes, 16 each
-        const int t = threadIdx.x - 192, row = t >> 3, j = t & 7;
-        int s = 0;
-        uint32_t phase = 0;
+        const int t = (threadIdx.x - 64 - 32 * T::kTakers) & 127, row = t >> 3, j = t & 7, group = (warp - 2 - T::kTakers) >> 2;
+        int s = 0, in = 0, turn = 0;  // whose stage it is
+        uint32_t phase = 1, in_phase = 0;
+        auto next = [&]() {
+            if (++s == kStages) s = 0, phase ^= 1;
+            if (++in == T::kRaws) in = 0, in_phase ^= 1;
+        };
         for (int64_t item = first; item < items && !dead; item += step) {
             item_of(item, m0, n0, k0, k1, part);
             uint32_t scale[4];
@@ -312,44 +375,61 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int64_t k = (int64_t)kb * 64 + row + 16 * i;
-                    scale[i] = kb < k1 && k < p.k ? __float_as_uint(__ldg(p.a_scale + k)) >> 23 : 127u;
+                    scale[i] = kb < k1 && k < p.k ? __float_as_uint(__ldg(p.a_scale + k)) : 127u << 23;
                 }
             };
-            fetch(k0);
+            fetch(k0 + (group + T::kGroups - turn) % T::kGroups);
             for (int kb = k0; kb < k1; kb++) {
-                if (!__all_sync(0xffffffffu, wait(&codes_in[s], phase))) break;
-                const unsigned char* raw = base + s * T::kStage + T::kA + T::kB;
-                unsigned char* to = base + s * T::kStage + (j >> 2) * 8192;
+                const bool mine = turn == group;
+                if (++turn == T::kGroups) turn = 0;
+                if (!mine) {
+                    next();
+                    continue;
+                }
+                if (!__all_sync(0xffffffffu, wait(&codes_in[in], in_phase))) break;
+                const unsigned char* raw = base + kStages * T::kStage + in * T::kRaw + row * 128 + 16 * j;
+                unsigned char* to = base + s * T::kStage + (j >> 2) * 8192 + row * 128;
+                // (the upper half of the threads of a row write their second piece first: eight threads meet all banks)
+                const int at0 = ((2 * (j & 3) + (j >> 2)) ^ (row & 7)) << 4, at1 = at0 ^ 16;
                 uint4 code[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) code[i] = *reinterpret_cast<const uint4*>(raw + (row + 16 * i) * 128 + 16 * j);
+                for (int i = 0; i < 4; i++) code[i] = *reinterpret_cast<const uint4*>(raw + i * 2048);
+                uint32_t nan = 0, v[4][8];
+                bool large = false;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int e = (int)scale[i] - 127, most = min(e, 7);
-                    const __nv_bfloat162 f = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)((most + 247) << 7)));
-                    const __nv_bfloat162 g = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)((e - most + 127) << 7)));
-                    const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
-                    uint32_t v[8];
+                    const uint32_t e = scale[i] >> 23;
+                    large |= e > 134;
+                    const __nv_bfloat162 f = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)((min(e, 134u) + 120u) << 7)));
+                    const uint4 c = j >> 2 ? make_uint4(code[i].z, code[i].w, code[i].x, code[i].y) : code[i];
+                    nan |= has_nan_code(c.x) | has_nan_code(c.y) | has_nan_code(c.z) | has_nan_code(c.w);
+                    codes_to_bf16(c.x, f, v[i][0], v[i][1]);
+                    codes_to_bf16(c.y, f, v[i][2], v[i][3]);
+                    codes_to_bf16(c.z, f, v[i][4], v[i][5]);
+                    codes_to_bf16(c.w, f, v[i][6], v[i][7]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&codes_out[in]);
+                if (!__all_sync(0xffffffffu, wait(&empty[s], phase))) break;
 #pragma unroll
-                    for (int q = 0; q < 4; q++) codes_to_bf16(w[q], f, e > 7, g, v[2 * q], v[2 * q + 1]);
-                    if ((has_nan_code(w[0]) | has_nan_code(w[1]) | has_nan_code(w[2]) | has_nan_code(w[3])) & 0x80808080u)
+                for (int i = 0; i < 4; i++) {
+                    *reinterpret_cast<uint4*>(to + i * 2048 + at0) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                    *reinterpret_cast<uint4*>(to + i * 2048 + at1) = make_uint4(v[i][4], v[i][5], v[i][6], v[i][7]);
+                }
+                if (large || nan & 0x80808080u) {
 #pragma unroll
-                        for (int q = 0; q < 16; q++)
-                            if ((w[q >> 2] >> 8 * (q & 3) & 0x7f) == 0x7f) v[q >> 1] |= 0x7fffu << 16 * (q & 1);
-                    const int r = row + 16 * i;
-                    // (the upper half of the threads of a row write their second piece first: eight threads meet all banks)
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int piece = h ^ (j >> 2);
-                        *reinterpret_cast<uint4*>(to + r * 128 + (((2 * (j & 3) + piece) ^ (r & 7)) << 4)) =
-                            piece ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(v[0], v[1], v[2], v[3]);
+                        for (int q = 0; q < 4; q++)
+                            codes_to_bf16_slowly(w[q], __uint_as_float(scale[i]), reinterpret_cast<uint32_t*>(to + i * 2048 + ((j >> 2) ^ (q >> 1) ? at1 : at0) + (q & 1) * 8));
                     }
                 }
-                fetch(kb + 1);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) arrive_at(PAIR ? of_rank(smem_u32(&ready[s]), 0) : smem_u32(&ready[s]));
-                if (++s == kStages) s = 0, phase ^= 1;
+                fetch(kb + T::kGroups);  // (behind the fence, which would wait for it)
+                next();
             }
         }
     }

@@ -116,18 +116,30 @@ __device__ __forceinline__ void store_typed(void* at, int64_t row_at, int type, 
     else
         store_eight<VEC>(static_cast<f16*>(at) + row_at, first, cols, v);
 }
-// Eight codes.  `all_finite`: of the row; then no value needs looking at but those that an activation's outputs have to keep.
+// Eight codes.  `all_finite`: of the row.  An activation's outputs are moved to where the nearest code is the one that they are to
+// have: those below the smallest code's value to that, those between the last code below 1 and 1 to that code's value (which is
+// 1 - 2^-4 up to scales of 2^6).
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, const float (&v)[8], uint32_t scale, int act, bool all_finite) {
-    const float by = one_over_scale(scale);
+    const float by = one_over_scale(scale), least = __uint_as_float(max(scale, 10u << 23) - (9u << 23));
     uint32_t q[4];
-    if (all_finite && act == B200_ACT_NONE && scale != kTopScale) {
+    if (all_finite && scale != kTopScale && (act == B200_ACT_NONE || (scale >= 10u << 23 && scale <= 133u << 23))) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) q[k] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * k] * by, v[2 * k + 1] * by), __NV_SATFINITE, __NV_E4M3);
+        for (int k = 0; k < 4; k++) {
+            float x[2] = {v[2 * k], v[2 * k + 1]};
+            if (act != B200_ACT_NONE) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) x[h] = x[h] > 0.f ? fmaxf(x[h], least) : x[h];
+                if (act != B200_ACT_RELU) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) x[h] = x[h] < 1.f ? fminf(x[h], 0.9375f) : x[h];
+                }
+            }
+            q[k] = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * by, x[1] * by), __NV_SATFINITE, __NV_E4M3);
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            q[k] = code_of_output(v[2 * k], scale, act) | (uint32_t)code_of_output(v[2 * k + 1], scale, act) << 8;
+        for (int k = 0; k < 4; k++) q[k] = code_of_output(v[2 * k], scale, act) | (uint32_t)code_of_output(v[2 * k + 1], scale, act) << 8;
     }
     if constexpr (VEC) {
         if (first < cols) *reinterpret_cast<uint2*>(row + first) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
@@ -508,7 +520,7 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_
     }
 }
 
-// ---- codes to values: the threads of a CTA `across` side by side, V codes each (eight or one), kUnpackRows rows in flight
+// ---- codes to values: the threads of a CTA `across` side by side, V codes each (sixteen or one), kUnpackRows rows in flight
 constexpr int kUnpackRows = 4;
 template <class TY, int V>
 static __global__ void __launch_bounds__(kRowThreads) unpack8_kernel(b200_unpack8_op a, int across) {
@@ -516,38 +528,40 @@ static __global__ void __launch_bounds__(kRowThreads) unpack8_kernel(b200_unpack
     const int64_t first = (int64_t)blockIdx.x * rows_at_once * kUnpackRows + (int)threadIdx.x / across;
     const uint8_t* q = static_cast<const uint8_t*>(a.q);
     for (int c = lane * V; c < a.cols; c += across * V) {
-        uint2 code[kUnpackRows];
+        uint4 code[kUnpackRows];
         float scale[kUnpackRows];
 #pragma unroll
         for (int r = 0; r < kUnpackRows; r++) {
             const int64_t row = min(first + (int64_t)r * rows_at_once, (int64_t)a.rows - 1);
-            if constexpr (V == 8)
-                code[r] = __ldcs(reinterpret_cast<const uint2*>(q + row * a.ldq + c));
+            if constexpr (V == 16)
+                code[r] = __ldcs(reinterpret_cast<const uint4*>(q + row * a.ldq + c));
             else
                 code[r].x = q[row * a.ldq + c];
             scale[r] = a.by_column ? 1.f : __ldg(a.scale + row);
         }
-        float by_column[V];
-#pragma unroll
-        for (int k = 0; k < V; k++) by_column[k] = a.by_column ? __ldg(a.scale + c + k) : 1.f;
 #pragma unroll
         for (int r = 0; r < kUnpackRows; r++) {
             const int64_t row = first + (int64_t)r * rows_at_once;
             if (row >= a.rows) break;
-            float v[V];
-#pragma unroll
-            for (int k = 0; k < V; k += V == 8 ? 2 : 1) {
-                const uint32_t pair = (k < 4 ? code[r].x : code[r].y) >> 8 * (k & 3);
-                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(pair & 0xffffu), __NV_E4M3);
-                const float2 f = __half22float2(__half2(h));
-                v[k] = f.x * scale[r] * by_column[k];
-                if constexpr (V == 8) v[k + 1] = f.y * scale[r] * by_column[k + 1];
-            }
             TY* y = static_cast<TY*>(a.y) + row * a.ldy + c;
-            if constexpr (V == 8)
-                store_eight<true>(y, 0, 8, v);
-            else
-                *y = from_float<TY>(v[0]);
+            if constexpr (V == 16) {
+                const uint32_t w[4] = {code[r].x, code[r].y, code[r].z, code[r].w};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        const uint32_t pair = w[2 * h + k / 4] >> 8 * (k & 3);
+                        const __half2_raw halves = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(pair & 0xffffu), __NV_E4M3);
+                        const float2 f = __half22float2(__half2(halves));
+                        v[k] = f.x * (a.by_column ? __ldg(a.scale + c + 8 * h + k) : scale[r]);
+                        v[k + 1] = f.y * (a.by_column ? __ldg(a.scale + c + 8 * h + k + 1) : scale[r]);
+                    }
+                    store_eight<true>(y, 8 * h, 16, v);
+                }
+            } else {
+                *y = from_float<TY>(to_float(e4m3{(uint8_t)code[r].x}) * (a.by_column ? __ldg(a.scale + c) : scale[r]));
+            }
         }
     }
 }

@@ -72,22 +72,26 @@ struct Plan {
     int parts, blocks;
 };
 constexpr int kSms = 148;  // that products are cut for
-constexpr int kStage256 = 560, kStage128 = 520, kStage64 = 400, kItem = 1500, kJoin = 6000, kJoinBytes = 2500, kPartsMost = 32;
+constexpr int kPartsMost = 32, kJoin = 6000, kJoinBytes = 2500;
+struct TileCost {
+    int columns, rows, units, stage, item;
+};
+constexpr TileCost kTiles[] = {{512, 256, kSms / 2, 1226, 5500}, {256, 256, kSms / 2, 687, 900}, {128, 128, kSms, 650, 900}, {64, 128, kSms, 450, 900}};
+constexpr int kStageCodes512 = 1403, kStageCodes256 = 1222;  // (narrower tiles turn codes more often)
 Plan plan_of(const Call& c) {
     const int64_t blocks = (c.p.k + c.block() - 1) / c.block();
     Plan best{};
     double least = 1e300;
-    for (int columns : {256, 128, 64}) {
-        if (columns == 64 && c.bytes()) continue;  // (boxes across are 128 columns there)
-        const int64_t rows = columns == 256 ? 256 : 128, units = columns == 256 ? kSms / 2 : kSms;
-        const int64_t tiles = ((c.p.m + rows - 1) / rows) * ((c.p.n + columns - 1) / columns);
-        const double stage = columns == 256 ? kStage256 : columns == 128 ? kStage128 : kStage64;
+    for (const TileCost& t : kTiles) {
+        if (t.columns == 64 && c.bytes()) continue;  // (boxes across are 128 columns there)
+        const int64_t tiles = ((c.p.m + t.rows - 1) / t.rows) * ((c.p.n + t.columns - 1) / t.columns);
+        const double stage = c.codes && t.columns >= 256 ? (t.columns == 512 ? kStageCodes512 : kStageCodes256) : t.stage;
         for (int64_t parts = 1; parts <= std::min<int64_t>(kPartsMost, blocks); parts++) {
-            if (parts > 1 && tiles * (parts - 1) >= 2 * units) break;
-            const int64_t each = (blocks + parts - 1) / parts, rounds = (tiles * parts + units - 1) / units;
-            double cost = (double)rounds * (each * stage + kItem);
+            if (parts > 1 && tiles * (parts - 1) >= 2 * t.units) break;
+            const int64_t each = (blocks + parts - 1) / parts, rounds = (tiles * parts + t.units - 1) / t.units;
+            double cost = (double)rounds * (each * stage + t.item);
             if (parts > 1) cost += kJoin + 8.0 * parts * c.p.m * c.p.n / kJoinBytes;
-            if (cost < least) least = cost, best = {columns, (int)((blocks + each - 1) / each), (int)each};
+            if (cost < least) least = cost, best = {t.columns, (int)((blocks + each - 1) / each), (int)each};
         }
     }
     return best;
@@ -119,13 +123,34 @@ int make_map(CUtensorMap* map, const Operand& o, int box_cols, int box_rows, boo
     return 0;
 }
 
+// The result, or its parts, as a stack of matrices, in boxes of 32 rows of 128 bytes.
+int make_result_map(CUtensorMap* map, const void* at, int type, int64_t ld, int64_t rows, int64_t cols, int64_t count) {
+    const Encode encode = encoder();
+    if (!encode) return fail(B200_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t row = (cuuint64_t)(rows == 1 ? (cols * type_bytes(type) + 15) / 16 * 16 : ld * type_bytes(type));
+    const cuuint64_t size[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)count}, stride[2] = {row, (cuuint64_t)rows * (cuuint64_t)(count > 1 ? ld * type_bytes(type) : row)};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / type_bytes(type)), 32, 1}, each[3] = {1, 1, 1};
+    const CUtensorMapDataType kind = type == B200_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == B200_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult rc = encode(map, kind, 3, const_cast<void*>(at), size, stride, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) on %lld rows of %lld, %lld apart", (int)rc, (long long)rows, (long long)cols, (long long)ld);
+    return 0;
+}
+
 template <int BN, bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
 int launch(const Call& c, cudaStream_t stream) {
-    constexpr bool PAIR = BN == 256;
+    constexpr bool PAIR = BN >= 256;
     using T = Tile<BN, PAIR, BYTES, A_ACROSS, B_ACROSS, CODES>;
-    CUtensorMap a, b;
+    CUtensorMap a, b, d{}, r{};
     if (int rc = CODES ? make_map(&a, c.a, 128, 64, false) : A_ACROSS ? make_map(&a, c.a, T::kBlock, T::kBlock, true) : make_map(&a, c.a, T::kBlock, 128, true)) return rc;
     if (int rc = B_ACROSS ? make_map(&b, c.b, T::kBlock, T::kBlock, true) : make_map(&b, c.b, T::kBlock, T::kOwnColumns, true)) return rc;
+    if (c.p.parts) {
+        if (int rc = make_result_map(&d, c.p.parts, B200_TYPE_F32, c.p.ldp, c.p.m, c.p.ldp, c.p.parts_n)) return rc;
+    } else if (c.p.boxes) {
+        if (int rc = make_result_map(&d, c.p.d, c.p.d_type, c.p.ldd, c.p.m, c.p.n, 1)) return rc;
+        if (c.p.residual)
+            if (int rc = make_result_map(&r, c.p.residual, c.p.d_type, c.p.ldr, c.p.m, c.p.n, 1)) return rc;
+    }
     auto kernel = product_kernel<BN, PAIR, BYTES, A_ACROSS, B_ACROSS, CODES>;
     static std::atomic<uint64_t> allowed;  // a bit per device
     int device = 0;
@@ -145,11 +170,12 @@ int launch(const Call& c, cudaStream_t stream) {
     attr.val.clusterDim = {PAIR ? 2u : 1u, 1, 1};
     config.attrs = &attr;
     config.numAttrs = 1;
-    OP_CK(cudaLaunchKernelEx(&config, kernel, a, b, c.p));
+    OP_CK(cudaLaunchKernelEx(&config, kernel, a, b, d, r, c.p));
     return 0;
 }
 template <bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
 int launch_columns(const Call& c, int columns, cudaStream_t stream) {
+    if (columns == 512) return launch<512, BYTES, A_ACROSS, B_ACROSS, CODES>(c, stream);
     if (columns == 256) return launch<256, BYTES, A_ACROSS, B_ACROSS, CODES>(c, stream);
     if constexpr (!BYTES)
         if (columns == 64) return launch<64, BYTES, A_ACROSS, B_ACROSS, CODES>(c, stream);
@@ -178,7 +204,7 @@ int run_product(Call c, char* space, cudaStream_t stream) {
     if (int rc = align(c.a, space, stream)) return rc;
     if (int rc = align(c.b, space, stream)) return rc;
     ProductArgs& p = c.p;
-    const int rows = plan.columns == 256 ? 256 : 128;
+    const int rows = plan.columns >= 256 ? 256 : 128;
     p.tiles_m = (int)((p.m + rows - 1) / rows);
     p.tiles_n = (int)((p.n + plan.columns - 1) / plan.columns);
     p.k_blocks = (int)((p.k + c.block() - 1) / c.block());
@@ -188,8 +214,8 @@ int run_product(Call c, char* space, cudaStream_t stream) {
     p.parts = plan.parts > 1 ? reinterpret_cast<float*>(space) : nullptr;
     p.form_type = c.b.type == B200_TYPE_BF16;
     const int size = type_bytes(p.d_type);
-    auto start = [&](const void* at, int64_t ld, int to) { return ((uintptr_t)at | (uintptr_t)(ld * size)) % to == 0; };
-    p.wide = start(p.d, p.ldd, 16) && (!p.residual || start(p.residual, p.ldr, 16)) ? (start(p.d, p.ldd, 32) ? 2 : 1) : 0;
+    auto starts = [&](const void* at, int64_t ld) { return (uintptr_t)at % 16 == 0 && (p.m == 1 || ld * size % 16 == 0); };
+    p.boxes = p.parts || (starts(p.d, p.ldd) && (!p.residual || starts(p.residual, p.ldr)));
     const int rc = c.bytes()    ? launch_columns<true, false, true, false>(c, plan.columns, stream)
                    : c.codes    ? launch_columns<false, true, true, true>(c, plan.columns, stream)
                    : c.a_across ? launch_columns<false, true, true, false>(c, plan.columns, stream)

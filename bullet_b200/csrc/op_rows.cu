@@ -254,11 +254,11 @@ int b200_op_unpack8(int device, void* stream, const b200_unpack8_op* op) {
     if (int rc = check_floats(who, "scale", op->scale)) return rc;
     OnDevice on(device);
     OP_CK(on.status);
-    const bool vec = op->cols % 8 == 0 && aligned8(op->q, op->ldq, B200_TYPE_E4M3) && aligned8(op->y, op->ldy, op->y_type);
-    const int across = threads_across(vec ? op->cols / 8 : op->cols), rows = kRowThreads / across * kUnpackRows;
+    const bool vec = op->cols % 16 == 0 && aligned(op->q, op->ldq, B200_TYPE_E4M3, 16) && aligned8(op->y, op->ldy, op->y_type);
+    const int across = threads_across(vec ? op->cols / 16 : op->cols), rows = kRowThreads / across * kUnpackRows;
     with_float(op->y_type, [&](auto y) {
         with_bool(vec, [&](auto v) {
-            unpack8_kernel<decltype(y), v() ? 8 : 1><<<(unsigned)(((int64_t)op->rows + rows - 1) / rows), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, across);
+            unpack8_kernel<decltype(y), v() ? 16 : 1><<<(unsigned)(((int64_t)op->rows + rows - 1) / rows), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, across);
         });
     });
     OP_CK(cudaGetLastError());

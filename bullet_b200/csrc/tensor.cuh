@@ -66,6 +66,16 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, in
                      : "memory");
 }
 
+// Boxes of a stack of matrices; what lies outside is 0, and not written.
+__device__ __forceinline__ void load_box3(uint32_t to, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void store_box3(const CUtensorMap* map, uint32_t from, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 // A tile's descriptor.  Both kinds have rows of 128 bytes with the 128-byte swizzle, eight rows are 1024 bytes.  Along k (K-major):
 // a row of the tile per m or n, 128 bytes of k; `column` unused.  Across (MN-major): a row per k, 128 bytes of m or n, the next
 // 128 bytes of m or n `column` bytes on.
@@ -132,9 +142,4 @@ __device__ __forceinline__ void load_sums32(uint32_t at, float (&v)[32]) {
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void store_32_bytes(void* at, const uint32_t (&v)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
-
 }  // namespace b200

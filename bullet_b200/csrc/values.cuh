@@ -84,7 +84,7 @@ __device__ __forceinline__ float one_over_scale(uint32_t scale) { return __uint_
 // The code of v / scale: nearest, halves to even, NaN for what is not finite; what would round up out of fp32 (kTopScale) rounds down.
 // For outputs of an activation: what is above 0 stays above 0, what is below 1 stays below 1.
 constexpr uint32_t kTopScale = 247u << 23;  // the largest there is: 256 times that is past fp32
-__device__ __forceinline__ uint8_t code_of_output(float v, uint32_t scale, int act) {
+static __device__ __noinline__ uint8_t code_of_output(float v, uint32_t scale, int act) {
     uint8_t q = __nv_cvt_float_to_fp8(v * one_over_scale(scale), __NV_SATFINITE, __NV_E4M3);
     if (!finite(v)) return 0x7f;
     if (scale == kTopScale && (q & 0x7f) >= 0x78) q = (q & 0x80) | 0x77;
