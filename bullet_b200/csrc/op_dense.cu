@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "kernels_few.cuh"
 #include "kernels_product.cuh"
 #include "kernels_rows.cuh"
 #include "op_call.h"
@@ -282,7 +283,42 @@ Call forward_call(const b200_dense_op* op) {
     p.d = op->y, p.ldd = op->ldy, p.d_type = op->y_type, p.act = op->act;
     return c;
 }
+// Few rows: dense_few_kernel.
+bool few_rows(const b200_dense_op* op) { return op->rows <= kFewRowsMost; }
+template <class T, bool VEC>
+int launch_few_typed(const b200_dense_op* op, cudaStream_t stream) {
+    const int groups = (op->out + kFewColumns - 1) / kFewColumns;
+    int ctas = 1;  // of a cluster: while there are SMs for them and enough of k
+    while (ctas < kFewClusterMost && groups * ctas * 2 <= 2 * kSms && op->in / (ctas * 2) >= 2 * kFewStep) ctas *= 2;
+    FewArgs f{*op, (op->in + ctas - 1) / ctas};
+    f.slice = (f.slice + kFewStep - 1) / kFewStep * kFewStep;
+    auto go = [&](auto kernel) {
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3((unsigned)(groups * ctas));
+        config.blockDim = dim3(256);
+        config.stream = stream;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {(unsigned)ctas, 1, 1};
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        return cudaLaunchKernelEx(&config, kernel, f);
+    };
+    OP_CK(op->rows == 1   ? go(dense_few_kernel<T, 1, VEC>)
+          : op->rows == 2 ? go(dense_few_kernel<T, 2, VEC>)
+          : op->rows <= 4 ? go(dense_few_kernel<T, 4, VEC>)
+                          : go(dense_few_kernel<T, 8, VEC>));
+    return 0;
+}
+template <class T>
+int launch_few(const b200_dense_op* op, cudaStream_t stream) {
+    constexpr int kBytes = 8 * sizeof(T);
+    const bool vec = op->out % 8 == 0 && (uintptr_t)op->w % kBytes == 0 && op->ldw * sizeof(T) % kBytes == 0;
+    return vec ? launch_few_typed<T, true>(op, stream) : launch_few_typed<T, false>(op, stream);
+}
+
 int64_t dense_bytes(const b200_dense_op* op) {
+    if (few_rows(op)) return 0;
     const int64_t bytes = op->rows ? call_bytes(forward_call(op)) : 0;
     return bytes ? bytes + 256 : 0;
 }
@@ -365,10 +401,12 @@ int b200_op_dense(int device, void* stream, const b200_dense_op* op) {
     if (int rc = check_workspace(who, op->workspace, op->workspace_bytes, dense_bytes(op))) return rc;
     OnDevice on(device);
     OP_CK(on.status);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (few_rows(op)) return packed ? launch_few<e4m3>(op, s) : op->x_type == B200_TYPE_BF16 ? launch_few<bf16>(op, s) : launch_few<f16>(op, s);
     Call c = forward_call(op);
     c.p.gave_up = gave_up_word(device);
     if (int rc = check_gave_up(who, c.p.gave_up)) return rc;
-    return run_product(c, aligned_space(op->workspace), static_cast<cudaStream_t>(stream));
+    return run_product(c, aligned_space(op->workspace), s);
 }
 
 int b200_op_dense_backward_workspace(const b200_dense_grad_op* op, int64_t* bytes) {
