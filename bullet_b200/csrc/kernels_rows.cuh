@@ -10,6 +10,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "values.cuh"
 
 namespace b200 {
@@ -116,30 +118,46 @@ __device__ __forceinline__ void store_typed(void* at, int64_t row_at, int type, 
     else
         store_eight<VEC>(static_cast<f16*>(at) + row_at, first, cols, v);
 }
-// Eight codes.  `all_finite`: of the row.  An activation's outputs are moved to where the nearest code is the one that they are to
-// have: those below the smallest code's value to that, those between the last code below 1 and 1 to that code's value (which is
-// 1 - 2^-4 up to scales of 2^6).
+// Eight elements of a row on their way to codes: what an activation's outputs have to keep, in the elements' own type where that is
+// bf16 (two at a time).  Those above 0 and below the smallest code's value are moved to that, those between the last code below 1
+// and 1 to that code's value, which is 1 - 2^-4 up to scales of 2^6; then the nearest code is the one that is wanted.
+__device__ __forceinline__ bool moves_outputs(uint32_t scale) { return scale >= 10u << 23 && scale <= 133u << 23; }
+__device__ __forceinline__ float least_value(uint32_t scale) { return __uint_as_float(scale - (9u << 23)); }
+__device__ __forceinline__ float moved_output(float v, float least, int act) {
+    v = v > 0.f ? fmaxf(v, least) : v;
+    return act != B200_ACT_RELU && v < 1.f ? fminf(v, 0.9375f) : v;
+}
+__device__ __forceinline__ uint32_t moved_outputs2(uint32_t w, uint32_t least2, int act) {
+    auto b = [](uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+    auto u = [](__nv_bfloat162 x) { return *reinterpret_cast<const uint32_t*>(&x); };
+    const uint32_t above = __hgt2_mask(b(w), b(0u));
+    w = (above & u(__hmax2(b(w), b(least2)))) | (~above & w);
+    if (act != B200_ACT_RELU) {
+        const uint32_t below = __hlt2_mask(b(w), b(0x3f803f80u));
+        w = (below & u(__hmin2(b(w), b(0x3f703f70u)))) | (~below & w);
+    }
+    return w;
+}
+// (v - v is 0, or NaN for what is not finite, which the code is then)
+__device__ __forceinline__ uint32_t two_codes(float a, float b, float by_a, float by_b) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(fmaf(a, by_a, a - a), fmaf(b, by_b, b - b)), __NV_SATFINITE, __NV_E4M3);
+}
+// Eight codes.
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, const float (&v)[8], uint32_t scale, int act, bool all_finite) {
-    const float by = one_over_scale(scale), least = __uint_as_float(max(scale, 10u << 23) - (9u << 23));
+__device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, const float (&v)[8], uint32_t scale, int act) {
+    const float by = one_over_scale(scale);
     uint32_t q[4];
-    if (all_finite && scale != kTopScale && (act == B200_ACT_NONE || (scale >= 10u << 23 && scale <= 133u << 23))) {
+    if (scale == kTopScale || (act != B200_ACT_NONE && !moves_outputs(scale))) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) q[k] = code_of_output(v[2 * k], scale, act) | (uint32_t)code_of_output(v[2 * k + 1], scale, act) << 8;
+    } else {
+        const float least = act != B200_ACT_NONE ? least_value(scale) : 0.f;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             float x[2] = {v[2 * k], v[2 * k + 1]};
-            if (act != B200_ACT_NONE) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) x[h] = x[h] > 0.f ? fmaxf(x[h], least) : x[h];
-                if (act != B200_ACT_RELU) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) x[h] = x[h] < 1.f ? fminf(x[h], 0.9375f) : x[h];
-                }
-            }
-            q[k] = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * by, x[1] * by), __NV_SATFINITE, __NV_E4M3);
+            if (act != B200_ACT_NONE) x[0] = moved_output(x[0], least, act), x[1] = moved_output(x[1], least, act);
+            q[k] = two_codes(x[0], x[1], by, by);
         }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++) q[k] = code_of_output(v[2 * k], scale, act) | (uint32_t)code_of_output(v[2 * k + 1], scale, act) << 8;
     }
     if constexpr (VEC) {
         if (first < cols) *reinterpret_cast<uint2*>(row + first) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
@@ -213,8 +231,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
     }
     if (a.y_type != B200_TYPE_E4M3) return;
     m = row_max(m, warps, largest[0]);
-    const bool all_finite = m < 0x7f800000u;
-    if (!all_finite) {  // the same in all threads of the row
+    if (m >= 0x7f800000u) {  // the same in all threads of the row
         m = 0;
 #pragma unroll
         for (int j = 0; j < NV; j++)
@@ -226,11 +243,14 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
     if ((threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.scale[p.row] = __uint_as_float(scale);
 #pragma unroll
     for (int j = 0; j < NV; j++)
-        store_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, v[j], scale, B200_ACT_NONE, all_finite);
+        store_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, v[j], scale, B200_ACT_NONE);
 }
 
+// Bound by the ALU pipe before HBM unless elements of 16 bits are compared two at a time: 131072 rows of 2048 bf16 outputs of CReLU
+// 207 us one by one.
 template <class TX, int NV, bool VEC>
 static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pack8_op a, int warps) {
+    constexpr bool TWO = VEC && sizeof(TX) == 2;
     __shared__ uint32_t largest[2][kRowWarpsMost];
     const RowPlace p = RowPlace::here<VEC>(warps);
     if (p.row >= a.rows) return;
@@ -238,29 +258,52 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pac
     const TX* xr = static_cast<const TX*>(a.x) + p.row * a.ldx;
 #pragma unroll
     for (int j = 0; j < NV; j++) x[j].load(xr, p.lane_at + p.step * j, a.cols);
-    float v[NV][8];
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        x[j].get(v[j]);
+        if constexpr (TWO) {  // magnitudes are in the order of their bits
+            m = __vmaxu2(m, x[j].raw[0].x & 0x7fff7fffu);
+            m = __vmaxu2(m, x[j].raw[0].y & 0x7fff7fffu);
+            m = __vmaxu2(m, x[j].raw[0].z & 0x7fff7fffu);
+            m = __vmaxu2(m, x[j].raw[0].w & 0x7fff7fffu);
+        } else {
+            float v[8];
+            x[j].get(v);
 #pragma unroll
-        for (int k = 0; k < 8; k++) m = max(m, magnitude_bits(v[j][k]));
+            for (int k = 0; k < 8; k++) m = max(m, magnitude_bits(v[k]));
+        }
+    }
+    if constexpr (TWO) {
+        float low, high;
+        unpack2<TX>(m, low, high);
+        m = max(magnitude_bits(low), magnitude_bits(high));
     }
     m = row_max(m, warps, largest[0]);
-    const bool all_finite = m < 0x7f800000u;
-    if (!all_finite) {
+    if (m >= 0x7f800000u) {
         m = 0;
 #pragma unroll
-        for (int j = 0; j < NV; j++)
+        for (int j = 0; j < NV; j++) {
+            float v[8];
+            x[j].get(v);
 #pragma unroll
-            for (int k = 0; k < 8; k++) m = max(m, finite_magnitude(v[j][k]));
+            for (int k = 0; k < 8; k++) m = max(m, finite_magnitude(v[k]));
+        }
         m = row_max(m, warps, largest[1]);
     }
     const uint32_t scale = scale_bits(m);
     if ((threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.scale[p.row] = __uint_as_float(scale);
+    const bool two = TWO && std::is_same<TX, bf16>::value && a.act != B200_ACT_NONE && scale != kTopScale && moves_outputs(scale);
+    const uint32_t least2 = two ? pack2<bf16>(least_value(scale), least_value(scale)) : 0;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-        store_codes<VEC>(static_cast<uint8_t*>(a.q) + p.row * a.ldq, p.lane_at + p.step * j, a.cols, v[j], scale, a.act, all_finite);
+    for (int j = 0; j < NV; j++) {
+        if (two) {
+            uint4& w = x[j].raw[0];
+            w = make_uint4(moved_outputs2(w.x, least2, a.act), moved_outputs2(w.y, least2, a.act), moved_outputs2(w.z, least2, a.act), moved_outputs2(w.w, least2, a.act));
+        }
+        float v[8];
+        x[j].get(v);
+        store_codes<VEC>(static_cast<uint8_t*>(a.q) + p.row * a.ldq, p.lane_at + p.step * j, a.cols, v, scale, two ? B200_ACT_NONE : a.act);
+    }
 }
 
 // The gradient.  A group of W warps takes rows group, group + groups, ...; dy * n of its columns is added up in registers over
@@ -336,22 +379,20 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b
     }
 }
 
-// out[c] = the sum of parts[...][c]: 32 columns a CTA, eight warps that take every eighth part.
-static __global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, int n_parts, int cols, float* out) {
-    __shared__ float sums[8][32];
+// out[c] = the sum of parts[...][c]: 32 columns a CTA, 32 warps that take every 32nd part.
+constexpr int kAddThreads = 1024;
+static __global__ void __launch_bounds__(kAddThreads) add_parts_kernel(const float* parts, int n_parts, int cols, float* out) {
+    __shared__ float sums[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (c < cols) {
 #pragma unroll 8
-        for (int k = warp; k < n_parts; k += 8) v += parts[(int64_t)k * cols + c];
+        for (int k = warp; k < n_parts; k += 32) v += __ldcg(parts + (int64_t)k * cols + c);
     }
-    sums[warp][lane] = v;
+    sums[lane][warp] = v;
     __syncthreads();
-    if (warp == 0 && c < cols) {
-        v = 0.f;
-        for (int k = 0; k < 8; k++) v += sums[k][lane];
-        out[c] = v;
-    }
+    v = warp_sum(sums[warp][lane]);  // a warp per column
+    if (lane == 0 && blockIdx.x * 32 + warp < cols) out[blockIdx.x * 32 + warp] = v;
 }
 
 // ---- rows of any length: a CTA of eight warps per row, element by element
@@ -499,6 +540,12 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_
             if (blockIdx.y == 0) *at = scale[k];
         }
     }
+    bool quick = true;
+    float by[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) by[k] = one_over_scale(scale[k]);
+#pragma unroll
+    for (int k = 0; k < V; k++) quick &= scale[k] != kTopScale && (a.act == B200_ACT_NONE || moves_outputs(scale[k]));
     const TX* x = static_cast<const TX*>(a.x) + p.column;
     uint8_t* q = static_cast<uint8_t*>(a.q) + p.column;
     for (; p.row < p.last; p.row += p.step * kColumnRows) {
@@ -509,8 +556,21 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_
         for (int r = 0; r < kColumnRows; r++) {
             if (p.row + r * p.step >= p.last) break;
             uint32_t code[V];
+            if (quick) {
+                if (a.act != B200_ACT_NONE)
 #pragma unroll
-            for (int k = 0; k < V; k++) code[k] = code_of_output(v[r][k], scale[k], a.act);
+                    for (int k = 0; k < V; k++) v[r][k] = moved_output(v[r][k], least_value(scale[k]), a.act);
+#pragma unroll
+                for (int k = 0; k < V; k += 2) {
+                    constexpr int kNext = V > 1 ? 1 : 0;
+                    const uint32_t two = two_codes(v[r][k], v[r][k + kNext], by[k], by[k + kNext]);
+                    code[k + kNext] = two >> 8;
+                    code[k] = two & 0xffu;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; k++) code[k] = code_of_output(v[r][k], scale[k], a.act);
+            }
             if constexpr (V == 8)
                 *reinterpret_cast<uint2*>(q + (p.row + r * p.step) * a.ldq) = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
                                                                                         code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
@@ -520,7 +580,7 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_
     }
 }
 
-// ---- codes to values: the threads of a CTA `across` side by side, V codes each (sixteen or one), kUnpackRows rows in flight
+// ---- codes to values: the threads of a CTA `across` side by side, V codes each (sixteen, eight or one), kUnpackRows rows in flight
 constexpr int kUnpackRows = 4;
 template <class TY, int V>
 static __global__ void __launch_bounds__(kRowThreads) unpack8_kernel(b200_unpack8_op a, int across) {
@@ -533,9 +593,12 @@ static __global__ void __launch_bounds__(kRowThreads) unpack8_kernel(b200_unpack
 #pragma unroll
         for (int r = 0; r < kUnpackRows; r++) {
             const int64_t row = min(first + (int64_t)r * rows_at_once, (int64_t)a.rows - 1);
-            if constexpr (V == 16)
+            if constexpr (V == 16) {
                 code[r] = __ldcs(reinterpret_cast<const uint4*>(q + row * a.ldq + c));
-            else
+            } else if constexpr (V == 8) {
+                const uint2 w = __ldcs(reinterpret_cast<const uint2*>(q + row * a.ldq + c));
+                code[r].x = w.x, code[r].y = w.y;
+            } else
                 code[r].x = q[row * a.ldq + c];
             scale[r] = a.by_column ? 1.f : __ldg(a.scale + row);
         }
@@ -544,10 +607,10 @@ static __global__ void __launch_bounds__(kRowThreads) unpack8_kernel(b200_unpack
             const int64_t row = first + (int64_t)r * rows_at_once;
             if (row >= a.rows) break;
             TY* y = static_cast<TY*>(a.y) + row * a.ldy + c;
-            if constexpr (V == 16) {
+            if constexpr (V > 1) {
                 const uint32_t w[4] = {code[r].x, code[r].y, code[r].z, code[r].w};
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < V / 8; h++) {
                     float v[8];
 #pragma unroll
                     for (int k = 0; k < 8; k += 2) {

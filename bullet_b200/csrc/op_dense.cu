@@ -474,7 +474,7 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
             go(bf16{}, e4m3{});
         else
             go(bf16{}, bf16{});
-        if (sums) add_parts_kernel<<<(op->out + 31) / 32, 256, 0, s>>>(sums, g.pieces, op->out, op->dbias);
+        if (sums) add_parts_kernel<<<(op->out + 31) / 32, kAddThreads, 0, s>>>(sums, g.pieces, op->out, op->dbias);
         OP_CK(cudaGetLastError());
     }
     const void* g = dz ? dz : op->dy;
