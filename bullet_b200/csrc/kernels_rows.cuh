@@ -24,15 +24,34 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// over `warps` warps, which are the CTA unless that is one; the same bits in every thread.  `shared`: one word per warp, and not
-// the one of the call before.
+// Over the `warps` warps of a row; the same bits in every thread.  `shared`: one word per warp of the CTA, and not the words of the call
+// before.  SEVERAL rows share a CTA, warps side by side; else a row of more than one warp has it to itself.  (Barriers by number: with
+// a number out of a register a CTA counts as using all sixteen, and half as many CTAs fit on an SM.)
+template <bool SEVERAL>
+__device__ __forceinline__ void row_sync(int warps) {
+    if constexpr (SEVERAL) {
+        const int group = (int)(threadIdx.x >> 5) / warps;
+        if (group == 0)
+            asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+        else if (group == 1)
+            asm volatile("bar.sync 2, %0;" ::"r"(32 * warps) : "memory");
+        else if (group == 2)
+            asm volatile("bar.sync 3, %0;" ::"r"(32 * warps) : "memory");
+        else
+            asm volatile("bar.sync 4, %0;" ::"r"(32 * warps) : "memory");
+    } else {
+        __syncthreads();
+    }
+}
+template <bool SEVERAL = false>
 __device__ __forceinline__ float row_sum(float v, int warps, float* shared) {
     v = warp_sum(v);
     if (warps == 1) return v;
-    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-    __syncthreads();
+    const int warp = threadIdx.x >> 5, first = SEVERAL ? warp / warps * warps : 0;
+    if ((threadIdx.x & 31) == 0) shared[warp] = v;
+    row_sync<SEVERAL>(warps);
     v = 0.f;
-    for (int k = 0; k < warps; k++) v += shared[k];
+    for (int k = 0; k < warps; k++) v += shared[first + k];
     return v;
 }
 __device__ __forceinline__ uint32_t row_max(uint32_t v, int warps, uint32_t* shared) {
@@ -118,25 +137,24 @@ __device__ __forceinline__ void store_typed(void* at, int64_t row_at, int type, 
     else
         store_eight<VEC>(static_cast<f16*>(at) + row_at, first, cols, v);
 }
-// Eight elements of a row on their way to codes: what an activation's outputs have to keep, in the elements' own type where that is
-// bf16 (two at a time).  Those above 0 and below the smallest code's value are moved to that, those between the last code below 1
-// and 1 to that code's value, which is 1 - 2^-4 up to scales of 2^6; then the nearest code is the one that is wanted.
+// Elements of a row on their way to codes: what an activation's outputs have to keep.  Those above 0 and below the smallest code's
+// value are moved to that, those between the last code below 1 and 1 to that code's value, which is 1 - 2^-4 up to scales of 2^6; then
+// the nearest code is the one that is wanted.  Magnitudes are in the order of their bits: less 1, what is not to move below the
+// least is 0, the largest of all; less 1's bits, what is below 1 comes last.  (131072 x 2048 bf16 outputs of CReLU with
+// comparisons and selections 185 us, with these additions in front of maxima and minima 161.)
 __device__ __forceinline__ bool moves_outputs(uint32_t scale) { return scale >= 10u << 23 && scale <= 133u << 23; }
-__device__ __forceinline__ float least_value(uint32_t scale) { return __uint_as_float(scale - (9u << 23)); }
-__device__ __forceinline__ float moved_output(float v, float least, int act) {
-    v = v > 0.f ? fmaxf(v, least) : v;
-    return act != B200_ACT_RELU && v < 1.f ? fminf(v, 0.9375f) : v;
+__device__ __forceinline__ uint32_t least_bits(uint32_t scale) { return scale - (9u << 23); }
+__device__ __forceinline__ float moved_output(float v, uint32_t least, int act) {
+    uint32_t s = __viaddmax_u32(__float_as_uint(v), 0xffffffffu, least - 1u);
+    if (act == B200_ACT_RELU) return __uint_as_float(s + 1u);
+    s = __viaddmin_u32(s, 1u - 0x3f800000u, 0x3f700000u - 0x3f800000u);
+    return __uint_as_float(s + 0x3f800000u);
 }
-__device__ __forceinline__ uint32_t moved_outputs2(uint32_t w, uint32_t least2, int act) {
-    auto b = [](uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
-    auto u = [](__nv_bfloat162 x) { return *reinterpret_cast<const uint32_t*>(&x); };
-    const uint32_t above = __hgt2_mask(b(w), b(0u));
-    w = (above & u(__hmax2(b(w), b(least2)))) | (~above & w);
-    if (act != B200_ACT_RELU) {
-        const uint32_t below = __hlt2_mask(b(w), b(0x3f803f80u));
-        w = (below & u(__hmin2(b(w), b(0x3f703f70u)))) | (~below & w);
-    }
-    return w;
+__device__ __forceinline__ uint32_t moved_outputs2(uint32_t w, uint32_t least, int act) {  // two bf16; `least`: in both halves
+    uint32_t s = __viaddmax_u16x2(w, 0xffffffffu, least - 0x00010001u);
+    if (act == B200_ACT_RELU) return __viaddmin_u16x2(s, 0x00010001u, 0xffffffffu);
+    s = __viaddmin_u16x2(s, 0xc081c081u, 0xfff0fff0u);
+    return __viaddmin_u16x2(s, 0x3f803f80u, 0xffffffffu);
 }
 // (v - v is 0, or NaN for what is not finite, which the code is then)
 __device__ __forceinline__ uint32_t two_codes(float a, float b, float by_a, float by_b) {
@@ -151,7 +169,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, c
 #pragma unroll
         for (int k = 0; k < 4; k++) q[k] = code_of_output(v[2 * k], scale, act) | (uint32_t)code_of_output(v[2 * k + 1], scale, act) << 8;
     } else {
-        const float least = act != B200_ACT_NONE ? least_value(scale) : 0.f;
+        const uint32_t least = least_bits(scale);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             float x[2] = {v[2 * k], v[2 * k + 1]};
@@ -171,15 +189,23 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, c
 // This thread's row and first elements.
 struct RowPlace {
     int64_t row;
+    bool leader;  // one thread of the row
     int lane_at, step, warps;  // columns lane_at + step * j, j < NV, are its vectors' first
-    template <bool VEC>
+    template <bool VEC, bool SEVERAL = false>
     __device__ __forceinline__ static RowPlace here(int warps) {
         RowPlace p;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         p.warps = warps;
-        p.row = warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
-        p.lane_at = (warps == 1 ? 0 : 256 * warp) + (VEC ? 8 * lane : lane);
         p.step = 256 * warps;
+        if constexpr (!SEVERAL) {  // (no divisions, which cost a short kernel 6 %)
+            p.row = warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
+            p.leader = lane == 0 && (warps == 1 || warp == 0);
+            p.lane_at = (warps == 1 ? 0 : 256 * warp) + (VEC ? 8 * lane : lane);
+            return p;
+        }
+        p.row = (int64_t)blockIdx.x * ((blockDim.x >> 5) / warps) + warp / warps;
+        p.leader = lane == 0 && warp % warps == 0;
+        p.lane_at = 256 * (warp % warps) + (VEC ? 8 * lane : lane);
         return p;
     }
 };
@@ -189,7 +215,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
     __shared__ float sums[kRowWarpsMost];
     __shared__ uint32_t largest[2][kRowWarpsMost];
     const RowPlace p = RowPlace::here<VEC>(warps);
-    if (p.row >= a.rows) return;  // (whole warps of their own)
+    if (p.row >= a.rows) return;  // (all warps of a row)
     Eight<VEC, TX> x[NV], r[NV];
     const TX* xr = static_cast<const TX*>(a.x) + p.row * a.ldx;
 #pragma unroll
@@ -214,7 +240,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
         for (int k = 0; k < 8; k++) squares = fmaf(v[j][k], v[j][k], squares);
     }
     const float rstd = 1.f / sqrtf(row_sum(squares, warps, sums) / (float)a.cols + a.eps);
-    if (a.rstd && (threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.rstd[p.row] = rstd;
+    if (a.rstd && p.leader) a.rstd[p.row] = rstd;
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -240,14 +266,14 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
         m = row_max(m, warps, largest[1]);
     }
     const uint32_t scale = scale_bits(m);
-    if ((threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.scale[p.row] = __uint_as_float(scale);
+    if (p.leader) a.scale[p.row] = __uint_as_float(scale);
 #pragma unroll
     for (int j = 0; j < NV; j++)
         store_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, v[j], scale, B200_ACT_NONE);
 }
 
-// Bound by the ALU pipe before HBM unless elements of 16 bits are compared two at a time: 131072 rows of 2048 bf16 outputs of CReLU
-// 207 us one by one.
+// Elements of 16 bits are compared two at a time: one by one the ALU pipe takes longer than HBM (131072 rows of 2048 bf16 outputs of
+// CReLU 207 us, so 161, for 805 MB).
 template <class TX, int NV, bool VEC>
 static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pack8_op a, int warps) {
     constexpr bool TWO = VEC && sizeof(TX) == 2;
@@ -291,9 +317,9 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pac
         m = row_max(m, warps, largest[1]);
     }
     const uint32_t scale = scale_bits(m);
-    if ((threadIdx.x & 31) == 0 && (warps == 1 || threadIdx.x == 0)) a.scale[p.row] = __uint_as_float(scale);
+    if (p.leader) a.scale[p.row] = __uint_as_float(scale);
     const bool two = TWO && std::is_same<TX, bf16>::value && a.act != B200_ACT_NONE && scale != kTopScale && moves_outputs(scale);
-    const uint32_t least2 = two ? pack2<bf16>(least_value(scale), least_value(scale)) : 0;
+    const uint32_t least2 = (least_bits(scale) >> 16) * 0x00010001u;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         if (two) {
@@ -312,8 +338,8 @@ template <class TX, class TD, int NV, bool VEC>
 static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b200_rms_norm_grad_op a, float* parts, int warps) {
     extern __shared__ float added[];  // [groups of the CTA][cols], where there are several
     __shared__ float sums[2][kRowWarpsMost];
-    const RowPlace p = RowPlace::here<VEC>(warps);
-    const int groups = warps == 1 ? blockDim.x >> 5 : 1;
+    const RowPlace p = RowPlace::here<VEC, true>(warps);
+    const int groups = (blockDim.x >> 5) / warps, group = (threadIdx.x >> 5) / warps;
     float dw[NV][8] = {};
     int turn = 0;
     for (int64_t row = p.row; row < a.rows; row += (int64_t)gridDim.x * groups, turn ^= 1) {
@@ -350,7 +376,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b
             }
         }
         if (!a.dx) continue;
-        const float mean = row_sum(dot, warps, sums[turn]) / (float)a.cols;
+        const float mean = row_sum<true>(dot, warps, sums[turn]) / (float)a.cols;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             float d[8] = {};
@@ -362,7 +388,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b
     }
     if (!a.dweight) return;
     float* part = parts + (int64_t)blockIdx.x * a.cols;
-    float* to = groups == 1 ? part : added + (int64_t)(threadIdx.x >> 5) * a.cols;
+    float* to = groups == 1 ? part : added + (int64_t)group * a.cols;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
@@ -509,22 +535,30 @@ __device__ __forceinline__ void load_columns(const T* at, float (&v)[1]) {
 }
 template <class TX, int V>
 static __global__ void __launch_bounds__(kRowThreads) column_scales_kernel(b200_pack8_op a, int across) {
+    __shared__ uint32_t largest[kRowThreads * V];
     ColumnPlace p(a.rows, across, V);
-    if (p.column >= a.cols) return;
     uint32_t m[V] = {};
     const TX* x = static_cast<const TX*>(a.x) + p.column;
-    for (; p.row < p.last; p.row += p.step * kColumnRows) {
-        float v[kColumnRows][V];
+    if (p.column < a.cols)
+        for (; p.row < p.last; p.row += p.step * kColumnRows) {
+            float v[kColumnRows][V];
 #pragma unroll
-        for (int r = 0; r < kColumnRows; r++) load_columns(x + min(p.row + r * p.step, p.last - 1) * a.ldx, v[r]);
+            for (int r = 0; r < kColumnRows; r++) load_columns(x + min(p.row + r * p.step, p.last - 1) * a.ldx, v[r]);
 #pragma unroll
-        for (int r = 0; r < kColumnRows; r++)
+            for (int r = 0; r < kColumnRows; r++)
 #pragma unroll
-            for (int k = 0; k < V; k++) m[k] = max(m[k], finite_magnitude(v[r][k]));
+                for (int k = 0; k < V; k++) m[k] = max(m[k], finite_magnitude(v[r][k]));
+        }
+    // one word per column and CTA: atomics of all threads took most of the time (65536 x 512 bf16: 430 us)
+#pragma unroll
+    for (int k = 0; k < V; k++) largest[k * kRowThreads + threadIdx.x] = m[k];
+    __syncthreads();
+    for (int c = threadIdx.x; c < across * V; c += kRowThreads) {
+        const int column = blockIdx.x * across * V + c;
+        uint32_t most = 0;
+        for (int r = 0; r < kRowThreads / across; r++) most = max(most, largest[c % V * kRowThreads + r * across + c / V]);
+        if (column < a.cols && most) atomicMax(reinterpret_cast<uint32_t*>(a.scale) + column, scale_bits(most));
     }
-#pragma unroll
-    for (int k = 0; k < V; k++)
-        if (m[k]) atomicMax(reinterpret_cast<uint32_t*>(a.scale) + p.column + k, scale_bits(m[k]));
 }
 template <class TX, int V>
 static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_pack8_op a, int across) {
@@ -559,7 +593,7 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_columns_kernel(b200_
             if (quick) {
                 if (a.act != B200_ACT_NONE)
 #pragma unroll
-                    for (int k = 0; k < V; k++) v[r][k] = moved_output(v[r][k], least_value(scale[k]), a.act);
+                    for (int k = 0; k < V; k++) v[r][k] = moved_output(v[r][k], least_bits(scale[k]), a.act);
 #pragma unroll
                 for (int k = 0; k < V; k += 2) {
                     constexpr int kNext = V > 1 ? 1 : 0;

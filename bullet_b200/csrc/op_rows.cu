@@ -25,17 +25,17 @@ struct RowShape {
 // Measured, us: norm with residual to 8 bits, 131072 x 2048 bf16, of 8 / 4 / 2 vectors 328 / 290 / 349; fp32 without residual 300 / 278 /
 // 259; gradient of 131072 x 2048 bf16 rows, of 4 / 2 / 1 505 / 405 / 614.
 constexpr int kFewRows = 148 * 4;
-RowShape row_shape(int64_t rows, int cols, int best) {
+RowShape row_shape(int64_t rows, int cols, int best, bool several) {
     RowShape s;
     const int needed = (cols + 255) / 256;  // vectors of one warp's lanes
     s.warps = std::max(1, std::min(kRowWarpsMost, rows <= kFewRows ? needed : (needed + best - 1) / best));
     s.vectors = (needed + s.warps - 1) / s.warps;
-    s.threads = s.warps == 1 ? 128 : 32 * s.warps;
-    s.groups = s.warps == 1 ? 4 : 1;
+    s.groups = several && rows > kFewRows ? kRowWarpsMost / s.warps : s.warps == 1 ? 4 : 1;
+    s.threads = 32 * s.warps * (int)s.groups;
     return s;
 }
-RowShape norm_shape(int64_t rows, int cols, int type) { return row_shape(rows, cols, type == B200_TYPE_F32 ? 2 : 4); }
-RowShape grad_shape(int64_t rows, int cols) { return row_shape(rows, cols, 2); }
+RowShape norm_shape(int64_t rows, int cols, int type) { return row_shape(rows, cols, type == B200_TYPE_F32 ? 2 : 4, false); }
+RowShape grad_shape(int64_t rows, int cols) { return row_shape(rows, cols, 2, true); }  // (fewer sums to leave behind)
 // f(std::integral_constant) for the smallest of 1, 2, 4, ... that holds `vectors`
 template <int Most, class F>
 void with_vectors(int vectors, F f) {
@@ -100,12 +100,12 @@ int check_norm_grad(const b200_rms_norm_grad_op* op, const char* who) {
     return 0;
 }
 
-// CTAs of the gradient, each of which leaves a row of sums: two per SM (a thread holds 24 to 32 values of eight columns), fewer where there are fewer rows.
+// CTAs of the gradient, each of which leaves a row of sums.
+constexpr int kGradCtas = 2;  // per SM
 int norm_grad_ctas(const b200_rms_norm_grad_op* op) {
     if (op->cols > kGradCols) return pieces(op->rows, op->cols, kRowThreads, 4);
     const RowShape g = grad_shape(op->rows, op->cols);
-    const int per_sm = g.warps == 1 ? 4 : std::max(1, 16 / g.warps);
-    return (int)std::min<int64_t>((op->rows + g.groups - 1) / g.groups, 148 * per_sm);
+    return (int)std::min<int64_t>((op->rows + g.groups - 1) / g.groups, 148 * kGradCtas);
 }
 int64_t norm_grad_workspace(const b200_rms_norm_grad_op* op) { return op->dweight && op->rows ? (int64_t)norm_grad_ctas(op) * op->cols * 4 : 0; }
 
@@ -224,10 +224,12 @@ int b200_op_pack8(int device, void* stream, const b200_pack8_op* op) {
     if (op->by_column) {
         const int across = threads_across(vec ? op->cols / 8 : op->cols), width = across * (vec ? 8 : 1);
         const dim3 grid((op->cols + width - 1) / width, pieces(op->rows, op->cols, width, kRowThreads / across));
+        // (every piece sends each column's magnitude to one address: two CTAs per SM at most)
+        const dim3 scales_grid(grid.x, std::max(1u, std::min(grid.y, 296u / grid.x)));
         OP_CK(cudaMemsetAsync(op->scale, 0, (size_t)op->cols * 4, s));
         with_float(op->x_type, [&](auto x) {
             with_bool(vec, [&](auto v) {
-                column_scales_kernel<decltype(x), v() ? 8 : 1><<<grid, kRowThreads, 0, s>>>(*op, across);
+                column_scales_kernel<decltype(x), v() ? 8 : 1><<<scales_grid, kRowThreads, 0, s>>>(*op, across);
                 pack8_columns_kernel<decltype(x), v() ? 8 : 1><<<grid, kRowThreads, 0, s>>>(*op, across);
             });
         });
