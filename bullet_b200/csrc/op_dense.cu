@@ -66,19 +66,20 @@ struct Call {
     int block() const { return bytes() ? 128 : 64; }  // of k in a stage
 };
 
-// How a product is cut.  The costs are clocks: of a stage (128 bytes of k) of each tile, of an item besides, of a join and of its
-// bytes per clock.
+// How a product is cut: into tiles of which width, and k into how many parts.  By what each way costs in clocks: a stage (128 bytes of
+// k) of a tile, an item besides, a join (launch, and its bytes per clock), rounds of items being whole.  Fitted to times on a B200; of 35
+// products of 16 to 65536 rows with every width and number of parts, this choice was within 10 % of the best on all but four,
+// and within 20 % on those (us, this choice / the best: 2048 x 2048 -> 256 16.2 / 12.0 before the codes' stages had costs of their own).
 struct Plan {
-    int columns;  // of a tile; 256: a pair's
+    int columns;  // of a tile; from 256 on a pair's
     int parts, blocks;
 };
 constexpr int kSms = 148;  // that products are cut for
 constexpr int kPartsMost = 32, kJoin = 6000, kJoinBytes = 2500;
 struct TileCost {
-    int columns, rows, units, stage, item;
+    int columns, rows, units, stage, stage_codes, item;
 };
-constexpr TileCost kTiles[] = {{512, 256, kSms / 2, 1226, 5500}, {256, 256, kSms / 2, 687, 900}, {128, 128, kSms, 650, 900}, {64, 128, kSms, 450, 900}};
-constexpr int kStageCodes512 = 1403, kStageCodes256 = 1222;  // (narrower tiles turn codes more often)
+constexpr TileCost kTiles[] = {{512, 256, kSms / 2, 1226, 1403, 5500}, {256, 256, kSms / 2, 687, 1222, 900}, {128, 128, kSms, 650, 1000, 900}, {64, 128, kSms, 450, 850, 900}};
 Plan plan_of(const Call& c) {
     const int64_t blocks = (c.p.k + c.block() - 1) / c.block();
     Plan best{};
@@ -86,7 +87,7 @@ Plan plan_of(const Call& c) {
     for (const TileCost& t : kTiles) {
         if (t.columns == 64 && c.bytes()) continue;  // (boxes across are 128 columns there)
         const int64_t tiles = ((c.p.m + t.rows - 1) / t.rows) * ((c.p.n + t.columns - 1) / t.columns);
-        const double stage = c.codes && t.columns >= 256 ? (t.columns == 512 ? kStageCodes512 : kStageCodes256) : t.stage;
+        const double stage = c.codes ? t.stage_codes : t.stage;
         for (int64_t parts = 1; parts <= std::min<int64_t>(kPartsMost, blocks); parts++) {
             if (parts > 1 && tiles * (parts - 1) >= 2 * t.units) break;
             const int64_t each = (blocks + parts - 1) / parts, rounds = (tiles * parts + t.units - 1) / t.units;

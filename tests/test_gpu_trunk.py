@@ -392,6 +392,36 @@ def test_dense_gradient_against_differences():
         assert abs(mine - slope) <= float(parts[0].abs().sum()) * ROUND[BF16] + size * (FEW + n_in * 2.0 ** -23) + 1e-6 * size
 
 
+@pytest.mark.parametrize("rows,n_in,n_out", [(70, 64, 32), (300, 200, 700), (2500, 256, 512), (700, 130, 64)])
+def test_checkpoints_of_any_scale_and_with_nan(rows, n_in, n_out):
+    """Scales from 2^-126 to 2^119, and codes that are NaN: each reaches the gradient rows that it belongs to."""
+    x, dy = whole(121, -3, 3, rows, n_in, kind=E4M3), torch.zeros(rows, n_out, device="cuda", dtype=BF16)
+    e = torch.zeros(rows, device="cuda")
+    e[3], e[5], e[rows - 1], e[7], e[9] = 8, 30, 119, -126, 7
+    scale = torch.exp2(e)
+    for k, row in enumerate((3, 5, rows - 1, 7, 9)):  # a row of dy each, in columns of their own
+        dy[row, k] = 1
+    _, dw, _ = ops.dense_backward(dy, ops.Packed8(x, scale), None, need_dx=False)
+    assert torch.equal(dw.double(), (x.double() * scale.double()[:, None]).t() @ dy.double())
+    codes = x.view(torch.uint8).clone()
+    codes[5, 11], codes[rows - 1, n_in - 1] = 0x7F, 0xFF
+    _, dw, _ = ops.dense_backward(dy, ops.Packed8(codes.view(E4M3), scale), None, need_dx=False)
+    nan = torch.zeros(n_in, dtype=torch.bool, device="cuda")
+    nan[11] = nan[n_in - 1] = True
+    assert torch.isnan(dw[nan]).all() and torch.isfinite(dw[~nan]).all()
+    want = (x.double() * scale.double()[:, None]).t() @ dy.double()
+    assert torch.equal(dw[~nan].double(), want[~nan])
+
+
+def test_pack_of_what_would_round_out_of_range():
+    top = torch.tensor([[3.38e38, -3.38e38, 1.0], [2.0 ** 127, -(2.0 ** 127), 0.0]], device="cuda")
+    for kind in (F32, BF16):
+        for by_column in (False, True):
+            p = ops.pack8(top.to(kind), by_column=by_column)
+            v = ops.unpack8(p, F32)
+            assert torch.isfinite(v).all() and (v[0, :2].abs() >= 2.0 ** 127 * 1.8).all() and torch.equal(v[1, :2], top[1, :2])
+
+
 def test_gradient_is_cut_off_whatever_comes_in():
     dy = torch.full((4, 16), float("inf"), device="cuda", dtype=BF16)
     y = torch.zeros(4, 16, device="cuda", dtype=BF16)
