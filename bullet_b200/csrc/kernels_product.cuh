@@ -21,9 +21,15 @@
 
 namespace b200 {
 
+// The tensor pipe cuts sums off where it adds to them, so that long sums lose: 131072 products of checkpoints and gradients, the sums'
+// error in 1 chain of 2048 stages 4e-5 of them, 228 stages 2.3e-6, 114 9e-7 (added up in fp32, 1.6e-7).  A sum is taken out after
+// kChainMost stages and added, rounded, to what memory holds.
+constexpr int kChainMost = 128;
+
 struct ProductArgs {
     int64_t m, n, k;
     int tiles_m, tiles_n, k_blocks, blocks_per_item, parts_n;  // parts_n: pieces of k
+    int chain;                                                 // stages that are added up in tensor memory (kChainMost)
     uint32_t form_type;                                        // of product_form
     const float* a_scale;                                      // per m (products of 8 bits) or per k (CODES)
     const float* b_scale;                                      // per n (products of 8 bits)
@@ -34,7 +40,7 @@ struct ProductArgs {
     int64_t ldd;
     int d_type, act;
     int boxes;     // rows of d and of the residual start on 16 bytes: TMA takes them; else element by element
-    float* parts;  // [parts_n][m][ldp], ldp = n up to a multiple of 8; null: none
+    float* parts;  // [parts_n][m][ldp], ldp = n up to a multiple of 8; null: none, there is one part of one chain
     int64_t ldp;
     int* gave_up;
 };
@@ -52,7 +58,8 @@ struct Tile {
     static constexpr int kGroups = CODES ? 3 : 0;              // of four warps that turn codes into bf16, a stage by turns
     static constexpr int kRaws = BN == 64 || BN == 512 ? kGroups : 2 * kGroups;  // codes on their way: a ring of their own
     static constexpr int kThreads = 64 + 32 * (kTakers + 4 * kGroups + (CODES ? 1 : 0));
-    static constexpr size_t kBoxes = kTakers * 4096;           // a box of the result on its way out for each
+    static constexpr int kBoxesEach = CODES ? 2 : 1;           // of the result on their way out (a chain's sums have to make room)
+    static constexpr size_t kBoxes = kTakers * kBoxesEach * 4096;
     static constexpr size_t kValues = kColumnValues ? (size_t)kTakers * 2 * kOwn * 4 : 0;
     static constexpr size_t kRest = 1024 + kBoxes + kValues + kRaws * kRaw;
     static constexpr int kFit = (int)((232448 - 1024 - kRest) / kStage), kStages = kFit < 8 ? kFit : 8;  // (1 KB for barriers)
@@ -238,42 +245,46 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
             const uint32_t form = product_form(p.form_type, A_ACROSS, B_ACROSS, T::kRows, BN / T::kWide);
             int s = 0, done = 0;
             uint32_t phase = 0;
-            for (int64_t item = first; item < items && !dead; item += step, done++) {
+            for (int64_t item = first; item < items && !dead; item += step) {
                 item_of(item, m0, n0, k0, k1, part);
-                const int half = done % T::kSums;
-                const uint32_t sums = memory + half * BN;
-                if (!wait(&sums_free[half], (done / T::kSums & 1) ^ 1)) break;
-                tensor_fence_after();
                 bool fine = true;
-                for (int kb = k0; kb < k1 && fine; kb++) {
-                    fine = wait(&full[s], phase) && (!CODES || wait(&ready[s], phase));
+                for (int kc = k0; kc < k1 && fine; kc += p.chain, done++) {
+                    const int half = done % T::kSums;
+                    const uint32_t sums = memory + half * BN;
+                    fine = wait(&sums_free[half], (done / T::kSums & 1) ^ 1);
                     if (!fine) break;
                     tensor_fence_after();
-                    const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA;
+                    for (int kb = kc; kb < min(kc + p.chain, k1); kb++) {
+                        fine = wait(&full[s], phase) && (!CODES || wait(&ready[s], phase));
+                        if (!fine) break;
+                        tensor_fence_after();
+                        const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA;
 #pragma unroll
-                    for (int q = 0; q < 4; q++)
+                        for (int q = 0; q < 4; q++)
 #pragma unroll
-                        for (int h = 0; h < T::kWide; h++)
-                            multiply<PAIR, BYTES>(sums + 256 * h, tile_descriptor(a_at + q * a_step, A_ACROSS ? column : 16),
-                                                  tile_descriptor(b_at + h * T::kBOne + q * b_step, B_ACROSS ? column : 16), form, kb > k0 || q > 0);
-                    when_multiplied<PAIR>(&empty[s]);
-                    if (++s == kStages) s = 0, phase ^= 1;
+                            for (int h = 0; h < T::kWide; h++)
+                                multiply<PAIR, BYTES>(sums + 256 * h, tile_descriptor(a_at + q * a_step, A_ACROSS ? column : 16),
+                                                      tile_descriptor(b_at + h * T::kBOne + q * b_step, B_ACROSS ? column : 16), form, kb > kc || q > 0);
+                        when_multiplied<PAIR>(&empty[s]);
+                        if (++s == kStages) s = 0, phase ^= 1;
+                    }
+                    when_multiplied<PAIR>(&sums_done[half]);
                 }
-                when_multiplied<PAIR>(&sums_done[half]);
             }
         }
     } else if (warp < 2 + T::kTakers) {  // takes sums out, kOwn columns of 32 rows
         const int quarter = warp & 3, taker = warp - 2, c0 = taker / 4 * T::kOwn;
-        unsigned char* box = base + kStages * T::kStage + T::kRaws * T::kRaw + taker * 4096;
+        unsigned char* boxes = base + kStages * T::kStage + T::kRaws * T::kRaw + taker * T::kBoxesEach * 4096;
+        unsigned char* box = boxes;
         float* bias = reinterpret_cast<float*>(base + kStages * T::kStage + T::kRaws * T::kRaw + T::kBoxes) + taker * 2 * T::kOwn;
         float* b_scale = bias + T::kOwn;
         const bool wide = p.boxes && (p.d_type == B200_TYPE_F32 || p.parts), adds = p.residual && !p.parts;
         const int width = wide ? 32 : 64;  // columns of a box
         uint32_t residuals = 0;
         int done = 0;
-        for (int64_t item = first; item < items; item += step, done++) {
+        bool fine = true;
+        for (int64_t item = first; item < items && fine; item += step) {
             item_of(item, m0, n0, k0, k1, part);
-            const int half = done % T::kSums;
             const int64_t rows0 = m0 + 128 * rank + 32 * quarter, m = rows0 + lane, own0 = n0 + c0;
             const int own = rows0 < p.m ? (int)min((int64_t)T::kOwn, p.n - own0) : 0;  // columns there are, 0 or less: nothing here
             const bool here = m < p.m;
@@ -294,56 +305,64 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
                 }
                 __syncwarp();
             }
-            const bool fine = __all_sync(0xffffffffu, wait(&sums_done[half], done / T::kSums & 1));
-            if (!fine) break;
-            tensor_fence_after();
-            const uint32_t sums = memory + ((uint32_t)quarter << 21) + half * BN + c0;
-            for (int c = 0; c < own; c += 32) {
-                float v[32];
-                load_sums32(sums + c, v);
-                if (!p.parts) finish_sums<BYTES, T::kColumnValues>(p, v, a_scale, bias + c, b_scale + c);
-                if (p.boxes) {
-                    const bool starts = c % width == 0, ends = (c + 32) % width == 0 || c + 32 >= own;
-                    if (starts) {
-                        if (adds) {
-                            if (c > 0) fetch_residual(c);
-                            if (!__all_sync(0xffffffffu, wait(&residual_in[taker], residuals & 1))) break;
-                            residuals++;
-                        } else {
-                            if (lane == 0) bulk_wait_read<0>();
+            for (int kc = k0; kc < k1; kc += p.chain, done++) {
+                const int half = done % T::kSums;
+                fine = __all_sync(0xffffffffu, wait(&sums_done[half], done / T::kSums & 1));
+                if (!fine) break;
+                if (kc > k0 && lane == 0) bulk_wait_all();  // what this part's chains before have left is in memory
+                tensor_fence_after();
+                const uint32_t sums = memory + ((uint32_t)quarter << 21) + half * BN + c0;
+                for (int c = 0; c < own; c += 32) {
+                    float v[32];
+                    load_sums32(sums + c, v);
+                    if (!p.parts) finish_sums<BYTES, T::kColumnValues>(p, v, a_scale, bias + c, b_scale + c);
+                    if (p.boxes) {
+                        const bool starts = c % width == 0, ends = (c + 32) % width == 0 || c + 32 >= own;
+                        if (starts) {
+                            if (adds) {
+                                if (c > 0) fetch_residual(c);
+                                if (!__all_sync(0xffffffffu, wait(&residual_in[taker], residuals & 1))) break;
+                                residuals++;
+                            } else {
+                                if constexpr (T::kBoxesEach == 2) box = box == boxes ? boxes + 4096 : boxes;
+                                if (lane == 0) bulk_wait_read<T::kBoxesEach - 1>();
+                                __syncwarp();
+                            }
+                        }
+                        unsigned char* row = box + lane * 128;
+                        if (wide)
+                            box_out<float>(row, lane, 0, v, adds);
+                        else if (p.d_type == B200_TYPE_BF16)
+                            box_out<bf16>(row, lane, starts ? 0 : 4, v, adds);
+                        else
+                            box_out<f16>(row, lane, starts ? 0 : 4, v, adds);
+                        if (ends) {
+                            fence_proxy_async();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (kc > k0)
+                                    add_box3(&d_map, smem_u32(box), (int)own0 + c / width * width, (int)rows0, part);
+                                else
+                                    store_box3(&d_map, smem_u32(box), (int)own0 + c / width * width, (int)rows0, part);
+                                bulk_commit();
+                            }
                             __syncwarp();
                         }
-                    }
-                    unsigned char* row = box + lane * 128;
-                    if (wide)
-                        box_out<float>(row, lane, 0, v, adds);
-                    else if (p.d_type == B200_TYPE_BF16)
-                        box_out<bf16>(row, lane, starts ? 0 : 4, v, adds);
-                    else
-                        box_out<f16>(row, lane, starts ? 0 : 4, v, adds);
-                    if (ends) {
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            store_box3(&d_map, smem_u32(box), (int)own0 + c / width * width, (int)rows0, part);
-                            bulk_commit();
-                        }
-                        __syncwarp();
-                    }
-                } else if (here) {
-                    for (int k = 0; k < 32; k++) {
-                        if (c + k >= own) break;
-                        float x = v[0];
+                    } else if (here) {
+                        for (int k = 0; k < 32; k++) {
+                            if (c + k >= own) break;
+                            float x = v[0];
 #pragma unroll
-                        for (int q = 1; q < 32; q++) x = q == k ? v[q] : x;
-                        if (adds) x += load_value(p.residual, m * p.ldr + own0 + c + k, p.d_type);
-                        store_value(p.d, m * p.ldd + own0 + c + k, p.d_type, x);
+                            for (int q = 1; q < 32; q++) x = q == k ? v[q] : x;
+                            if (adds) x += load_value(p.residual, m * p.ldr + own0 + c + k, p.d_type);
+                            store_value(p.d, m * p.ldd + own0 + c + k, p.d_type, x);
+                        }
                     }
                 }
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_at(PAIR ? of_rank(smem_u32(&sums_free[half]), 0) : smem_u32(&sums_free[half]));
             }
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_at(PAIR ? of_rank(smem_u32(&sums_free[half]), 0) : smem_u32(&sums_free[half]));
         }
         if (lane == 0) bulk_wait_all();
     } else if (CODES && warp == T::kThreads / 32 - 1) {

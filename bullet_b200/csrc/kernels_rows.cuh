@@ -66,6 +66,21 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, int warps, uint32_t* sha
 __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t finite_magnitude(float v) { return finite(v) ? magnitude_bits(v) : 0u; }
 
+// 32 bytes of a lane: neighbouring lanes' stand side by side, where two loads of 16 bytes would take twice the way through L1.  `stream`: not
+// to be read again.
+template <bool STREAM>
+__device__ __forceinline__ void load_32_bytes(const void* at, uint32_t (&w)[8]) {
+    if constexpr (STREAM)
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(at));
+    else
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(at));
+}
+// Whether all of eight elements 32 apart are there: all but a row's last eights, which alone are looked at one by one.
+__device__ __forceinline__ bool whole_eight(int first, int cols) { return first + 7 * 32 < cols; }
 // Eight elements from `first` on (VEC) or from `first` on in steps of 32; those at or past `cols` are 0.
 template <bool VEC, class T>
 struct Eight {
@@ -75,15 +90,26 @@ struct Eight {
     __device__ __forceinline__ void load(const T* row, int first, int cols) {
         if constexpr (VEC) {
             if (first < cols) {
-#pragma unroll
-                for (int k = 0; k < kWords; k++) raw[k] = __ldcs(reinterpret_cast<const uint4*>(row + first) + k);
+                if constexpr (sizeof(T) == 4) {
+                    uint32_t w[8];
+                    load_32_bytes<true>(row + first, w);
+                    raw[0] = make_uint4(w[0], w[1], w[2], w[3]), raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                } else {
+                    raw[0] = __ldcs(reinterpret_cast<const uint4*>(row + first));
+                }
             } else {
 #pragma unroll
                 for (int k = 0; k < kWords; k++) raw[k] = make_uint4(0, 0, 0, 0);
             }
         } else {
+            const T* at = row + first;
+            if (whole_eight(first, cols)) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) one[k] = first + 32 * k < cols ? __ldcs(row + first + 32 * k) : from_float<T>(0.f);
+                for (int k = 0; k < 8; k++) one[k] = __ldcs(at + 32 * k);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) one[k] = first + 32 * k < cols ? __ldcs(at + 32 * k) : from_float<T>(0.f);
+            }
         }
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {
@@ -103,26 +129,46 @@ struct Eight {
 };
 template <bool VEC>
 __device__ __forceinline__ void load_weights(const float* w, int first, int cols, float (&v)[8]) {
-    if constexpr (VEC) {
-        const float4 a = first < cols ? __ldg(reinterpret_cast<const float4*>(w + first)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 b = first < cols ? __ldg(reinterpret_cast<const float4*>(w + first) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
+    if (!w) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = first + 32 * k < cols ? __ldg(w + first + 32 * k) : 0.f;
+        for (int k = 0; k < 8; k++) v[k] = 1.f;
+        return;
+    }
+    if constexpr (VEC) {
+        uint32_t u[8] = {};
+        if (first < cols) load_32_bytes<false>(w + first, u);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = __uint_as_float(u[k]);
+    } else {
+        const float* at = w + first;
+        if (whole_eight(first, cols)) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __ldg(at + 32 * k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = first + 32 * k < cols ? __ldg(at + 32 * k) : 0.f;
+        }
     }
 }
 template <bool VEC, class T>
 __device__ __forceinline__ void store_eight(T* row, int first, int cols, const float (&v)[8]) {
     if constexpr (!VEC) {
+        T* at = row + first;
+        if (whole_eight(first, cols)) {
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (first + 32 * k < cols) row[first + 32 * k] = from_float<T>(v[k]);
+            for (int k = 0; k < 8; k++) at[32 * k] = from_float<T>(v[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (first + 32 * k < cols) at[32 * k] = from_float<T>(v[k]);
+        }
     } else if (first < cols) {
         uint4* at = reinterpret_cast<uint4*>(row + first);
         if constexpr (sizeof(T) == 4) {
-            at[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-            at[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])),
+                         "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])),
+                         "r"(__float_as_uint(v[7]))
+                         : "memory");
         } else {
             at[0] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
         }
@@ -160,14 +206,22 @@ __device__ __forceinline__ uint32_t moved_outputs2(uint32_t w, uint32_t least, i
 __device__ __forceinline__ uint32_t two_codes(float a, float b, float by_a, float by_b) {
     return __nv_cvt_float2_to_fp8x2(make_float2(fmaf(a, by_a, a - a), fmaf(b, by_b, b - b)), __NV_SATFINITE, __NV_E4M3);
 }
+// (one call for eight: their code stands beside that of the kernels' usual way otherwise, which then misses the instruction cache)
+static __device__ __noinline__ uint2 codes_slowly(float v0, float v1, float v2, float v3, float v4, float v5, float v6, float v7, uint32_t scale, int act) {
+    const float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
+    uint32_t q[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) q[k] = code_of_output(v[k], scale, act);
+    return make_uint2(q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24);
+}
 // Eight codes.
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, const float (&v)[8], uint32_t scale, int act) {
     const float by = one_over_scale(scale);
     uint32_t q[4];
-    if (scale == kTopScale || (act != B200_ACT_NONE && !moves_outputs(scale))) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) q[k] = code_of_output(v[2 * k], scale, act) | (uint32_t)code_of_output(v[2 * k + 1], scale, act) << 8;
+    if (__builtin_expect(scale == kTopScale || (act != B200_ACT_NONE && !moves_outputs(scale)), 0)) {
+        const uint2 u = codes_slowly(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], scale, act);
+        q[0] = u.x & 0xffffu, q[1] = u.x >> 16, q[2] = u.y & 0xffffu, q[3] = u.y >> 16;
     } else {
         const uint32_t least = least_bits(scale);
 #pragma unroll
@@ -180,9 +234,15 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, c
     if constexpr (VEC) {
         if (first < cols) *reinterpret_cast<uint2*>(row + first) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
     } else {
+        uint8_t* at = row + first;
+        if (whole_eight(first, cols)) {
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (first + 32 * k < cols) row[first + 32 * k] = (uint8_t)(q[k / 2] >> 8 * (k & 1));
+            for (int k = 0; k < 8; k++) at[32 * k] = (uint8_t)(q[k / 2] >> 8 * (k & 1));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (first + 32 * k < cols) at[32 * k] = (uint8_t)(q[k / 2] >> 8 * (k & 1));
+        }
     }
 }
 
@@ -210,8 +270,30 @@ struct RowPlace {
     }
 };
 
-template <class TX, int NV, bool VEC>
-static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_norm_op a, int warps) {
+// 1 / sqrt(mean), and what its rounding to fp32 leaves of it: a Newton step from the rounded root, with its error in 64 bits.
+__device__ __forceinline__ float root_of_mean(double mean, float& rest) {
+    const float first = 1.f / sqrtf((float)mean);
+    const float error = (float)fma(-mean * (double)first, (double)first, 1.0);
+    const float by = first * 0.5f * error, rstd = first + by;
+    const bool fine = finite(rstd) && finite(by);
+    rest = fine ? by - (rstd - first) : 0.f;
+    return fine ? rstd : first;
+}
+// t * rstd * w in fp32 may round onto a halfway point of two codes or across it: one code in 10^6 came out as its neighbour.  A
+// product within two units of one (bits 19 to 0 of the significand near 0x80000) is formed again: the fp32 number next to the exact one
+// towards 0, with its last bit set where it is not exact itself, so that it lies on the right side.
+__device__ __forceinline__ bool near_halfway(float y) { return (__float_as_uint(y) - 0x7fffeu) * 4096u < 5u * 4096u; }
+template <class TX>
+static __device__ __noinline__ float exact_for_code(const TX* x, const TX* residual, const float* weight, float rstd, float rest) {
+    const float t = residual ? to_float(*x) + to_float(*residual) : to_float(*x), w = weight ? *weight : 1.f;
+    const float n = t * rstd, n_rest = fmaf(t, rest, fmaf(t, rstd, -n)), y = n * w;
+    const float y_rest = fmaf(n_rest, w, fmaf(n, w, -y));
+    const uint32_t bits = __float_as_uint(y), opposite = (bits ^ __float_as_uint(y_rest)) >> 31;
+    return y_rest != 0.f && finite(y_rest) ? __uint_as_float((bits - opposite) | 1u) : y;
+}
+
+template <class TX, int NV, bool VEC, bool CODES>
+static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_norm_op a, int warps, double one_over_cols) {
     __shared__ float sums[kRowWarpsMost];
     __shared__ uint32_t largest[2][kRowWarpsMost];
     const RowPlace p = RowPlace::here<VEC>(warps);
@@ -239,37 +321,49 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
 #pragma unroll
         for (int k = 0; k < 8; k++) squares = fmaf(v[j][k], v[j][k], squares);
     }
-    const float rstd = 1.f / sqrtf(row_sum(squares, warps, sums) / (float)a.cols + a.eps);
+    float rest;
+    const float rstd = root_of_mean((double)row_sum(squares, warps, sums) * one_over_cols + (double)a.eps, rest);
     if (a.rstd && p.leader) a.rstd[p.row] = rstd;
-    uint32_t m = 0;
+    float most = 0.f;  // (NaN, which no scale is to know of, loses against every number)
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         float w[8];
-        if (a.weight) load_weights<VEC>(a.weight, p.lane_at + p.step * j, a.cols, w);
+        load_weights<VEC>(a.weight, p.lane_at + p.step * j, a.cols, w);
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            v[j][k] *= rstd;
-            if (a.weight) v[j][k] *= w[k];
-            // (past the columns there are zeros, and zeros times an infinite rstd, which no code is to know of)
-            if (VEC ? p.lane_at + p.step * j < a.cols : p.lane_at + p.step * j + 32 * k < a.cols) m = max(m, magnitude_bits(v[j][k]));
+            v[j][k] = v[j][k] * rstd * w[k];
+            if constexpr (CODES) most = fmaxf(most, fabsf(v[j][k]));
         }
-        if (a.y_type != B200_TYPE_E4M3) store_typed<VEC>(a.y, p.row * a.ldy, a.y_type, p.lane_at + p.step * j, a.cols, v[j]);
+        if constexpr (!CODES) store_typed<VEC>(a.y, p.row * a.ldy, a.y_type, p.lane_at + p.step * j, a.cols, v[j]);
     }
-    if (a.y_type != B200_TYPE_E4M3) return;
-    m = row_max(m, warps, largest[0]);
-    if (m >= 0x7f800000u) {  // the same in all threads of the row
-        m = 0;
+    if constexpr (CODES) {
+        uint32_t m = row_max(magnitude_bits(most), warps, largest[0]);
+        if (m >= 0x7f800000u) {  // the same in all threads of the row
+            m = 0;
 #pragma unroll
-        for (int j = 0; j < NV; j++)
+            for (int j = 0; j < NV; j++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) m = max(m, finite_magnitude(v[j][k]));
-        m = row_max(m, warps, largest[1]);
+                for (int k = 0; k < 8; k++) m = max(m, finite_magnitude(v[j][k]));
+            m = row_max(m, warps, largest[1]);
+        }
+        const uint32_t scale = scale_bits(m);
+        if (p.leader) a.scale[p.row] = __uint_as_float(scale);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            uint32_t past = 0xffffffffu;
+#pragma unroll
+            for (int k = 0; k < 8; k++) past = __viaddmin_u32(__float_as_uint(v[j][k]) << 12, 0u - (0x7fffeu << 12), past);
+            if (past < 5u << 12) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int c = p.lane_at + p.step * j + (VEC ? k : 32 * k);
+                    if (near_halfway(v[j][k]) && c < a.cols)
+                        v[j][k] = exact_for_code(xr + c, a.residual ? static_cast<const TX*>(a.residual) + p.row * a.ldr + c : nullptr, a.weight ? a.weight + c : nullptr, rstd, rest);
+                }
+            }
+            store_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, v[j], scale, B200_ACT_NONE);
+        }
     }
-    const uint32_t scale = scale_bits(m);
-    if (p.leader) a.scale[p.row] = __uint_as_float(scale);
-#pragma unroll
-    for (int j = 0; j < NV; j++)
-        store_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, v[j], scale, B200_ACT_NONE);
 }
 
 // Elements of 16 bits are compared two at a time: one by one the ALU pipe takes longer than HBM (131072 rows of 2048 bf16 outputs of
@@ -363,15 +457,14 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             float w[8];
-            if (a.weight) load_weights<VEC>(a.weight, p.lane_at + p.step * j, a.cols, w);
+            load_weights<VEC>(a.weight, p.lane_at + p.step * j, a.cols, w);
             s[j].get(n[j]);
             dy[j].get(g[j]);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                // (past the columns both are 0, and stay so where rstd is infinite)
-                n[j][k] = (VEC ? p.lane_at + p.step * j < a.cols : p.lane_at + p.step * j + 32 * k < a.cols) ? n[j][k] * rstd : 0.f;
+                n[j][k] *= rstd;  // (past the columns 0; NaN where rstd is infinite, as all of the row's dx is then)
                 dw[j][k] = fmaf(g[j][k], n[j][k], dw[j][k]);
-                if (a.weight) g[j][k] *= w[k];
+                g[j][k] *= w[k];
                 dot = fmaf(g[j][k], n[j][k], dot);
             }
         }

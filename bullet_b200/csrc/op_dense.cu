@@ -72,7 +72,9 @@ struct Call {
 // and within 20 % on those (us, this choice / the best: 2048 x 2048 -> 256 16.2 / 12.0 before the codes' stages had costs of their own).
 struct Plan {
     int columns;  // of a tile; from 256 on a pair's
-    int parts, blocks;
+    int parts, blocks;  // pieces of k and the stages of each
+    int chains() const { return (blocks + kChainMost - 1) / kChainMost; }
+    bool joined() const { return parts > 1 || chains() > 1; }
 };
 constexpr int kSms = 148;  // that products are cut for
 constexpr int kPartsMost = 32, kJoin = 6000, kJoinBytes = 2500;
@@ -91,14 +93,15 @@ Plan plan_of(const Call& c) {
         for (int64_t parts = 1; parts <= std::min<int64_t>(kPartsMost, blocks); parts++) {
             if (parts > 1 && tiles * (parts - 1) >= 2 * t.units) break;
             const int64_t each = (blocks + parts - 1) / parts, rounds = (tiles * parts + t.units - 1) / t.units;
-            double cost = (double)rounds * (each * stage + t.item);
-            if (parts > 1) cost += kJoin + 8.0 * parts * c.p.m * c.p.n / kJoinBytes;
+            const int64_t chains = (each + kChainMost - 1) / kChainMost;
+            double cost = (double)rounds * (each * stage + t.item * (t.columns == 512 ? chains : 1));
+            if (parts > 1 || chains > 1) cost += kJoin + 8.0 * parts * c.p.m * c.p.n / kJoinBytes;
             if (cost < least) least = cost, best = {t.columns, (int)((blocks + each - 1) / each), (int)each};
         }
     }
     return best;
 }
-int64_t parts_bytes(const Call& c, const Plan& plan) { return plan.parts > 1 ? (int64_t)plan.parts * c.p.m * ((c.p.n + 7) / 8 * 8) * 4 : 0; }
+int64_t parts_bytes(const Call& c, const Plan& plan) { return plan.joined() ? (int64_t)plan.parts * c.p.m * ((c.p.n + 7) / 8 * 8) * 4 : 0; }
 int64_t call_bytes(const Call& c) { return c.a.copy_bytes() + c.b.copy_bytes() + (parts_bytes(c, plan_of(c)) + 255) / 256 * 256; }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -213,7 +216,8 @@ int run_product(Call c, char* space, cudaStream_t stream) {
     p.blocks_per_item = plan.blocks;
     p.parts_n = plan.parts;
     p.ldp = (p.n + 7) / 8 * 8;
-    p.parts = plan.parts > 1 ? reinterpret_cast<float*>(space) : nullptr;
+    p.chain = (plan.blocks + plan.chains() - 1) / plan.chains();
+    p.parts = plan.joined() ? reinterpret_cast<float*>(space) : nullptr;
     p.form_type = c.b.type == B200_TYPE_BF16;
     const int size = type_bytes(p.d_type);
     auto starts = [&](const void* at, int64_t ld) { return (uintptr_t)at % 16 == 0 && (p.m == 1 || ld * size % 16 == 0); };

@@ -70,7 +70,7 @@ int threads_across(int vectors) {
     return t;
 }
 bool aligned(const void* at, int64_t ld, int type, int to) { return ((uintptr_t)at | (uintptr_t)(ld * type_bytes(type))) % to == 0; }
-bool aligned8(const void* at, int64_t ld, int type) { return aligned(at, ld, type, type == B200_TYPE_E4M3 ? 8 : 16); }  // vectors of eight elements
+bool aligned8(const void* at, int64_t ld, int type) { return aligned(at, ld, type, 8 * type_bytes(type)); }  // vectors of eight elements
 
 int check_norm(const b200_rms_norm_op* op, const char* who) {
     if (!op) return fail(B200_ERR_ARG, "%s: null operator description", who);
@@ -129,12 +129,16 @@ int b200_op_rms_norm(int device, void* stream, const b200_rms_norm_op* op) {
         with_float(op->x_type, [&](auto x) { rms_norm_any_kernel<decltype(x)><<<any_ctas(op->rows), kRowThreads, 0, s>>>(*op); });
     } else {
         const bool vec = op->cols % 8 == 0 && aligned8(op->x, op->ldx, op->x_type) && aligned8(op->y, op->ldy, op->y_type) && (!op->residual || aligned8(op->residual, op->ldr, op->x_type)) &&
-                         (!op->sum || aligned8(op->sum, op->lds, op->x_type)) && (uintptr_t)op->weight % 16 == 0;
+                         (!op->sum || aligned8(op->sum, op->lds, op->x_type)) && (uintptr_t)op->weight % 32 == 0;
         const RowShape g = norm_shape(op->rows, op->cols, op->x_type);
         with_float(op->x_type, [&](auto x) {
             with_bool(vec, [&](auto v) {
                 with_vectors<kRowVectors>(g.vectors, [&](auto nv) {
-                    rms_norm_kernel<decltype(x), nv(), v()><<<(unsigned)((op->rows + g.groups - 1) / g.groups), g.threads, 0, s>>>(*op, g.warps);
+                    auto go = [&](auto kernel) { kernel<<<(unsigned)((op->rows + g.groups - 1) / g.groups), g.threads, 0, s>>>(*op, g.warps, 1.0 / op->cols); };
+                    if (op->y_type == B200_TYPE_E4M3)
+                        go(rms_norm_kernel<decltype(x), nv(), v(), true>);
+                    else
+                        go(rms_norm_kernel<decltype(x), nv(), v(), false>);
                 });
             });
         });
@@ -186,7 +190,7 @@ int b200_op_rms_norm_backward(int device, void* stream, const b200_rms_norm_grad
         });
     } else if (op->dx || op->dweight) {
         const bool vec = op->cols % 8 == 0 && aligned8(op->dy, op->lddy, op->dy_type) && aligned8(op->sum, op->lds, op->x_type) && (!op->dx || aligned8(op->dx, op->lddx, op->x_type)) &&
-                         (!op->dsum || aligned8(op->dsum, op->ldds, op->x_type)) && (uintptr_t)op->weight % 16 == 0;
+                         (!op->dsum || aligned8(op->dsum, op->ldds, op->x_type)) && (uintptr_t)op->weight % 32 == 0;
         const RowShape g = grad_shape(op->rows, op->cols);
         const size_t shared = op->dweight && g.groups > 1 ? (size_t)g.groups * op->cols * 4 : 0;  // at most 4 x 1024 floats
         with_float(op->x_type, [&](auto x) {
@@ -224,8 +228,8 @@ int b200_op_pack8(int device, void* stream, const b200_pack8_op* op) {
     if (op->by_column) {
         const int across = threads_across(vec ? op->cols / 8 : op->cols), width = across * (vec ? 8 : 1);
         const dim3 grid((op->cols + width - 1) / width, pieces(op->rows, op->cols, width, kRowThreads / across));
-        // (every piece sends each column's magnitude to one address: two CTAs per SM at most)
-        const dim3 scales_grid(grid.x, std::max(1u, std::min(grid.y, 296u / grid.x)));
+        // (every piece sends each column's magnitude to one address: four CTAs per SM at most)
+        const dim3 scales_grid(grid.x, std::max(1u, std::min(grid.y, 592u / grid.x)));
         OP_CK(cudaMemsetAsync(op->scale, 0, (size_t)op->cols * 4, s));
         with_float(op->x_type, [&](auto x) {
             with_bool(vec, [&](auto v) {

@@ -76,6 +76,10 @@ __device__ __forceinline__ void store_box3(const CUtensorMap* map, uint32_t from
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
+__device__ __forceinline__ void add_box3(const CUtensorMap* map, uint32_t from, int x, int y, int z) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 // A tile's descriptor.  Both kinds have rows of 128 bytes with the 128-byte swizzle, eight rows are 1024 bytes.  Along k (K-major):
 // a row of the tile per m or n, 128 bytes of k; `column` unused.  Across (MN-major): a row per k, 128 bytes of m or n, the next
 // 128 bytes of m or n `column` bytes on.

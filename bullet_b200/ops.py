@@ -73,8 +73,8 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 def _like(t: torch.Tensor, dtype):
     """An empty matrix without gaps, of t's shape (empty_like is the quicker way to one, where t has none)."""
-    if t.dtype is dtype and t.is_contiguous():
-        return torch.empty_like(t)
+    if t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
     return torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
@@ -159,7 +159,7 @@ def pack8(x, act: int = ACT_NONE, by_column: bool = False) -> Packed8:
     then stays where it was."""
     ldx = _matrix(x, "x", types=_FLOATS)
     rows, cols = x.shape
-    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
+    codes = _like(x, torch.float8_e4m3fn)
     scale = torch.empty(cols if by_column else rows, dtype=torch.float32, device=x.device)
     op = _lib.CPack8(rows, cols, _TYPES[x.dtype], _act(act), int(by_column), ldx, cols, x.data_ptr(), codes.data_ptr(), scale.data_ptr())
     _call(_lib.load().b200_op_pack8, x.device, op)
@@ -172,7 +172,7 @@ def unpack8(packed: Packed8, dtype=torch.bfloat16):
     if dtype not in _FLOATS:
         raise ValueError(f"dtype: {dtype} is not taken here")
     rows, cols = packed.codes.shape
-    y = torch.empty((rows, cols), dtype=dtype, device=packed.codes.device)
+    y = _like(packed.codes, dtype)
     op = _lib.CUnpack8(rows, cols, _TYPES[dtype], int(packed.by_column), ldq, cols, packed.codes.data_ptr(), scale, y.data_ptr())
     _call(_lib.load().b200_op_unpack8, y.device, op)
     return y

@@ -365,6 +365,27 @@ def test_dense_gradient(rows, n_in, n_out, codes, act):
     near(db, dz.sum(0), 0, dz.abs().sum(0) * (rows * 2.0 ** -23 + FEW))
 
 
+@pytest.mark.parametrize("codes", [False, True])
+def test_long_sums_keep_their_bits(codes):
+    """Sums over many rows, of one sign and of both: the pipe that multiplies cuts off what it adds, so they are taken out on the way.
+    Bound: the 4 x 128 additions between two takings-out cut off less than 2^-23 of the magnitudes' sum each, and adding up what
+    was taken out rounds at most 64 times.  (Without, 32768 additions: 2^-8.)"""
+    rows, n_in, n_out = 131072, 256, 64
+    x = torch.rand(rows, n_in, device="cuda", generator=gen(87))
+    dy = torch.cat([torch.rand(rows, 32, device="cuda", generator=gen(88)), normal(89, rows, 32)], 1).to(BF16)
+    x = ops.pack8(x) if codes else x.to(BF16)
+    xv = (ops.unpack8(x, F32) if codes else x).double()
+    _, dw, _ = ops.dense_backward(dy, x, None, need_dx=False, need_dbias=False)
+    near(dw, xv.t() @ dy.double(), 0, (4 * 128 + 64) * 2.0 ** -23 * (xv.abs().t() @ dy.double().abs()))
+
+
+@pytest.mark.parametrize("rows,n_in,n_out", [(30, 20000, 72), (700, 16392, 520)])
+def test_dense_of_many_inputs(rows, n_in, n_out):
+    x, w = whole(85, -2, 2, rows, n_in), whole(86, -2, 2, n_in, n_out)
+    r = whole(87, -9, 9, rows, n_out, kind=F32)
+    assert torch.equal(ops.dense(x, w, residual=r, out_dtype=F32).double(), x.double() @ w.double() + r.double())
+
+
 def test_dense_gradient_against_differences():
     rows, n_in, n_out, h = 40, 64, 48, 1e-6
     x, w = normal(91, rows, n_in).to(BF16), (normal(92, n_in, n_out) * n_in ** -0.5).to(BF16)
