@@ -550,3 +550,60 @@ def test_refusals_of_tensors():
     with pytest.raises(_lib.B200Error):
         ops.dense_backward(normal(1, 4, 16).to(F16), ops.pack8(x), w.to(F16))
     assert math.isfinite(float(ops.dense(x, w).float().sum()))
+
+
+def test_the_example_trains():
+    """The trunk of examples/residual_trunk.py behind the feature transformer: its output is that of the same network in 64 bits but for
+    the roundings to 8 bits, its gradients are those of the same formulas in 64 bits from the activations that it kept, but for the
+    roundings of passed-on gradients to bf16, and the loss falls."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "residual_trunk.py")
+    spec = importlib.util.spec_from_file_location("residual_trunk", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    trunk = example.Trunk(128, 64, 96, 2)
+    x, dout = normal(141, 300, 128).clamp(min=0), normal(142, 300, 1).to(BF16)
+    out, kept = trunk.forward(x)
+    dx = trunk.backward(dout, kept)
+    w = {k: v.double() for k, v in trunk.w.value.items()}
+    stream = norm_of(x.double(), w["norm_in"]) @ w["in"]
+    for k in range(2):
+        h = (norm_of(stream, w[f"norm{k}"]) @ w[f"up{k}"] + w[f"bias_up{k}"]).clamp(0, 1)
+        stream = stream + h @ w[f"down{k}"] + w[f"bias_down{k}"]
+    want = norm_of(stream, w["norm_out"]) @ w["out"] + w["bias_out"]
+
+    def off(a, b):
+        return float((a.double() - b).norm() / b.norm())
+
+    # nearest codes of four bits are off by 2^-5.8 in the mean square at most: of a norm's output and a weight, twice, behind which
+    # the stream's own part dilutes them
+    assert off(out, want) < 0.1
+
+    def norm_back(dn, stream, rstd, weight):
+        t, g = stream.double().requires_grad_(), weight.clone().requires_grad_()
+        return torch.autograd.grad((norm_of(t, g) * dn).sum(), (t, g))
+
+    b = {k: v.double() for k, v in trunk.w.bf16.items()}
+    values = [[ops.unpack8(t, F32).double() if isinstance(t, ops.Packed8) else t.double() for t in step] for step in kept]
+    grads, d = {}, dout.double()
+    n, stream, rstd = values[-1]
+    grads["out"], grads["bias_out"] = n.t() @ d, d.sum(0)
+    d, grads["norm_out"] = norm_back(d @ b["out"].t(), stream, rstd, w["norm_out"])
+    for k in (1, 0):
+        n, stream, rstd, h = values[1 + k]
+        grads[f"down{k}"], grads[f"bias_down{k}"] = h.t() @ d, d.sum(0)
+        dz = (d @ b[f"down{k}"].t()) * ((h > 0) & (h < 1))
+        grads[f"up{k}"], grads[f"bias_up{k}"] = n.t() @ dz, dz.sum(0)
+        through, grads[f"norm{k}"] = norm_back(dz @ b[f"up{k}"].t(), stream, rstd, w[f"norm{k}"])
+        d = d + through
+    n, stream, rstd = values[0]
+    grads["in"] = n.t() @ d
+    dx_want, grads["norm_in"] = norm_back(d @ b["in"].t(), stream, rstd, w["norm_in"])
+    # at most ten roundings to bf16 one behind the other, of 2^-9 each, and a stream whose sum is kept in bf16 while rstd is that of the sum
+    assert off(dx, dx_want) < 12 * 2.0 ** -8 and grads.keys() == trunk.w.gradient.keys()
+    for k, g in trunk.w.gradient.items():
+        assert off(g, grads[k]) < 12 * 2.0 ** -8, k
+    losses = example.train(steps=40, batch=2048, width=128, hidden=256, blocks=2, ft_out=128, report=None)
+    assert sum(losses[-4:]) < 0.9 * sum(losses[:4])
