@@ -16,6 +16,7 @@
 // shared memory to another: a power of two as scale makes that exact, so there is no product of other values than those
 // that the checkpoint stands for, and no copy of it in 16 bits in memory.
 #pragma once
+#include "launch.cuh"
 #include "tensor.cuh"
 #include "values.cuh"
 
@@ -189,6 +190,7 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
     if (PAIR) cluster_sync();
     tensor_fence_after();
     const uint32_t memory = memory_at;
+    step_begin(nullptr);  // (behind the own memory and barriers: what a kernel of the same call left is read from here on)
 
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, items = tiles * p.parts_n;
     const int64_t first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
@@ -467,6 +469,7 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
 
 // The pieces of k added up in order, and what finish_sums does to whole sums.  A thread takes four columns.
 static __global__ void __launch_bounds__(256) join_kernel(const ProductArgs p) {
+    step_begin(nullptr);
     const int64_t per_row = p.ldp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= p.m * per_row) return;
     const int64_t m = i / per_row, n = i % per_row * 4;
@@ -510,6 +513,7 @@ template <class TD, class TY, int V>
 static __global__ void __launch_bounds__(256) dense_dz_kernel(b200_dense_grad_op a, TD* dz, int64_t ldz, float* parts, int across) {
     constexpr int kAhead = 4;
     __shared__ float added[256 * V];
+    step_begin(nullptr);
     const int lane = (int)threadIdx.x % across, column = (blockIdx.x * across + lane) * V, step = 256 / across;
     const int64_t first = (int64_t)a.rows * blockIdx.y / gridDim.y, last = (int64_t)a.rows * (blockIdx.y + 1) / gridDim.y;
     const TD* dy = static_cast<const TD*>(a.dy) + column;

@@ -12,6 +12,7 @@
 
 #include <type_traits>
 
+#include "launch.cuh"
 #include "values.cuh"
 
 namespace b200 {
@@ -434,6 +435,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b
     __shared__ float sums[2][kRowWarpsMost];
     const RowPlace p = RowPlace::here<VEC, true>(warps);
     const int groups = (blockDim.x >> 5) / warps, group = (threadIdx.x >> 5) / warps;
+    step_begin(nullptr);
     float dw[NV][8] = {};
     int turn = 0;
     for (int64_t row = p.row; row < a.rows; row += (int64_t)gridDim.x * groups, turn ^= 1) {
@@ -502,6 +504,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b
 constexpr int kAddThreads = 1024;
 static __global__ void __launch_bounds__(kAddThreads) add_parts_kernel(const float* parts, int n_parts, int cols, float* out) {
     __shared__ float sums[32][33];
+    step_begin(nullptr);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (c < cols) {

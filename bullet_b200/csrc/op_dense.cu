@@ -61,6 +61,7 @@ Operand operand(const void* at, int64_t ld, int64_t rows, int64_t cols, int type
 struct Call {
     Operand a, b;
     bool a_across, b_across, codes;  // codes: a is an 8-bit checkpoint with a scale per k
+    bool follows;                    // a kernel of the same call stands before it on the stream
     ProductArgs p;
     bool bytes() const { return a.type == B200_TYPE_E4M3 && !codes; }
     int block() const { return bytes() ? 128 : 64; }  // of k in a stage
@@ -170,11 +171,13 @@ int launch(const Call& c, cudaStream_t stream) {
     config.blockDim = dim3(T::kThreads);
     config.dynamicSmemBytes = T::kShared;
     config.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {PAIR ? 2u : 1u, 1, 1};
-    config.attrs = &attr;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attrs[2] = {};
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim = {PAIR ? 2u : 1u, 1, 1};
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attrs;
+    config.numAttrs = c.follows ? 2 : 1;
     OP_CK(cudaLaunchKernelEx(&config, kernel, a, b, d, r, c.p));
     return 0;
 }
@@ -229,8 +232,7 @@ int run_product(Call c, char* space, cudaStream_t stream) {
                                 : launch_columns<false, false, false, false>(c, plan.columns, stream);
     if (rc) return rc;
     if (p.parts) {
-        join_kernel<<<(unsigned)((p.m * (p.ldp / 4) + 255) / 256), 256, 0, stream>>>(p);
-        OP_CK(cudaGetLastError());
+        OP_CK(launch_step(true, join_kernel, (unsigned)((p.m * (p.ldp / 4) + 255) / 256), 256, 0, stream, p));
     }
     return 0;
 }
@@ -479,18 +481,20 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
             go(bf16{}, e4m3{});
         else
             go(bf16{}, bf16{});
-        if (sums) add_parts_kernel<<<(op->out + 31) / 32, kAddThreads, 0, s>>>(sums, g.pieces, op->out, op->dbias);
         OP_CK(cudaGetLastError());
+        if (sums) OP_CK(launch_step(true, add_parts_kernel, (op->out + 31) / 32, kAddThreads, 0, s, sums, g.pieces, op->out, op->dbias));
     }
     const void* g = dz ? dz : op->dy;
     const int64_t ldg = dz ? space.ldz : op->lddy;
     if (op->dx) {
         Call c = dx_call(op, g, ldg);
+        c.follows = dz || sums;
         c.p.gave_up = word;
         if (int rc = run_product(c, base + space.products, s)) return rc;
     }
     if (op->dw) {
         Call c = dw_call(op, g, ldg);
+        c.follows = dz || sums || op->dx;
         c.p.gave_up = word;
         if (int rc = run_product(c, base + space.products, s)) return rc;
     }

@@ -203,8 +203,8 @@ int b200_op_rms_norm_backward(int device, void* stream, const b200_rms_norm_grad
             });
         });
     }
-    if (op->dweight) add_parts_kernel<<<(op->cols + 31) / 32, kAddThreads, 0, s>>>(parts, ctas, op->cols, op->dweight);
     OP_CK(cudaGetLastError());
+    if (op->dweight) OP_CK(launch_step(true, add_parts_kernel, (op->cols + 31) / 32, kAddThreads, 0, s, parts, ctas, op->cols, op->dweight));
     return 0;
 }
 
