@@ -511,7 +511,7 @@ static __global__ void __launch_bounds__(256) align_rows_kernel(const E* from, i
 // rows: parts[piece][out] (or null).  HBM bound.  The threads of a CTA are `across` side by side, V columns each.
 template <class TD, class TY, int V>
 static __global__ void __launch_bounds__(256) dense_dz_kernel(b200_dense_grad_op a, TD* dz, int64_t ldz, float* parts, int across) {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;  // rows (131072 x 2048 from 8-bit outputs: 4 260 us, 8 228)
     __shared__ float added[256 * V];
     step_begin(nullptr);
     const int lane = (int)threadIdx.x % across, column = (blockIdx.x * across + lane) * V, step = 256 / across;

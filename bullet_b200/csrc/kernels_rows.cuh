@@ -188,7 +188,7 @@ __device__ __forceinline__ void store_typed(void* at, int64_t row_at, int type, 
 // value are moved to that, those between the last code below 1 and 1 to that code's value, which is 1 - 2^-4 up to scales of 2^6; then
 // the nearest code is the one that is wanted.  Magnitudes are in the order of their bits: less 1, what is not to move below the
 // least is 0, the largest of all; less 1's bits, what is below 1 comes last.  (131072 x 2048 bf16 outputs of CReLU with
-// comparisons and selections 185 us, with these additions in front of maxima and minima 161.)
+// comparisons and selections 185 us, with these additions in front of maxima and minima 161, in a kernel of its own 134.)
 __device__ __forceinline__ bool moves_outputs(uint32_t scale) { return scale >= 10u << 23 && scale <= 133u << 23; }
 __device__ __forceinline__ uint32_t least_bits(uint32_t scale) { return scale - (9u << 23); }
 __device__ __forceinline__ float moved_output(float v, uint32_t least, int act) {
@@ -215,23 +215,28 @@ static __device__ __noinline__ uint2 codes_slowly(float v0, float v1, float v2, 
     for (int k = 0; k < 8; k++) q[k] = code_of_output(v[k], scale, act);
     return make_uint2(q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24);
 }
-// Eight codes.
-template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* row, int first, int cols, const float (&v)[8], uint32_t scale, int act) {
-    const float by = one_over_scale(scale);
-    uint32_t q[4];
-    if (__builtin_expect(scale == kTopScale || (act != B200_ACT_NONE && !moves_outputs(scale)), 0)) {
-        const uint2 u = codes_slowly(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], scale, act);
-        q[0] = u.x & 0xffffu, q[1] = u.x >> 16, q[2] = u.y & 0xffffu, q[3] = u.y >> 16;
-    } else {
+// Eight codes, as q[k] two each: where the scale is a usual one, else slowly.
+template <bool MOVES>
+__device__ __forceinline__ bool usual_scale(uint32_t scale) { return scale != kTopScale && (!MOVES || moves_outputs(scale)); }
+template <bool MOVES>
+__device__ __forceinline__ void eight_codes(const float (&v)[8], uint32_t scale, bool usual, int act, uint32_t (&q)[4]) {
+    if (__builtin_expect(usual, 1)) {
+        const float by = one_over_scale(scale);
         const uint32_t least = least_bits(scale);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            float x[2] = {v[2 * k], v[2 * k + 1]};
-            if (act != B200_ACT_NONE) x[0] = moved_output(x[0], least, act), x[1] = moved_output(x[1], least, act);
-            q[k] = two_codes(x[0], x[1], by, by);
+            if constexpr (MOVES)
+                q[k] = two_codes(moved_output(v[2 * k], least, act), moved_output(v[2 * k + 1], least, act), by, by);
+            else
+                q[k] = two_codes(v[2 * k], v[2 * k + 1], by, by);
         }
+    } else {
+        const uint2 u = codes_slowly(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], scale, act);
+        q[0] = u.x & 0xffffu, q[1] = u.x >> 16, q[2] = u.y & 0xffffu, q[3] = u.y >> 16;
     }
+}
+template <bool VEC>
+__device__ __forceinline__ void put_codes(uint8_t* row, int first, int cols, const uint32_t (&q)[4]) {
     if constexpr (VEC) {
         if (first < cols) *reinterpret_cast<uint2*>(row + first) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
     } else {
@@ -348,6 +353,7 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
             m = row_max(m, warps, largest[1]);
         }
         const uint32_t scale = scale_bits(m);
+        const bool usual = usual_scale<false>(scale);
         if (p.leader) a.scale[p.row] = __uint_as_float(scale);
 #pragma unroll
         for (int j = 0; j < NV; j++) {
@@ -362,14 +368,17 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_kernel(b200_rms_n
                         v[j][k] = exact_for_code(xr + c, a.residual ? static_cast<const TX*>(a.residual) + p.row * a.ldr + c : nullptr, a.weight ? a.weight + c : nullptr, rstd, rest);
                 }
             }
-            store_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, v[j], scale, B200_ACT_NONE);
+            uint32_t q[4];
+            eight_codes<false>(v[j], scale, usual, B200_ACT_NONE, q);
+            put_codes<VEC>(static_cast<uint8_t*>(a.y) + p.row * a.ldy, p.lane_at + p.step * j, a.cols, q);
         }
     }
 }
 
 // Elements of 16 bits are compared two at a time: one by one the ALU pipe takes longer than HBM (131072 rows of 2048 bf16 outputs of
-// CReLU 207 us, so 161, for 805 MB).
-template <class TX, int NV, bool VEC>
+// CReLU 207 us, so 134, for 805 MB; plain values 120).
+// OUTPUTS: of an activation.
+template <class TX, int NV, bool VEC, bool OUTPUTS>
 static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pack8_op a, int warps) {
     constexpr bool TWO = VEC && sizeof(TX) == 2;
     __shared__ uint32_t largest[2][kRowWarpsMost];
@@ -413,17 +422,20 @@ static __global__ void __launch_bounds__(kRowThreads) pack8_rows_kernel(b200_pac
     }
     const uint32_t scale = scale_bits(m);
     if (p.leader) a.scale[p.row] = __uint_as_float(scale);
-    const bool two = TWO && std::is_same<TX, bf16>::value && a.act != B200_ACT_NONE && scale != kTopScale && moves_outputs(scale);
-    const uint32_t least2 = (least_bits(scale) >> 16) * 0x00010001u;
+    const bool usual = usual_scale<OUTPUTS>(scale);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        if (two) {
-            uint4& w = x[j].raw[0];
-            w = make_uint4(moved_outputs2(w.x, least2, a.act), moved_outputs2(w.y, least2, a.act), moved_outputs2(w.z, least2, a.act), moved_outputs2(w.w, least2, a.act));
-        }
+        constexpr bool kTwoMoved = OUTPUTS && TWO && std::is_same<TX, bf16>::value;
+        uint32_t q[4];
         float v[8];
+        if (kTwoMoved && usual) {
+            const uint32_t least = (least_bits(scale) >> 16) * 0x00010001u;
+            uint4& w = x[j].raw[0];
+            w = make_uint4(moved_outputs2(w.x, least, a.act), moved_outputs2(w.y, least, a.act), moved_outputs2(w.z, least, a.act), moved_outputs2(w.w, least, a.act));
+        }
         x[j].get(v);
-        store_codes<VEC>(static_cast<uint8_t*>(a.q) + p.row * a.ldq, p.lane_at + p.step * j, a.cols, v, scale, two ? B200_ACT_NONE : a.act);
+        eight_codes<OUTPUTS && !kTwoMoved>(v, scale, usual, a.act, q);
+        put_codes<VEC>(static_cast<uint8_t*>(a.q) + p.row * a.ldq, p.lane_at + p.step * j, a.cols, q);
     }
 }
 

@@ -34,6 +34,7 @@ RowShape row_shape(int64_t rows, int cols, int best, bool several) {
     s.threads = 32 * s.warps * (int)s.groups;
     return s;
 }
+RowShape pack_shape(int64_t rows, int cols) { return row_shape(rows, cols, 8, false); }
 RowShape norm_shape(int64_t rows, int cols, int type) { return row_shape(rows, cols, type == B200_TYPE_F32 ? 2 : 4, false); }
 RowShape grad_shape(int64_t rows, int cols) { return row_shape(rows, cols, 2, true); }  // (fewer sums to leave behind)
 // f(std::integral_constant) for the smallest of 1, 2, 4, ... that holds `vectors`
@@ -240,11 +241,15 @@ int b200_op_pack8(int device, void* stream, const b200_pack8_op* op) {
     } else if (op->cols > kRowCols) {
         with_float(op->x_type, [&](auto x) { pack8_rows_any_kernel<decltype(x)><<<any_ctas(op->rows), kRowThreads, 0, s>>>(*op); });
     } else {
-        const RowShape g = norm_shape(op->rows, op->cols, op->x_type);
+        const RowShape g = pack_shape(op->rows, op->cols);
         with_float(op->x_type, [&](auto x) {
             with_bool(vec, [&](auto v) {
                 with_vectors<kRowVectors>(g.vectors, [&](auto nv) {
-                    pack8_rows_kernel<decltype(x), nv(), v()><<<(unsigned)((op->rows + g.groups - 1) / g.groups), g.threads, 0, s>>>(*op, g.warps);
+                    auto go = [&](auto kernel) { kernel<<<(unsigned)((op->rows + g.groups - 1) / g.groups), g.threads, 0, s>>>(*op, g.warps); };
+                    if (op->act == B200_ACT_NONE)
+                        go(pack8_rows_kernel<decltype(x), nv(), v(), false>);
+                    else
+                        go(pack8_rows_kernel<decltype(x), nv(), v(), true>);
                 });
             });
         });
