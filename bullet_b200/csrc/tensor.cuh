@@ -14,18 +14,19 @@ namespace b200 {
 struct Waits {
     volatile int* dead;  // of the CTA, in shared memory
     int* gave_up;        // the host's
+    static constexpr uint32_t kAsleepNs = 100000;
     __device__ __forceinline__ static bool arrived(uint64_t* bar, uint32_t parity) {  // by threads of either CTA of a pair
         uint32_t ok;
         asm volatile(
-            "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+            "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
             : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(kAsleepNs)  // (asleep until then: warps that ask again and again cost power)
             : "memory");
         return ok != 0;
     }
     __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
         if (arrived(bar, parity)) return true;
-        for (int tries = 0; tries < 1000000 && !*dead; tries++)
+        for (int tries = 0; tries < 20000 && !*dead; tries++)
             if (arrived(bar, parity)) return true;
         if (!*dead) {
             *dead = 1;
