@@ -4,6 +4,7 @@ Tolerances.  A value rounded to a type with p significand bits is off by at most
 fp16).  A sum of k products in 32 bits is off by at most k 2^-23 of the sum of their magnitudes, in any order and whether a step
 rounds or cuts off; products of small whole numbers are exact, and have to come out exactly.  A code of 8 bits is off by half a step of its
 binade.  2^-18 covers the few roundings of elementwise arithmetic in 32 bits."""
+import ctypes
 import math
 
 import pytest
@@ -297,9 +298,11 @@ def test_dense_of_matrices_inside_larger_ones(rows, n_in, n_out, kind, pads):
     codes = kind is E4M3
     op = _lib.CDense(rows, n_in, n_out, 3 if codes else 1, 1, 0, n_in + px, n_out + pw, n_out + pr, n_out + pr, x.data_ptr(), one.data_ptr() if codes else None,
                      w.data_ptr(), one.data_ptr() if codes else None, None, r.data_ptr(), y.data_ptr())
-    lib = _lib.load()
-    space = ops._space(lib.b200_op_dense_workspace, op, x.device)  # noqa: F841
-    ops._call(lib.b200_op_dense, x.device, op)
+    lib, need = _lib.load(), ctypes.c_int64()
+    _lib.check(lib.b200_op_dense_workspace(ctypes.byref(op), ctypes.byref(need)))
+    space = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")[at % 2 * 16:]  # (aligned to 16 bytes and no more)
+    op.workspace, op.workspace_bytes = space.data_ptr(), need.value
+    _lib.check(lib.b200_op_dense(0, torch.cuda.current_stream().cuda_stream, ctypes.byref(op)))
     assert torch.equal(y[:, :n_out].double(), want.to(BF16).double())
     assert (y[:, n_out:] == 77).all() and (holder[:at] == 77).all() and (holder[at + rows * (n_out + pr):] == 77).all()
 
