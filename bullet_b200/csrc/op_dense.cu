@@ -68,9 +68,9 @@ struct Call {
 };
 
 // How a product is cut: into tiles of which width, and k into how many parts.  By what each way costs in clocks: a stage (128 bytes of
-// k) of a tile, an item besides, a join (launch, and its bytes per clock), rounds of items being whole.  Fitted to times on a B200; of 35
-// products of 16 to 65536 rows with every width and number of parts, this choice was within 10 % of the best on all but four,
-// and within 20 % on those (us, this choice / the best: 2048 x 2048 -> 256 16.2 / 12.0 before the codes' stages had costs of their own).
+// k) of a tile, an item besides, a join (launch, and its bytes per clock), rounds of items being whole.  Fitted to times on a B200: of 33
+// products of 16 to 65536 rows, timed with every width and up to ten numbers of parts, this choice is within 10 % of the best on all
+// but two (us, it and the best: 16 x 2048 -> 1024 10.8 and 8.7, gradient of 256 x 256 weights from 16384 rows 17.4 and 15.2).
 struct Plan {
     int columns;  // of a tile; from 256 on a pair's
     int parts, blocks;  // pieces of k and the stages of each
@@ -78,11 +78,11 @@ struct Plan {
     bool joined() const { return parts > 1 || chains() > 1; }
 };
 constexpr int kSms = 148;  // that products are cut for
-constexpr int kPartsMost = 32, kJoin = 6000, kJoinBytes = 2500;
+constexpr int kPartsMost = 32, kJoin = 4500, kJoinBytes = 2500;
 struct TileCost {
     int columns, rows, units, stage, stage_codes, item;
 };
-constexpr TileCost kTiles[] = {{512, 256, kSms / 2, 1226, 1403, 5500}, {256, 256, kSms / 2, 687, 1222, 900}, {128, 128, kSms, 650, 1000, 900}, {64, 128, kSms, 450, 850, 900}};
+constexpr TileCost kTiles[] = {{512, 256, kSms / 2, 1226, 1403, 5500}, {256, 256, kSms / 2, 687, 1222, 900}, {128, 128, kSms, 650, 1000, 900}, {64, 128, kSms, 600, 950, 900}};
 Plan plan_of(const Call& c) {
     const int64_t blocks = (c.p.k + c.block() - 1) / c.block();
     Plan best{};
