@@ -184,6 +184,12 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
     }
+    if (threadIdx.x == 32) {
+        know_map(&a_map);
+        know_map(&b_map);
+        if (p.boxes) know_map(&d_map);
+    }
+    __syncwarp();
     if (warp == 1) tensor_memory_take<PAIR>(&memory_at, T::kMemory);
     tensor_fence_before();
     __syncthreads();

@@ -83,7 +83,7 @@ struct TileCost {
     int columns, rows, units, stage, stage_codes, item;
 };
 constexpr TileCost kTiles[] = {{512, 256, kSms / 2, 1226, 1403, 5500}, {256, 256, kSms / 2, 687, 1222, 900}, {128, 128, kSms, 650, 1000, 900}, {64, 128, kSms, 600, 950, 900}};
-Plan plan_of(const Call& c) {
+Plan reckoned_plan(const Call& c) {
     const int64_t blocks = (c.p.k + c.block() - 1) / c.block();
     Plan best{};
     double least = 1e300;
@@ -101,6 +101,19 @@ Plan plan_of(const Call& c) {
         }
     }
     return best;
+}
+// The same, from the last ones that this thread asked for (2 us to reckon, and a gradient asks six times).
+Plan plan_of(const Call& c) {
+    struct Known {
+        int64_t m, n, k;
+        int kind;
+        Plan plan;
+    };
+    thread_local Known known[16] = {};
+    const int kind = 1 + c.bytes() + 2 * c.codes;  // (0: a place that holds none)
+    Known& at = known[(c.p.m * 7 + c.p.n * 3 + c.p.k + kind) & 15];
+    if (at.kind != kind || at.m != c.p.m || at.n != c.p.n || at.k != c.p.k) at = {c.p.m, c.p.n, c.p.k, kind, reckoned_plan(c)};
+    return at.plan;
 }
 int64_t parts_bytes(const Call& c, const Plan& plan) { return plan.joined() ? (int64_t)plan.parts * c.p.m * ((c.p.n + 7) / 8 * 8) * 4 : 0; }
 int64_t call_bytes(const Call& c) { return c.a.copy_bytes() + c.b.copy_bytes() + (parts_bytes(c, plan_of(c)) + 255) / 256 * 256; }
@@ -254,7 +267,8 @@ DzShape dz_shape(const b200_dense_grad_op* op) {
     s.across = 1;
     while (s.across < 256 && s.across < vectors) s.across *= 2;
     const int ctas = (vectors + s.across - 1) / s.across, at_once = 256 / s.across * 4;
-    s.pieces = std::max(1, std::min(op->rows / at_once, std::max(1, kSms * 4 / ctas)));
+    // (few rows: one piece, whose sums are the result, and no second launch)
+    s.pieces = op->rows <= 4 * at_once ? 1 : std::max(1, std::min(op->rows / at_once, std::max(1, kSms * 4 / ctas)));
     s.grid = dim3(ctas, s.pieces);
     return s;
 }
@@ -369,7 +383,8 @@ GradSpace grad_space(const b200_dense_grad_op* op) {
     s.ldz = (op->out + 7) / 8 * 8;
     s.dz_made = op->act != B200_ACT_NONE && (op->dx || op->dw);
     s.dz = next(s.dz_made ? op->rows * s.ldz * 2 : 0);
-    s.sums = next(op->dbias ? (int64_t)dz_shape(op).pieces * op->out * 4 : 0);
+    const int pieces = dz_shape(op).pieces;
+    s.sums = next(op->dbias && pieces > 1 ? (int64_t)pieces * op->out * 4 : 0);
     const void* g = s.dz_made ? nullptr : op->dy;  // (dz is aligned, as NULL is)
     const int64_t ldg = s.dz_made ? s.ldz : op->lddy;
     s.products = next(std::max(op->dx ? call_bytes(dx_call(op, g, ldg)) : 0, op->dw ? call_bytes(dw_call(op, g, ldg)) : 0));
@@ -464,9 +479,9 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
     if (int rc = check_gave_up(who, word)) return rc;
     char* base = aligned_space(op->workspace);
     void* dz = space.dz_made ? base + space.dz : nullptr;
-    float* sums = op->dbias ? reinterpret_cast<float*>(base + space.sums) : nullptr;
+    const DzShape g = dz_shape(op);
+    float* sums = !op->dbias ? nullptr : g.pieces == 1 ? op->dbias : reinterpret_cast<float*>(base + space.sums);
     if (dz || sums) {
-        const DzShape g = dz_shape(op);
         auto go = [&](auto d, auto y) {
             using TD = decltype(d);
             using TY = decltype(y);
@@ -482,18 +497,18 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
         else
             go(bf16{}, bf16{});
         OP_CK(cudaGetLastError());
-        if (sums) OP_CK(launch_step(true, add_parts_kernel, (op->out + 31) / 32, kAddThreads, 0, s, sums, g.pieces, op->out, op->dbias));
+        if (sums && g.pieces > 1) OP_CK(launch_step(true, add_parts_kernel, (op->out + 31) / 32, kAddThreads, 0, s, sums, g.pieces, op->out, op->dbias));
     }
-    const void* g = dz ? dz : op->dy;
-    const int64_t ldg = dz ? space.ldz : op->lddy;
+    const void* gradient = dz ? dz : op->dy;
+    const int64_t ld_gradient = dz ? space.ldz : op->lddy;
     if (op->dx) {
-        Call c = dx_call(op, g, ldg);
+        Call c = dx_call(op, gradient, ld_gradient);
         c.follows = dz || sums;
         c.p.gave_up = word;
         if (int rc = run_product(c, base + space.products, s)) return rc;
     }
     if (op->dw) {
-        Call c = dw_call(op, g, ldg);
+        Call c = dw_call(op, gradient, ld_gradient);
         c.follows = dz || sums || op->dx;
         c.p.gave_up = word;
         if (int rc = run_product(c, base + space.products, s)) return rc;

@@ -54,6 +54,9 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
+// has a map fetched before its first use
+__device__ __forceinline__ void know_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 // A box of a matrix into shared memory; the bytes are counted at `bar`, a barrier of this CTA or (PAIR) of either.  x in elements,
 // a multiple of 16 bytes.
 template <bool PAIR>
