@@ -356,15 +356,24 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
                             }
                             __syncwarp();
                         }
-                    } else if (here) {
-                        for (int k = 0; k < 32; k++) {
-                            if (c + k >= own) break;
-                            float x = v[0];
+                    } else {  // through the box as fp32, a row of 32 elements at a time
+                        box_out<float>(box + lane * 128, lane, 0, v, false);
+                        __syncwarp();
+                        const int64_t column = own0 + c + lane;
+                        const int64_t last = p.m - 1;
+                        if (c + lane < own) {
+                            for (int r0 = 0; r0 < 32; r0 += 16) {
+                                float x[16];  // (what is added is read before anything is written, which might be the same for all that is known)
 #pragma unroll
-                            for (int q = 1; q < 32; q++) x = q == k ? v[q] : x;
-                            if (adds) x += load_value(p.residual, m * p.ldr + own0 + c + k, p.d_type);
-                            store_value(p.d, m * p.ldd + own0 + c + k, p.d_type, x);
+                                for (int r = 0; r < 16; r++) x[r] = adds ? load_value(p.residual, min(rows0 + r0 + r, last) * p.ldr + column, p.d_type) : 0.f;
+#pragma unroll
+                                for (int r = 0; r < 16; r++) {
+                                    x[r] += *reinterpret_cast<const float*>(box + (r0 + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                                    if (rows0 + r0 + r <= last) store_value(p.d, (rows0 + r0 + r) * p.ldd + column, p.d_type, x[r]);
+                                }
+                            }
                         }
+                        __syncwarp();
                     }
                 }
                 tensor_fence_before();
@@ -499,18 +508,31 @@ static __global__ void __launch_bounds__(256) join_kernel(const ProductArgs p) {
     }
 }
 
-// A matrix whose rows do not start on 16 bytes, copied to one whose rows do.  E: bytes of an element.
-template <class E>
-static __global__ void __launch_bounds__(256) align_rows_kernel(const E* from, int64_t ld, E* to, int64_t ld_to, int64_t rows, int64_t cols) {
-    const int64_t per = (cols + 255) / 256, i = blockIdx.x;
-    const int64_t row0 = i / per * 8, c = i % per * 256 + threadIdx.x;
-    if (c >= cols) return;
-    E v[8];
+// A matrix whose rows do not start on 16 bytes, copied to one whose rows do, side by side.  A thread puts 16 bytes together out of the
+// five words of four that they lie in, of which it loads those that hold any byte of the row.
+constexpr int kAlignPieces = 4;  // of a thread, in flight
+static __global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* from, int64_t apart, uint4* to, int64_t rows, int64_t bytes) {
+    const int64_t per_row = (bytes + 15) / 16, all = rows * per_row;
+    uint32_t w[kAlignPieces][5];
+    int shift[kAlignPieces];
 #pragma unroll
-    for (int r = 0; r < 8; r++) v[r] = from[min(row0 + r, rows - 1) * ld + c];
+    for (int q = 0; q < kAlignPieces; q++) {
+        const int64_t i = (int64_t)blockIdx.x * 256 * kAlignPieces + q * 256 + threadIdx.x;
+        if (i >= all) continue;
+        const uint8_t* row = from + i / per_row * apart;
+        const uint8_t* at = row + i % per_row * 16;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>((uintptr_t)at & ~(uintptr_t)3);
+        shift[q] = 8 * (int)((uintptr_t)at & 3);
 #pragma unroll
-    for (int r = 0; r < 8; r++)
-        if (row0 + r < rows) to[(row0 + r) * ld_to + c] = v[r];
+        for (int k = 0; k < 5; k++) w[q][k] = reinterpret_cast<const uint8_t*>(words + k) < row + bytes ? words[k] : 0u;
+    }
+#pragma unroll
+    for (int q = 0; q < kAlignPieces; q++) {
+        const int64_t i = (int64_t)blockIdx.x * 256 * kAlignPieces + q * 256 + threadIdx.x;
+        if (i < all)
+            to[i] = make_uint4(__funnelshift_r(w[q][0], w[q][1], shift[q]), __funnelshift_r(w[q][1], w[q][2], shift[q]), __funnelshift_r(w[q][2], w[q][3], shift[q]),
+                               __funnelshift_r(w[q][3], w[q][4], shift[q]));
+    }
 }
 
 // dz = act'(y) * dy, rounded to dy's type (dz: rows of ldz, or null), and the sums of the unrounded values over pieces of the

@@ -208,12 +208,9 @@ int align(Operand& o, char*& space, cudaStream_t stream) {
     if (o.aligned()) return 0;
     void* to = space;
     space += o.copy_bytes();
-    const int64_t grid = (o.rows + 7) / 8 * ((o.cols + 255) / 256);
+    const int64_t pieces = o.rows * (o.copy_ld() * type_bytes(o.type) / 16), grid = (pieces + 256 * kAlignPieces - 1) / (256 * kAlignPieces);
     if (grid > INT32_MAX) return fail(B200_ERR_UNSUPPORTED, "too many elements in rows that do not start on 16 bytes");
-    if (type_bytes(o.type) == 1)
-        align_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>(static_cast<const uint8_t*>(o.at), o.ld, static_cast<uint8_t*>(to), o.copy_ld(), o.rows, o.cols);
-    else
-        align_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>(static_cast<const uint16_t*>(o.at), o.ld, static_cast<uint16_t*>(to), o.copy_ld(), o.rows, o.cols);
+    align_rows_kernel<<<(unsigned)grid, 256, 0, stream>>>(static_cast<const uint8_t*>(o.at), o.bytes_of_row(), static_cast<uint4*>(to), o.rows, o.cols * type_bytes(o.type));
     OP_CK(cudaGetLastError());
     o.ld = o.copy_ld();
     o.at = to;
@@ -381,7 +378,8 @@ GradSpace grad_space(const b200_dense_grad_op* op) {
         return at;
     };
     s.ldz = (op->out + 7) / 8 * 8;
-    s.dz_made = op->act != B200_ACT_NONE && (op->dx || op->dw);
+    // (dz is dy without an activation, but for two products of one that does not start on 16 bytes)
+    s.dz_made = (op->dx || op->dw) && (op->act != B200_ACT_NONE || !operand(op->dy, op->lddy, op->rows, op->out, op->dy_type).aligned());
     s.dz = next(s.dz_made ? op->rows * s.ldz * 2 : 0);
     const int pieces = dz_shape(op).pieces;
     s.sums = next(op->dbias && pieces > 1 ? (int64_t)pieces * op->out * 4 : 0);
