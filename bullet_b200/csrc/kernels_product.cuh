@@ -151,6 +151,25 @@ __device__ __forceinline__ void box_out(unsigned char* row, int r, int first_pie
     }
 }
 
+// A column of a box of fp32, the residual added, element by element; sixteen of the residual are on their way at a time.
+template <class T>
+static __device__ __forceinline__ void column_out(const ProductArgs& p, const unsigned char* box, int lane, int64_t rows0, int64_t column, bool adds) {
+    const T* residual = static_cast<const T*>(p.residual) + column;
+    T* d = static_cast<T*>(p.d) + column;
+    const int64_t last = p.m - 1;
+    for (int r0 = 0; r0 < 32 && rows0 + r0 <= last; r0 += 16) {
+        T added[16];
+        if (adds)
+#pragma unroll
+            for (int r = 0; r < 16; r++) added[r] = residual[min(rows0 + r0 + r, last) * p.ldr];
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const float x = *reinterpret_cast<const float*>(box + (r0 + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            if (rows0 + r0 + r <= last) d[(rows0 + r0 + r) * p.ldd] = from_float<T>(adds ? x + to_float(added[r]) : x);
+        }
+    }
+}
+
 template <int BN, bool PAIR, bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
 static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACROSS, CODES>::kThreads), 1)
     product_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap d_map,
@@ -359,19 +378,13 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
                     } else {  // through the box as fp32, a row of 32 elements at a time
                         box_out<float>(box + lane * 128, lane, 0, v, false);
                         __syncwarp();
-                        const int64_t column = own0 + c + lane;
-                        const int64_t last = p.m - 1;
                         if (c + lane < own) {
-                            for (int r0 = 0; r0 < 32; r0 += 16) {
-                                float x[16];  // (what is added is read before anything is written, which might be the same for all that is known)
-#pragma unroll
-                                for (int r = 0; r < 16; r++) x[r] = adds ? load_value(p.residual, min(rows0 + r0 + r, last) * p.ldr + column, p.d_type) : 0.f;
-#pragma unroll
-                                for (int r = 0; r < 16; r++) {
-                                    x[r] += *reinterpret_cast<const float*>(box + (r0 + r) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                                    if (rows0 + r0 + r <= last) store_value(p.d, (rows0 + r0 + r) * p.ldd + column, p.d_type, x[r]);
-                                }
-                            }
+                            if (p.d_type == B200_TYPE_F32)
+                                column_out<float>(p, box, lane, rows0, own0 + c + lane, adds);
+                            else if (p.d_type == B200_TYPE_BF16)
+                                column_out<bf16>(p, box, lane, rows0, own0 + c + lane, adds);
+                            else
+                                column_out<f16>(p, box, lane, rows0, own0 + c + lane, adds);
                         }
                         __syncwarp();
                     }
