@@ -62,6 +62,7 @@ static __global__ void __launch_bounds__(256) dense_few_kernel(const FewArgs f) 
     const b200_dense_op& a = f.op;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
+    cluster_arrive();  // (the first CTA has to be there before its memory is written)
     uint32_t ctas;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
     const int n0 = (int)(blockIdx.x / ctas) * kFewColumns, n = n0 + 8 * (lane & 7), columns = min(8, a.out - n);
@@ -103,6 +104,7 @@ static __global__ void __launch_bounds__(256) dense_few_kernel(const FewArgs f) 
             if (lane < 8) sums[warp][r][8 * lane + c] = v;
         }
     __syncthreads();
+    cluster_wait();
     for (int i = threadIdx.x; i < ROWS * kFewColumns; i += 256) {
         float v = 0.f;
 #pragma unroll

@@ -44,6 +44,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
+// the same in two halves
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // `local`, an address of shared memory, in CTA `rank` of the cluster
 __device__ __forceinline__ uint32_t of_rank(uint32_t local, uint32_t rank) {
     uint32_t at;
