@@ -108,9 +108,7 @@ __device__ __forceinline__ void finish_sums(const ProductArgs& p, float (&v)[32]
             const float4 b = reinterpret_cast<const float4*>(bias)[g];
             v[4 * g] += b.x, v[4 * g + 1] += b.y, v[4 * g + 2] += b.z, v[4 * g + 3] += b.w;
         }
-        if (p.act != B200_ACT_NONE)
-#pragma unroll
-            for (int k = 0; k < 32; k++) v[k] = activate(v[k], p.act);
+        activate_all(v, p.act);
     }
 }
 // Half of a row of a box (16 bits: 32 columns of 64; fp32: 32 columns, the whole), the residual there added, in place.  Rows of 128 bytes

@@ -95,12 +95,35 @@ static __device__ __noinline__ uint8_t code_of_output(float v, uint32_t scale, i
 }
 
 // NaN stays NaN in all of them.
+__device__ __forceinline__ float at_least_0(float z) {
+    asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z));
+    return z;
+}
+__device__ __forceinline__ float at_most_1(float z) {
+    asm("min.NaN.f32 %0, %0, 0f3F800000;" : "+f"(z));
+    return z;
+}
 __device__ __forceinline__ float activate(float z, int act) {
     if (act == B200_ACT_NONE) return z;
-    z = z < 0.f ? 0.f : z;
+    z = at_least_0(z);
     if (act == B200_ACT_RELU) return z;
-    z = z > 1.f ? 1.f : z;
+    z = at_most_1(z);
     return act == B200_ACT_SCRELU ? z * z : z;
+}
+template <int N>
+__device__ __forceinline__ void activate_all(float (&z)[N], int act) {  // (one question for all)
+    if (act == B200_ACT_NONE) return;
+    if (act == B200_ACT_RELU) {
+#pragma unroll
+        for (int k = 0; k < N; k++) z[k] = at_least_0(z[k]);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) z[k] = at_most_1(at_least_0(z[k]));
+    if (act == B200_ACT_SCRELU) {
+#pragma unroll
+        for (int k = 0; k < N; k++) z[k] *= z[k];
+    }
 }
 // dy times the activation's derivative, taken from its output; 0 where that is cut off, whatever dy is.
 __device__ __forceinline__ float gradient_from_output(float dy, float y, int act) {
