@@ -383,7 +383,12 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
  *     Any ld and any address aligned to the element will do; 16-byte aligned rows are faster.  Indices are 64-bit;
  *   - no rows: nothing is done (gradients of weights become 0) and B200_OK returned;
  *   - outputs overlap neither inputs nor one another;
- *   - all sums are held in 32 bits and taken in the same order by every call of the same shape: equal inputs give equal bits;
+ *   - scratch is lent by the caller: b200_op_*_workspace says how many bytes the very operation needs that is then called
+ *     (its addresses and distances count);
+ *   - all sums are held in 32 bits and taken in the same order by every call of the same shape and alignment: equal inputs
+ *     give equal bits;
+ *   - a kernel that waits too long for its own copies or products gives up, and the next dense call returns
+ *     B200_ERR_STATE;
  *   - a B200_TYPE_E4M3 matrix holds codes of 8 bits (four significand bits, largest value 448, no infinities) and goes with
  *     a scale, a power of two in fp32, per row (or per column, where said): it stands for code * scale. */
 #define B200_ACT_RELU 3 /* these operators only; 0 to 2 as above */
@@ -437,7 +442,8 @@ int b200_op_rms_norm_backward(int device, void* stream, const b200_rms_norm_grad
  * even one; infinities and NaN become NaN.  `act` names the activation whose outputs these are: for B200_ACT_RELU, _CRELU
  * and _SCRELU a value above 0 keeps a code above 0, for the latter two a value below 1 one that stands for less than 1, so
  * that the activation's gradient is cut off where it would have been without the rounding.
- * A power of two as scale leaves every value exact in bf16 and fp32. */
+ * A power of two as scale leaves every value exact in bf16 and fp32, down to their smallest numbers; a value that would round
+ * up out of fp32 rounds down. */
 typedef struct b200_pack8_op {
     int32_t rows, cols;
     int32_t x_type;    /* B200_TYPE_F32, _BF16 or _F16 */
