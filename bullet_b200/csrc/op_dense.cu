@@ -264,8 +264,9 @@ DzShape dz_shape(const b200_dense_grad_op* op) {
     s.across = 1;
     while (s.across < 256 && s.across < vectors) s.across *= 2;
     const int ctas = (vectors + s.across - 1) / s.across, at_once = 256 / s.across * 4;
-    // (few rows: one piece, whose sums are the result, and no second launch)
-    s.pieces = op->rows <= 4 * at_once ? 1 : std::max(1, std::min(op->rows / at_once, std::max(1, kSms * 4 / ctas)));
+    // Few rows: one piece, whose sums are the result, and no second launch.  Many: as many pieces as run at once, two to an SM (5003 x 1024
+    // with dz, and the parts' sums: four to an SM 10.8 + 5.6 us, three 11.3 + 8, two 8.9 + 5; 16384 x 1024: 23.4, 26.3, 21.5 + 6.7).
+    s.pieces = op->rows <= 4 * at_once ? 1 : std::max(1, std::min(op->rows / at_once, std::max(1, kSms * 2 / ctas)));
     s.grid = dim3(ctas, s.pieces);
     return s;
 }
