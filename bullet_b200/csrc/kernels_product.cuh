@@ -44,6 +44,10 @@ struct ProductArgs {
     float* parts;  // [parts_n][m][ldp], ldp = n up to a multiple of 8; null: none, there is one part of one chain
     int64_t ldp;
     int* gave_up;
+    // The kernel before it on the stream is a product of the same call, whose result it does not read: it starts while that one's last
+    // tiles run, on the SMs that they leave over, and waits for it at the end instead (gradient of 5003 rows, 2048 -> 1024 73.6 us without,
+    // 69.7 so; 16384 rows, 512 -> 256 47.6 and 43.0; 131072 rows, 2048 -> 512 605 and 602).
+    int beside;
 };
 
 template <int BN, bool PAIR, bool BYTES, bool A_ACROSS, bool B_ACROSS, bool CODES>
@@ -213,7 +217,12 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
     if (PAIR) cluster_sync();
     tensor_fence_after();
     const uint32_t memory = memory_at;
-    step_begin(nullptr);  // (behind the own memory and barriers: what a kernel of the same call left is read from here on)
+    // (behind the own memory and barriers: what a kernel of the same call left is read from here on; that before the one that it stands
+    // beside has completed, as that one waited for it before it let this one in)
+    if (p.beside)
+        step_lets_in();
+    else
+        step_begin(nullptr);
 
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, items = tiles * p.parts_n;
     const int64_t first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
@@ -491,6 +500,7 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
         tensor_fence_after();
         tensor_memory_give<PAIR>(memory, T::kMemory);
     }
+    if (p.beside) step_waits();  // who waits for this kernel waits for both
 }
 
 // The pieces of k added up in order, and what finish_sums does to whole sums.  A thread takes four columns.

@@ -7,6 +7,8 @@
 // So the kernel before may still be writing when a kernel begins, and its output is read with loads that are coherent (__ldcg, plain
 // ones), never through the read-only path (__ldg, ld.global.nc, const __restrict__), which wants data that nobody writes from the
 // kernel's first instruction on.  What the kernels before that one wrote is finished by then.
+// A kernel that reads nothing of the kernel before may let its successor in at once and wait (step_waits) at its end: who waits for it
+// then waits for both.
 // This takes most of the 3 us out of every boundary between two kernels of a step.
 //
 // Time stamps of the phases are written by the first thread of the kernels themselves: an event with timing between two
@@ -22,10 +24,12 @@ __device__ __forceinline__ unsigned long long clock_ns() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
+__device__ __forceinline__ void step_waits() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void step_lets_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // first statement of a step's kernel; `stamp`: where its start time goes, or null
 __device__ __forceinline__ void step_begin(unsigned long long* stamp) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    step_waits();
+    step_lets_in();
     if (stamp && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) *stamp = clock_ns();
 }
 

@@ -500,15 +500,18 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
     }
     const void* gradient = dz ? dz : op->dy;
     const int64_t ld_gradient = dz ? space.ldz : op->lddy;
+    bool dx_alone = false;  // its product is the last kernel so far, and uses no workspace
     if (op->dx) {
         Call c = dx_call(op, gradient, ld_gradient);
         c.follows = dz || sums;
         c.p.gave_up = word;
+        dx_alone = call_bytes(c) == 0;
         if (int rc = run_product(c, base + space.products, s)) return rc;
     }
     if (op->dw) {
         Call c = dw_call(op, gradient, ld_gradient);
         c.follows = dz || sums || op->dx;
+        c.p.beside = dx_alone && c.a.aligned() && c.b.aligned();
         c.p.gave_up = word;
         if (int rc = run_product(c, base + space.products, s)) return rc;
     }

@@ -499,6 +499,35 @@ def test_calls_run_on_the_current_stream_and_in_graphs(rows):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("rows,cols,out", [(5003, 2048, 1024), (16384, 512, 256), (700, 256, 2048)])
+def test_gradients_of_one_call_are_those_of_two_and_all_there_for_who_follows(rows, cols, out, packed):
+    """The two products of a call may run beside each other: a copy right behind the call has to find both results."""
+    dy, w = normal(401, rows, out).to(BF16), normal(402, cols, out).to(BF16)
+    x, y = torch.rand(rows, cols, device="cuda", generator=gen(403)).to(BF16), torch.rand(rows, out, device="cuda", generator=gen(404)).to(BF16)
+    act = ACT_CRELU if packed else ACT_SCRELU
+    if packed:
+        x, y = ops.pack8(x, act=act), ops.pack8(y, act=act)
+    dx = ops.dense_backward(dy, x, w, y=y, act=act, need_dw=False)[0]
+    dw = ops.dense_backward(dy, x, w, y=y, act=act, need_dx=False)[1]
+
+    def both():
+        got = ops.dense_backward(dy, x, w, y=y, act=act)[:2]
+        copies = [t.clone() for t in got]
+        for t in got:
+            t.zero_()
+        return copies
+
+    for got in [both() for _ in range(5)]:
+        assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = both()
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(captured[0], dx) and torch.equal(captured[1], dw)
+
+
 def test_long_matrices_pass_32_bit_offsets():
     """More than 2^31 elements: the last rows are those of the plain forms, by the bounds of the tests above."""
     rows, cols, n = (1 << 20) + 37, 2056, 40
