@@ -44,9 +44,10 @@ struct ProductArgs {
     float* parts;  // [parts_n][m][ldp], ldp = n up to a multiple of 8; null: none, there is one part of one chain
     int64_t ldp;
     int* gave_up;
-    // The kernel before it on the stream is a product of the same call, whose result it does not read: it starts while that one's last
-    // tiles run, on the SMs that they leave over, and waits for it at the end instead (gradient of 5003 rows, 2048 -> 1024 73.6 us without,
-    // 69.7 so; 16384 rows, 512 -> 256 47.6 and 43.0; 131072 rows, 2048 -> 512 605 and 602).
+    // The kernel before it on the stream is one of the same call whose result it does not read (the bias's sums joined, the other product
+    // of a gradient): it starts while that one's last CTAs run, on the SMs that they leave over, and waits for it at the end instead.
+    // Gradients, us: 5003 rows, 2048 -> 1024 73.6 without, 69.7 beside the other product; 16384 rows, 512 -> 256 47.6 and 43.0; 131072
+    // rows, 2048 -> 512 605 and 602.  Beside the joined sums as well: 2000 rows, 512 -> 512 36.6 and 35.3, 5003 rows 70.0 and 69.6.
     int beside;
 };
 

@@ -480,6 +480,7 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
     void* dz = space.dz_made ? base + space.dz : nullptr;
     const DzShape g = dz_shape(op);
     float* sums = !op->dbias ? nullptr : g.pieces == 1 ? op->dbias : reinterpret_cast<float*>(base + space.sums);
+    bool beside = false;  // the last kernel so far neither writes what the next product reads nor the other way round
     if (dz || sums) {
         auto go = [&](auto d, auto y) {
             using TD = decltype(d);
@@ -496,22 +497,23 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
         else
             go(bf16{}, bf16{});
         OP_CK(cudaGetLastError());
-        if (sums && g.pieces > 1) OP_CK(launch_step(true, add_parts_kernel, (op->out + 31) / 32, kAddThreads, 0, s, sums, g.pieces, op->out, op->dbias));
+        beside = sums && g.pieces > 1;
+        if (beside) OP_CK(launch_step(true, add_parts_kernel, (op->out + 31) / 32, kAddThreads, 0, s, sums, g.pieces, op->out, op->dbias));
     }
     const void* gradient = dz ? dz : op->dy;
     const int64_t ld_gradient = dz ? space.ldz : op->lddy;
-    bool dx_alone = false;  // its product is the last kernel so far, and uses no workspace
     if (op->dx) {
         Call c = dx_call(op, gradient, ld_gradient);
         c.follows = dz || sums;
+        c.p.beside = beside && c.a.aligned() && c.b.aligned();
         c.p.gave_up = word;
-        dx_alone = call_bytes(c) == 0;
+        beside = call_bytes(c) == 0;
         if (int rc = run_product(c, base + space.products, s)) return rc;
     }
     if (op->dw) {
         Call c = dw_call(op, gradient, ld_gradient);
         c.follows = dz || sums || op->dx;
-        c.p.beside = dx_alone && c.a.aligned() && c.b.aligned();
+        c.p.beside = beside && c.a.aligned() && c.b.aligned();
         c.p.gave_up = word;
         if (int rc = run_product(c, base + space.products, s)) return rc;
     }
