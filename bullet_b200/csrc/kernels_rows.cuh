@@ -185,11 +185,12 @@ __device__ __forceinline__ void store_typed(void* at, int64_t row_at, int type, 
         store_eight<VEC>(static_cast<f16*>(at) + row_at, first, cols, v);
 }
 // Elements of a row on their way to codes: what an activation's outputs have to keep.  Those above 0 and below the smallest code's
-// value are moved to that, those between the last code below 1 and 1 to that code's value, which is 1 - 2^-4 up to scales of 2^6; then
-// the nearest code is the one that is wanted.  Magnitudes are in the order of their bits: less 1, what is not to move below the
-// least is 0, the largest of all; less 1's bits, what is below 1 comes last.  (131072 x 2048 bf16 outputs of CReLU with
-// comparisons and selections 185 us, with these additions in front of maxima and minima 161, in a kernel of its own 134.)
-__device__ __forceinline__ bool moves_outputs(uint32_t scale) { return scale >= 10u << 23 && scale <= 133u << 23; }
+// value are moved to that, those between the last code below 1 and 1 to that code's value, which is 1 - 2^-4 up to scales of 2^5 (at
+// 2^6 one is the smallest normal code, and the code below it 1 - 2^-3); then the nearest code is the one that is wanted.  Magnitudes
+// are in the order of their bits: less 1, what is not to move below the least is 0, the largest of all; less 1's bits, what is below 1
+// comes last.  (131072 x 2048 bf16 outputs of CReLU with comparisons and selections 185 us, with these additions in front of maxima and
+// minima 161, in a kernel of its own 134.)
+__device__ __forceinline__ bool moves_outputs(uint32_t scale) { return scale >= 10u << 23 && scale <= 132u << 23; }
 __device__ __forceinline__ uint32_t least_bits(uint32_t scale) { return scale - (9u << 23); }
 __device__ __forceinline__ float moved_output(float v, uint32_t least, int act) {
     uint32_t s = __viaddmax_u32(__float_as_uint(v), 0xffffffffu, least - 1u);

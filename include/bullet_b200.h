@@ -441,7 +441,8 @@ int b200_op_rms_norm_backward(int device, void* stream, const b200_rms_norm_grad
  * brings the largest finite magnitude to 448 or below (1 where there is none but 0); codes are the nearest, halves to the
  * even one; infinities and NaN become NaN.  `act` names the activation whose outputs these are: for B200_ACT_RELU, _CRELU
  * and _SCRELU a value above 0 keeps a code above 0, for the latter two a value below 1 one that stands for less than 1, so
- * that the activation's gradient is cut off where it would have been without the rounding.
+ * that the activation's gradient is cut off where it would have been without the rounding (up to scales of 2^8, past which no
+ * code lies between 0 and 1; outputs of _CRELU and _SCRELU have 2^-8 at most).
  * A power of two as scale leaves every value exact in bf16 and fp32, down to their smallest numbers; a value that would round
  * up out of fp32 rounds down. */
 typedef struct b200_pack8_op {

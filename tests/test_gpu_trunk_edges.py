@@ -1,0 +1,49 @@
+"""The dense trunk's operators at the edges of their ranges: scales of every size, what an activation's codes have to keep, waits that gave
+up.  Expected values are the definitions in 64 bits; where a test asks for equality, every value on the way is exact."""
+import pytest
+import torch
+
+from bullet_b200 import ops
+from bullet_b200.configs import ACT_CRELU, ACT_NONE, ACT_RELU, ACT_SCRELU
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16, E4M3 = torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def kept(v, scale, act):
+    """The values of the codes of an activation's outputs `v` at a scale: the nearest (halves to the even one), but above 0 what was above 0,
+    and for outputs that are cut off at 1 below 1 what was below 1.  Scales up to 2^8, past which no code lies between."""
+    codes = torch.arange(127, device=v.device, dtype=torch.uint8).view(E4M3).double()
+    q = (v / scale).float().to(E4M3).double()  # (in fp32 exactly: a power of two)
+    if act != ACT_NONE:
+        q = torch.where((v > 0) & (q == 0), codes[1], q)
+    if act in (ACT_CRELU, ACT_SCRELU):
+        q = torch.where((v > 0) & (v < 1) & (q * scale >= 1), codes[codes * scale < 1].max(), q)
+    return q * scale
+
+
+# Scales 2^e around those at which the codes below 1 and above 0 change places: 2^5 is the last at which 15/16 is a code, 2^-117 the last at
+# which half the smallest code is a normal number.
+@pytest.mark.parametrize("e", [-120, -118, -117, -116, -20, -9, -8, -7, -1, 0, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("act", [ACT_NONE, ACT_CRELU, ACT_SCRELU, ACT_RELU])
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+def test_codes_of_outputs_keep_the_mask_at_every_scale(e, act, kind):
+    if kind is F16 and not -8 <= e <= 7:
+        pytest.skip("past fp16")
+    scale = 2.0 ** e
+    one = torch.tensor(1.0, dtype=kind)
+    last = torch.nextafter(one, one * 0).item()
+    below_one = [1.0, last, 0.999, 0.97, 0.95, 0.94, 0.9375, 0.93, 0.91, 0.9, 0.88, 0.876, 0.875, 0.8, 0.76, 0.75, 0.7, 0.6, 0.51, 0.5, 0.49, 0.3, 0.1]
+    of_scale = [scale * f for f in (2.0 ** -12, 2.0 ** -10, 2.0 ** -9, 1.4 * 2.0 ** -9, 1.5 * 2.0 ** -9, 2.0 ** -6, 0.3, 1.0, 17.3, 239.0, 299.0)]
+    values = torch.tensor([v for v in below_one + of_scale if v < 300 * scale] + [0.0], dtype=torch.float64, device="cuda").to(kind)
+    top = torch.tensor([300 * scale], dtype=torch.float64, device="cuda").to(kind)
+    for cols in (96, 77, 1100, 17000):  # vectors or single elements, one warp or several, rows past registers
+        x = torch.zeros(5, cols, device="cuda", dtype=kind)
+        for r in range(5):
+            x[r, r:r + len(values)] = values
+            x[r, cols - 1] = top[0]
+        want = kept(x.double(), scale, act)
+        p = ops.pack8(x, act=act)
+        assert (p.scale == scale).all() and torch.equal(ops.unpack8(p, F32).double(), want), cols
+        p = ops.pack8(x.t().contiguous(), act=act, by_column=True)
+        assert (p.scale == scale).all() and torch.equal(ops.unpack8(p, F32).t().double(), want), cols
