@@ -14,7 +14,7 @@
 //
 // CODES: a is an 8-bit checkpoint with a scale per k.  Four more warps turn its codes into bf16 on the way from one place in
 // shared memory to another: a power of two as scale makes that exact, so there is no product of other values than those
-// that the checkpoint stands for, and no copy of it in 16 bits in memory.
+// that the checkpoint stands for, and no copy of it in 16 bits in memory.  (With other scales the values are rounded to bf16.)
 #pragma once
 #include "launch.cuh"
 #include "tensor.cuh"
@@ -91,7 +91,7 @@ __device__ __forceinline__ void codes_to_bf16(uint32_t w, __nv_bfloat162 f, uint
     low = t[0], high = t[1];
 }
 __device__ __forceinline__ uint32_t has_nan_code(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }  // & 0x80808080
-// Four codes one by one into memory, for NaN and scales past 2^7.
+// Four codes one by one into memory, rounded to bf16: for NaN, scales past 2^7 and scales that are no powers of two.
 static __device__ __noinline__ void codes_to_bf16_slowly(uint32_t w, float scale, uint32_t* to) {
 #pragma unroll 1
     for (int q = 0; q < 4; q++) reinterpret_cast<bf16*>(to)[q] = __float2bfloat16_rn(to_float(e4m3{(uint8_t)(w >> 8 * q)}) * scale);
@@ -452,11 +452,11 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
 #pragma unroll
                 for (int i = 0; i < 4; i++) code[i] = *reinterpret_cast<const uint4*>(raw + i * 2048);
                 uint32_t nan = 0, v[4][8];
-                bool large = false;
+                bool slow = false;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint32_t e = scale[i] >> 23;
-                    large |= e > 134;
+                    slow |= scale[i] - (1u << 23) > 133u << 23 || (scale[i] & 0x7fffffu);  // (2^-126 to 2^7 are not)
                     const __nv_bfloat162 f = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)((min(e, 134u) + 120u) << 7)));
                     const uint4 c = j >> 2 ? make_uint4(code[i].z, code[i].w, code[i].x, code[i].y) : code[i];
                     nan |= has_nan_code(c.x) | has_nan_code(c.y) | has_nan_code(c.z) | has_nan_code(c.w);
@@ -473,7 +473,7 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
                     *reinterpret_cast<uint4*>(to + i * 2048 + at0) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
                     *reinterpret_cast<uint4*>(to + i * 2048 + at1) = make_uint4(v[i][4], v[i][5], v[i][6], v[i][7]);
                 }
-                if (large || nan & 0x80808080u) {
+                if (slow || nan & 0x80808080u) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};

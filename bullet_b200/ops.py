@@ -30,7 +30,8 @@ _calls.set_library_error(_lib.B200Error)
 
 
 class Packed8(NamedTuple):
-    """Codes of 8 bits and their scales, powers of two: one per row, or with `by_column` one per column."""
+    """Codes of 8 bits and their scales: one per row, or with `by_column` one per column.  The scales that pack8 and rms_norm make are powers
+    of two, which leaves the values exact in bf16; with others dense_backward rounds a checkpoint's values to bf16 for dw."""
 
     codes: torch.Tensor
     scale: torch.Tensor

@@ -390,7 +390,8 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
  *   - a kernel that waits too long for its own copies or products gives up, and the next dense call returns
  *     B200_ERR_STATE;
  *   - a B200_TYPE_E4M3 matrix holds codes of 8 bits (four significand bits, largest value 448, no infinities) and goes with
- *     a scale, a power of two in fp32, per row (or per column, where said): it stands for code * scale. */
+ *     a scale in fp32 per row (or per column, where said): it stands for code * scale.  Scales that these operators make are
+ *     powers of two; others may be given, and dw then takes a checkpoint's values rounded to bf16. */
 #define B200_ACT_RELU 3 /* these operators only; 0 to 2 as above */
 #define B200_TYPE_F32 0
 #define B200_TYPE_BF16 1

@@ -47,3 +47,47 @@ def test_codes_of_outputs_keep_the_mask_at_every_scale(e, act, kind):
         assert (p.scale == scale).all() and torch.equal(ops.unpack8(p, F32).double(), want), cols
         p = ops.pack8(x.t().contiguous(), act=act, by_column=True)
         assert (p.scale == scale).all() and torch.equal(ops.unpack8(p, F32).t().double(), want), cols
+
+
+def near(got, want, absolute):
+    off = (got.double() - want.double()).abs() - absolute
+    assert not torch.isnan(off).any() and off.max() <= 0, float(off.max())
+
+
+def random(seed, *shape):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=g)
+
+
+def of_any_scale(rows, n_in):
+    x, scale = random(1, rows, n_in), torch.exp(random(4, rows))
+    x[4] = 320  # (beside a scale below fp32's normal numbers: the value is a normal one)
+    scale[1], scale[2], scale[3], scale[4] = 0.0, -1.5, 1 + 2.0 ** -23, 2.0 ** -130
+    return x.to(E4M3), scale
+
+
+@pytest.mark.parametrize("rows,n_in,n_out", [(70, 64, 32), (300, 200, 700), (2500, 256, 512)])
+def test_scales_that_are_no_powers_of_two_mean_the_same_to_unpack_and_the_gradients(rows, n_in, n_out):
+    """unpack8 and both gradients take a scale as it is.  The weights' gradient multiplies bf16: each value is rounded by 2^-9 of
+    itself there, which is nothing for powers of two.  Sums as in the other tests: 2^-23 of their magnitudes' sum a term."""
+    (x, scale), y = of_any_scale(rows, n_in), random(7, rows, n_out).abs().clamp(max=1).to(E4M3)
+    w, dy = random(2, n_in, n_out).to(BF16), random(3, rows, n_out).to(BF16)
+    packed = ops.Packed8(x, scale)
+    xv = x.double() * scale.double()[:, None]
+    assert torch.equal(ops.unpack8(packed, F32), (x.float() * scale[:, None]))
+    _, dw, _ = ops.dense_backward(dy, packed, None, need_dx=False)
+    size = xv.abs().t() @ dy.double().abs()
+    near(dw, xv.t() @ dy.double(), size * (2.0 ** -9 + rows * 2.0 ** -23))
+    alone = torch.zeros_like(dy)  # a row at a time
+    for k, row in enumerate((1, 2, 3, 4, 5)):
+        alone[row, k] = 1
+    _, dw, _ = ops.dense_backward(alone, packed, None, need_dx=False)
+    assert torch.equal(dw, (xv.to(BF16).double().t() @ alone.double()).float())
+    # dz is cut off by the value that y stands for
+    sy = torch.exp(random(6, rows))
+    yv = y.double() * sy.double()[:, None]
+    dx, _, db = ops.dense_backward(dy, None, w, y=ops.Packed8(y, sy), act=ACT_CRELU, need_dw=False)
+    dz = torch.where((yv > 0) & ((y.float() * sy[:, None]) < 1), dy.double(), torch.zeros_like(yv))
+    near(db, dz.sum(0), dz.abs().sum(0) * (rows * 2.0 ** -23))
+    near(dx, dz @ w.double().t(), (dz.abs() @ w.double().abs().t()) * (n_out * 2.0 ** -23 + 2.0 ** -8))
