@@ -119,7 +119,7 @@ static __global__ void __launch_bounds__(256) dense_few_kernel(const FewArgs f) 
         if (row >= a.rows || column >= a.out) continue;
         float v = 0.f;
         for (uint32_t k = 0; k < ctas; k++) v += (&pieces[k][0][0])[i];
-        if constexpr (sizeof(T) == 1) v *= a.x_scale[row] * a.w_scale[column];
+        if constexpr (sizeof(T) == 1) v = scaled(v, a.x_scale[row], a.w_scale[column]);
         if (a.bias) v += a.bias[column];
         v = activate(v, a.act);
         if (a.residual) v += load_value(a.residual, row * a.ldr + column, a.y_type);

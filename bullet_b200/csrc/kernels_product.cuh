@@ -97,14 +97,22 @@ static __device__ __noinline__ void codes_to_bf16_slowly(uint32_t w, float scale
     for (int q = 0; q < 4; q++) reinterpret_cast<bf16*>(to)[q] = __float2bfloat16_rn(to_float(e4m3{(uint8_t)(w >> 8 * q)}) * scale);
 }
 
-// 32 sums of a row as whole sums end: scales, bias (of these columns, in shared memory), activation.
+// (one function: 32 times in line it would stand in the way of the usual scales' code)
+static __device__ __noinline__ float scaled_slowly(float v, float a, float b) { return scaled(v, a, b); }
+// 32 sums of a row as whole sums end: scales, bias (of these columns, in shared memory), activation.  `usual`: all products of two
+// scales that the warp meets are normal numbers.
 template <bool BYTES, bool VALUES>
-__device__ __forceinline__ void finish_sums(const ProductArgs& p, float (&v)[32], float a_scale, const float* bias, const float* b_scale) {
+__device__ __forceinline__ void finish_sums(const ProductArgs& p, float (&v)[32], float a_scale, const float* bias, const float* b_scale, bool usual) {
     if constexpr (BYTES) {
+        if (__builtin_expect(usual, 1)) {
 #pragma unroll
-        for (int g = 0; g < 8; g++) {
-            const float4 b = reinterpret_cast<const float4*>(b_scale)[g];
-            v[4 * g] *= a_scale * b.x, v[4 * g + 1] *= a_scale * b.y, v[4 * g + 2] *= a_scale * b.z, v[4 * g + 3] *= a_scale * b.w;
+            for (int g = 0; g < 8; g++) {
+                const float4 b = reinterpret_cast<const float4*>(b_scale)[g];
+                v[4 * g] *= a_scale * b.x, v[4 * g + 1] *= a_scale * b.y, v[4 * g + 2] *= a_scale * b.z, v[4 * g + 3] *= a_scale * b.w;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 32; k++) v[k] = scaled_slowly(v[k], a_scale, b_scale[k]);
         }
     }
     if constexpr (VALUES) {
@@ -332,11 +340,22 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
                 }
             };
             if (adds && p.boxes && own > 0) fetch_residual(0);
+            bool usual = true;
             if constexpr (T::kColumnValues) {
                 __syncwarp();
+                uint32_t least = 0x7f7fffffu, most = 0;  // of the scales, by their bits
                 for (int c = lane; c < T::kOwn; c += 32) {
                     bias[c] = p.bias && c < own ? __ldg(p.bias + own0 + c) : 0.f;
-                    if constexpr (BYTES) b_scale[c] = c < own ? __ldg(p.b_scale + own0 + c) : 0.f;
+                    if constexpr (BYTES) {
+                        const float b = c < own ? __ldg(p.b_scale + own0 + c) : 0.f;
+                        b_scale[c] = b;
+                        const uint32_t size = __float_as_uint(b) & 0x7fffffffu;
+                        if (c < own) least = min(least, size), most = max(most, size);
+                    }
+                }
+                if constexpr (BYTES) {
+                    least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
+                    usual = __all_sync(0xffffffffu, normal(a_scale * __uint_as_float(least)) && normal(a_scale * __uint_as_float(most)));
                 }
                 __syncwarp();
             }
@@ -350,7 +369,7 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
                 for (int c = 0; c < own; c += 32) {
                     float v[32];
                     load_sums32(sums + c, v);
-                    if (!p.parts) finish_sums<BYTES, T::kColumnValues>(p, v, a_scale, bias + c, b_scale + c);
+                    if (!p.parts) finish_sums<BYTES, T::kColumnValues>(p, v, a_scale, bias + c, b_scale + c, usual);
                     if (p.boxes) {
                         const bool starts = c % width == 0, ends = (c + 32) % width == 0 || c + 32 >= own;
                         if (starts) {
@@ -522,7 +541,7 @@ static __global__ void __launch_bounds__(256) join_kernel(const ProductArgs p) {
     for (int k = 0; k < 4; k++) {
         if (n + k >= p.n) return;
         float x = v[k];
-        if (p.b_scale) x *= a_scale * p.b_scale[n + k];
+        if (p.b_scale) x = scaled(x, a_scale, p.b_scale[n + k]);
         if (p.bias) x += p.bias[n + k];
         x = activate(x, p.act);
         if (p.residual) x += load_value(p.residual, m * p.ldr + n + k, p.d_type);

@@ -81,6 +81,15 @@ __device__ __forceinline__ uint32_t scale_bits(uint32_t magnitude) {
 }
 __device__ __forceinline__ float one_over_scale(uint32_t scale) { return __uint_as_float((254u << 23) - scale); }
 
+// A sum of products of codes times both scales.  The scales' product may leave fp32's normal numbers where the result does not (or, for
+// v = 0, become infinite): then the larger scale first, which takes v out of them only if the result is out as well.
+__device__ __forceinline__ bool normal(float v) { return (__float_as_uint(v) & 0x7fffffffu) - 0x800000u < 0x7f000000u; }
+__device__ __forceinline__ float scaled(float v, float a, float b) {
+    const float s = a * b;
+    if (normal(s)) return v * s;
+    return fabsf(a) > fabsf(b) ? v * a * b : v * b * a;
+}
+
 // The code of v / scale: nearest, halves to even, NaN for what is not finite; what would round up out of fp32 (kTopScale) rounds down.
 // For outputs of an activation: what is above 0 stays above 0, what is below 1 stays below 1.
 constexpr uint32_t kTopScale = 247u << 23;  // the largest there is: 256 times that is past fp32

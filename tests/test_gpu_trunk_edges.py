@@ -91,3 +91,27 @@ def test_scales_that_are_no_powers_of_two_mean_the_same_to_unpack_and_the_gradie
     dz = torch.where((yv > 0) & ((y.float() * sy[:, None]) < 1), dy.double(), torch.zeros_like(yv))
     near(db, dz.sum(0), dz.abs().sum(0) * (rows * 2.0 ** -23))
     near(dx, dz @ w.double().t(), (dz.abs() @ w.double().abs().t()) * (n_out * 2.0 ** -23 + 2.0 ** -8))
+
+
+@pytest.mark.parametrize("rows,n_in,n_out", [(3, 64, 40), (8, 1024, 64), (17, 2048, 16), (70, 64, 32), (300, 200, 700), (1000, 96, 520), (2500, 256, 512)])
+def test_dense_at_scales_whose_product_is_out_of_range(rows, n_in, n_out):
+    """Whole numbers in codes, scales of 2^-126 to 2^119: what the scales make of an exact sum, rounded once.  A sum of 0 stays 0."""
+    x, w = (3 * random(11, rows, n_in)).round().clamp(-3, 3), (2 * random(12, n_in, n_out)).round().clamp(-2, 2)
+    x[0] = 0
+    ex, ew = (60 * random(13, rows)).round().clamp(-126, 119), (60 * random(14, n_out)).round().clamp(-126, 119)
+    ex[0], ex[1], ew[0], ew[1] = 119, -126, 119, -126
+    want = (x.double() @ w.double()) * torch.exp2(ex.double())[:, None] * torch.exp2(ew.double())
+    y = ops.dense(ops.Packed8(x.to(E4M3), torch.exp2(ex.double()).float()), ops.Packed8(w.to(E4M3), torch.exp2(ew.double()).float(), True), out_dtype=F32)
+    assert torch.equal(y, want.float())
+
+
+@pytest.mark.parametrize("rows,n_in,n_out", [(70, 64, 32), (300, 200, 700), (2500, 256, 512)])
+def test_dense_takes_scales_that_are_no_powers_of_two(rows, n_in, n_out):
+    x, scale = of_any_scale(rows, n_in)
+    w = random(2, n_in, n_out).to(BF16)
+    packed = ops.Packed8(x, scale)
+    xv = x.double() * scale.double()[:, None]
+    w8 = ops.pack8(w, by_column=True)
+    sw = w8.scale * torch.exp(random(5, n_out))
+    wv = w8.codes.double() * sw.double()
+    near(ops.dense(packed, ops.Packed8(w8.codes, sw, True), out_dtype=F32), xv @ wv, (xv.abs() @ wv.abs()) * (n_in * 2.0 ** -23 + 2.0 ** -20))
