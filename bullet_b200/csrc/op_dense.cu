@@ -242,7 +242,7 @@ int run_product(Call c, char* space, cudaStream_t stream) {
                                 : launch_columns<false, false, false, false>(c, plan.columns, stream);
     if (rc) return rc;
     if (p.parts) {
-        OP_CK(launch_step(true, join_kernel, (unsigned)((p.m * (p.ldp / 4) + 255) / 256), 256, 0, stream, p));
+        OP_CK(launch_step(true, c.bytes() ? join_kernel<true> : join_kernel<false>, (unsigned)((p.m * (p.ldp / 4) + 255) / 256), 256, 0, stream, p));
     }
     return 0;
 }
