@@ -214,6 +214,7 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_proxy_async();
     }
+    if (threadIdx.x == 64 && p.beside) step_takes_over();  // (beside the preparations; the barrier below is behind it)
     if (threadIdx.x == 32) {
         know_map(&a_map);
         know_map(&b_map);
@@ -227,11 +228,10 @@ static __global__ void __launch_bounds__((Tile<BN, PAIR, BYTES, A_ACROSS, B_ACRO
     tensor_fence_after();
     const uint32_t memory = memory_at;
     // (behind the own memory and barriers: what a kernel of the same call left is read from here on; that before the one that it stands
-    // beside has completed, as that one waited for it before it let this one in)
-    if (p.beside)
-        step_lets_in();
-    else
-        step_begin(nullptr);
+    // beside, dz, has completed: dense_dz_kernel -> [joined sums of the bias ->] dx -> dw, and of these the first behind dense_dz_kernel
+    // waits for it before it lets the next one in)
+    if (!p.beside) step_waits();
+    if (threadIdx.x == 32) step_hands_on();
 
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, items = tiles * p.parts_n;
     const int64_t first = blockIdx.x / kCtas, step = gridDim.x / kCtas;

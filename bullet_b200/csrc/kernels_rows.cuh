@@ -535,7 +535,8 @@ static __global__ void __launch_bounds__(kRowThreads) rms_norm_backward_kernel(b
 constexpr int kAddThreads = 1024;
 static __global__ void __launch_bounds__(kAddThreads) add_parts_kernel(const float* parts, int n_parts, int cols, float* out) {
     __shared__ float sums[32][33];
-    step_begin(nullptr);
+    step_waits();
+    if (threadIdx.x == 0) step_hands_on();  // (products of the same call may start beside it)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (c < cols) {

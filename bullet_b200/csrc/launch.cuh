@@ -8,7 +8,10 @@
 // ones), never through the read-only path (__ldg, ld.global.nc, const __restrict__), which wants data that nobody writes from the
 // kernel's first instruction on.  What the kernels before that one wrote is finished by then.
 // A kernel that reads nothing of the kernel before may let its successor in at once and wait (step_waits) at its end: who waits for it
-// then waits for both.
+// then waits for both.  What it reads of kernels further back has to be complete: each kernel in between has waited for its own
+// predecessor, or has been let in by one that had, before it lets anybody in.  Waiting is what makes memory visible, though, and only to
+// the grid that waits; so such chains let in with step_hands_on, and a kernel that starts without waiting takes over (step_takes_over)
+// before it reads.
 // This takes most of the 3 us out of every boundary between two kernels of a step.
 //
 // Time stamps of the phases are written by the first thread of the kernels themselves: an event with timing between two
@@ -26,6 +29,8 @@ __device__ __forceinline__ unsigned long long clock_ns() {
 }
 __device__ __forceinline__ void step_waits() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void step_lets_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void step_hands_on() { asm volatile("fence.acq_rel.gpu;\ngriddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void step_takes_over() { asm volatile("fence.acq_rel.gpu;\nfence.proxy.async.global;" ::: "memory"); }  // (for TMA too)
 // first statement of a step's kernel; `stamp`: where its start time goes, or null
 __device__ __forceinline__ void step_begin(unsigned long long* stamp) {
     step_waits();

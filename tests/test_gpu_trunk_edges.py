@@ -115,3 +115,36 @@ def test_dense_takes_scales_that_are_no_powers_of_two(rows, n_in, n_out):
     sw = w8.scale * torch.exp(random(5, n_out))
     wv = w8.codes.double() * sw.double()
     near(ops.dense(packed, ops.Packed8(w8.codes, sw, True), out_dtype=F32), xv @ wv, (xv.abs() @ wv.abs()) * (n_in * 2.0 ** -23 + 2.0 ** -20))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("rows,n_in,n_out", [(5003, 2048, 1024), (16384, 512, 256), (2000, 512, 512), (700, 256, 2048), (60, 64, 48)])
+def test_all_three_gradients_of_a_call_are_there_for_who_follows(rows, n_in, n_out, packed):
+    """The bias's sums are joined while the products run, and those beside each other: copies right behind a call find what calls
+    for one gradient each give, eagerly and in a graph, also when dz changes from call to call."""
+    act = ACT_CRELU if packed else ACT_SCRELU
+    w = random(21, n_in, n_out).to(BF16)
+    x, y = random(22, rows, n_in).abs().clamp(max=1).to(BF16), random(23, rows, n_out).abs().clamp(max=1).to(BF16)
+    if packed:
+        x, y = ops.pack8(x, act=act), ops.pack8(y, act=act)
+    dys = [random(24 + k, rows, n_out).to(BF16) for k in range(3)]
+    needs = [dict(need_dx=k == 0, need_dw=k == 1, need_dbias=k == 2) for k in range(3)]
+    want = [[ops.dense_backward(dy, x, w, y=y, act=act, **needs[k])[k] for k in range(3)] for dy in dys]
+
+    def one(dy):
+        got = ops.dense_backward(dy, x, w, y=y, act=act)
+        copies = [t.clone() for t in got]
+        for t in got:
+            t.zero_()
+        return copies
+
+    for got in [[one(dy) for dy in dys] for _ in range(4)]:
+        assert all(torch.equal(a, b) for g, v in zip(got, want) for a, b in zip(g, v))
+    dy = dys[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = one(dy)
+    for k in (1, 2, 0, 1):
+        dy.copy_(dys[k])
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
