@@ -388,6 +388,7 @@ extern "C" {
     pub fn b200_op_dense(device: c_int, stream: *mut c_void, op: *const b200_dense_op) -> c_int;
     pub fn b200_op_dense_backward_workspace(op: *const b200_dense_grad_op, bytes: *mut i64) -> c_int;
     pub fn b200_op_dense_backward(device: c_int, stream: *mut c_void, op: *const b200_dense_grad_op) -> c_int;
+    pub fn b200_op_dense_gave_up(device: c_int, word: *mut *mut i32) -> c_int;
 
     pub fn b200_map_chess768(records: *const c_void, n: i32, stm: *mut i32, nstm: *mut i32, nnz: i32) -> c_int;
     pub fn b200_map_chess_buckets_mirrored(

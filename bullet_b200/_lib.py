@@ -26,7 +26,7 @@ SYMBOLS = (
     "b200_grad_zero_range", "b200_batch_upload_records", "b200_set_host_threads", "b200_step_exchange",
     "b200_batch_upload_records_gpu", "b200_slot_read", "b200_probe_bandwidth", "b200_net_set_optimiser",
     "b200_op_rms_norm", "b200_op_rms_norm_backward_workspace", "b200_op_rms_norm_backward", "b200_op_pack8", "b200_op_unpack8",
-    "b200_op_dense_workspace", "b200_op_dense", "b200_op_dense_backward_workspace", "b200_op_dense_backward",
+    "b200_op_dense_workspace", "b200_op_dense", "b200_op_dense_backward_workspace", "b200_op_dense_backward", "b200_op_dense_gave_up",
 )
 
 
@@ -187,6 +187,7 @@ def load() -> ctypes.CDLL:
         "b200_op_dense": [ctypes.c_int, vp, ctypes.POINTER(CDense)],
         "b200_op_dense_backward_workspace": [ctypes.POINTER(CDenseGrad), ctypes.POINTER(i64)],
         "b200_op_dense_backward": [ctypes.c_int, vp, ctypes.POINTER(CDenseGrad)],
+        "b200_op_dense_gave_up": [ctypes.c_int, ctypes.POINTER(ctypes.POINTER(i32))],
         "b200_map_chess768": [vp, i32, vp, vp, i32],
         "b200_map_chess_buckets_mirrored": [vp, i32, vp, vp, vp, i32],
         "b200_map_ataxx147": [vp, i32, vp, vp, i32],

@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbullet_b200.so")
 TENSOR_CALLS = os.path.join(HERE, "_tensor_calls.so")
-SOURCES = ["net.cu", "op_ft_forward.cu", "op_rows.cu", "op_dense.cu", "probe.cu", "host_pack.cpp", "checkpoint.cpp", "saved_format.cpp"]
+SOURCES = ["net.cu", "op_ft_forward.cu", "op_rows.cu", "op_dense.cu", "gave_up.cu", "probe.cu", "host_pack.cpp", "checkpoint.cpp", "saved_format.cpp"]
 
 
 def _nvcc() -> str:

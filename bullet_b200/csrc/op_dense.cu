@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "gave_up.h"
 #include "kernels_few.cuh"
 #include "kernels_product.cuh"
 #include "kernels_rows.cuh"
@@ -11,34 +12,10 @@ namespace {
 
 using namespace b200;
 
-// ---- the host's word for waits that gave up (Waits)
-
-// Memory of the library image that both sides may touch at any time; kernels touch it only if there is something to report.
-static __managed__ int g_gave_up;
-
-// Its address for kernels, or null where the device cannot share such memory while it is running.
-int* gave_up_word(int device) {
-    constexpr int kDevices = 64;
-    static std::atomic<signed char> known[kDevices];  // 0 not asked yet, 1 yes, -1 no
-    if (device < 0 || device >= kDevices) return nullptr;
-    if (known[device] == 0) {
-        int concurrent = 0;
-        if (cudaDeviceGetAttribute(&concurrent, cudaDevAttrConcurrentManagedAccess, device) != cudaSuccess) concurrent = 0;
-        if (concurrent) {  // (hints: the word stays in host memory)
-            cudaMemAdvise(&g_gave_up, sizeof g_gave_up, cudaMemAdviseSetPreferredLocation, cudaCpuDeviceId);
-            cudaMemAdvise(&g_gave_up, sizeof g_gave_up, cudaMemAdviseSetAccessedBy, device);
-        }
-        cudaGetLastError();
-        known[device] = concurrent ? 1 : -1;
-    }
-    return known[device] > 0 ? &g_gave_up : nullptr;
-}
+// A wait of a kernel before that gave up (Waits) is reported by the next call on its device.
 int check_gave_up(const char* who, int* word) {
-    if (word && *reinterpret_cast<volatile int*>(word)) {
-        *reinterpret_cast<volatile int*>(word) = 0;
-        return fail(B200_ERR_STATE, "%s: a kernel of a call before waited too long for its own copies or products; that call's outputs are not valid", who);
-    }
-    return 0;
+    if (!take_gave_up(word)) return 0;
+    return fail(B200_ERR_STATE, "%s: a kernel of a call before on this device waited too long for its own copies or products; that call's outputs are not valid", who);
 }
 
 // ---- products
@@ -423,10 +400,11 @@ int b200_op_dense(int device, void* stream, const b200_dense_op* op) {
     OnDevice on(device);
     OP_CK(on.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int* word = gave_up_word(device);
+    if (int rc = check_gave_up(who, word)) return rc;
     if (few_rows(op)) return packed ? launch_few<e4m3>(op, s) : op->x_type == B200_TYPE_BF16 ? launch_few<bf16>(op, s) : launch_few<f16>(op, s);
     Call c = forward_call(op);
-    c.p.gave_up = gave_up_word(device);
-    if (int rc = check_gave_up(who, c.p.gave_up)) return rc;
+    c.p.gave_up = word;
     return run_product(c, aligned_space(op->workspace), s);
 }
 

@@ -14,6 +14,7 @@ checks and allocations are compiled (csrc/tensor_calls.cpp).
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -91,3 +92,14 @@ def dense_backward(dy, x, w, y=None, act: int = ACT_NONE, dskip=None, dw_dtype=t
     x, x_scale = _of_rows(x, "x")
     y, y_scale = _of_rows(y, "y")
     return _calls.dense_backward(dy, x, x_scale, w, y, y_scale, act, dskip, dw_dtype, need_dx, need_dw, need_dbias)
+
+
+def gave_up(device: int) -> bool:
+    """Whether a wait of dense kernels on a device gave up since this was last asked, or reported by a call: the outputs of what ran
+    there are not valid then.  For programs that replay graphs, behind a synchronisation; other calls report by B200Error."""
+    word = ctypes.POINTER(ctypes.c_int32)()
+    _lib.check(_lib.load().b200_op_dense_gave_up(device, ctypes.byref(word)))
+    if not word or not word[0]:
+        return False
+    word[0] = 0
+    return True

@@ -387,8 +387,9 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
  *     (its addresses and distances count);
  *   - all sums are held in 32 bits and taken in the same order by every call of the same shape and alignment: equal inputs
  *     give equal bits;
- *   - a kernel that waits too long for its own copies or products gives up, and the next dense call returns
- *     B200_ERR_STATE;
+ *   - a dense kernel that waits too long for its own copies or products gives up, which leaves its call's outputs invalid; the
+ *     next call of b200_op_dense or its gradient with rows on the device, whoever makes it, returns B200_ERR_STATE, once, and
+ *     does nothing else.  Programs that replay graphs, or that want to know whose call it was, ask b200_op_dense_gave_up;
  *   - a B200_TYPE_E4M3 matrix holds codes of 8 bits (four significand bits, largest value 448, no infinities) and goes with
  *     a scale in fp32 per row (or per column, where said): it stands for code * scale.  Scales that these operators make are
  *     powers of two; others may be given, and dw then takes a checkpoint's values rounded to bf16. */
@@ -518,6 +519,11 @@ typedef struct b200_dense_grad_op {
 } b200_dense_grad_op;
 int b200_op_dense_backward_workspace(const b200_dense_grad_op* op, int64_t* bytes);
 int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* op);
+
+/* The word that the dense kernels of `device` set to 1 where a wait gave up: host memory that may be read at any time, and set
+ * back to 0, which the call that returns B200_ERR_STATE does as well.  Read behind a synchronisation, it tells of all work
+ * before that, replayed graphs included.  *word is NULL where the device cannot share memory while it is running. */
+int b200_op_dense_gave_up(int device, int32_t** word);
 
 /* ---- bandwidth probes: the measured denominators for kernels whose table stays in L2.  kind 0: every SM
  * reads a buffer of `bytes` bytes `reps` times with 16-byte loads (a buffer well below the L2 size measures L2,

@@ -1,9 +1,11 @@
 """The dense trunk's operators at the edges of their ranges: scales of every size, what an activation's codes have to keep, waits that gave
 up.  Expected values are the definitions in 64 bits; where a test asks for equality, every value on the way is exact."""
+import ctypes
+
 import pytest
 import torch
 
-from bullet_b200 import ops
+from bullet_b200 import _lib, ops
 from bullet_b200.configs import ACT_CRELU, ACT_NONE, ACT_RELU, ACT_SCRELU
 
 pytestmark = pytest.mark.gpu
@@ -148,3 +150,26 @@ def test_all_three_gradients_of_a_call_are_there_for_who_follows(rows, n_in, n_o
         dy.copy_(dys[k])
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
+
+
+def test_a_wait_that_gave_up_is_reported_once_by_the_next_dense_call():
+    """The host sets the word that kernels would."""
+    word = ctypes.POINTER(ctypes.c_int32)()
+    _lib.check(_lib.load().b200_op_dense_gave_up(0, ctypes.byref(word)))
+    few, many, w = random(31, 3, 64).to(BF16), random(32, 300, 64).to(BF16), random(33, 64, 48).to(BF16)
+    dy = random(34, 300, 48).to(BF16)
+    for call in (lambda: ops.dense(few, w), lambda: ops.dense(many, w), lambda: ops.dense_backward(dy, many, w), lambda: ops.dense_backward(dy, many, w, need_dw=False)):
+        call()
+        torch.cuda.synchronize()
+        assert word[0] == 0
+        word[0] = 1
+        assert ops.dense(few[:0], w).shape == (0, 48)  # (no rows: nothing is asked)
+        with pytest.raises(_lib.B200Error) as e:
+            call()
+        assert e.value.code == -2 and "not valid" in str(e.value) and word[0] == 0
+        call()
+    assert not ops.gave_up(0)
+    word[0] = 1
+    assert ops.gave_up(0) and not ops.gave_up(0)
+    ops.dense(few, w)
+    assert _lib.load().b200_op_dense_gave_up(0, None) == -1
