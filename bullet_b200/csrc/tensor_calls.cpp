@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -56,7 +57,11 @@ bool among(at::ScalarType t, Types types) {
 using Tensor = const at::Tensor&;
 at::Tensor tensor(PyObject* o, const char* what) {
     if (!THPVariable_Check(o)) refuse(std::string(what) + ": a tensor is wanted");
-    return THPVariable_Unpack(o);
+    Tensor t = THPVariable_Unpack(o);
+    // (the outputs have no history: a weight would stay where it is without a word)
+    if (t.requires_grad() && at::GradMode::is_enabled())
+        refuse(std::string(what) + ": requires a gradient, which these calls do not record: take the *_backward calls, under torch.no_grad() or in an autograd.Function");
+    return t;
 }
 std::optional<at::Tensor> maybe_tensor(PyObject* o, const char* what) {
     if (o == Py_None) return std::nullopt;

@@ -102,3 +102,18 @@ def test_tensor_calls_name_what_is_wrong():
         ops.dense(ops.Packed8(x, x), x)
     with pytest.raises(ValueError, match="dy: "):
         ops.dense_backward(x, x, x)
+
+
+def test_tensors_whose_gradient_would_be_lost_are_refused():
+    torch = pytest.importorskip("torch")
+    from bullet_b200 import ops
+
+    x, w = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(8, 8, dtype=torch.bfloat16, requires_grad=True)
+    of_w = w * 2
+    for call in (lambda: ops.rms_norm(w), lambda: ops.rms_norm(x, torch.ones(8, requires_grad=True)), lambda: ops.rms_norm(x, residual=of_w), lambda: ops.dense(x, w),
+                 lambda: ops.dense(of_w, x), lambda: ops.pack8(w), lambda: ops.dense_backward(x, x, w), lambda: ops.rms_norm_backward(x, of_w, x),
+                 lambda: ops.unpack8(ops.Packed8(x, torch.ones(4, requires_grad=True)))):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="a matrix on a CUDA device is wanted|this type is not taken here"):  # (on to the next check)
+            call()
