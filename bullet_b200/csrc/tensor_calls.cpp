@@ -20,7 +20,7 @@
 
 namespace {
 
-PyObject* library_error = nullptr;  // bullet_b200._lib.B200Error
+PyObject *library_error = nullptr, *memory_error = nullptr;  // bullet_b200._lib.B200Error, torch.OutOfMemoryError
 
 // What ends a call with a Python exception, which is set already.
 struct Raised {};
@@ -314,14 +314,21 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return Call(args);
     } catch (const Raised&) {
         return nullptr;
-    } catch (const std::exception& e) {  // torch's own, out of memory among them
+    } catch (const c10::OutOfMemoryError& e) {
+        PyErr_SetString(memory_error, e.what());
+        return nullptr;
+    } catch (const std::exception& e) {  // torch's other ones
         PyErr_SetString(PyExc_RuntimeError, e.what());
         return nullptr;
     }
 }
-PyObject* set_library_error(PyObject*, PyObject* cls) {
-    Py_INCREF(cls);
-    Py_XSETREF(library_error, cls);
+PyObject* set_errors(PyObject*, PyObject* args) {
+    PyObject *library, *memory;
+    if (!PyArg_ParseTuple(args, "OO", &library, &memory)) return nullptr;
+    Py_INCREF(library);
+    Py_XSETREF(library_error, library);
+    Py_INCREF(memory);
+    Py_XSETREF(memory_error, memory);
     Py_RETURN_NONE;
 }
 
@@ -332,7 +339,7 @@ PyMethodDef methods[] = {B200_ENTRY(rms_norm, 5),
                          B200_ENTRY(unpack8, 4),
                          B200_ENTRY(dense, 8),
                          B200_ENTRY(dense_backward, 12),
-                         {"set_library_error", set_library_error, METH_O, nullptr},
+                         {"set_errors", set_errors, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -9,9 +9,9 @@
 
 Weights are [in, out], which is the networks' column-major out x in matrix.  Matrices may have any distance between rows, the
 elements of a row are consecutive.  Calls enqueue on torch's current stream of their tensors' device and do not wait; new
-tensors come from torch's allocator.  Arguments that do not fit raise ValueError, what the library refuses B200Error.
-Nothing is recorded for autograd: gradients are the *_backward calls', and a tensor that requires one is refused while torch
-records.  The checks and allocations are compiled (csrc/tensor_calls.cpp).
+tensors come from torch's allocator.  Arguments that do not fit raise ValueError, what the library refuses B200Error, want of
+memory torch.OutOfMemoryError.  Nothing is recorded for autograd: gradients are the *_backward calls', and a tensor that requires
+one is refused while torch records.  The checks and allocations are compiled (csrc/tensor_calls.cpp).
 """
 from __future__ import annotations
 
@@ -28,7 +28,7 @@ try:
     from . import _tensor_calls as _calls
 except ImportError as e:
     raise ImportError(f"bullet_b200._tensor_calls is missing or not built for this torch: build it with `python -m bullet_b200.build` ({e})") from e
-_calls.set_library_error(_lib.B200Error)
+_calls.set_errors(_lib.B200Error, torch.OutOfMemoryError)
 
 
 class Packed8(NamedTuple):

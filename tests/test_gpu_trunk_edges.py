@@ -173,3 +173,11 @@ def test_a_wait_that_gave_up_is_reported_once_by_the_next_dense_call():
     assert ops.gave_up(0) and not ops.gave_up(0)
     ops.dense(few, w)
     assert _lib.load().b200_op_dense_gave_up(0, None) == -1
+
+
+def test_want_of_memory_is_torchs_error():
+    """A result of 1 TB, which the allocator refuses at once: callers that catch torch's error go on with less."""
+    x, w = torch.zeros(1 << 20, 16, device="cuda", dtype=BF16), torch.zeros(16, 1 << 19, device="cuda", dtype=BF16)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.dense(x, w)
+    assert (ops.dense(x[:100], w[:, :64]) == 0).all()
