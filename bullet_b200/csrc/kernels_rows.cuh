@@ -288,7 +288,10 @@ __device__ __forceinline__ float root_of_mean(double mean, float& rest) {
 }
 // t * rstd * w in fp32 may round onto a halfway point of two codes or across it: one code in 10^6 came out as its neighbour.  A
 // product within two units of one (bits 19 to 0 of the significand near 0x80000) is formed again: the fp32 number next to the exact one
-// towards 0, with its last bit set where it is not exact itself, so that it lies on the right side.
+// towards 0, with its last bit set where it is not exact itself, so that it lies on the right side.  So the roundings of rstd and of both
+// products move no code.  What still may: the sum of squares, which is an fp32 sum, and all of them for codes below the smallest
+// normal one (2^-6 of the scale), whose halfway points lie elsewhere.  100 M codes of fp32 rows of 2048: 18 neighbours of the nearest,
+// without this 60; 16384 of those rows 37.6 us, without this 33.8.
 __device__ __forceinline__ bool near_halfway(float y) { return (__float_as_uint(y) - 0x7fffeu) * 4096u < 5u * 4096u; }
 template <class TX>
 static __device__ __noinline__ float exact_for_code(const TX* x, const TX* residual, const float* weight, float rstd, float rest) {
@@ -549,7 +552,7 @@ static __global__ void __launch_bounds__(kAddThreads) add_parts_kernel(const flo
     if (lane == 0 && blockIdx.x * 32 + warp < cols) out[blockIdx.x * 32 + warp] = v;
 }
 
-// ---- rows of any length: a CTA of eight warps per row, element by element
+// ---- rows of any length: a CTA of eight warps per row, element by element (a norm's codes are those of its fp32 products here)
 
 __device__ __forceinline__ float cta_sum(float v, float* shared) {
     v = row_sum(v, kRowWarpsMost, shared);

@@ -401,7 +401,9 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
 
 /* sum = x + residual; rstd = 1 / sqrt(mean(sum^2) + eps); y = sum * rstd * weight, per row.  The norm is taken of the sum
  * before that is rounded to x_type.  y in 8 bits: each row's scale is the smallest power of two from 2^-126 on that brings
- * the row's largest magnitude to 448 or below. */
+ * the row's largest magnitude to 448 or below, and codes are the nearest of y.  The sum of squares is held in 32 bits, which moves a
+ * code in 10^6 or fewer to its neighbour; the roundings behind it move none (but for values below 2^-6 of the scale, and in rows
+ * of more than 16384). */
 typedef struct b200_rms_norm_op {
     int32_t rows, cols;
     int32_t x_type;        /* B200_TYPE_F32, _BF16 or _F16: of x, residual and sum */

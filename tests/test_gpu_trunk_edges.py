@@ -181,3 +181,30 @@ def test_want_of_memory_is_torchs_error():
     with pytest.raises(torch.OutOfMemoryError):
         ops.dense(x, w)
     assert (ops.dense(x[:100], w[:, :64]) == 0).all()
+
+
+@pytest.mark.parametrize("cols", [96, 777, 2048, 8192])
+@pytest.mark.parametrize("kind,with_residual", [(F32, False), (F32, True), (BF16, True), (F16, False)])
+def test_roundings_of_a_norms_product_move_no_code(cols, kind, with_residual):
+    """Whole numbers, whose squares add up exactly, and weights that put every product next to a halfway point between two codes (normal
+    ones): the code is that of total * rstd * weight before any rounding of the two products and of rstd."""
+    rows, eps = 64, 2.0 ** -10
+    g = torch.Generator(device="cuda")
+    g.manual_seed(cols)
+    sizes = torch.tensor([1.0, 2.0, 4.0, 8.0], device="cuda")[torch.randint(0, 4, (1, cols), device="cuda", generator=g)].expand(rows, cols)
+    total = (sizes.gather(1, torch.rand(rows, cols, device="cuda", generator=g).argsort(1)) * (2 * torch.randint(0, 2, (rows, cols), device="cuda", generator=g) - 1)).double()
+    rstd = 1 / torch.sqrt(total[0].square().mean() + eps)  # of every row: they are in another order only
+    halfway = (8.5 + torch.randint(0, 8, (cols,), device="cuda", generator=g).double()) * torch.exp2(torch.randint(-2, 1, (cols,), device="cuda", generator=g).double())
+    w = (halfway / rstd).float()
+    r = torch.randint(-4, 5, (rows, cols), device="cuda", generator=g).to(kind) if with_residual else None
+    x = (total if r is None else total - r.double()).to(kind)
+    y, _, got_rstd = ops.rms_norm(x, w, residual=r, eps=eps, out_dtype=E4M3)
+    assert torch.equal(got_rstd, rstd.float().expand(rows))
+    want = total * rstd * w.double()
+    code = want.abs() / y.scale.double()[:, None]  # at least 2^-6: normal codes
+    step = torch.exp2(torch.floor(torch.log2(code)) - 3)
+    assert (y.scale.double() >= want.abs().amax(1) / 448).all() and (y.scale.double() < want.abs().amax(1) / 224).all() and code.min() >= 2.0 ** -6
+    clear = ((code / step).frac() - 0.5).abs() > 2.0 ** -45  # (where 64 bits tell on which side it lies)
+    assert clear.float().mean() > 0.95
+    nearest = torch.round(code / step) * step * want.sign()
+    assert torch.equal(y.codes.double()[clear], nearest[clear])
