@@ -11,6 +11,9 @@
 namespace b200 {
 
 constexpr int kFewColumns = 64, kFewAhead = 8, kFewStep = 32, kFewChunk = kFewAhead * kFewStep;  // of k: by one load of all threads, by eight
+// Up to eight rows: sixteen would not fit in 48 KB of shared memory, and at eight the tiles of kernels_product.cuh come near.  1 / 2 / 4 / 8
+// rows here and there, us: 2048 -> 1024 3.6 / 3.9 / 5.4 / 7.9 and 8.4, 512 -> 512 3.2 / 3.6 / 4.2 / 5.2 and 6.8, 512 -> 2048 3.5 / 4.0 / 5.0 /
+// 7.0 and 6.9, 2048 -> 16 3.4 / 3.7 / 4.6 / 5.7 and 7.5; in 8 bits 2048 -> 1024 3.8 / 4.3 / 5.5 / 7.4 and 8.2.
 constexpr int kFewRowsMost = 8, kFewClusterMost = 8;
 
 struct FewArgs {

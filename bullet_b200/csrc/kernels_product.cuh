@@ -8,11 +8,12 @@
 //
 // A CTA (or, PAIR, a pair of two SMs that share a tile of 256 rows and each fetch half of its columns) takes items, a tile of
 // the result times a piece of k, one after another.  One thread has TMA fetch boxes of 128 bytes by rows, with the 128-byte
-// swizzle, into a ring of stages; one issues the products of a stage as it arrives, with sums in tensor memory; eight warps take
-// finished sums out, a thread a row, while the products of the next item go to the other half of tensor memory, and hand them to
-// TMA in boxes of 32 rows of 128 bytes, in which the residual lies already.  With k cut (`parts`) the pieces' sums go to memory in fp32 and join_kernel adds them up in order.
+// swizzle, into a ring of stages; one issues the products of a stage as it arrives, with sums in tensor memory; kTakers warps take
+// finished sums out, a thread a row, while the products of the next item go to the other half of tensor memory (tiles of 512 columns
+// fill all of it, and their products wait), and hand them to TMA in boxes of 32 rows of 128 bytes, in which the residual lies already.
+// With k cut (`parts`) the pieces' sums go to memory in fp32 and join_kernel adds them up in order.
 //
-// CODES: a is an 8-bit checkpoint with a scale per k.  Four more warps turn its codes into bf16 on the way from one place in
+// CODES: a is an 8-bit checkpoint with a scale per k.  Twelve more warps (kGroups of four) turn its codes into bf16 on the way from one place in
 // shared memory to another: a power of two as scale makes that exact, so there is no product of other values than those
 // that the checkpoint stands for, and no copy of it in 16 bits in memory.  (With other scales the values are rounded to bf16.)
 #pragma once

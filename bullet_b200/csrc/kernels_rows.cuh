@@ -1,10 +1,11 @@
 // Kernels over the rows of a matrix: root-mean-square norm and its gradient, 8-bit packing.
 //
-// All of them are bound by HBM where there are many rows, by latency where there are few.  A row is read once: W warps hold it in
+// With many rows all of them are bound by HBM but the norm to 8 bits, whose work per element shows beside it (16384 fp32 rows of 2048 37.6 us
+// for 25.6 of traffic, 131072 bf16 rows with residual 306 for 287); with few rows latency counts.  A row is read once: W warps hold it in
 // registers, NV vectors of eight elements a lane, from its first load to the last store, so that the norm's sum, the largest
-// magnitude for the scale and the codes cost no second pass.  One warp takes up to 2048 columns by itself (no barrier anywhere, 16
-// loads of 16 bytes a lane in flight with a residual); wider rows, and narrower ones when there are too few rows for a warp each to
-// fill the GPU, are shared by the warps of a CTA.  A vector's elements lie side by side where rows start on 16 bytes, else 32 apart, so that
+// magnitude for the scale and the codes cost no second pass.  One warp takes up to 2048 columns by itself in packing, 1024 in a norm of
+// 16 bits, 512 in one of fp32 and in the gradient (no barrier anywhere); wider rows, and narrower ones when there are too few rows for a
+// warp each to fill the GPU, are shared by the warps of a CTA.  A vector's elements lie side by side where rows start on 16 bytes, else 32 apart, so that
 // loads of single elements are coalesced.  Rows that do not fit in registers are taken by the *_any_ kernels, a CTA per row,
 // in passes over L2.
 #pragma once

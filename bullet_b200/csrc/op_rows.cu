@@ -23,7 +23,8 @@ struct RowShape {
 // A lane takes `best` vectors where the row has them, so that a warp has 4 KB on their way and registers for many warps; wider rows have
 // more warps, up to kRowWarpsMost, then more vectors.  With fewer rows than the GPU has warps to spare (kFewRows) a row is shared out, a vector a lane.
 // Measured, us: norm with residual to 8 bits, 131072 x 2048 bf16, of 8 / 4 / 2 vectors 328 / 290 / 349; fp32 without residual 300 / 278 /
-// 259; gradient of 131072 x 2048 bf16 rows, of 4 / 2 / 1 505 / 405 / 614.
+// 259; gradient of 131072 x 2048 bf16 rows, of 4 / 2 / 1 505 / 405 / 614.  Norm to 8 bits of 592 rows of 2048 shared out 3.5, as above 4.5; of
+// 1000 rows 5.3 and 4.9, of 2300 rows 9.1 and 8.3; of rows of 520 3.0 and 3.7, 3.3 and 3.9, 4.5 and 4.4.
 constexpr int kFewRows = 148 * 4;
 RowShape row_shape(int64_t rows, int cols, int best, bool several) {
     RowShape s;
@@ -101,8 +102,9 @@ int check_norm_grad(const b200_rms_norm_grad_op* op, const char* who) {
     return 0;
 }
 
-// CTAs of the gradient, each of which leaves a row of sums.
-constexpr int kGradCtas = 2;  // per SM
+// CTAs of the gradient per SM, each of which leaves a row of sums: as many as run at once.  Of 1 / 2 / 3 / 4, us: 5003 x 520 bf16 13.6 / 10.7 /
+// 14.3 / 12.9, 5003 x 1024 14.1 / 11.8 / 15.7 / 14.5, 131072 x 1024 fp32 344 / 231 / 282 / 234, 131072 x 2048 bf16 470 / 310 / 390 / 314.
+constexpr int kGradCtas = 2;
 int norm_grad_ctas(const b200_rms_norm_grad_op* op) {
     if (op->cols > kGradCols) return pieces(op->rows, op->cols, kRowThreads, 4);
     const RowShape g = grad_shape(op->rows, op->cols);

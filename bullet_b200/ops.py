@@ -76,7 +76,8 @@ def unpack8(packed: Packed8, dtype=torch.bfloat16):
 
 def dense(x, w, bias=None, act: int = ACT_NONE, residual=None, out_dtype=None):
     """act(x @ w + bias) + residual.  x and w: matrices of one 16-bit type, or both Packed8 (w by column).  `out_dtype`: fp32 or 16
-    bits; default x's type, bf16 for codes."""
+    bits; default x's type, bf16 for codes.  dense_backward wants act(x @ w + bias) by itself: to train a layer that has both, call
+    without the residual, and add it behind (rms_norm does, on its way)."""
     x, x_scale = _of_rows(x, "x")
     w_scale = None
     if w.__class__ is Packed8:
@@ -89,7 +90,9 @@ def dense(x, w, bias=None, act: int = ACT_NONE, residual=None, out_dtype=None):
 def dense_backward(dy, x, w, y=None, act: int = ACT_NONE, dskip=None, dw_dtype=torch.float32, need_dx: bool = True, need_dw: bool = True,
                    need_dbias: bool = True):
     """(dx, dw, dbias) of act(x @ w + bias); None for what is not needed.  x and y (the layer's output before a residual; not
-    needed with ACT_NONE) are matrices of dy's type or 8-bit checkpoints; dskip is added to dx."""
+    needed with ACT_NONE) are matrices of dy's type or 8-bit checkpoints; dskip is added to dx.  The gradient at the pre-activation
+    enters both products in dy's type: behind ACT_SCRELU it is rounded to 16 bits (2^-9 of itself in bf16), also where dw is fp32;
+    dbias is of the values before that."""
     x, x_scale = _of_rows(x, "x")
     y, y_scale = _of_rows(y, "y")
     return _calls.dense_backward(dy, x, x_scale, w, y, y_scale, act, dskip, dw_dtype, need_dx, need_dw, need_dbias)

@@ -380,7 +380,9 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
  *   - they only enqueue on `stream` (NULL = the default stream), allocate nothing, leave the thread's current device as it
  *     was and may be captured into a graph (each once outside a capture before); memory of theirs is the caller's until the stream has passed the call;
  *   - matrices have rows of consecutive elements; `ld*` is the distance of two rows in elements, at least their length.
- *     Any ld and any address aligned to the element will do; 16-byte aligned rows are faster.  Indices are 64-bit;
+ *     Any ld and any address aligned to the element will do.  Faster are, in products, rows that start on 16 bytes; over rows
+ *     (norm, packing, dz) multiples of eight columns in rows that start on eight elements (fp32: 32 bytes), with a norm's
+ *     weight on 32 bytes: all matrices of a call, or its rows are read element by element.  Indices are 64-bit;
  *   - no rows: nothing is done (gradients of weights become 0) and B200_OK returned;
  *   - outputs overlap neither inputs nor one another;
  *   - scratch is lent by the caller: b200_op_*_workspace says how many bytes the very operation needs that is then called
@@ -471,7 +473,8 @@ typedef struct b200_unpack8_op {
 } b200_unpack8_op;
 int b200_op_unpack8(int device, void* stream, const b200_unpack8_op* op);
 
-/* y = act(x W + bias) + residual for rows of `in` inputs.  W is column-major out x in like the weights of a network:
+/* y = act(x W + bias) + residual for rows of `in` inputs (a layer with both that is to be trained is called without the residual, as its
+ * gradient wants act(x W + bias) by itself).  W is column-major out x in like the weights of a network:
  * w[i * ldw + o].  x and W are both bf16, both fp16, or both codes of 8 bits, x with a scale per row, W with one per output
  * (b200_op_pack8 with by_column). */
 typedef struct b200_dense_op {
@@ -509,7 +512,7 @@ typedef struct b200_dense_grad_op {
     const void* dy;        /* [rows][out] */
     const void* x;         /* [rows][in]; may be NULL without dw */
     const float* x_scale;  /* [rows], x_type E4M3 only */
-    const void* y;         /* [rows][out]; may be NULL with B200_ACT_NONE */
+    const void* y;         /* [rows][out]: act(x W + bias), without a residual; may be NULL with B200_ACT_NONE */
     const float* y_scale;  /* [rows], y_type E4M3 only */
     const void* w;         /* [in][out] as above; may be NULL without dx */
     const void* dskip;     /* [rows][in], or NULL */
