@@ -20,12 +20,15 @@ int* gave_up_word(int device) {
     static std::atomic<signed char> known[kDevices];  // 0 not asked yet, 1 yes, -1 no
     if (device < 0 || device >= kDevices) return nullptr;
     if (known[device] == 0) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (the first call may be one that a stream captures)
+        cudaThreadExchangeStreamCaptureMode(&mode);
         int concurrent = 0;
         if (cudaDeviceGetAttribute(&concurrent, cudaDevAttrConcurrentManagedAccess, device) != cudaSuccess) concurrent = 0;
         if (concurrent) {  // (hints: the words stay in host memory)
             cudaMemAdvise(g_gave_up, sizeof g_gave_up, cudaMemAdviseSetPreferredLocation, cudaCpuDeviceId);
             cudaMemAdvise(g_gave_up, sizeof g_gave_up, cudaMemAdviseSetAccessedBy, device);
         }
+        cudaThreadExchangeStreamCaptureMode(&mode);
         cudaGetLastError();
         known[device] = concurrent ? 1 : -1;
     }

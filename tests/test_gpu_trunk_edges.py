@@ -1,6 +1,9 @@
 """The dense trunk's operators at the edges of their ranges: scales of every size, what an activation's codes have to keep, waits that gave
 up.  Expected values are the definitions in 64 bits; where a test asks for equality, every value on the way is exact."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -208,3 +211,24 @@ def test_roundings_of_a_norms_product_move_no_code(cols, kind, with_residual):
     assert clear.float().mean() > 0.95
     nearest = torch.round(code / step) * step * want.sign()
     assert torch.equal(y.codes.double()[clear], nearest[clear])
+
+
+FIRST_CALL = """
+import sys
+import torch
+from bullet_b200 import ops
+x, w = torch.ones(int(sys.argv[1]), 64, device="cuda").bfloat16(), torch.ones(64, 48, device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.dense(x, w)
+graph.replay()
+assert (y == 64).all()
+"""
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_the_first_dense_call_of_a_process_may_be_captured(rows):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL, str(rows)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
