@@ -41,7 +41,7 @@ struct ProductArgs {
     void* d;
     int64_t ldd;
     int d_type, act;
-    int boxes;     // rows of d and of the residual start on 16 bytes: TMA takes them; else element by element
+    int boxes;     // rows of d start and end on 16 bytes, those of the residual start on them: TMA takes them; else element by element
     float* parts;  // [parts_n][m][ldp], ldp = n up to a multiple of 8; null: none, there is one part of one chain
     int64_t ldp;
     int* gave_up;

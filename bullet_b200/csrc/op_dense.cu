@@ -211,7 +211,8 @@ int run_product(Call c, char* space, cudaStream_t stream) {
     p.form_type = c.b.type == B200_TYPE_BF16;
     const int size = type_bytes(p.d_type);
     auto starts = [&](const void* at, int64_t ld) { return (uintptr_t)at % 16 == 0 && (p.m == 1 || ld * size % 16 == 0); };
-    p.boxes = p.parts || (starts(p.d, p.ldd) && (!p.residual || starts(p.residual, p.ldr)));
+    // (rows end on 16 bytes as well: boxes that were cut off inside 16 bytes wrote into what lies behind the row)
+    p.boxes = p.parts || (p.n * size % 16 == 0 && starts(p.d, p.ldd) && (!p.residual || starts(p.residual, p.ldr)));
     const int rc = c.bytes()    ? launch_columns<true, false, true, false>(c, plan.columns, stream)
                    : c.codes    ? launch_columns<false, true, true, true>(c, plan.columns, stream)
                    : c.a_across ? launch_columns<false, true, true, false>(c, plan.columns, stream)

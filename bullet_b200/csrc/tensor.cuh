@@ -73,7 +73,7 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, in
                      : "memory");
 }
 
-// Boxes of a stack of matrices; what lies outside is 0, and not written.
+// Boxes of a stack of matrices; what lies outside is 0, and not written if the matrix's rows end on 16 bytes.
 __device__ __forceinline__ void load_box3(uint32_t to, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y),
                  "r"(z), "r"(bar)

@@ -232,3 +232,60 @@ def test_the_first_dense_call_of_a_process_may_be_captured(rows):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", FIRST_CALL, str(rows)], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
+
+
+class Inside:
+    """A matrix inside a larger buffer of `fill`: `at` elements behind its start, `pad` more elements a row."""
+
+    def __init__(self, rows, cols, kind, at, pad, fill):
+        self.raw = torch.full((at + rows * (cols + pad) + 64,), fill, device="cuda").to(kind)
+        self.ld, self.address = cols + pad, self.raw.data_ptr() + at * self.raw.element_size()
+        self.view = self.raw[at:at + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+
+    @classmethod
+    def of(cls, t, at, pad):
+        m = cls(*t.shape, t.dtype, at, pad, float("nan"))
+        m.view.copy_(t)
+        return m
+
+    def taken(self, fill):
+        """Its values; everything around it has to be `fill`."""
+        v = self.view.clone()
+        self.view.fill_(fill)
+        assert (self.raw == fill).all()
+        return v
+
+
+# Rows that start on 16 bytes and end inside 16, in and out, of one row and of more
+@pytest.mark.parametrize("rows,n_in,n_out", [(1, 23, 7), (1, 2, 549), (9, 7, 1), (40, 23, 331), (300, 517, 23), (2000, 9, 70)])
+@pytest.mark.parametrize("dw_kind", [F32, BF16])
+def test_what_lies_behind_rows_that_end_inside_16_bytes(rows, n_in, n_out, dw_kind):
+    def pad(cols, kind):  # to the next 16 bytes, and 16 more
+        each = 8 if kind is BF16 else 4
+        return -cols % each + each
+
+    x, w = random(41, rows, n_in).mul(2).round().clamp(-3, 3).to(BF16), random(42, n_in, n_out).round().clamp(-2, 2).to(BF16)
+    dy = random(43, rows, n_out).round().clamp(-1, 1).to(BF16)
+    mx, mw, mdy = (Inside.of(t, 8, pad(t.shape[1], BF16)) for t in (x, w, dy))
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    code = {F32: 0, BF16: 1}
+
+    def run(op, size, call):
+        need = ctypes.c_int64()
+        _lib.check(size(ctypes.byref(op), ctypes.byref(need)))
+        space = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+        op.workspace, op.workspace_bytes = space.data_ptr(), need.value
+        _lib.check(call(0, stream, ctypes.byref(op)))
+
+    for kind in (F32, BF16):
+        y = Inside(rows, n_out, kind, 8, pad(n_out, kind), 77.0)
+        op = _lib.CDense(rows, n_in, n_out, 1, code[kind], 0, mx.ld, mw.ld, 0, y.ld, mx.address, None, mw.address, None, None, None, y.address)
+        run(op, lib.b200_op_dense_workspace, lib.b200_op_dense)
+        assert torch.equal(y.taken(77.0), (x.double() @ w.double()).to(kind))
+    dx, dw = Inside(rows, n_in, BF16, 8, pad(n_in, BF16), 77.0), Inside(n_in, n_out, dw_kind, 8, pad(n_out, dw_kind), 77.0)
+    db = torch.empty(n_out, device="cuda")
+    op = _lib.CDenseGrad(rows, n_in, n_out, 1, 1, 1, code[dw_kind], 0, mdy.ld, mx.ld, 0, mw.ld, 0, dx.ld, dw.ld, mdy.address, mx.address, None, None, None, mw.address, None, dx.address,
+                         dw.address, db.data_ptr())
+    run(op, lib.b200_op_dense_backward_workspace, lib.b200_op_dense_backward)
+    assert torch.equal(dx.taken(77.0), (dy.double() @ w.double().t()).to(BF16)) and torch.equal(dw.taken(77.0), (x.double().t() @ dy.double()).to(dw_kind))
+    assert torch.equal(db.double(), dy.double().sum(0))
