@@ -195,6 +195,55 @@ pub struct b200_unpack8_op {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct b200_pack4_op {
+    pub rows: i32,
+    pub cols: i32,
+    pub x_type: i32,
+    pub by_column: i32,
+    pub ldx: i64,
+    pub ldq: i64,
+    pub x: *const c_void,
+    pub q: *mut c_void,
+    pub scale: *mut u8,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_unpack4_op {
+    pub rows: i32,
+    pub cols: i32,
+    pub y_type: i32,
+    pub by_column: i32,
+    pub ldq: i64,
+    pub ldy: i64,
+    pub q: *const c_void,
+    pub scale: *const u8,
+    pub y: *mut c_void,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_dense4_op {
+    pub rows: i32,
+    pub r#in: i32,
+    pub out: i32,
+    pub y_type: i32,
+    pub act: i32,
+    pub ldx: i64,
+    pub ldw: i64,
+    pub ldr: i64,
+    pub ldy: i64,
+    pub x: *const c_void,
+    pub x_scale: *const u8,
+    pub w: *const c_void,
+    pub w_scale: *const u8,
+    pub bias: *const f32,
+    pub residual: *const c_void,
+    pub y: *mut c_void,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct b200_dense_op {
     pub rows: i32,
     pub r#in: i32,
@@ -388,6 +437,9 @@ extern "C" {
     pub fn b200_op_dense(device: c_int, stream: *mut c_void, op: *const b200_dense_op) -> c_int;
     pub fn b200_op_dense_backward_workspace(op: *const b200_dense_grad_op, bytes: *mut i64) -> c_int;
     pub fn b200_op_dense_backward(device: c_int, stream: *mut c_void, op: *const b200_dense_grad_op) -> c_int;
+    pub fn b200_op_pack4(device: c_int, stream: *mut c_void, op: *const b200_pack4_op) -> c_int;
+    pub fn b200_op_unpack4(device: c_int, stream: *mut c_void, op: *const b200_unpack4_op) -> c_int;
+    pub fn b200_op_dense4(device: c_int, stream: *mut c_void, op: *const b200_dense4_op) -> c_int;
     pub fn b200_op_dense_gave_up(device: c_int, word: *mut *mut i32) -> c_int;
 
     pub fn b200_map_chess768(records: *const c_void, n: i32, stm: *mut i32, nstm: *mut i32, nnz: i32) -> c_int;

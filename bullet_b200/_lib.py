@@ -27,6 +27,7 @@ SYMBOLS = (
     "b200_batch_upload_records_gpu", "b200_slot_read", "b200_probe_bandwidth", "b200_net_set_optimiser",
     "b200_op_rms_norm", "b200_op_rms_norm_backward_workspace", "b200_op_rms_norm_backward", "b200_op_pack8", "b200_op_unpack8",
     "b200_op_dense_workspace", "b200_op_dense", "b200_op_dense_backward_workspace", "b200_op_dense_backward", "b200_op_dense_gave_up",
+    "b200_op_pack4", "b200_op_unpack4", "b200_op_dense4",
 )
 
 
@@ -88,6 +89,24 @@ class CDenseGrad(ctypes.Structure):
 
     _fields_ = _fields("rows in_ out dy_type x_type y_type dw_type act", "lddy ldx ldy ldw ldskip lddx lddw",
                        "dy x x_scale y y_scale w dskip dx dw dbias workspace", last="workspace_bytes")
+
+
+class CPack4(ctypes.Structure):
+    """b200_pack4_op"""
+
+    _fields_ = _fields("rows cols x_type by_column", "ldx ldq", "x q scale")
+
+
+class CUnpack4(ctypes.Structure):
+    """b200_unpack4_op"""
+
+    _fields_ = _fields("rows cols y_type by_column", "ldq ldy", "q scale y")
+
+
+class CDense4(ctypes.Structure):
+    """b200_dense4_op"""
+
+    _fields_ = _fields("rows in_ out y_type act", "ldx ldw ldr ldy", "x x_scale w w_scale bias residual y")
 
 
 class CSavedFormat(ctypes.Structure):
@@ -187,6 +206,9 @@ def load() -> ctypes.CDLL:
         "b200_op_dense": [ctypes.c_int, vp, ctypes.POINTER(CDense)],
         "b200_op_dense_backward_workspace": [ctypes.POINTER(CDenseGrad), ctypes.POINTER(i64)],
         "b200_op_dense_backward": [ctypes.c_int, vp, ctypes.POINTER(CDenseGrad)],
+        "b200_op_pack4": [ctypes.c_int, vp, ctypes.POINTER(CPack4)],
+        "b200_op_unpack4": [ctypes.c_int, vp, ctypes.POINTER(CUnpack4)],
+        "b200_op_dense4": [ctypes.c_int, vp, ctypes.POINTER(CDense4)],
         "b200_op_dense_gave_up": [ctypes.c_int, ctypes.POINTER(ctypes.POINTER(i32))],
         "b200_map_chess768": [vp, i32, vp, vp, i32],
         "b200_map_chess_buckets_mirrored": [vp, i32, vp, vp, vp, i32],

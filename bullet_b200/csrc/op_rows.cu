@@ -1,19 +1,13 @@
 // Operator-level entry points over the rows of a matrix: b200_op_rms_norm and its gradient, b200_op_pack8, b200_op_unpack8.
 #include <algorithm>
-#include <type_traits>
 
 #include "kernels_rows.cuh"
 #include "op_call.h"
+#include "with_type.h"
 
 namespace {
 
 using namespace b200;
-
-// f(element type) for one of the float types
-template <class F>
-auto with_float(int type, F f) {
-    return type == B200_TYPE_F32 ? f(float{}) : type == B200_TYPE_BF16 ? f(bf16{}) : f(f16{});
-}
 
 // How a launch deals rows out: `warps` of a CTA to a row (1: every warp one of its own), `vectors` of eight elements a lane.
 struct RowShape {
@@ -49,13 +43,6 @@ void with_vectors(int vectors, F f) {
         f(std::integral_constant<int, 4>{});
     else
         f(std::integral_constant<int, Most == 4 ? 4 : 8>{});
-}
-template <class F>
-void with_bool(bool b, F f) {
-    if (b)
-        f(std::true_type{});
-    else
-        f(std::false_type{});
 }
 constexpr int kRowVectors = 8, kGradVectors = 4;  // most of a lane
 constexpr int kRowCols = 256 * kRowWarpsMost * kRowVectors, kGradCols = 256 * kRowWarpsMost * kGradVectors;

@@ -259,6 +259,86 @@ PyObject* dense(PyObject* const* a) {
     return THPVariable_Wrap(y);
 }
 
+// ---- 4 bits
+
+// Rows of codes along `length`, and their scales.
+struct Codes4 {
+    at::Tensor codes, scale;
+    int64_t rows, length, ld;
+    const uint8_t* scale_at() const { return static_cast<const uint8_t*>(scale.data_ptr()); }
+};
+int64_t length_of(PyObject* o, const char* what) {
+    const long long n = PyLong_AsLongLong(o);
+    if (n == -1 && PyErr_Occurred()) throw Raised{};
+    if (n < 0 || n > INT32_MAX) refuse(std::string(what) + ": a length of " + std::to_string(n));
+    return n;
+}
+Codes4 codes4(PyObject* codes, PyObject* scale, PyObject* length, const char* what) {
+    Codes4 c{tensor(codes, what), tensor(scale, what), 0, length_of(length, what), 0};
+    if (c.codes.scalar_type() != at::kByte) refuse(std::string(what) + ": codes are torch.uint8");
+    c.ld = rows_apart(c.codes, what);
+    c.rows = c.codes.size(0);
+    const int64_t groups = (c.length + 31) / 32;
+    if (c.codes.size(1) != groups * 16) refuse(std::string(what) + ": " + std::to_string(groups * 16) + " bytes a row are wanted for a length of " + std::to_string(c.length));
+    if (c.rows <= 1 || groups == 0) c.ld = groups * 16;  // (there is no second row)
+    if (c.ld % 16 || reinterpret_cast<uintptr_t>(c.codes.data_ptr()) % 16) refuse(std::string(what) + ": rows of codes must start on 16 bytes");
+    if (c.scale.scalar_type() != at::kByte || c.scale.dim() != 1 || c.scale.size(0) != B200_FOUR_SCALES(c.rows, c.length) || !c.scale.is_contiguous() ||
+        c.scale.device() != c.codes.device() || reinterpret_cast<uintptr_t>(c.scale.data_ptr()) % 16)
+        refuse(std::string(what) + ": scales are " + std::to_string(B200_FOUR_SCALES(c.rows, c.length)) + " consecutive torch.uint8 on 16 bytes on the same device");
+    return c;
+}
+
+// (x, by_column) -> (codes, scale)
+PyObject* pack4(PyObject* const* a) {
+    const at::Tensor x = tensor(a[0], "x");
+    b200_pack4_op op{};
+    op.by_column = truth(a[1]);
+    op.ldx = matrix(x, "x", kFloats);
+    const int64_t rows = op.by_column ? x.size(1) : x.size(0), length = op.by_column ? x.size(0) : x.size(1);
+    const at::Tensor codes = empty({rows, (length + 31) / 32 * 16}, at::kByte, x), scale = empty({B200_FOUR_SCALES(rows, length)}, at::kByte, x);
+    op.rows = (int)x.size(0), op.cols = (int)x.size(1), op.x_type = type_of(x.scalar_type());
+    op.ldq = codes.size(1);
+    op.x = x.data_ptr(), op.q = codes.data_ptr(), op.scale = static_cast<uint8_t*>(scale.data_ptr());
+    check(b200_op_pack4(device_of(x), stream_of(x), &op));
+    return tuple<2>({codes, scale});
+}
+
+// (codes, scale, length, by_column, dtype) -> values
+PyObject* unpack4(PyObject* const* a) {
+    const Codes4 q = codes4(a[0], a[1], a[2], "packed");
+    b200_unpack4_op op{};
+    op.by_column = truth(a[3]);
+    const at::ScalarType out = dtype(a[4], "dtype");
+    if (!among(out, kFloats)) refuse("dtype: this type is not taken here");
+    const int64_t rows = op.by_column ? q.length : q.rows, cols = op.by_column ? q.rows : q.length;
+    const at::Tensor y = empty({rows, cols}, out, q.codes);
+    op.rows = (int)rows, op.cols = (int)cols, op.y_type = type_of(out);
+    op.ldq = q.ld, op.ldy = cols;
+    op.q = q.codes.data_ptr(), op.scale = q.scale_at(), op.y = y.data_ptr();
+    check(b200_op_unpack4(device_of(y), stream_of(y), &op));
+    return THPVariable_Wrap(y);
+}
+
+// (x codes, x scale, x length, w codes, w scale, w length, bias, act, residual, out_dtype) -> y
+PyObject* dense4(PyObject* const* a) {
+    const auto bias = maybe_tensor(a[6], "bias"), residual = maybe_tensor(a[8], "residual");
+    const Codes4 x = codes4(a[0], a[1], a[2], "x"), w = codes4(a[3], a[4], a[5], "w");
+    b200_dense4_op op{};
+    op.act = act_of(a[7]);
+    if (x.length != w.length) refuse("x and w: lengths of " + std::to_string(x.length) + " and " + std::to_string(w.length));
+    if (w.codes.device() != x.codes.device()) refuse("w: on another device");
+    const at::ScalarType out = a[9] != Py_None ? dtype(a[9], "out_dtype") : at::kBFloat16;
+    if (!among(out, kFloats)) refuse("out_dtype: this type is not taken here");
+    op.bias = vector(bias, "bias", w.rows, x.codes);
+    if (residual) op.ldr = matrix(*residual, "residual", out, x.rows, w.rows, x.codes), op.residual = residual->data_ptr();
+    const at::Tensor y = empty({x.rows, w.rows}, out, x.codes);
+    op.rows = (int)x.rows, op.in = (int)x.length, op.out = (int)w.rows, op.y_type = type_of(out);
+    op.ldx = x.ld, op.ldw = w.ld, op.ldy = w.rows;
+    op.x = x.codes.data_ptr(), op.x_scale = x.scale_at(), op.w = w.codes.data_ptr(), op.w_scale = w.scale_at(), op.y = y.data_ptr();
+    check(b200_op_dense4(device_of(y), stream_of(y), &op));
+    return THPVariable_Wrap(y);
+}
+
 // (dy, x, x_scale, w, y, y_scale, act, dskip, dw_dtype, need_dx, need_dw, need_dbias) -> (dx, dw, dbias); what is not needed None
 PyObject* dense_backward(PyObject* const* a) {
     const at::Tensor dy = tensor(a[0], "dy");
@@ -339,6 +419,9 @@ PyMethodDef methods[] = {B200_ENTRY(rms_norm, 5),
                          B200_ENTRY(unpack8, 4),
                          B200_ENTRY(dense, 8),
                          B200_ENTRY(dense_backward, 12),
+                         B200_ENTRY(pack4, 2),
+                         B200_ENTRY(unpack4, 5),
+                         B200_ENTRY(dense4, 10),
                          {"set_errors", set_errors, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

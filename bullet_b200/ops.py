@@ -40,6 +40,16 @@ class Packed8(NamedTuple):
     by_column: bool = False
 
 
+class Packed4(NamedTuple):
+    """Codes of 4 bits (e2m1) along the axis that a product sums over, `length` of them a row in whole groups of 32, and their scales, a power of
+    two for each group: torch.uint8 both, laid out as include/bullet_b200.h says.  `by_column`: a row of codes is a column of the matrix."""
+
+    codes: torch.Tensor
+    scale: torch.Tensor
+    length: int
+    by_column: bool = False
+
+
 def _of_rows(p, what: str):
     """(matrix, scales) of a matrix (None) or of codes with a scale per row."""
     if p.__class__ is not Packed8:
@@ -74,10 +84,27 @@ def unpack8(packed: Packed8, dtype=torch.bfloat16):
     return _calls.unpack8(packed.codes, packed.scale, packed.by_column, dtype)
 
 
+def pack4(x, by_column: bool = False) -> Packed4:
+    """x in 4 bits with a scale for every 32 elements of a row (weights [in, out]: of a column).  A group with an infinity or a NaN becomes NaN."""
+    codes, scale = _calls.pack4(x, by_column)
+    return Packed4(codes, scale, x.shape[0 if by_column else 1], bool(by_column))
+
+
+def unpack4(packed: Packed4, dtype=torch.bfloat16):
+    """The values that codes stand for (exact in bf16 and fp32): a matrix as pack4 was given."""
+    return _calls.unpack4(packed.codes, packed.scale, packed.length, packed.by_column, dtype)
+
+
 def dense(x, w, bias=None, act: int = ACT_NONE, residual=None, out_dtype=None):
-    """act(x @ w + bias) + residual.  x and w: matrices of one 16-bit type, or both Packed8 (w by column).  `out_dtype`: fp32 or 16
-    bits; default x's type, bf16 for codes.  dense_backward wants act(x @ w + bias) by itself: to train a layer that has both, call
+    """act(x @ w + bias) + residual.  x and w: matrices of one 16-bit type, or both Packed8, or both Packed4 (w by column).  `out_dtype`: fp32 or 16
+    bits; default x's type, bf16 for codes.  The gradient of a layer on Packed4 is dense_backward's at unpack4's values.  dense_backward wants act(x @ w + bias) by itself: to train a layer that has both, call
     without the residual, and add it behind (rms_norm does, on its way)."""
+    if x.__class__ is Packed4 or w.__class__ is Packed4:
+        if x.__class__ is not w.__class__:
+            raise ValueError("x and w: both in 4 bits or neither")
+        if x.by_column or not w.by_column:
+            raise ValueError("x and w: codes of x by row and of w by column are wanted")
+        return _calls.dense4(x.codes, x.scale, x.length, w.codes, w.scale, w.length, bias, act, residual, out_dtype)
     x, x_scale = _of_rows(x, "x")
     w_scale = None
     if w.__class__ is Packed8:

@@ -390,7 +390,7 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
  *   - all sums are held in 32 bits and taken in the same order by every call of the same shape and alignment: equal inputs
  *     give equal bits;
  *   - a dense kernel that waits too long for its own copies or products gives up, which leaves its call's outputs invalid; the
- *     next call of b200_op_dense or its gradient with rows on the device, whoever makes it, returns B200_ERR_STATE, once, and
+ *     next call of b200_op_dense, its gradient or b200_op_dense4 with rows on the device, whoever makes it, returns B200_ERR_STATE, once, and
  *     does nothing else.  Programs that replay graphs, or that want to know whose call it was, ask b200_op_dense_gave_up;
  *   - a B200_TYPE_E4M3 matrix holds codes of 8 bits (four significand bits, largest value 448, no infinities) and goes with
  *     a scale in fp32 per row (or per column, where said): it stands for code * scale.  Scales that these operators make are
@@ -524,6 +524,59 @@ typedef struct b200_dense_grad_op {
 } b200_dense_grad_op;
 int b200_op_dense_backward_workspace(const b200_dense_grad_op* op, int64_t* bytes);
 int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* op);
+
+/* ---- matrices in 4 bits, for dense layers at twice the rate and half the bytes of 8.
+ * A code is e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and, with 8 added, their negatives.  Codes lie along the axis that a product sums over, of length
+ * `n`: two to a byte, the even element in the low half, in rows of (n + 31) / 32 groups of 16 bytes; ld of codes is in BYTES, and rows
+ * start on 16.  What lies in a group past n is code 0.  The 32 elements of a group share a scale, a byte e that stands for
+ * 2^(e - 127), 255 for NaN, which the whole group is then.  Scales lie in tiles of 512 bytes, of 128 rows by four groups, the tiles of 128
+ * rows side by side: with `across` = (groups + 3) / 4, that of row r and group g at
+ *     (r / 128 * across + g / 4) * 512 + r % 32 * 16 + r % 128 / 32 * 4 + g % 4,
+ * which is B200_FOUR_SCALES(rows, n) bytes from an address on 16 bytes; bytes that belong to no group of the matrix are 127. */
+#define B200_FOUR_SCALES(rows, n) (((int64_t)(rows) + 127) / 128 * (((int64_t)(n) + 127) / 128) * 512)
+
+/* Activations (or weights) to 4 bits, and back.  by_column 0: rows of x become rows of codes.  by_column 1: columns do, `cols` rows of codes along
+ * the rows of x, as weights [in][out] are wanted by b200_op_dense4.  The scale is the smallest power of two from 2^-126 on that brings the
+ * group's largest magnitude to 6 or below (2^0 where there is none but 0); codes are the nearest, halves to the even one; a group with an
+ * infinity or a NaN becomes NaN.  Values are exact in bf16 and fp32; one that would round up out of fp32 rounds down. */
+typedef struct b200_pack4_op {
+    int32_t rows, cols;    /* of x */
+    int32_t x_type;        /* B200_TYPE_F32, _BF16 or _F16 */
+    int32_t by_column;
+    int64_t ldx, ldq;
+    const void* x;
+    void* q;               /* out: codes */
+    uint8_t* scale;        /* out */
+} b200_pack4_op;
+int b200_op_pack4(int device, void* stream, const b200_pack4_op* op);
+typedef struct b200_unpack4_op {
+    int32_t rows, cols;    /* of y */
+    int32_t y_type;        /* B200_TYPE_F32, _BF16 or _F16 */
+    int32_t by_column;
+    int64_t ldq, ldy;
+    const void* q;
+    const uint8_t* scale;
+    void* y;               /* out */
+} b200_unpack4_op;
+int b200_op_unpack4(int device, void* stream, const b200_unpack4_op* op);
+
+/* y = act(x W + bias) + residual, as b200_op_dense, with x and W in 4 bits: x by row, W by column, both along `in`.  Products are exact and
+ * summed in 32 bits, which cut a sum off by up to 2^-23 of the largest on the way at each 64 of `in`; what scales bring below 2^-126 may
+ * become 0.  Its gradient is that of b200_op_dense at the values that the codes stand for (b200_op_unpack4: exact in bf16). */
+typedef struct b200_dense4_op {
+    int32_t rows, in, out;
+    int32_t y_type;        /* B200_TYPE_F32, _BF16 or _F16: of residual and y */
+    int32_t act;           /* B200_ACT_* */
+    int64_t ldx, ldw, ldr, ldy;
+    const void* x;         /* `rows` rows of codes */
+    const uint8_t* x_scale;
+    const void* w;         /* `out` rows of codes */
+    const uint8_t* w_scale;
+    const float* bias;     /* [out], or NULL */
+    const void* residual;  /* [rows][out], or NULL */
+    void* y;               /* out */
+} b200_dense4_op;
+int b200_op_dense4(int device, void* stream, const b200_dense4_op* op);
 
 /* The word that the dense kernels of `device` set to 1 where a wait gave up: host memory that may be read at any time, and set
  * back to 0, which the call that returns B200_ERR_STATE does as well.  Read behind a synchronisation, it tells of all work
