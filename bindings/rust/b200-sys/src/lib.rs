@@ -244,6 +244,66 @@ pub struct b200_dense4_op {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct b200_embed_op {
+    pub rows: i32,
+    pub slots: i32,
+    pub n: i32,
+    pub cols: i32,
+    pub table_type: i32,
+    pub y_type: i32,
+    pub wide_ids: i32,
+    pub ldids: i64,
+    pub ldt: i64,
+    pub ldy: i64,
+    pub ids: *const c_void,
+    pub table: *const c_void,
+    pub y: *mut c_void,
+    pub scale: f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_embed_grad_op {
+    pub rows: i32,
+    pub slots: i32,
+    pub n: i32,
+    pub cols: i32,
+    pub dy_type: i32,
+    pub dtable_type: i32,
+    pub wide_ids: i32,
+    pub ldids: i64,
+    pub lddy: i64,
+    pub lddt: i64,
+    pub ids: *const c_void,
+    pub dy: *const c_void,
+    pub dtable: *mut c_void,
+    pub workspace: *mut c_void,
+    pub scale: f32,
+    pub workspace_bytes: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_gradient {
+    pub g: *const c_void,
+    pub out: *mut c_void,
+    pub n: i64,
+    pub r#type: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct b200_clip_op {
+    pub count: i32,
+    pub gradients: *const b200_gradient,
+    pub norm: *mut f32,
+    pub workspace: *mut c_void,
+    pub max_norm: f32,
+    pub workspace_bytes: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct b200_dense_op {
     pub rows: i32,
     pub r#in: i32,
@@ -440,6 +500,11 @@ extern "C" {
     pub fn b200_op_pack4(device: c_int, stream: *mut c_void, op: *const b200_pack4_op) -> c_int;
     pub fn b200_op_unpack4(device: c_int, stream: *mut c_void, op: *const b200_unpack4_op) -> c_int;
     pub fn b200_op_dense4(device: c_int, stream: *mut c_void, op: *const b200_dense4_op) -> c_int;
+    pub fn b200_op_embed(device: c_int, stream: *mut c_void, op: *const b200_embed_op) -> c_int;
+    pub fn b200_op_embed_backward_workspace(op: *const b200_embed_grad_op, bytes: *mut i64) -> c_int;
+    pub fn b200_op_embed_backward(device: c_int, stream: *mut c_void, op: *const b200_embed_grad_op) -> c_int;
+    pub fn b200_op_clip_gradients_workspace(op: *const b200_clip_op, bytes: *mut i64) -> c_int;
+    pub fn b200_op_clip_gradients(device: c_int, stream: *mut c_void, op: *const b200_clip_op) -> c_int;
     pub fn b200_op_dense_gave_up(device: c_int, word: *mut *mut i32) -> c_int;
 
     pub fn b200_map_chess768(records: *const c_void, n: i32, stm: *mut i32, nstm: *mut i32, nnz: i32) -> c_int;

@@ -27,7 +27,8 @@ SYMBOLS = (
     "b200_batch_upload_records_gpu", "b200_slot_read", "b200_probe_bandwidth", "b200_net_set_optimiser",
     "b200_op_rms_norm", "b200_op_rms_norm_backward_workspace", "b200_op_rms_norm_backward", "b200_op_pack8", "b200_op_unpack8",
     "b200_op_dense_workspace", "b200_op_dense", "b200_op_dense_backward_workspace", "b200_op_dense_backward", "b200_op_dense_gave_up",
-    "b200_op_pack4", "b200_op_unpack4", "b200_op_dense4",
+    "b200_op_pack4", "b200_op_unpack4", "b200_op_dense4", "b200_op_embed", "b200_op_embed_backward_workspace", "b200_op_embed_backward",
+    "b200_op_clip_gradients_workspace", "b200_op_clip_gradients",
 )
 
 
@@ -107,6 +108,30 @@ class CDense4(ctypes.Structure):
     """b200_dense4_op"""
 
     _fields_ = _fields("rows in_ out y_type act", "ldx ldw ldr ldy", "x x_scale w w_scale bias residual y")
+
+
+class CEmbed(ctypes.Structure):
+    """b200_embed_op"""
+
+    _fields_ = _fields("rows slots n cols table_type y_type wide_ids", "ldids ldt ldy", "ids table y", f32="scale")
+
+
+class CEmbedGrad(ctypes.Structure):
+    """b200_embed_grad_op"""
+
+    _fields_ = _fields("rows slots n cols dy_type dtable_type wide_ids", "ldids lddy lddt", "ids dy dtable workspace", f32="scale", last="workspace_bytes")
+
+
+class CGradient(ctypes.Structure):
+    """b200_gradient"""
+
+    _fields_ = [("g", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n", ctypes.c_int64), ("type", ctypes.c_int32)]
+
+
+class CClip(ctypes.Structure):
+    """b200_clip_op"""
+
+    _fields_ = _fields("count", "", "gradients norm workspace", f32="max_norm", last="workspace_bytes")
 
 
 class CSavedFormat(ctypes.Structure):
@@ -209,6 +234,11 @@ def load() -> ctypes.CDLL:
         "b200_op_pack4": [ctypes.c_int, vp, ctypes.POINTER(CPack4)],
         "b200_op_unpack4": [ctypes.c_int, vp, ctypes.POINTER(CUnpack4)],
         "b200_op_dense4": [ctypes.c_int, vp, ctypes.POINTER(CDense4)],
+        "b200_op_embed": [ctypes.c_int, vp, ctypes.POINTER(CEmbed)],
+        "b200_op_embed_backward_workspace": [ctypes.POINTER(CEmbedGrad), ctypes.POINTER(i64)],
+        "b200_op_embed_backward": [ctypes.c_int, vp, ctypes.POINTER(CEmbedGrad)],
+        "b200_op_clip_gradients_workspace": [ctypes.POINTER(CClip), ctypes.POINTER(i64)],
+        "b200_op_clip_gradients": [ctypes.c_int, vp, ctypes.POINTER(CClip)],
         "b200_op_dense_gave_up": [ctypes.c_int, ctypes.POINTER(ctypes.POINTER(i32))],
         "b200_map_chess768": [vp, i32, vp, vp, i32],
         "b200_map_chess_buckets_mirrored": [vp, i32, vp, vp, vp, i32],

@@ -18,7 +18,7 @@ LIB = os.path.join(HERE, "libbullet_b200.so")
 HEADER = os.path.join(HERE, "..", "include", "bullet_b200.h")
 TENSOR_CALLS = os.path.join(HERE, "_tensor_calls.so")
 MADE_FOR = os.path.join(HERE, "_tensor_calls.made_for")
-SOURCES = ["net.cu", "op_ft_forward.cu", "op_rows.cu", "op_dense.cu", "op_four.cu", "gave_up.cu", "probe.cu", "host_pack.cpp", "checkpoint.cpp", "saved_format.cpp"]
+SOURCES = ["net.cu", "op_ft_forward.cu", "op_rows.cu", "op_dense.cu", "op_four.cu", "op_table.cu", "op_clip.cu", "gave_up.cu", "probe.cu", "host_pack.cpp", "checkpoint.cpp", "saved_format.cpp"]
 
 
 def _nvcc() -> str:

@@ -15,6 +15,7 @@
 
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "../../include/bullet_b200.h"
 
@@ -339,6 +340,127 @@ PyObject* dense4(PyObject* const* a) {
     return THPVariable_Wrap(y);
 }
 
+// ---- rows named by ids
+
+double number(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw Raised{};
+    return v;
+}
+// Lists of ids, [rows] or [rows][slots].
+template <class Op>
+at::Tensor lists(PyObject* o, Op& op, Tensor beside) {
+    const at::Tensor ids = tensor(o, "ids");
+    if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) refuse("ids: torch.int32 or torch.int64 are wanted");
+    if (ids.dim() < 1 || ids.dim() > 2 || ids.device() != beside.device()) refuse("ids: a vector, or a matrix of lists, on the same device is wanted");
+    const int64_t rows = ids.size(0), slots = ids.dim() == 2 ? ids.size(1) : 1;
+    if (rows > INT32_MAX || slots > INT32_MAX) refuse("ids: too many");
+    if (ids.dim() == 2 && slots > 1 && ids.stride(1) != 1) refuse("ids: a list's must be consecutive");
+    if (rows > 1 && ids.stride(0) < slots) refuse("ids: lists must not overlap");
+    op.rows = (int)rows, op.slots = (int)slots, op.wide_ids = ids.scalar_type() == at::kLong;
+    op.ldids = rows > 1 ? ids.stride(0) : slots;
+    op.ids = ids.data_ptr();
+    return ids;
+}
+
+// (table, ids, scale, out_dtype) -> y
+PyObject* embed(PyObject* const* a) {
+    const at::Tensor table = tensor(a[0], "table");
+    b200_embed_op op{};
+    op.ldt = matrix(table, "table", kFloats);
+    const at::Tensor ids = lists(a[1], op, table);
+    op.scale = (float)number(a[2]);
+    const at::ScalarType out = a[3] == Py_None ? table.scalar_type() : dtype(a[3], "out_dtype");
+    if (!among(out, kFloats)) refuse("out_dtype: this type is not taken here");
+    const at::Tensor y = empty({op.rows, table.size(1)}, out, table);
+    op.n = (int)table.size(0), op.cols = (int)table.size(1), op.table_type = type_of(table.scalar_type()), op.y_type = type_of(out);
+    op.ldy = op.cols;
+    op.table = table.data_ptr(), op.y = y.data_ptr();
+    check(b200_op_embed(device_of(table), stream_of(table), &op));
+    return THPVariable_Wrap(y);
+}
+
+// (dy, ids, n, scale, dtype) -> dtable
+PyObject* embed_backward(PyObject* const* a) {
+    const at::Tensor dy = tensor(a[0], "dy");
+    b200_embed_grad_op op{};
+    op.lddy = matrix(dy, "dy", kFloats);
+    const at::Tensor ids = lists(a[1], op, dy);
+    if (ids.size(0) != dy.size(0)) refuse("ids: " + std::to_string(ids.size(0)) + " lists where " + std::to_string(dy.size(0)) + " are wanted");
+    const int64_t n = length_of(a[2], "n");
+    op.scale = (float)number(a[3]);
+    const at::ScalarType out = dtype(a[4], "dtype");
+    if (!among(out, kFloats)) refuse("dtype: this type is not taken here");
+    const at::Tensor dtable = empty({n, dy.size(1)}, out, dy);
+    op.n = (int)n, op.cols = (int)dy.size(1), op.dy_type = type_of(dy.scalar_type()), op.dtable_type = type_of(out);
+    op.lddt = op.cols;
+    op.dy = dy.data_ptr(), op.dtable = dtable.data_ptr();
+    const at::Tensor held = space(b200_op_embed_backward_workspace, op, dy);
+    check(b200_op_embed_backward(device_of(dy), stream_of(dy), &op));
+    return THPVariable_Wrap(dtable);
+}
+
+// ---- the norm of gradients
+
+struct Reference {
+    PyObject* o;
+    ~Reference() { Py_XDECREF(o); }
+};
+// (gradients, max_norm, out) -> (outputs or None, norm); max_norm None: the norm alone; out None: new tensors
+PyObject* clip_gradients(PyObject* const* a) {
+    const Reference list{PySequence_Fast(a[0], "gradients: a sequence of tensors is wanted")};
+    if (!list.o) throw Raised{};
+    const bool writes = a[1] != Py_None;
+    const Reference outs{writes && a[2] != Py_None ? PySequence_Fast(a[2], "out: a sequence of tensors is wanted") : nullptr};
+    if (writes && a[2] != Py_None && !outs.o) throw Raised{};
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(list.o);
+    if (count == 0 || count > INT32_MAX) refuse("gradients: at least one tensor is wanted");
+    if (outs.o && PySequence_Fast_GET_SIZE(outs.o) != count) refuse("out: " + std::to_string(count) + " tensors are wanted");
+    std::vector<at::Tensor> held;
+    std::vector<b200_gradient> gradients(count);
+    held.reserve(2 * count);
+    for (Py_ssize_t k = 0; k < count; k++) {
+        auto name = [&](const char* what) { return std::string(what) + "[" + std::to_string(k) + "]"; };
+        PyObject* o = PySequence_Fast_GET_ITEM(list.o, k);
+        if (!THPVariable_Check(o)) refuse(name("gradients") + ": a tensor is wanted");
+        held.push_back(tensor(o, "gradients"));
+        const at::Tensor g = held.back();
+        if (!g.is_cuda() || g.device() != held.front().device()) refuse(name("gradients") + ": on another device than the first, or on none");
+        if (!among(g.scalar_type(), kFloats)) refuse(name("gradients") + ": this type is not taken here");
+        if (!g.is_non_overlapping_and_dense()) refuse(name("gradients") + ": elements must lie side by side");
+        gradients[k] = {g.data_ptr(), nullptr, g.numel(), type_of(g.scalar_type())};
+    }
+    for (Py_ssize_t k = 0; writes && k < count; k++) {
+        const at::Tensor g = held[k];
+        if (outs.o) {
+            held.push_back(tensor(PySequence_Fast_GET_ITEM(outs.o, k), "out"));
+            Tensor t = held.back();
+            if (t.scalar_type() != g.scalar_type() || t.sizes() != g.sizes() || t.strides() != g.strides() || t.device() != g.device())
+                refuse("out[" + std::to_string(k) + "]: not of its gradient's type, shape, strides and device");
+        } else {
+            held.push_back(at::detail::empty_strided_cuda(g.sizes(), g.strides(), g.scalar_type(), g.device()));
+        }
+        gradients[k].out = held.back().data_ptr();
+    }
+    Tensor first = held.front();
+    const at::Tensor norm = empty({}, at::kFloat, first);
+    b200_clip_op op{};
+    op.count = (int)count, op.gradients = gradients.data(), op.norm = static_cast<float*>(norm.data_ptr());
+    op.max_norm = writes ? (float)number(a[1]) : 0.f;
+    if (writes && !(op.max_norm >= 0)) refuse("max_norm: 0 or above is wanted");
+    const at::Tensor scratch = space(b200_op_clip_gradients_workspace, op, first);
+    check(b200_op_clip_gradients(device_of(first), stream_of(first), &op));
+    if (!writes) return Py_BuildValue("(ON)", Py_None, THPVariable_Wrap(norm));
+    const Reference clipped{PyList_New(count)};
+    if (!clipped.o) throw Raised{};
+    for (Py_ssize_t k = 0; k < count; k++) {
+        PyObject* o = THPVariable_Wrap(held[count + k]);
+        if (!o) throw Raised{};
+        PyList_SET_ITEM(clipped.o, k, o);
+    }
+    return Py_BuildValue("(ON)", clipped.o, THPVariable_Wrap(norm));
+}
+
 // (dy, x, x_scale, w, y, y_scale, act, dskip, dw_dtype, need_dx, need_dw, need_dbias) -> (dx, dw, dbias); what is not needed None
 PyObject* dense_backward(PyObject* const* a) {
     const at::Tensor dy = tensor(a[0], "dy");
@@ -422,6 +544,9 @@ PyMethodDef methods[] = {B200_ENTRY(rms_norm, 5),
                          B200_ENTRY(pack4, 2),
                          B200_ENTRY(unpack4, 5),
                          B200_ENTRY(dense4, 10),
+                         B200_ENTRY(embed, 4),
+                         B200_ENTRY(embed_backward, 5),
+                         B200_ENTRY(clip_gradients, 3),
                          {"set_errors", set_errors, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

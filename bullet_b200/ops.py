@@ -125,6 +125,28 @@ def dense_backward(dy, x, w, y=None, act: int = ACT_NONE, dskip=None, dw_dtype=t
     return _calls.dense_backward(dy, x, x_scale, w, y, y_scale, act, dskip, dw_dtype, need_dx, need_dw, need_dbias)
 
 
+def embed(table, ids, scale: float = 1.0, out_dtype=None):
+    """scale * the sum of table[ids[r][s]] over s, for every list r of `ids`: [rows, slots], or [rows] for one each, in int32 or int64.  Ids outside
+    [0, len(table)), as -1, name no row and add nothing.  Sums are of 32 bits; `out_dtype`: default the table's type."""
+    return _calls.embed(table, ids, scale, out_dtype)
+
+
+def embed_backward(dy, ids, n: int, scale: float = 1.0, dtype=torch.float32):
+    """The gradient of embed at its table, [n, cols]: row t is scale * the sum of dy[r] over all ids[r][s] == t, in their order, 0 where there are none."""
+    return _calls.embed_backward(dy, ids, n, scale, dtype)
+
+
+def gradient_norm(gradients):
+    """The norm of all elements of tensors (fp32, bf16, fp16, of any shape, their elements side by side) together: a tensor of no dimension."""
+    return _calls.clip_gradients(gradients, None, None)[1]
+
+
+def clip_gradients(gradients, max_norm: float, out=None):
+    """([tensors], norm): the gradients times max_norm / norm where their norm together is above max_norm (and finite), else as they are.  `out`:
+    where they go; may be `gradients`, or any of them, themselves, which are then written only if they change."""
+    return _calls.clip_gradients(gradients, max_norm, out)
+
+
 def gave_up(device: int) -> bool:
     """Whether a wait of dense kernels on a device gave up since this was last asked, or reported by a call: the outputs of what ran
     there are not valid then.  For programs that replay graphs, behind a synchronisation; other calls report by B200Error."""

@@ -578,6 +578,59 @@ typedef struct b200_dense4_op {
 } b200_dense4_op;
 int b200_op_dense4(int device, void* stream, const b200_dense4_op* op);
 
+/* ---- rows of a table that lists of ids name, as embeddings of features or of an output bucket: y[r] = scale * sum over s of table[ids[r][s]], sums
+ * taken in the order of the slots.  An id outside [0, n), as the -1 behind the last of a list, names no row and adds nothing.  At most 2^31 - 2^16
+ * ids.  (The reference's sparse affine, crates/compiler/src/tensor/operation/sparse.rs:103-115, without its bias, in these types.) */
+typedef struct b200_embed_op {
+    int32_t rows, slots, n, cols;  /* lists, ids of a list, rows of the table, columns */
+    int32_t table_type, y_type;    /* B200_TYPE_F32, _BF16 or _F16 */
+    int32_t wide_ids;              /* 0: int32, 1: int64 */
+    int64_t ldids, ldt, ldy;
+    const void* ids;
+    const void* table;             /* [n][cols] */
+    void* y;                       /* out: [rows][cols] */
+    float scale;
+} b200_embed_op;
+int b200_op_embed(int device, void* stream, const b200_embed_op* op);
+
+/* Its gradient at the table: dtable[t] = scale * sum of dy[r] over all r, s with ids[r][s] == t, 0 for a row that none names.  The ids are sorted
+ * and the sums taken in the order of the lists, stretches of 64 by themselves where there are more. */
+typedef struct b200_embed_grad_op {
+    int32_t rows, slots, n, cols;
+    int32_t dy_type, dtable_type;  /* B200_TYPE_F32, _BF16 or _F16 */
+    int32_t wide_ids;
+    int64_t ldids, lddy, lddt;
+    const void* ids;
+    const void* dy;                /* [rows][cols] */
+    void* dtable;                  /* out: [n][cols], all of it */
+    void* workspace;               /* 16-byte aligned; may be NULL where none is needed */
+    float scale;
+    int64_t workspace_bytes;
+} b200_embed_grad_op;
+int b200_op_embed_backward_workspace(const b200_embed_grad_op* op, int64_t* bytes);
+int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* op);
+
+/* ---- the gradients of a step together: norm = sqrt(sum of the squares of all elements), and out = share * g with share = max_norm / norm where the
+ * norm is finite and above max_norm, else 1 (so a norm that is not finite changes nothing, and says so).  Squares are summed in 32 bits for 32
+ * elements, beyond in 64; a norm past fp32 is infinity, its share is right all the same.  Elements lie side by side.  `out` may be the gradient
+ * itself, which is then read and written only if it changes, or memory that overlaps no other gradient and output; NULL: counted, not written. */
+typedef struct b200_gradient {
+    const void* g;
+    void* out;
+    int64_t n;
+    int32_t type;                  /* B200_TYPE_F32, _BF16 or _F16: of both */
+} b200_gradient;
+typedef struct b200_clip_op {
+    int32_t count;
+    const b200_gradient* gradients; /* [count], HOST memory, read by the call */
+    float* norm;                   /* out: [1] */
+    void* workspace;               /* 16-byte aligned */
+    float max_norm;                /* read where anything is written; 0 or above */
+    int64_t workspace_bytes;
+} b200_clip_op;
+int b200_op_clip_gradients_workspace(const b200_clip_op* op, int64_t* bytes);
+int b200_op_clip_gradients(int device, void* stream, const b200_clip_op* op);
+
 /* The word that the dense kernels of `device` set to 1 where a wait gave up: host memory that may be read at any time, and set
  * back to 0, which the call that returns B200_ERR_STATE does as well.  Read behind a synchronisation, it tells of all work
  * before that, replayed graphs included.  *word is NULL where the device cannot share memory while it is running. */
