@@ -6,9 +6,17 @@
 // multiplies codes and scales as they are (tcgen05.mma.kind::mxf4.block_scale): nothing is turned into wider types.
 //
 // As product_kernel (kernels_product.cuh): CTAs, or pairs of them, take tiles one after another; one thread has TMA fetch stages of 128 bytes of
-// k = 256 codes, 128-byte swizzled, and their scales' tiles; one copies the scales on into tensor memory and issues the products; eight warps
-// take finished sums out and hand them to TMA in boxes of 32 rows of 128 bytes.
+// k = 256 codes, 128-byte swizzled; one warp issues the products; eight or sixteen take finished sums out, 32 columns at a time, and hand them to TMA in boxes
+// of 32 rows of 64 bytes.  (Eight warps for a tile of 256 columns, 64 at a time: 7000 clocks a tile, most of them spent fetching instructions.)
 // Sums stay in tensor memory over all of k: the pipe cuts a sum off at each of its k / 64 additions, by 2^-24 of it or so.
+//
+// Scales have to lie in tensor memory.  They come with the stages, and four more warps, one for each 32 lanes, carry them on through registers.  The pipe's own
+// copies from shared memory (tcgen05.cp, 512 bytes each) take it 100 clocks a piece, in which it multiplies nothing: six of them 330 ns of a stage's 800, where
+// four products of 256 x 256 x 64 are 280 and the stage's way out of L2 310 to 400.  (Loaded from global memory by those warps, two stages ahead: 1500,
+// as each arrival at a barrier waits for the loads on their way.)
+// Two tiles' sums of 256 columns and the scales of five stages do not fit in 512 columns: the tiles overlap by half, which is taken out first.
+// (Scales of two stages, and an overlap of 64 columns: the way from the products that last used a place, by way of those warps, to those that use it
+// next is longer than one stage's products: 1050 ns a stage.)
 #pragma once
 #include "kernels_four.cuh"
 #include "product_out.cuh"
@@ -18,52 +26,100 @@ namespace b200 {
 template <int BN, bool PAIR>
 struct Tile4 {
     static constexpr int kRows = PAIR ? 256 : 128, kOwnColumns = PAIR ? BN / 2 : BN;  // of b, that this CTA fetches
-    static constexpr int kCodes = 256;                                                // of k in a stage: 128 bytes
-    static constexpr uint32_t kA = 128 * 128, kB = kOwnColumns * 128;
-    static constexpr int kScaleTiles = (BN + 127) / 128;  // of b's rows: each CTA of a pair wants all of them
-    static constexpr uint32_t kAScales = 1024, kBScales = kScaleTiles * 1024, kStage = kA + kB + kAScales + kBScales;
-    static constexpr int kTakers = 8, kOwn = BN * 4 / kTakers;  // warps that take sums out, columns of each
-    static constexpr int kThreads = 64 + 32 * kTakers;
-    static constexpr size_t kBoxes = kTakers * 4096, kValues = (size_t)kTakers * kOwn * 4, kRest = 1024 + kBoxes + kValues;
+    static constexpr int kScaleTiles = (BN + 127) / 128;                              // of b's rows: each CTA of a pair wants all of them
+    static constexpr uint32_t kA = 128 * 128, kB = kOwnColumns * 128, kAScales = 1024, kScales = kAScales * (1 + kScaleTiles), kStage = kA + kB + kScales;
+    static constexpr int kTakers = BN / 16, kGroups = kTakers / 4;  // warps that take sums out: a quarter of the rows, 32 columns of every 32 kGroups
+    static constexpr int kThreads = 64 + 32 * kTakers + 128;
+    static constexpr uint32_t kBox = 32 * 64;
+    static constexpr size_t kBoxes = kTakers * kBox, kValues = (size_t)kTakers * 64 * 4, kRest = 1024 + kBoxes + kValues;
     static constexpr int kFit = (int)((232448 - 1024 - kRest) / kStage), kStages = kFit < 8 ? kFit : 8;
     static constexpr size_t kShared = kRest + (size_t)kStages * kStage;
-    static constexpr int kSums = BN == 256 ? 1 : 2;                          // tiles whose sums there is room for
-    static constexpr uint32_t kScaleColumns = 2 * (4 + 4 * kScaleTiles);     // of tensor memory for a stage's scales
-    static constexpr uint32_t kScalesAt = 512 - 2 * kScaleColumns;           // two stages' by turns
-    static_assert(kSums * BN <= kScalesAt && kStages >= 3, "");
-    static_assert(kStage % 1024 == 0, "the swizzle wants stages on 1024 bytes");
+    static constexpr int kScaleWords = 2 * 4 * (1 + kScaleTiles);              // columns of tensor memory for a stage's: a's of two tiles of k, b's
+    static constexpr int kSumsApart = 128;                                     // of two tiles: those of 256 columns share half of their places
+    static constexpr bool kShares = BN > kSumsApart;
+    static constexpr uint32_t kScalesAt = kSumsApart + BN;
+    static_assert(kScalesAt + kStages * kScaleWords <= 512 && kStages >= 3, "");
+    static_assert(2 * 32 * kGroups == BN && (!kShares || 32 * kGroups == kSumsApart), "a warp takes 32 columns twice, those of shared places together");
 };
 
-// A box of a stack of scales' tiles into shared memory; the bytes are counted at `bar`, of this CTA or (PAIR) of either.
-template <bool PAIR>
-__device__ __forceinline__ void load_scales(uint32_t to, const CUtensorMap* map, int y, int z, uint32_t bar) {
-    if constexpr (PAIR)
-        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(0),
-                     "r"(y), "r"(z), "r"(bar)
-                     : "memory");
-    else
-        load_box3(to, map, 0, y, z, bar);
+// A row of 64 bytes of a box, the residual there added, in place: v from `from` on, 32 values of 16 bits or 16 of fp32.  64-byte swizzle; r: the row's number.
+template <class T>
+__device__ __forceinline__ void box_out64(unsigned char* row, int r, const float (&v)[32], int from, bool residual) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        uint4* at = reinterpret_cast<uint4*>(row + ((k ^ (r >> 1 & 3)) << 4));
+        constexpr int kEach = 16 / sizeof(T);
+        float x[kEach];
+#pragma unroll
+        for (int q = 0; q < kEach; q++) x[q] = v[from + kEach * k + q];
+        if (residual) {
+            const uint4 o = *at;
+            const uint32_t u[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if constexpr (sizeof(T) == 4) {
+                    x[q] += __uint_as_float(u[q]);
+                } else {
+                    float low, high;
+                    unpack2<T>(u[q], low, high);
+                    x[2 * q] += low, x[2 * q + 1] += high;
+                }
+            }
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if constexpr (sizeof(T) == 4)
+                w[q] = __float_as_uint(x[q]);
+            else
+                w[q] = pack2<T>(x[2 * q], x[2 * q + 1]);
+        }
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
-// A tile of scales, 32 rows of 16 bytes, from shared memory into four columns of tensor memory, once for each of its four parts of 32 lanes (PAIR: of
-// both CTAs, from and to the same places of each).
-template <bool PAIR>
-__device__ __forceinline__ void scales_on(uint32_t to, uint32_t smem) {
-    const uint64_t from = (uint64_t)((smem & 0x3ffffu) >> 4) | (uint64_t)(128u >> 4 | 1u << 14) << 32;  // (eight rows are 128 bytes, no swizzle)
-    if constexpr (PAIR)
-        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(from) : "memory");
-    else
-        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(from) : "memory");
+// Sixteen columns of a box of fp32, the residual added, element by element: half a warp a row.
+template <class T>
+static __device__ __forceinline__ void columns_out16(const ProductArgs& p, const unsigned char* box, int lane, int64_t rows0, int64_t column0, bool adds) {
+    const int64_t column = column0 + (lane & 15);
+    if (column >= p.n) return;
+#pragma unroll 4
+    for (int k = 0; k < 16; k++) {
+        const int r = 2 * k + (lane >> 4);
+        const int64_t row = rows0 + r;
+        if (row >= p.m) break;
+        float x = *reinterpret_cast<const float*>(box + r * 64 + (((lane >> 2 & 3) ^ (r >> 1 & 3)) << 4) + (lane & 3) * 4);
+        if (adds) x += to_float(static_cast<const T*>(p.residual)[row * p.ldr + column]);
+        static_cast<T*>(p.d)[row * p.ldd + column] = from_float<T>(x);
+    }
+}
+// Four columns of a warp's 32 lanes into tensor memory.  What was put is there behind scales_stored().
+__device__ __forceinline__ void put_scales(uint32_t to, const uint4& w) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+}
+__device__ __forceinline__ void scales_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// An arrival that says nothing of memory but tensor memory, whose instructions the fence in front of it orders.  (One that releases waits for all else that
+// the warp has had to do with memory: 1500 clocks between the scales' stores and those who wait for them.)
+__device__ __forceinline__ void arrive_for_tensor_memory(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // Form of a product of e2m1 with exponents as scales: `half` says which two bytes of a word of scales belong to its 64 of k.
 __device__ __forceinline__ uint32_t four_form(int m, int n, uint32_t half) {
     return half << 5 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(m >> 4) << 24 | half << 30;
 }
+// One of the warp's lanes, the same one every time.
+__device__ __forceinline__ bool elected() {
+    uint32_t is;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+    return is != 0;
+}
+// a, b: where the tiles lie in shared memory, in pieces of 16 bytes
 template <bool PAIR>
-__device__ __forceinline__ void multiply4(uint32_t sums, uint64_t a, uint64_t b, uint32_t form, uint32_t a_scales, uint32_t b_scales, bool add) {
-#define B200_MULTIPLY4(group)                                                                                                                       \
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::" group ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n}" ::"r"( \
-                     sums),                                                                                                                         \
-                 "l"(a), "l"(b), "r"(form), "r"((int)add), "r"(a_scales), "r"(b_scales)                                                             \
+__device__ __forceinline__ void multiply4(uint32_t sums, uint32_t a, uint32_t b, uint32_t form, uint32_t a_scales, uint32_t b_scales, bool add) {
+    // (tile_descriptor's: rows of 128 bytes along k, 128-byte swizzle)
+#define B200_MULTIPLY4(group)                                                                                                                                                   \
+    asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 a, {%1, %7};\nmov.b64 b, {%2, %7};\ntcgen05.mma.cta_group::" group                           \
+                 ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%5], [%6], p;\n}" ::"r"(sums),                                                                         \
+                 "r"((a & 0x3fffu) | 1u << 16), "r"((b & 0x3fffu) | 1u << 16), "r"(form), "r"((int)add), "r"(a_scales), "r"(b_scales), "r"(64u | 1u << 14 | 2u << 29)             \
                  : "memory")
     if constexpr (PAIR)
         B200_MULTIPLY4("2");
@@ -79,18 +135,19 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
     using T = Tile4<BN, PAIR>;
     constexpr int kStages = T::kStages, kCtas = PAIR ? 2 : 1;
     extern __shared__ unsigned char raw_smem[];
-    __shared__ uint64_t full[kStages], empty[kStages], sums_done[2], sums_free[2], residual_in[T::kTakers];
+    __shared__ uint64_t full[kStages], empty[kStages], scales_in[kStages], sums_done[2], sums_free[2], residual_in[T::kTakers];
     __shared__ uint32_t memory_at;
     __shared__ int dead;
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_rank() : 0;
-    const Waits wait{&dead, p.gave_up};
+    const WaitsFor<false> wait{&dead, p.gave_up};
     if (threadIdx.x == 0) {
         dead = 0;
         for (int s = 0; s < kStages; s++) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], 1 + 4 * kCtas);  // (the codes, and each warp that carries scales on)
             mbar_init(&empty[s], 1);
+            mbar_init(&scales_in[s], 1);
         }
         for (int k = 0; k < T::kTakers; k++) mbar_init(&residual_in[k], 1);
         for (int k = 0; k < 2; k++) {
@@ -125,130 +182,175 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
                 const int m0 = (int)(tile / p.tiles_n * T::kRows) + 128 * (int)rank, n0 = (int)(tile % p.tiles_n * BN);
                 for (int kb = 0; kb < p.k_blocks; kb++) {
                     if (!wait(&empty[s], phase)) break;
-                    const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA, scales_at = b_at + T::kB;
+                    const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA;
                     const uint32_t bar = PAIR ? of_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
-                    if (rank == 0) mbar_expect_tx(&full[s], kCtas * T::kStage);
+                    if (rank == 0) mbar_expect_tx(&full[s], kCtas * (T::kA + T::kB));
+                    mbar_expect_tx(&scales_in[s], T::kScales);
+                    load_box3(b_at + T::kB, &a_scale_map, 0, 2 * kb, m0 >> 7, smem_u32(&scales_in[s]));
+                    load_box3(b_at + T::kB + T::kAScales, &b_scale_map, 0, 2 * kb, n0 >> 7, smem_u32(&scales_in[s]));
                     load_box<PAIR>(a_at, &a_map, kb * 128, m0, bar);
                     load_box<PAIR>(b_at, &b_map, kb * 128, n0 + (PAIR ? T::kOwnColumns * (int)rank : 0), bar);
-                    load_scales<PAIR>(scales_at, &a_scale_map, 2 * kb, m0 >> 7, bar);
-                    load_scales<PAIR>(scales_at + T::kAScales, &b_scale_map, 2 * kb, n0 >> 7, bar);
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {  // multiplies
-            int s = 0, done = 0;
-            uint32_t phase = 0, turn = 0;
+        if (rank == 0) {  // multiplies: the whole warp keeps count, one lane issues (operands that all lanes agree on need no way into uniform registers)
+            const bool issues = elected();
+            const uint32_t a0 = smem_u32(base) >> 4, form = four_form(T::kRows, BN, 0), other = four_form(T::kRows, BN, 1);
+            const int whole = (int)(p.k / 256), rest = (int)((p.k % 256 + 63) / 64);  // stages, and products of the last one (past k there may be no scales)
+            int s = 0;
+            uint32_t phase = 0, done = 0;
             for (int64_t tile = first; tile < tiles && !dead; tile += step, done++) {
-                const int half = done % T::kSums;
-                const uint32_t sums = memory + half * BN;
-                bool fine = wait(&sums_free[half], (done / T::kSums & 1) ^ 1);
-                if (!fine) break;
+                const uint32_t half = done & 1, sums = memory + half * T::kSumsApart;
+                bool fine = T::kShares ? done == 0 || wait(&sums_free[0], done - 1 & 1) : wait(&sums_free[half], (done >> 1 & 1) ^ 1);
+                if (!__all_sync(0xffffffffu, fine)) break;
                 tensor_fence_after();
                 for (int kb = 0; kb < p.k_blocks; kb++) {
-                    fine = wait(&full[s], phase);
-                    if (!fine) break;
+                    if (!__all_sync(0xffffffffu, wait(&full[s], phase))) break;
                     tensor_fence_after();
-                    const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA, scales_at = b_at + T::kB;
-                    const int quarters = (int)min((int64_t)4, (p.k - (int64_t)kb * 256 + 63) / 64);  // (past k there may be no scales)
-                    // (the products before the last ones with these columns are done with them: the pipe takes copies and products in order)
-                    const uint32_t a_scales = memory + T::kScalesAt + turn * T::kScaleColumns, b_scales = a_scales + 8;
-                    turn ^= 1;
-                    for (int g = 0; 2 * g < quarters; g++) {
-                        scales_on<PAIR>(a_scales + 4 * g, scales_at + 512 * g);
+                    const uint32_t a_at = a0 + s * (T::kStage / 16), b_at = a_at + T::kA / 16, a_scales = memory + T::kScalesAt + s * T::kScaleWords, b_scales = a_scales + 8;
+                    if (issues) {
+                        auto product = [&](int q) {
+                            const uint32_t g = q >> 1, part = (uint32_t)(q & 1) << 31;
+                            multiply4<PAIR>(sums, a_at + 2 * q, b_at + 2 * q, q & 1 ? other : form, a_scales + 4 * g + part, b_scales + 4 * T::kScaleTiles * g + part, kb > 0 || q > 0);
+                        };
+                        if (kb < whole) {
 #pragma unroll
-                        for (int t = 0; t < T::kScaleTiles; t++)
-                            scales_on<PAIR>(b_scales + 4 * T::kScaleTiles * g + 4 * t, scales_at + T::kAScales + 1024 * t + 512 * g);
+                            for (int q = 0; q < 4; q++) product(q);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 4; q++)
+                                if (q < rest) product(q);
+                        }
+                        when_multiplied<PAIR>(&empty[s]);
+                        if (kb + 1 == p.k_blocks) when_multiplied<PAIR>(&sums_done[half]);
                     }
-                    for (int q = 0; q < quarters; q++) {
-                        const uint32_t part = (uint32_t)(q & 1), g = (uint32_t)q >> 1;
-                        multiply4<PAIR>(sums, tile_descriptor(a_at + q * 32, 16), tile_descriptor(b_at + q * 32, 16), four_form(T::kRows, BN, part),
-                                        a_scales + 4 * g + (part << 31), b_scales + 4 * T::kScaleTiles * g + (part << 31), kb > 0 || q > 0);
-                    }
-                    when_multiplied<PAIR>(&empty[s]);
+                    __syncwarp();
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
-                when_multiplied<PAIR>(&sums_done[half]);
             }
         }
-    } else {  // takes sums out, kOwn columns of 32 rows
-        const int quarter = warp & 3, taker = warp - 2, c0 = taker / 4 * T::kOwn;
-        unsigned char* box = base + kStages * T::kStage + taker * 4096;
-        float* bias = reinterpret_cast<float*>(base + kStages * T::kStage + T::kBoxes) + taker * T::kOwn;
-        const bool wide = p.boxes && p.d_type == B200_TYPE_F32, adds = p.residual;
-        const int width = wide ? 32 : 64;  // columns of a box
+    } else if (warp < 2 + T::kTakers) {  // takes sums out: 32 rows, twice 32 columns
+        constexpr int kApart = 32 * T::kGroups;
+        const int quarter = warp & 3, taker = warp - 2, c0 = taker / 4 * 32;
+        unsigned char* box = base + kStages * T::kStage + taker * T::kBox;
+        float* bias = reinterpret_cast<float*>(base + kStages * T::kStage + T::kBoxes) + taker * 64;
+        const bool wide = p.d_type == B200_TYPE_F32, adds = p.residual;
+        int64_t bias_at = -1;
         uint32_t residuals = 0;
-        int done = 0;
-        for (int64_t tile = first; tile < tiles; tile += step, done++) {
+        int64_t done = 0;
+        bool fine = true;
+        for (int64_t tile = first; tile < tiles && fine; tile += step, done++) {
+            // of two tiles that share places the second half of the one, and the first half of the other, first
+            const int half = done & 1, turned = T::kShares && half == 0 ? kApart : 0;
             const int64_t rows0 = tile / p.tiles_n * T::kRows + 128 * rank + 32 * quarter, own0 = tile % p.tiles_n * BN + c0;
-            const int own = rows0 < p.m ? (int)min((int64_t)T::kOwn, p.n - own0) : 0;  // columns there are, 0 or less: nothing here
+            const int own = rows0 < p.m ? (int)min((int64_t)BN, p.n - own0) : 0;  // columns there are from own0 on, 0 or less: nothing here
             auto fetch_residual = [&](int c) {
                 if (lane == 0) {
                     bulk_wait_read<0>();
-                    mbar_expect_tx(&residual_in[taker], 4096);
+                    mbar_expect_tx(&residual_in[taker], T::kBox);
                     load_box3(smem_u32(box), &r_map, (int)own0 + c, (int)rows0, 0, smem_u32(&residual_in[taker]));
                 }
             };
-            if (adds && p.boxes && own > 0) fetch_residual(0);
-            __syncwarp();
-            for (int c = lane; c < T::kOwn; c += 32) bias[c] = p.bias && c < own ? __ldg(p.bias + own0 + c) : 0.f;
-            __syncwarp();
-            const int half = done % T::kSums;
-            if (!__all_sync(0xffffffffu, wait(&sums_done[half], done / T::kSums & 1))) break;
+            bool fetched = adds && p.boxes && turned < own;  // the first box's residual is on its way
+            if (fetched) fetch_residual(turned);
+            if (bias_at != own0) {
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 2; k++) bias[32 * k + lane] = p.bias && kApart * k + lane < own ? __ldg(p.bias + own0 + kApart * k + lane) : 0.f;
+                bias_at = own > 0 ? own0 : -1;  // (rows past the last: nothing was loaded)
+                __syncwarp();
+            }
+            fine = __all_sync(0xffffffffu, wait(&sums_done[half], done >> 1 & 1));
+            if (!fine) break;
             tensor_fence_after();
-            const uint32_t sums = memory + ((uint32_t)quarter << 21) + half * BN + c0;
-            for (int c = 0; c < own; c += 32) {
+            const uint32_t sums = memory + ((uint32_t)quarter << 21) + half * T::kSumsApart + c0;
+#pragma unroll 1
+            for (int k = 0; k < 2; k++) {
+                const int c1 = (kApart * k + turned) % BN;
                 float v[32];
-                load_sums32(sums + c, v);
-                finish_sums<false, true>(p, v, 1.f, bias + c, nullptr, true);
-                if (p.boxes) {
-                    const bool starts = c % width == 0, ends = (c + 32) % width == 0 || c + 32 >= own;
-                    if (starts) {
-                        if (adds) {
-                            if (c > 0) fetch_residual(c);
-                            if (!__all_sync(0xffffffffu, wait(&residual_in[taker], residuals & 1))) break;
-                            residuals++;
-                        } else {
-                            if (lane == 0) bulk_wait_read<0>();
-                            __syncwarp();
-                        }
+                if (c1 < own) load_sums32(sums + c1, v);
+                if (k == (T::kShares ? 0 : 1)) {  // the next tile, once the places that it shares are read (or all); every warp has read the tile before
+                    tensor_fence_before();
+                    __syncwarp();
+                    uint64_t* bar = &sums_free[T::kShares ? 0 : half];
+                    if (lane == 0) arrive_for_tensor_memory(PAIR ? of_rank(smem_u32(bar), 0) : smem_u32(bar));
+                }
+                if (c1 >= own) continue;
+                finish_sums<false, true>(p, v, 1.f, bias + (c1 ? 32 : 0), nullptr, true);
+                unsigned char* row = box + lane * 64;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {  // (fp32, and what is written element by element: 16 columns a box)
+                    const int c = c1 + 16 * h;
+                    if (h && ((p.boxes && !wide) || c >= own)) break;
+                    if (adds && p.boxes) {
+                        if (!fetched) fetch_residual(c);
+                        fetched = false;
+                        fine = __all_sync(0xffffffffu, wait(&residual_in[taker], residuals & 1));
+                        if (!fine) break;
+                        residuals++;
+                    } else if (p.boxes) {
+                        if (lane == 0) bulk_wait_read<0>();
+                        __syncwarp();
                     }
-                    unsigned char* row = box + lane * 128;
-                    if (wide)
-                        box_out<float>(row, lane, 0, v, adds);
+                    if (wide || !p.boxes)
+                        box_out64<float>(row, lane, v, 16 * h, adds && p.boxes);
                     else if (p.d_type == B200_TYPE_BF16)
-                        box_out<bf16>(row, lane, starts ? 0 : 4, v, adds);
+                        box_out64<bf16>(row, lane, v, 0, adds);
                     else
-                        box_out<f16>(row, lane, starts ? 0 : 4, v, adds);
-                    if (ends) {
+                        box_out64<f16>(row, lane, v, 0, adds);
+                    if (p.boxes) {
                         fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) {
-                            store_box3(&d_map, smem_u32(box), (int)own0 + c / width * width, (int)rows0, 0);
+                            store_box3(&d_map, smem_u32(box), (int)own0 + c, (int)rows0, 0);
                             bulk_commit();
                         }
                         __syncwarp();
-                    }
-                } else {  // through the box as fp32, a row of 32 elements at a time
-                    box_out<float>(box + lane * 128, lane, 0, v, false);
-                    __syncwarp();
-                    if (c + lane < own) {
-                        if (p.d_type == B200_TYPE_F32)
-                            column_out<float>(p, box, lane, rows0, own0 + c + lane, adds);
+                    } else {
+                        __syncwarp();
+                        if (wide)
+                            columns_out16<float>(p, box, lane, rows0, own0 + c, adds);
                         else if (p.d_type == B200_TYPE_BF16)
-                            column_out<bf16>(p, box, lane, rows0, own0 + c + lane, adds);
+                            columns_out16<bf16>(p, box, lane, rows0, own0 + c, adds);
                         else
-                            column_out<f16>(p, box, lane, rows0, own0 + c + lane, adds);
+                            columns_out16<f16>(p, box, lane, rows0, own0 + c, adds);
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_at(PAIR ? of_rank(smem_u32(&sums_free[half]), 0) : smem_u32(&sums_free[half]));
         }
         if (lane == 0) bulk_wait_all();
+    } else {  // carries scales on, 32 lanes of them
+        const uint32_t to = memory + ((uint32_t)(warp & 3) << 21) + T::kScalesAt;
+        int s = 0;
+        uint32_t phase = 0;
+        bool fine = true;
+        for (int64_t tile = first; tile < tiles && fine && !dead; tile += step) {
+            for (int kb = 0; kb < p.k_blocks; kb++) {
+                // (they were fetched behind the products that last used this place, here and in tensor memory)
+                fine = __all_sync(0xffffffffu, wait(&scales_in[s], phase));
+                if (!fine) break;
+                tensor_fence_after();
+                // tiles of a's scales for 128 of k each, then for each 128 of k those of b
+                const uint4* from = reinterpret_cast<const uint4*>(base + s * T::kStage + T::kA + T::kB) + lane;
+                uint4 w[T::kScaleWords / 4];
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    w[g] = from[32 * g];
+#pragma unroll
+                    for (int t = 0; t < T::kScaleTiles; t++) w[2 + T::kScaleTiles * g + t] = from[(T::kAScales + 1024 * t + 512 * g) / 16];
+                }
+#pragma unroll
+                for (int k = 0; k < T::kScaleWords / 4; k++) put_scales(to + s * T::kScaleWords + 4 * k, w[k]);
+                scales_stored();
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_for_tensor_memory(PAIR ? of_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]));
+                if (++s == kStages) s = 0, phase ^= 1;
+            }
+        }
     }
     __syncwarp();
     if (dead) {  // what is in flight lands before the CTA's memory goes

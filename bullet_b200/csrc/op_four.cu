@@ -82,9 +82,9 @@ int launch_product(const b200_dense4_op* op, ProductArgs p, cudaStream_t stream)
     if (int rc = make_scales_map(&a_scale, op->x_scale, p.m, p.k, 1)) return rc;
     if (int rc = make_scales_map(&b_scale, op->w_scale, p.n, p.k, T::kScaleTiles)) return rc;
     if (p.boxes) {
-        if (int rc = make_result_map(&d, p.d, p.d_type, p.ldd, p.m, p.n, 1)) return rc;
+        if (int rc = make_result_map(&d, p.d, p.d_type, p.ldd, p.m, p.n, 1, 64)) return rc;
         if (p.residual)
-            if (int rc = make_result_map(&r, p.residual, p.d_type, p.ldr, p.m, p.n, 1)) return rc;
+            if (int rc = make_result_map(&r, p.residual, p.d_type, p.ldr, p.m, p.n, 1, 64)) return rc;
     }
     auto kernel = product4_kernel<BN, PAIR>;
     static std::atomic<uint64_t> allowed;  // a bit per device

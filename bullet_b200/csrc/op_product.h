@@ -28,16 +28,16 @@ inline Encode encoder() {
     }
     return reinterpret_cast<Encode>(found.load());
 }
-// The result, or its parts, as a stack of matrices, in boxes of 32 rows of 128 bytes.
-inline int make_result_map(CUtensorMap* map, const void* at, int type, int64_t ld, int64_t rows, int64_t cols, int64_t count) {
+// The result, or its parts, as a stack of matrices, in boxes of 32 rows of 128 (or 64) bytes, swizzled over as many.
+inline int make_result_map(CUtensorMap* map, const void* at, int type, int64_t ld, int64_t rows, int64_t cols, int64_t count, int bytes = 128) {
     const Encode encode = encoder();
     if (!encode) return fail(B200_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
     const cuuint64_t row = (cuuint64_t)(rows == 1 ? (cols * type_bytes(type) + 15) / 16 * 16 : ld * type_bytes(type));
     const cuuint64_t size[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)count}, stride[2] = {row, (cuuint64_t)rows * (cuuint64_t)(count > 1 ? ld * type_bytes(type) : row)};
-    const cuuint32_t box[3] = {(cuuint32_t)(128 / type_bytes(type)), 32, 1}, each[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)(bytes / type_bytes(type)), 32, 1}, each[3] = {1, 1, 1};
     const CUtensorMapDataType kind = type == B200_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == B200_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const CUresult rc = encode(map, kind, 3, const_cast<void*>(at), size, stride, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult rc = encode(map, kind, 3, const_cast<void*>(at), size, stride, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) on %lld rows of %lld, %lld apart", (int)rc, (long long)rows, (long long)cols, (long long)ld);
     return 0;
 }

@@ -10,18 +10,26 @@ namespace b200 {
 
 // A wait that gives up: the CTA's other waits then end at once, everybody runs on to the end without issuing more, and the host
 // hears of it.  What is waited for are this kernel's own copies and products, which always land; the limit only keeps a broken
-// program from hanging the device.
-struct Waits {
+// program from hanging the device.  CLUSTER: what is waited for makes ordinary writes of the pair's other CTA visible; else this CTA's, and what TMA
+// and the tensor pipe leave (which takes a thread 100 clocks less).
+template <bool CLUSTER>
+struct WaitsFor {
     volatile int* dead;  // of the CTA, in shared memory
     int* gave_up;        // the host's
     static constexpr uint32_t kAsleepNs = 100000;
     __device__ __forceinline__ static bool arrived(uint64_t* bar, uint32_t parity) {  // by threads of either CTA of a pair
         uint32_t ok;
-        asm volatile(
-            "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity), "r"(kAsleepNs)  // (asleep until then: warps that ask again and again cost power)
-            : "memory");
+        // (asleep until then: warps that ask again and again cost power)
+        if constexpr (CLUSTER)
+            asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+                         : "=r"(ok)
+                         : "r"(smem_u32(bar)), "r"(parity), "r"(kAsleepNs)
+                         : "memory");
+        else
+            asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+                         : "=r"(ok)
+                         : "r"(smem_u32(bar)), "r"(parity), "r"(kAsleepNs)
+                         : "memory");
         return ok != 0;
     }
     __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
@@ -35,6 +43,7 @@ struct Waits {
         return false;
     }
 };
+using Waits = WaitsFor<true>;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
