@@ -12,18 +12,21 @@
 //
 // Scales have to lie in tensor memory.  They come with the stages, and four more warps, one for each 32 lanes, carry them on through registers.  The pipe's own
 // copies from shared memory (tcgen05.cp, 512 bytes each) take it 100 clocks a piece, in which it multiplies nothing: six of them 330 ns of a stage's 800, where
-// four products of 256 x 256 x 64 are 280 and the stage's way out of L2 310 to 400.  (Loaded from global memory by those warps, two stages ahead: 1500,
-// as each arrival at a barrier waits for the loads on their way.)
+// its four products of 256 x 256 x 64 are 280 and a stage is now 290.  (Loaded from global memory by those warps: 1500, as each arrival at a barrier
+// waited for the loads on their way.)
 // Two tiles' sums of 256 columns and the scales of five stages do not fit in 512 columns: the tiles overlap by half, which is taken out first.
 // (Scales of two stages, and an overlap of 64 columns: the way from the products that last used a place, by way of those warps, to those that use it
 // next is longer than one stage's products: 1050 ns a stage.)
+//
+// Measured, us: 131072 x 2048 -> 512 73 (3.8 PFLOP/s, under the power cap: 64 with codes of zeros; a tile's eight stages 2.3 us, 0.95 until the next one's begin, 3.6
+// together; HBM 42); 16384 x 1024 -> 2048 24, with a residual 37.
 #pragma once
 #include "kernels_four.cuh"
 #include "product_out.cuh"
 
 namespace b200 {
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool ADDS>
 struct Tile4 {
     static constexpr int kRows = PAIR ? 256 : 128, kOwnColumns = PAIR ? BN / 2 : BN;  // of b, that this CTA fetches
     static constexpr int kScaleTiles = (BN + 127) / 128;                              // of b's rows: each CTA of a pair wants all of them
@@ -31,7 +34,7 @@ struct Tile4 {
     static constexpr int kTakers = BN / 16, kGroups = kTakers / 4;  // warps that take sums out: a quarter of the rows, 32 columns of every 32 kGroups
     static constexpr int kThreads = 64 + 32 * kTakers + 128;
     static constexpr uint32_t kBox = 32 * 64;
-    static constexpr size_t kBoxes = kTakers * kBox, kValues = (size_t)kTakers * 64 * 4, kRest = 1024 + kBoxes + kValues;
+    static constexpr size_t kBoxes = kTakers * kBox * (ADDS ? 2 : 1), kValues = (size_t)kTakers * 64 * 4, kRest = 1024 + kBoxes + kValues;
     static constexpr int kFit = (int)((232448 - 1024 - kRest) / kStage), kStages = kFit < 8 ? kFit : 8;
     static constexpr size_t kShared = kRest + (size_t)kStages * kStage;
     static constexpr int kScaleWords = 2 * 4 * (1 + kScaleTiles);              // columns of tensor memory for a stage's: a's of two tiles of k, b's
@@ -128,14 +131,14 @@ __device__ __forceinline__ void multiply4(uint32_t sums, uint32_t a, uint32_t b,
 #undef B200_MULTIPLY4
 }
 
-template <int BN, bool PAIR>
-static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
+template <int BN, bool PAIR, bool ADDS>
+static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
     product4_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap a_scale_map,
                     const __grid_constant__ CUtensorMap b_scale_map, const __grid_constant__ CUtensorMap d_map, const __grid_constant__ CUtensorMap r_map, const ProductArgs p) {
-    using T = Tile4<BN, PAIR>;
+    using T = Tile4<BN, PAIR, ADDS>;
     constexpr int kStages = T::kStages, kCtas = PAIR ? 2 : 1;
     extern __shared__ unsigned char raw_smem[];
-    __shared__ uint64_t full[kStages], empty[kStages], scales_in[kStages], sums_done[2], sums_free[2], residual_in[T::kTakers];
+    __shared__ uint64_t full[kStages], empty[kStages], scales_in[kStages], sums_done[2], sums_free[2], residual_in[2 * T::kTakers];
     __shared__ uint32_t memory_at;
     __shared__ int dead;
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
@@ -149,7 +152,7 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
             mbar_init(&empty[s], 1);
             mbar_init(&scales_in[s], 1);
         }
-        for (int k = 0; k < T::kTakers; k++) mbar_init(&residual_in[k], 1);
+        for (int k = 0; k < 2 * T::kTakers; k++) mbar_init(&residual_in[k], 1);
         for (int k = 0; k < 2; k++) {
             mbar_init(&sums_done[k], 1);
             mbar_init(&sums_free[k], T::kTakers * kCtas);
@@ -234,27 +237,47 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
     } else if (warp < 2 + T::kTakers) {  // takes sums out: 32 rows, twice 32 columns
         constexpr int kApart = 32 * T::kGroups;
         const int quarter = warp & 3, taker = warp - 2, c0 = taker / 4 * 32;
-        unsigned char* box = base + kStages * T::kStage + taker * T::kBox;
+        unsigned char* const boxes = base + kStages * T::kStage + taker * T::kBox * (ADDS ? 2 : 1);
         float* bias = reinterpret_cast<float*>(base + kStages * T::kStage + T::kBoxes) + taker * 64;
-        const bool wide = p.d_type == B200_TYPE_F32, adds = p.residual;
+        const bool wide = p.d_type == B200_TYPE_F32;
         int64_t bias_at = -1;
-        uint32_t residuals = 0;
-        int64_t done = 0;
+        // Where the boxes lie, in their order: of two tiles that share places the second half of the one, and the first half of the other, first; fp32, and what
+        // is written element by element, 16 columns a box.
+        struct Where {
+            int64_t tile;
+            uint32_t done;
+            int k, h;
+        };
+        auto column_of = [&](uint32_t done, int k) { return (kApart * k + (T::kShares && (done & 1) == 0 ? kApart : 0)) % BN; };  // of the tile, behind c0
+        auto first_row = [&](int64_t tile) { return tile / p.tiles_n * T::kRows + 128 * rank + 32 * quarter; };
+        auto first_column = [&](const Where& w) { return w.tile % p.tiles_n * BN + c0 + column_of(w.done, w.k) + 16 * w.h; };
+        // ADDS and boxes: a box's residual is on its way while the box before it is filled.  (Loaded into registers, 64 bytes of a lane's row, it takes
+        // twice the time: 16384 x 1024 -> 2048 37 us so, 71 in registers, 41 with one box; without a residual 24.)
+        Where next{first, 0, 0, 0};
+        uint32_t filled = 0;  // boxes
+        auto fetch_residual = [&](uint32_t number) {
+            auto on = [&] {
+                next.h = wide && next.h == 0;
+                if (next.h == 0 && (next.k ^= 1) == 0) next.tile += step, next.done++;
+            };
+            while (next.tile < tiles && (first_row(next.tile) >= p.m || first_column(next) >= p.n)) on();
+            if (next.tile >= tiles) return;
+            if (lane == 0) {
+                bulk_wait_read<0>();
+                uint64_t* bar = &residual_in[2 * taker + (number & 1)];
+                mbar_expect_tx(bar, T::kBox);
+                load_box3(smem_u32(boxes + (number & 1) * T::kBox), &r_map, (int)first_column(next), (int)first_row(next.tile), 0, smem_u32(bar));
+            }
+            on();
+        };
+        const bool ahead = ADDS && p.boxes;
+        if (ahead) fetch_residual(0);
+        uint32_t done = 0;
         bool fine = true;
         for (int64_t tile = first; tile < tiles && fine; tile += step, done++) {
-            // of two tiles that share places the second half of the one, and the first half of the other, first
-            const int half = done & 1, turned = T::kShares && half == 0 ? kApart : 0;
-            const int64_t rows0 = tile / p.tiles_n * T::kRows + 128 * rank + 32 * quarter, own0 = tile % p.tiles_n * BN + c0;
+            const int half = done & 1;
+            const int64_t rows0 = first_row(tile), own0 = tile % p.tiles_n * BN + c0;
             const int own = rows0 < p.m ? (int)min((int64_t)BN, p.n - own0) : 0;  // columns there are from own0 on, 0 or less: nothing here
-            auto fetch_residual = [&](int c) {
-                if (lane == 0) {
-                    bulk_wait_read<0>();
-                    mbar_expect_tx(&residual_in[taker], T::kBox);
-                    load_box3(smem_u32(box), &r_map, (int)own0 + c, (int)rows0, 0, smem_u32(&residual_in[taker]));
-                }
-            };
-            bool fetched = adds && p.boxes && turned < own;  // the first box's residual is on its way
-            if (fetched) fetch_residual(turned);
             if (bias_at != own0) {
                 __syncwarp();
 #pragma unroll
@@ -268,7 +291,7 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
             const uint32_t sums = memory + ((uint32_t)quarter << 21) + half * T::kSumsApart + c0;
 #pragma unroll 1
             for (int k = 0; k < 2; k++) {
-                const int c1 = (kApart * k + turned) % BN;
+                const int c1 = column_of(done, k);
                 float v[32];
                 if (c1 < own) load_sums32(sums + c1, v);
                 if (k == (T::kShares ? 0 : 1)) {  // the next tile, once the places that it shares are read (or all); every warp has read the tile before
@@ -279,27 +302,27 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
                 }
                 if (c1 >= own) continue;
                 finish_sums<false, true>(p, v, 1.f, bias + (c1 ? 32 : 0), nullptr, true);
-                unsigned char* row = box + lane * 64;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {  // (fp32, and what is written element by element: 16 columns a box)
+                for (int h = 0; h < 2; h++) {
                     const int c = c1 + 16 * h;
                     if (h && ((p.boxes && !wide) || c >= own)) break;
-                    if (adds && p.boxes) {
-                        if (!fetched) fetch_residual(c);
-                        fetched = false;
-                        fine = __all_sync(0xffffffffu, wait(&residual_in[taker], residuals & 1));
+                    unsigned char* box = boxes + (ahead ? (filled & 1) * T::kBox : 0);
+                    unsigned char* row = box + lane * 64;
+                    if (ahead) {
+                        fetch_residual(filled + 1);
+                        fine = __all_sync(0xffffffffu, wait(&residual_in[2 * taker + (filled & 1)], filled >> 1 & 1));
                         if (!fine) break;
-                        residuals++;
+                        filled++;
                     } else if (p.boxes) {
                         if (lane == 0) bulk_wait_read<0>();
                         __syncwarp();
                     }
                     if (wide || !p.boxes)
-                        box_out64<float>(row, lane, v, 16 * h, adds && p.boxes);
+                        box_out64<float>(row, lane, v, 16 * h, ahead);
                     else if (p.d_type == B200_TYPE_BF16)
-                        box_out64<bf16>(row, lane, v, 0, adds);
+                        box_out64<bf16>(row, lane, v, 0, ahead);
                     else
-                        box_out64<f16>(row, lane, v, 0, adds);
+                        box_out64<f16>(row, lane, v, 0, ahead);
                     if (p.boxes) {
                         fence_proxy_async();
                         __syncwarp();
@@ -311,11 +334,11 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR>::kThreads), 1)
                     } else {
                         __syncwarp();
                         if (wide)
-                            columns_out16<float>(p, box, lane, rows0, own0 + c, adds);
+                            columns_out16<float>(p, box, lane, rows0, own0 + c, ADDS);
                         else if (p.d_type == B200_TYPE_BF16)
-                            columns_out16<bf16>(p, box, lane, rows0, own0 + c, adds);
+                            columns_out16<bf16>(p, box, lane, rows0, own0 + c, ADDS);
                         else
-                            columns_out16<f16>(p, box, lane, rows0, own0 + c, adds);
+                            columns_out16<f16>(p, box, lane, rows0, own0 + c, ADDS);
                         __syncwarp();
                     }
                 }

@@ -33,17 +33,20 @@ dim3 column_grid(int64_t columns, int64_t groups) { return dim3((unsigned)((colu
 
 // ---- products
 
-// Which tile: by what each way costs in clocks, a stage (256 of k) and the rest of a tile, rounds of tiles being whole.
+// Which tile: by what each way costs in ns, from the launch to the first stage, a stage (256 of k), the rest of each tile after the first; rounds of tiles
+// being whole.  Fitted to times of 16 to 131072 rows, 256 to 4096 inputs, 64 to 2048 outputs with either tile: of 75 such layers the choice is the quicker
+// one in all.  Us, 128 x 128 and 256 x 256 of a pair: 300 rows 2048 -> 1024 6.9 and 8.9, 5003 rows 1024 -> 512 7.5 and 7.9, 16384 rows 11.2 and
+// 10.3, 2048 -> 2048 44.9 and 35.6, 131072 rows 1024 -> 64 18.1 and 19.1, 2048 -> 512 94.0 and 72.9.
 struct Way {
-    int columns, rows, units, stage, tile;
+    int columns, rows, units, start, stage, tile;
 };
-constexpr Way kWays[] = {{256, 256, kSms / 2, 900, 4000}, {128, 128, kSms, 800, 2500}};
+constexpr Way kWays[] = {{256, 256, kSms / 2, 6600, 290, 1500}, {128, 128, kSms, 4500, 290, 850}};
 int columns_of(int64_t m, int64_t n, int64_t blocks) {
     int best = 0;
     int64_t least = INT64_MAX;
     for (const Way& w : kWays) {
         const int64_t tiles = ((m + w.rows - 1) / w.rows) * ((n + w.columns - 1) / w.columns), rounds = (tiles + w.units - 1) / w.units;
-        const int64_t cost = rounds * (blocks * w.stage + w.tile);
+        const int64_t cost = w.start + rounds * blocks * w.stage + (rounds - 1) * w.tile;
         if (cost < least) least = cost, best = w.columns;
     }
     return best;
@@ -71,9 +74,9 @@ int make_scales_map(CUtensorMap* map, const void* at, int64_t rows, int64_t n, i
     return 0;
 }
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool ADDS>
 int launch_product(const b200_dense4_op* op, ProductArgs p, cudaStream_t stream) {
-    using T = Tile4<BN, PAIR>;
+    using T = Tile4<BN, PAIR, ADDS>;
     p.tiles_m = (int)((p.m + T::kRows - 1) / T::kRows);
     p.tiles_n = (int)((p.n + BN - 1) / BN);
     CUtensorMap a, b, a_scale, b_scale, d{}, r{};
@@ -86,7 +89,7 @@ int launch_product(const b200_dense4_op* op, ProductArgs p, cudaStream_t stream)
         if (p.residual)
             if (int rc = make_result_map(&r, p.residual, p.d_type, p.ldr, p.m, p.n, 1, 64)) return rc;
     }
-    auto kernel = product4_kernel<BN, PAIR>;
+    auto kernel = product4_kernel<BN, PAIR, ADDS>;
     static std::atomic<uint64_t> allowed;  // a bit per device
     int device = 0;
     OP_CK(cudaGetDevice(&device));
@@ -213,7 +216,8 @@ int b200_op_dense4(int device, void* stream, const b200_dense4_op* op) {
     auto starts = [&](const void* at, int64_t ld) { return (uintptr_t)at % 16 == 0 && (p.m == 1 || ld * size % 16 == 0); };
     // (rows end on 16 bytes as well: boxes that were cut off inside 16 bytes would write into what lies behind the row)
     p.boxes = p.n * size % 16 == 0 && starts(p.d, p.ldd) && (!p.residual || starts(p.residual, p.ldr));
-    return columns_of(p.m, p.n, p.k_blocks) == 256 ? launch_product<256, true>(op, p, s) : launch_product<128, false>(op, p, s);
+    if (columns_of(p.m, p.n, p.k_blocks) == 256) return p.residual ? launch_product<256, true, true>(op, p, s) : launch_product<256, true, false>(op, p, s);
+    return p.residual ? launch_product<128, false, true>(op, p, s) : launch_product<128, false, false>(op, p, s);
 }
 
 }  // extern "C"
