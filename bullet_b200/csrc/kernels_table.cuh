@@ -1,9 +1,12 @@
 // Rows of a table that lists of ids name: their sums per list, and the gradient, the sums of the lists' gradients per row of the table.
 //
-// The gradient's sums are taken in the order of the lists, so ids are sorted first, stably: by counting, a digit of up to eight bits a pass
-// (pass_count_kernel, pass_scan_kernel, pass_place_kernel).  Then a thread takes eight columns of one table row and adds the rows up that its
-// stretch of the sorted ids names.  Stretches of more than kStretch are cut at multiples of kStretch of the sorted order, whose sums go to
-// memory and are joined in order: a piece has parts of two such stretches at most, its first id's and its last one's.
+// Bound by L2's way to the SMs (16384 lists of 17 rows of 2 KB are 590 MB out of a table of 25), with few lists by latency.  A warp takes a list, or a row of the
+// table, and the columns that its lanes cover with 16 bytes each (fewer in narrow matrices; single elements 32 apart where rows do not start on 16 bytes).
+// Its lanes load 32 indices side by side and hand them round, and kAhead rows are on their way at a time.
+//
+// The gradient's sums are taken in the order of the lists, so ids are sorted first, stably, by counting digits of up to eight bits: one CTA for up to kSortOne
+// ids, else three kernels a pass.  Ids that name no row are left out by the first pass.  Then a warp adds up the rows that a table row's stretch of the
+// sorted ids names.  Stretches of more than `piece` are listed and cut into as many, whose sums go to memory and are joined in order.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -13,7 +16,7 @@
 
 namespace b200 {
 
-constexpr int kTableThreads = 256;
+constexpr int kTableThreads = 256, kAhead = 8;  // rows on their way
 
 // ---- sums of rows
 
@@ -23,162 +26,245 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int64_t i, int wide, i
     return id >= 0 && id < n ? id : -1;
 }
 
-template <bool VEC, class T>
-struct Row8 {
-    T v[8];
-    __device__ __forceinline__ void load(const T* row, int64_t first, int64_t cols) {
-        if constexpr (VEC) {
-#pragma unroll
-            for (int k = 0; k < (int)sizeof(T) / 2; k++) reinterpret_cast<uint4*>(v)[k] = __ldg(reinterpret_cast<const uint4*>(row + first) + k);
+// A lane's columns of a warp's: BYTES side by side, or with BYTES 0 as many single elements as 16 bytes hold, 32 apart.
+template <class T, int BYTES>
+struct Lanes {
+    static constexpr int kEach = (BYTES ? BYTES : 16) / (int)sizeof(T), kWarp = 32 * kEach;
+    static __device__ __forceinline__ int64_t first(int64_t chunk) { return chunk * kWarp + (threadIdx.x & 31) * (BYTES ? kEach : 1); }
+    T v[kEach];
+    __device__ __forceinline__ void load(const T* row, int64_t at, int64_t cols) {
+        if constexpr (BYTES == 16) {
+            if (at < cols) *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(row + at));
+        } else if constexpr (BYTES == 8) {
+            if (at < cols) *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(row + at));
+        } else if constexpr (BYTES == 4) {
+            if (at < cols) *reinterpret_cast<uint32_t*>(v) = __ldg(reinterpret_cast<const uint32_t*>(row + at));
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = first + k < cols ? __ldg(row + first + k) : from_float<T>(0.f);
+            for (int k = 0; k < kEach; k++)
+                if (at + 32 * k < cols) v[k] = __ldg(row + at + 32 * k);
         }
     }
-    __device__ __forceinline__ void add(float (&sum)[8]) const {
+    __device__ __forceinline__ void add(float (&sum)[kEach]) const {
+        if constexpr (sizeof(T) == 2 && kEach > 1) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum[k] += to_float(v[k]);
+            for (int k = 0; k < kEach; k += 2) {
+                uint32_t w;
+                memcpy(&w, v + k, 4);
+                float low, high;
+                unpack2<T>(w, low, high);
+                sum[k] += low, sum[k + 1] += high;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kEach; k++) sum[k] += to_float(v[k]);
+        }
     }
 };
-template <bool VEC>
-__device__ __forceinline__ void store_typed(void* y, int64_t row_at, int64_t first, int64_t cols, int type, const float (&v)[8]) {
-    if (type == B200_TYPE_F32)
-        store_values<VEC>(static_cast<float*>(y) + row_at, first, cols, v);
-    else if (type == B200_TYPE_BF16)
-        store_values<VEC>(static_cast<bf16*>(y) + row_at, first, cols, v);
-    else
-        store_values<VEC>(static_cast<f16*>(y) + row_at, first, cols, v);
+// kEach sums to a row of `type`, whose elements start where those of T did (VEC: on as many elements together).
+template <class T, int BYTES, bool VEC>
+__device__ __forceinline__ void store_sums(void* y, int64_t row_at, int64_t at, int64_t cols, int type, const float (&v)[Lanes<T, BYTES>::kEach]) {
+    constexpr int kEach = Lanes<T, BYTES>::kEach;
+    if constexpr (BYTES != 0 && VEC && kEach > 1) {
+        if (at >= cols) return;
+        if (type == B200_TYPE_F32) {
+            float* to = static_cast<float*>(y) + row_at + at;
+            if constexpr (kEach >= 4) {
+#pragma unroll
+                for (int k = 0; k < kEach; k += 4) *reinterpret_cast<float4*>(to + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+            } else {
+                *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+            }
+        } else {
+            uint32_t w[kEach / 2];
+#pragma unroll
+            for (int k = 0; k < kEach / 2; k++) w[k] = type == B200_TYPE_BF16 ? pack2<bf16>(v[2 * k], v[2 * k + 1]) : pack2<f16>(v[2 * k], v[2 * k + 1]);
+            uint16_t* to = static_cast<uint16_t*>(y) + row_at + at;
+            if constexpr (kEach == 8)
+                *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+            else if constexpr (kEach == 4)
+                *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<uint32_t*>(to) = w[0];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kEach; k++) {
+            const int64_t c = at + (BYTES ? k : 32 * k);
+            if (c < cols) store_value(y, row_at + c, type, v[k]);
+        }
+    }
 }
-
-constexpr int kSlotsAhead = 8;
-// A thread takes eight columns of a list.
-template <class T, bool VEC>
-static __global__ void __launch_bounds__(kTableThreads) embed_kernel(b200_embed_op a) {
-    Place p((int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads, (a.cols + 7) / 8);
-    const T* table = static_cast<const T*>(a.table);
-    for (; p.row < a.rows; p.next()) {
-        float sum[8] = {};
-        for (int s = 0; s < a.slots; s += kSlotsAhead) {
-            int64_t id[kSlotsAhead];
-            Row8<VEC, T> row[kSlotsAhead];
+// Adds the rows that the lanes in `mask` name, in the lanes' order.
+template <class T, int BYTES, int AHEAD>
+__device__ __forceinline__ void add_named(const T* rows, int64_t ld, int64_t at, int64_t cols, int index, unsigned mask, float (&sum)[Lanes<T, BYTES>::kEach]) {
+    while (mask) {
+        Lanes<T, BYTES> row[AHEAD];
+        const int there = min(AHEAD, __popc(mask));
 #pragma unroll
-            for (int k = 0; k < kSlotsAhead; k++) id[k] = s + k < a.slots ? id_at(a.ids, p.row * a.ldids + s + k, a.wide_ids, a.n) : -1;
-#pragma unroll
-            for (int k = 0; k < kSlotsAhead; k++)
-                if (id[k] >= 0) row[k].load(table + id[k] * a.ldt, p.at * 8, a.cols);
-#pragma unroll
-            for (int k = 0; k < kSlotsAhead; k++)
-                if (id[k] >= 0) row[k].add(sum);
+        for (int k = 0; k < AHEAD; k++) {
+            const int64_t r = __shfl_sync(0xffffffffu, index, __ffs(mask) - 1);  // (0 left: lane 31's, and not used)
+            mask &= mask - 1;
+            if (k < there) row[k].load(rows + r * ld, at, cols);
         }
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum[k] *= a.scale;
-        store_typed<VEC>(a.y, p.row * a.ldy, p.at * 8, a.cols, a.y_type, sum);
+        for (int k = 0; k < AHEAD; k++)
+            if (k < there) row[k].add(sum);
+    }
+}
+
+// VEC: a row of y takes a lane's elements together.
+template <class T, int BYTES, int AHEAD>
+static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES == 0 ? 2 : 4) embed_kernel(b200_embed_op a, int vec) {
+    using L = Lanes<T, BYTES>;
+    const int lane = threadIdx.x & 31;
+    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), (a.cols + L::kWarp - 1ll) / L::kWarp);
+    for (; p.row < a.rows; p.next()) {
+        const int64_t at = L::first(p.at);
+        float sum[L::kEach] = {};
+        for (int s = 0; s < a.slots; s += 32) {
+            const int64_t id = s + lane < a.slots ? id_at(a.ids, p.row * a.ldids + s + lane, a.wide_ids, a.n) : -1;
+            add_named<T, BYTES, AHEAD>(static_cast<const T*>(a.table), a.ldt, at, a.cols, (int)id, __ballot_sync(0xffffffffu, id >= 0), sum);
+        }
+#pragma unroll
+        for (int k = 0; k < L::kEach; k++) sum[k] *= a.scale;
+        if (vec)
+            store_sums<T, BYTES, true>(a.y, p.row * a.ldy, at, a.cols, a.y_type, sum);
+        else
+            store_sums<T, BYTES, false>(a.y, p.row * a.ldy, at, a.cols, a.y_type, sum);
     }
 }
 
 // ---- ids sorted
 
-constexpr int kSortThreads = 256, kSortEach = 16, kSortTile = kSortThreads * kSortEach, kSortWarps = kSortThreads / 32;
+constexpr int kSortThreads = 256, kSortEach = 8, kSortTile = kSortThreads * kSortEach, kSortWarps = kSortThreads / 32;
 struct SortPass {
     const void* ids;       // the first pass's, in lists
     int64_t ldids;
-    int slots, wide, n;
+    uint32_t slots;
+    int wide, n;
     const int2* from;      // the later ones': (id, list)
     int2* to;
-    int64_t count;         // of ids
+    uint32_t count;        // of ids, there or not
+    int* there;            // how many are: left by the first pass, which the later ones read
     int shift, bits;       // of the digit
-    int* counts;           // [1 << bits][tiles]
+    int* counts;           // [1 << bits][tiles], and behind them [1 << bits]: of a digit all
     int tiles;
 };
-// Element i of a pass: an id (n: none) and the list that it stands in.
-__device__ __forceinline__ int2 sort_element(const SortPass& p, int64_t i) {
+// Element i of a pass, (id, list); (-1, ..) for an id that names no row.
+__device__ __forceinline__ int2 sort_element(const SortPass& p, uint32_t i) {
     if (p.from) return __ldcg(p.from + i);
-    const int64_t list = i / p.slots, id = id_at(p.ids, list * p.ldids + i % p.slots, p.wide, p.n);
-    return make_int2(id < 0 ? p.n : (int)id, (int)list);
+    const uint32_t list = i / p.slots;
+    return make_int2((int)id_at(p.ids, list * p.ldids + (i - list * p.slots), p.wide, p.n), (int)list);
 }
 __device__ __forceinline__ int sort_digit(const SortPass& p, int id) { return id >> p.shift & ((1 << p.bits) - 1); }
 
-static __global__ void __launch_bounds__(kSortThreads) pass_count_kernel(SortPass p) {
+static __global__ void __launch_bounds__(kSortThreads) pass_count_kernel(SortPass p, int* cleared) {
     __shared__ int count[256];
     step_begin(nullptr);
+    if (blockIdx.x == 0 && threadIdx.x < 2 && !p.from) cleared[threadIdx.x] = 0;
     count[threadIdx.x] = 0;
     __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * kSortTile;
-#pragma unroll 4
+    const uint32_t first = blockIdx.x * (uint32_t)kSortTile, all = p.from ? (uint32_t)__ldcg(p.there) : p.count;
+    int id[kSortEach];
+#pragma unroll
     for (int k = 0; k < kSortEach; k++) {
-        const int64_t i = first + k * kSortThreads + threadIdx.x;
-        if (i < p.count) atomicAdd(count + sort_digit(p, sort_element(p, i).x), 1);
+        const uint32_t i = first + k * kSortThreads + threadIdx.x;
+        id[k] = i < all ? sort_element(p, i).x : -1;
     }
+#pragma unroll
+    for (int k = 0; k < kSortEach; k++)
+        if (id[k] >= 0) atomicAdd(count + sort_digit(p, id[k]), 1);
     __syncthreads();
     if (threadIdx.x < 1 << p.bits) p.counts[(int64_t)threadIdx.x * p.tiles + blockIdx.x] = count[threadIdx.x];
 }
-// Counts to where each tile's first element of each digit goes: one CTA.
-static __global__ void __launch_bounds__(1024) pass_scan_kernel(int* counts, int64_t n) {
-    __shared__ int sums[32];
-    step_begin(nullptr);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int before = 0;
-    for (int64_t base = 0; base < n; base += 4096) {
-        const int64_t i = base + threadIdx.x * 4;
-        int v[4], own = 0;
+// The sum of the values of the CTA's threads before this one; `sums`: 33 words, whose last one is then the sum of all.
+__device__ __forceinline__ int sum_before(int own, int* sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
+    int run = own;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            v[k] = i + k < n ? __ldcg(counts + i + k) : 0;
-            own += v[k];
-        }
-        int run = own;
+    for (int o = 1; o < 32; o *= 2) {
+        const int u = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += u;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = run;
+    __syncthreads();
+    if (warp == 0) {
+        const int mine = lane < warps ? sums[lane] : 0;
+        int w = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-            const int u = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += u;
+            const int u = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += u;
         }
-        if (lane == 31) sums[warp] = run;
-        __syncthreads();
-        if (warp == 0) {
-            int w = sums[lane];
+        sums[lane] = w - mine;
+        if (lane == 31) sums[32] = w;
+    }
+    __syncthreads();
+    return sums[warp] + run - own;
+}
+// Of each digit, counts to sums of the tiles before, and the sum of all: a warp a digit.
+static __global__ void __launch_bounds__(kSortThreads) pass_sum_kernel(int* counts, int digits, int tiles) {
+    step_begin(nullptr);
+    const int lane = threadIdx.x & 31, digit = blockIdx.x * kSortWarps + (threadIdx.x >> 5);
+    if (digit >= digits) return;
+    int* own = counts + (int64_t)digit * tiles;
+    int before = 0;
+    for (int base = 0; base < tiles; base += 256) {
+        int v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = base + 32 * k + lane < tiles ? __ldcg(own + base + 32 * k + lane) : 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            int run = v[k];
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
-                const int u = __shfl_up_sync(0xffffffffu, w, o);
-                if (lane >= o) w += u;
+                const int u = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += u;
             }
-            sums[lane] = w;
+            if (base + 32 * k + lane < tiles) own[base + 32 * k + lane] = before + run - v[k];
+            before += __shfl_sync(0xffffffffu, run, 31);
         }
-        __syncthreads();
-        int at = before + (warp ? sums[warp - 1] : 0) + run - own;
-        before += sums[31];
+    }
+    if (lane == 0) counts[(int64_t)digits * tiles + digit] = before;
+}
+// An element's rank among its warp's of the same digit, which take EACH x 32 neighbours in order; count: the warp's, of each digit, counted on.
+template <int EACH>
+__device__ __forceinline__ void warp_ranks(const int (&digit)[EACH], int (&rank)[EACH], int* count) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (i + k < n) counts[i + k] = at;
-            at += v[k];
-        }
-        __syncthreads();
+    for (int k = 0; k < EACH; k++) {
+        const unsigned same = __match_any_sync(0xffffffffu, digit[k]);
+        rank[k] = digit[k] >= 0 ? count[digit[k]] + __popc(same & ((1u << lane) - 1)) : 0;
+        __syncwarp();
+        if (digit[k] >= 0 && same >> lane == 1u) count[digit[k]] = rank[k] + 1;  // (the last of them)
+        __syncwarp();
     }
 }
-// A warp takes kSortEach x 32 neighbours in order: an element's rank among its warp's of the same digit, then the warps before, then the tiles.
+// A warp's elements by their ranks, then the warps before, then the tiles.
 static __global__ void __launch_bounds__(kSortThreads) pass_place_kernel(SortPass p) {
-    __shared__ int count[kSortWarps][256];
+    __shared__ int count[kSortWarps][256], sums[33];
     step_begin(nullptr);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int k = threadIdx.x; k < kSortWarps * 256; k += kSortThreads) count[k >> 8][k & 255] = 0;
     __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * kSortTile + warp * 32 * kSortEach + lane;
+    const uint32_t first = blockIdx.x * (uint32_t)kSortTile + warp * 32 * kSortEach + lane, all = p.from ? (uint32_t)__ldcg(p.there) : p.count;
     int2 element[kSortEach];
-    int rank[kSortEach];
+    int digit[kSortEach], rank[kSortEach];
 #pragma unroll
-    for (int k = 0; k < kSortEach; k++) element[k] = first + k * 32 < p.count ? sort_element(p, first + k * 32) : make_int2(-1, 0);
+    for (int k = 0; k < kSortEach; k++) element[k] = first + k * 32 < all ? sort_element(p, first + k * 32) : make_int2(-1, 0);
 #pragma unroll
-    for (int k = 0; k < kSortEach; k++) {
-        const bool here = first + k * 32 < p.count;
-        const int digit = here ? sort_digit(p, element[k].x) : 256 + lane;
-        const unsigned same = __match_any_sync(0xffffffffu, digit);
-        if (here) rank[k] = count[warp][digit] + __popc(same & ((1u << lane) - 1));
-        __syncwarp();
-        if (here && (same >> lane) == 1u) count[warp][digit] = rank[k] + 1;  // (the last of them)
-        __syncwarp();
-    }
-    __syncthreads();
-    if (threadIdx.x < 1 << p.bits) {
-        int at = __ldcg(p.counts + (int64_t)threadIdx.x * p.tiles + blockIdx.x);
+    for (int k = 0; k < kSortEach; k++) digit[k] = element[k].x >= 0 ? sort_digit(p, element[k].x) : -1;
+    warp_ranks(digit, rank, count[warp]);
+    const int digits = 1 << p.bits;
+    const int of_digit = threadIdx.x < digits ? __ldcg(p.counts + (int64_t)digits * p.tiles + threadIdx.x) : 0;
+    const int before = threadIdx.x < digits ? __ldcg(p.counts + (int64_t)threadIdx.x * p.tiles + blockIdx.x) : 0;
+    const int digits_before = sum_before(of_digit, sums);  // (behind its barriers the counts are complete)
+    if (!p.from && threadIdx.x == 0 && blockIdx.x == 0) *p.there = sums[32];
+    if (threadIdx.x < digits) {
+        int at = digits_before + before;
+#pragma unroll
         for (int w = 0; w < kSortWarps; w++) {
             const int own = count[w][threadIdx.x];
             count[w][threadIdx.x] = at;
@@ -188,19 +274,16 @@ static __global__ void __launch_bounds__(kSortThreads) pass_place_kernel(SortPas
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSortEach; k++)
-        if (first + k * 32 < p.count) p.to[count[warp][sort_digit(p, element[k].x)] + rank[k]] = element[k];
+        if (digit[k] >= 0) p.to[count[warp][digit[k]] + rank[k]] = element[k];
 }
 
-// start[t]: where row t's stretch of the sorted ids begins, t up to n.  A thread per place between two ids fills in the rows that begin there; where
-// there are many (ids far apart) its warp does.
-static __global__ void __launch_bounds__(kTableThreads) stretches_kernel(const int2* sorted, int64_t count, int n, int* start) {
-    step_begin(nullptr);
-    const int64_t i = (int64_t)blockIdx.x * kTableThreads + threadIdx.x;
+// start[t]: where row t's stretch of the sorted ids begins, t up to n.  What lies between two neighbours, `before` at place i - 1 and `id` at i, is filled in by
+// the thread of the second one; where that is much (ids far apart) by its warp, whose places are in a row.
+__device__ __forceinline__ void fill_starts(int64_t i, int before, int id, int* start) {
     const int lane = threadIdx.x & 31;
-    const int before = i == 0 || i > count ? -1 : __ldcg(sorted + i - 1).x, id = i < count ? __ldcg(sorted + i).x : n;
-    const int gap = i <= count ? id - before : 0;
+    const int64_t gap = (int64_t)id - before;
     if (gap > 0 && gap <= 32)
-        for (int t = before + 1; t <= id; t++) start[t] = (int)i;
+        for (int64_t t = before + 1ll; t <= id; t++) start[t] = (int)i;
     for (unsigned wide = __ballot_sync(0xffffffffu, gap > 32); wide; wide &= wide - 1) {
         const int from = __ffs(wide) - 1;
         const int b = __shfl_sync(0xffffffffu, before, from), e = __shfl_sync(0xffffffffu, id, from);
@@ -208,87 +291,168 @@ static __global__ void __launch_bounds__(kTableThreads) stretches_kernel(const i
         for (int64_t t = b + 1ll + lane; t <= e; t += 32) start[t] = at;
     }
 }
+static __global__ void __launch_bounds__(kTableThreads) starts_kernel(const int2* sorted, const int* there, int n, int* start) {
+    step_begin(nullptr);
+    const int64_t i = (int64_t)blockIdx.x * kTableThreads + threadIdx.x, count = __ldcg(there);
+    const int before = i == 0 ? -1 : i <= count ? __ldcg(sorted + i - 1).x : n, id = i < count ? __ldcg(sorted + i).x : n;
+    fill_starts(i, before, id, start);
+}
+
+// Stretches of more than `piece`: `rows` (row, its first piece), `pieces` (row, where the piece begins); how many of each in counts[0] and [1].  In no order of
+// theirs: it says where a piece's sum is kept, not in which order they are joined.
+struct Long {
+    int* counts;
+    int2 *rows, *pieces;
+    int piece;
+};
+__device__ __forceinline__ void list_long(const Long& l, int t, int from, int to) {  // a whole warp, a row a lane (from == to: none)
+    const int lane = threadIdx.x & 31, own = to - from > l.piece ? (to - from + l.piece - 1) / l.piece : 0;
+    int first = 0;
+    if (own) {
+        first = atomicAdd(l.counts + 1, own);
+        l.rows[atomicAdd(l.counts, 1)] = make_int2(t, first);
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, own > 0); left; left &= left - 1) {
+        const int who = __ffs(left) - 1;
+        const int n = __shfl_sync(0xffffffffu, own, who), at = __shfl_sync(0xffffffffu, first, who), row = __shfl_sync(0xffffffffu, t, who), begin = __shfl_sync(0xffffffffu, from, who);
+        for (int k = lane; k < n; k += 32) l.pieces[at + k] = make_int2(row, begin + k * l.piece);
+    }
+}
+static __global__ void __launch_bounds__(kTableThreads) list_long_kernel(const int* start, int n, Long l) {
+    step_begin(nullptr);
+    const int64_t t = (int64_t)blockIdx.x * kTableThreads + threadIdx.x;
+    list_long(l, (int)t, t < n ? __ldcg(start + t) : 0, t < n ? __ldcg(start + t + 1) : 0);
+}
+
+// All passes for up to kSortOne ids, the starts and the long stretches: one CTA, the ids in shared memory between the passes.
+constexpr int kOneThreads = 1024, kOneEach = 8, kSortOne = kOneThreads * kOneEach;
+static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p, int passes, int* start, Long l) {
+    extern __shared__ int2 pairs[];                               // [kSortOne]
+    int* const count = reinterpret_cast<int*>(pairs + kSortOne);  // [32][(1 << bits) + 1]
+    __shared__ int totals[256], sums[33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, apart = digits + 1;
+    int2 element[kOneEach];
+    int digit[kOneEach], rank[kOneEach], all = (int)p.count;
+    if (threadIdx.x < 2) l.counts[threadIdx.x] = 0;
+#pragma unroll
+    for (int k = 0; k < kOneEach; k++) {
+        const int i = (warp * kOneEach + k) * 32 + lane;
+        element[k] = i < all ? sort_element(p, i) : make_int2(-1, 0);
+    }
+    for (int pass = 0; pass < passes; pass++, p.shift += p.bits) {
+        if (pass)
+#pragma unroll
+            for (int k = 0; k < kOneEach; k++) {
+                const int i = (warp * kOneEach + k) * 32 + lane;
+                element[k] = i < all ? pairs[i] : make_int2(-1, 0);
+            }
+        for (int k = threadIdx.x; k < 32 * apart; k += kOneThreads) count[k] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kOneEach; k++) digit[k] = element[k].x >= 0 ? sort_digit(p, element[k].x) : -1;
+        warp_ranks(digit, rank, count + warp * apart);
+        __syncthreads();
+        for (int d = warp; d < digits; d += 32) {  // a lane a warp's count
+            const int own = count[lane * apart + d];
+            int run = own;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int u = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += u;
+            }
+            count[lane * apart + d] = run - own;
+            if (lane == 31) totals[d] = run;
+        }
+        __syncthreads();
+        const int before = sum_before(threadIdx.x < digits ? totals[threadIdx.x] : 0, sums);
+        all = sums[32];
+        if (threadIdx.x < digits) totals[threadIdx.x] = before;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kOneEach; k++)
+            if (digit[k] >= 0) pairs[totals[digit[k]] + count[warp * apart + digit[k]] + rank[k]] = element[k];
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < all; i += kOneThreads) p.to[i] = pairs[i];
+    for (int i = threadIdx.x; i - lane <= all; i += kOneThreads) {  // (whole warps)
+        const int before = i == 0 ? -1 : i <= all ? pairs[i - 1].x : p.n, id = i < all ? pairs[i].x : p.n;
+        fill_starts(i, before, id, start);
+    }
+    if (all <= l.piece) return;
+    __syncthreads();
+    for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads) list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0);
+}
 
 // ---- the gradient
 
-constexpr int kStretch = 64, kRowsAhead = 8;
 struct TableGrad {
     b200_embed_grad_op a;
     const int2* sorted;
     const int* start;
-    float* parts;  // [2][pieces][ldp]: of a piece's first id, and of its last one where that is another
-    int64_t ldp, pieces;
+    Long l;
+    float* parts;  // [pieces][ldp]
+    int64_t ldp;
+    int cuts;      // there may be long stretches
+    int vec;       // a row of dtable takes a lane's elements together
 };
-// The sum of what stretch [from, to) of the sorted ids names.
-template <class T, bool VEC>
-__device__ __forceinline__ void add_stretch(const TableGrad& g, int from, int to, int64_t first, float (&sum)[8]) {
-    const T* dy = static_cast<const T*>(g.a.dy);
-    for (int s = from; s < to; s += kRowsAhead) {
-        Row8<VEC, T> row[kRowsAhead];
-        int list[kRowsAhead];
-#pragma unroll
-        for (int k = 0; k < kRowsAhead; k++) list[k] = s + k < to ? __ldcg(&g.sorted[s + k].y) : -1;
-#pragma unroll
-        for (int k = 0; k < kRowsAhead; k++)
-            if (list[k] >= 0) row[k].load(dy + list[k] * g.a.lddy, first, g.a.cols);
-#pragma unroll
-        for (int k = 0; k < kRowsAhead; k++)
-            if (list[k] >= 0) row[k].add(sum);
-    }
-}
-// Rows of the table, then pieces.
-template <class T, bool VEC>
-static __global__ void __launch_bounds__(kTableThreads) embed_backward_kernel(TableGrad g) {
+// Pieces of the long stretches, then rows of the table.
+template <class T, int BYTES, int AHEAD>
+static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES == 0 ? 2 : 4) embed_backward_kernel(TableGrad g) {
+    using L = Lanes<T, BYTES>;
     step_begin(nullptr);
-    Place p((int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads, (g.a.cols + 7) / 8);
-    for (; p.row < g.a.n + g.pieces; p.next()) {
-        const int64_t first = p.at * 8;
-        if (p.row < g.a.n) {
-            const int from = __ldcg(g.start + p.row), to = __ldcg(g.start + p.row + 1);
-            if (to - from > kStretch) continue;
-            float sum[8] = {};
-            add_stretch<T, VEC>(g, from, to, first, sum);
-#pragma unroll
-            for (int k = 0; k < 8; k++) sum[k] *= g.a.scale;
-            store_typed<VEC>(g.a.dtable, p.row * g.a.lddt, first, g.a.cols, g.a.dtable_type, sum);
+    const int lane = threadIdx.x & 31;
+    const int64_t pieces = g.cuts ? __ldcg(g.l.counts + 1) : 0, all = pieces + g.a.n;
+    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), (g.a.cols + L::kWarp - 1ll) / L::kWarp);
+    for (; p.row < all; p.next()) {
+        const int64_t at = L::first(p.at), t = p.row - pieces;
+        int from, to;
+        if (t < 0) {
+            const int2 piece = __ldcg(g.l.pieces + p.row);
+            from = piece.y, to = min(from + g.l.piece, __ldcg(g.start + piece.x + 1));
         } else {
-            const int64_t piece = p.row - g.a.n;
-            const int all = __ldcg(g.start + g.a.n), begin = (int)(piece * kStretch), end = min(begin + kStretch, all);
-            if (begin >= end) continue;
-            const int id[2] = {__ldcg(&g.sorted[begin].x), __ldcg(&g.sorted[end - 1].x)};
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if (h && id[1] == id[0]) break;
-                const int from = __ldcg(g.start + id[h]), to = __ldcg(g.start + id[h] + 1);
-                if (to - from <= kStretch) continue;
-                float sum[8] = {};
-                add_stretch<T, VEC>(g, max(from, begin), min(to, end), first, sum);
-                store_values<true>(g.parts + (h * g.pieces + piece) * g.ldp, first, g.a.cols, sum);
-            }
+            from = __ldcg(g.start + t), to = __ldcg(g.start + t + 1);
+            if (to - from > g.l.piece) continue;
         }
+        float sum[L::kEach] = {};
+        int list = from + lane < to ? __ldcg(&g.sorted[from + lane].y) : 0;
+        for (int s = from; s < to; s += 32) {
+            const int next = s + 32 + lane < to ? __ldcg(&g.sorted[s + 32 + lane].y) : 0;
+            add_named<T, BYTES, AHEAD>(static_cast<const T*>(g.a.dy), g.a.lddy, at, g.a.cols, list, to - s >= 32 ? 0xffffffffu : (1u << (to - s)) - 1, sum);
+            list = next;
+        }
+        if (t < 0) {
+            store_sums<T, BYTES, true>(g.parts, p.row * g.ldp, at, g.a.cols, B200_TYPE_F32, sum);
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < L::kEach; k++) sum[k] *= g.a.scale;
+        if (g.vec)
+            store_sums<T, BYTES, true>(g.a.dtable, t * g.a.lddt, at, g.a.cols, g.a.dtable_type, sum);
+        else
+            store_sums<T, BYTES, false>(g.a.dtable, t * g.a.lddt, at, g.a.cols, g.a.dtable_type, sum);
     }
 }
-// Rows with stretches that were cut.
-template <bool VEC>
+// Long stretches: a thread four columns of one.
 static __global__ void __launch_bounds__(kTableThreads) embed_join_kernel(TableGrad g) {
     step_begin(nullptr);
-    Place p((int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads, (g.a.cols + 7) / 8);
-    for (; p.row < g.a.n; p.next()) {
-        const int from = __ldcg(g.start + p.row), to = __ldcg(g.start + p.row + 1);
-        if (to - from <= kStretch) continue;
-        const int64_t first = p.at * 8;
-        const int piece0 = from / kStretch, piece1 = (to - 1) / kStretch;
-        float sum[8] = {};
-#pragma unroll 4
-        for (int piece = piece0; piece <= piece1; piece++) {
-            const bool last = piece == piece0 && __ldcg(&g.sorted[piece * kStretch].x) != p.row;  // (it begins behind the piece's first id)
-            const float* part = g.parts + ((last ? g.pieces : 0) + piece) * g.ldp + first;
-            const float4 u = __ldcg(reinterpret_cast<const float4*>(part)), v = __ldcg(reinterpret_cast<const float4*>(part) + 1);
-            sum[0] += u.x, sum[1] += u.y, sum[2] += u.z, sum[3] += u.w, sum[4] += v.x, sum[5] += v.y, sum[6] += v.z, sum[7] += v.w;
+    Place p((int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads, (g.a.cols + 3) / 4);
+    const int rows = __ldcg(g.l.counts);
+    for (; p.row < rows; p.next()) {
+        const int2 row = __ldcg(g.l.rows + p.row);
+        const int n = (__ldcg(g.start + row.x + 1) - __ldcg(g.start + row.x) + g.l.piece - 1) / g.l.piece;
+        const int64_t at = p.at * 4;
+        const float* parts = g.parts + row.y * g.ldp + at;
+        float sum[4] = {};
+        for (int k = 0; k < n; k += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = k + i < n ? __ldcg(reinterpret_cast<const float4*>(parts + (k + i) * g.ldp)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum[0] += v[i].x, sum[1] += v[i].y, sum[2] += v[i].z, sum[3] += v[i].w;
         }
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum[k] *= g.a.scale;
-        store_typed<VEC>(g.a.dtable, p.row * g.a.lddt, first, g.a.cols, g.a.dtable_type, sum);
+        for (int k = 0; k < 4; k++)
+            if (at + k < g.a.cols) store_value(g.a.dtable, row.x * g.a.lddt + at + k, g.a.dtable_type, sum[k] * g.a.scale);
     }
 }
 

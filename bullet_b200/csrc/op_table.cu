@@ -1,5 +1,6 @@
 // Operator-level entry points of tables whose rows are named by ids: b200_op_embed and its gradient.
 #include <algorithm>
+#include <atomic>
 
 #include "kernels_table.cuh"
 #include "op_call.h"
@@ -23,18 +24,44 @@ int check_ids(const char* who, const void* ids, int64_t ld, int rows, int slots,
     if (ld < slots || ld > INT64_MAX / 8 / (rows > 0 ? rows : 1)) return fail(B200_ERR_ARG, "%s: ld of ids is %lld, with lists of %d", who, (long long)ld, slots);
     return 0;
 }
-bool vectors(const void* at, int64_t ld, int cols, int type) { return cols % 8 == 0 && ((uintptr_t)at | (uintptr_t)(ld * type_bytes(type))) % 16 == 0; }
-unsigned ctas_for(int64_t places) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((places + kTableThreads - 1) / kTableThreads, kTableSms * 8)); }
+// How many bytes of a row of `type` a lane takes: 16 where rows start on them, fewer where the warp would have lanes to spare, 0 (single elements) where rows start anywhere.
+int bytes_of(const void* at, int64_t ld, int cols, int type) {
+    const int size = type_bytes(type);
+    for (int bytes = 16; bytes >= 4; bytes /= 2) {
+        if (bytes > 4 && cols * size <= 16 * bytes) continue;  // (half the lanes or fewer)
+        if (((uintptr_t)at | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)cols * size)) % bytes == 0) return bytes;
+        if (cols * size > 128 * 4) return 0;  // (wide rows of pieces smaller than 16 bytes: elements)
+    }
+    return 0;
+}
+// Whether rows of `type` take `each` elements together.
+bool together(const void* at, int64_t ld, int type, int each) {
+    const int64_t bytes = std::min(16, each * type_bytes(type));
+    return ((uintptr_t)at | (uintptr_t)(ld * type_bytes(type))) % bytes == 0;
+}
+template <class F>
+void with_bytes(int bytes, F f) {
+    if (bytes == 16)
+        f(std::integral_constant<int, 16>{});
+    else if (bytes == 8)
+        f(std::integral_constant<int, 8>{});
+    else if (bytes == 4)
+        f(std::integral_constant<int, 4>{});
+    else
+        f(std::integral_constant<int, 0>{});
+}
+unsigned ctas_for(int64_t warps) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((warps + kTableThreads / 32 - 1) / (kTableThreads / 32), kTableSms * 8)); }
 
-// How ids are sorted: in passes of equal digits, by whole tiles.
+// How ids are sorted: in passes of equal digits, by whole tiles, or by one CTA.
 struct Sorting {
     int64_t count;
     int passes, bits, tiles;
+    bool one() const { return count <= kSortOne; }
 };
 Sorting sorting_of(const b200_embed_grad_op* op) {
     Sorting s{(int64_t)op->rows * op->slots};
     int wanted = 1;
-    while (wanted < 31 && op->n >> wanted) wanted++;  // (n itself stands for no row)
+    while (wanted < 31 && (op->n - 1) >> wanted) wanted++;
     s.passes = (wanted + 7) / 8;
     s.bits = (wanted + s.passes - 1) / s.passes;
     s.tiles = (int)((s.count + kSortTile - 1) / kSortTile);
@@ -42,8 +69,10 @@ Sorting sorting_of(const b200_embed_grad_op* op) {
 }
 // Where the parts of a gradient's workspace begin, in bytes.
 struct Space {
-    int64_t pairs, more_pairs, counts, start, parts, all;
-    int64_t pieces, ldp;
+    int64_t pairs, more_pairs, counts, start, numbers, rows, pieces, parts, all;
+    int64_t ldp;
+    int piece;
+    bool cuts;
 };
 Space space_of(const b200_embed_grad_op* op) {
     Space s{};
@@ -55,12 +84,23 @@ Space space_of(const b200_embed_grad_op* op) {
     };
     const Sorting sort = sorting_of(op);
     s.pairs = next(sort.count * 8);
-    s.more_pairs = next(sort.passes > 1 ? sort.count * 8 : 0);
-    s.counts = next(((int64_t)sort.tiles << sort.bits) * 4);
+    if (!sort.one()) {
+        s.more_pairs = next(sort.passes > 1 ? sort.count * 8 : 0);
+        s.counts = next((((int64_t)sort.tiles + 1) << sort.bits) * 4);
+    }
     s.start = next((op->n + 1ll) * 4);
-    s.pieces = sort.count > kStretch ? (sort.count + kStretch - 1) / kStretch : 0;  // (shorter lists have no stretch that is cut)
-    s.ldp = (op->cols + 7ll) / 8 * 8;
-    s.parts = next(2 * s.pieces * s.ldp * 4);
+    s.numbers = next(16);
+    // Pieces short enough for a few thousand warps to share the longest stretches, and no more of them than that takes room for.
+    s.piece = 64;
+    while (s.piece < 512 && sort.count / s.piece > 8192) s.piece *= 2;
+    s.cuts = sort.count > s.piece;
+    if (s.cuts) {  // (a stretch that is cut has more than `piece` ids, so their pieces are fewer than twice the whole ones)
+        const int64_t rows = std::min<int64_t>(op->n, sort.count / s.piece), pieces = sort.count / s.piece + rows;
+        s.rows = next(rows * 8);
+        s.pieces = next(pieces * 8);
+        s.ldp = (op->cols + 7ll) / 8 * 8;
+        s.parts = next(pieces * s.ldp * 4);
+    }
     return s;
 }
 
@@ -86,9 +126,18 @@ int b200_op_embed(int device, void* stream, const b200_embed_op* op) {
     if (int rc = check_matrix(who, "y", op->y, op->ldy, op->rows, op->cols, op->y_type)) return rc;
     OnDevice on(device);
     OP_CK(on.status);
+    const int bytes = bytes_of(op->table, op->ldt, op->cols, op->table_type);
     with_float(op->table_type, [&](auto t) {
-        with_bool(vectors(op->table, op->ldt, op->cols, op->table_type) && vectors(op->y, op->ldy, op->cols, op->y_type), [&](auto v) {
-            embed_kernel<decltype(t), v()><<<ctas_for((int64_t)op->rows * ((op->cols + 7) / 8)), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op);
+        with_bytes(bytes, [&](auto b) {
+            using L = Lanes<decltype(t), b()>;
+            const int64_t warps = op->rows * ((op->cols + L::kWarp - 1ll) / L::kWarp);
+            const int vec = together(op->y, op->ldy, op->y_type, L::kEach);
+            auto go = [&](auto kernel) { kernel<<<ctas_for(warps), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, vec); };
+            // (few warps: as much on its way as registers hold)
+            if (warps <= kTableSms * 8)
+                go(embed_kernel<decltype(t), b(), 2 * kAhead>);
+            else
+                go(embed_kernel<decltype(t), b(), kAhead>);
         });
     });
     OP_CK(cudaGetLastError());
@@ -122,30 +171,53 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     char* base = static_cast<char*>(op->workspace);
     const Sorting sort = sorting_of(op);
     int2* pairs[2] = {reinterpret_cast<int2*>(base + space.pairs), reinterpret_cast<int2*>(base + space.more_pairs)};
-    SortPass p{};
-    p.ids = op->ids, p.ldids = op->ldids, p.slots = op->slots, p.wide = op->wide_ids, p.n = op->n;
-    p.count = sort.count, p.tiles = sort.tiles, p.counts = reinterpret_cast<int*>(base + space.counts), p.bits = sort.bits;
-    for (int k = 0; k < sort.passes; k++) {
-        p.to = pairs[k & 1];
-        p.shift = k * sort.bits;
-        OP_CK(launch_step(k > 0, pass_count_kernel, sort.tiles, kSortThreads, 0, s, p));
-        OP_CK(launch_step(true, pass_scan_kernel, 1, 1024, 0, s, p.counts, (int64_t)sort.tiles << sort.bits));
-        OP_CK(launch_step(true, pass_place_kernel, sort.tiles, kSortThreads, 0, s, p));
-        p.from = p.to;
-    }
     int* start = reinterpret_cast<int*>(base + space.start);
-    OP_CK(launch_step(true, stretches_kernel, (unsigned)((sort.count + kTableThreads) / kTableThreads), kTableThreads, 0, s, p.from, sort.count, op->n, start));
-    const TableGrad g{*op, p.from, start, reinterpret_cast<float*>(base + space.parts), space.ldp, space.pieces};
-    const bool vec_out = vectors(op->dtable, op->lddt, op->cols, op->dtable_type);
-    const int64_t across = (op->cols + 7) / 8;
+    int* numbers = reinterpret_cast<int*>(base + space.numbers);
+    const Long l{numbers, reinterpret_cast<int2*>(base + space.rows), reinterpret_cast<int2*>(base + space.pieces), space.piece};
+    SortPass p{};
+    p.ids = op->ids, p.ldids = op->ldids, p.slots = (uint32_t)op->slots, p.wide = op->wide_ids, p.n = op->n;
+    p.count = (uint32_t)sort.count, p.tiles = sort.tiles, p.bits = sort.bits, p.to = pairs[0];
+    if (sort.one()) {
+        const size_t shared = kSortOne * 8 + (((size_t)32 << sort.bits) + 32) * 4;
+        static std::atomic<uint64_t> allowed;  // a bit per device
+        if (device >= 64 || !(allowed >> device & 1)) {
+            OP_CK(cudaFuncSetAttribute(sort_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortOne * 8 + 32 * 257 * 4));
+            if (device < 64) allowed |= (uint64_t)1 << device;
+        }
+        sort_one_kernel<<<1, kOneThreads, shared, s>>>(p, sort.passes, start, l);
+        OP_CK(cudaGetLastError());
+    } else {
+        p.counts = reinterpret_cast<int*>(base + space.counts);
+        p.there = numbers + 2;
+        for (int k = 0; k < sort.passes; k++) {
+            p.to = pairs[k & 1];
+            p.shift = k * sort.bits;
+            OP_CK(launch_step(k > 0, pass_count_kernel, sort.tiles, kSortThreads, 0, s, p, numbers));
+            OP_CK(launch_step(true, pass_sum_kernel, ((1 << sort.bits) + kSortWarps - 1) / kSortWarps, kSortThreads, 0, s, p.counts, 1 << sort.bits, sort.tiles));
+            OP_CK(launch_step(true, pass_place_kernel, sort.tiles, kSortThreads, 0, s, p));
+            p.from = p.to;
+        }
+        OP_CK(launch_step(true, starts_kernel, (unsigned)((sort.count + kTableThreads) / kTableThreads), kTableThreads, 0, s, p.to, p.there, op->n, start));
+        OP_CK(launch_step(true, list_long_kernel, (unsigned)((op->n + kTableThreads - 1ll) / kTableThreads), kTableThreads, 0, s, start, op->n, l));
+    }
+    TableGrad g{*op, p.to, start, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
+    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type);
     cudaError_t rc = cudaSuccess;
     with_float(op->dy_type, [&](auto t) {
-        with_bool(vectors(op->dy, op->lddy, op->cols, op->dy_type) && vec_out, [&](auto v) {
-            rc = launch_step(true, embed_backward_kernel<decltype(t), v()>, ctas_for((op->n + space.pieces) * across), kTableThreads, 0, s, g);
+        with_bytes(bytes, [&](auto b) {
+            using L = Lanes<decltype(t), b()>;
+            g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kEach);
+            const int64_t across = (op->cols + L::kWarp - 1ll) / L::kWarp, most = (op->n + (space.cuts ? 2 * sort.count / space.piece : 0)) * across;
+            // (few warps: as much on its way as registers hold)
+            rc = most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), 2 * kAhead>, ctas_for(most), kTableThreads, 0, s, g)
+                                        : launch_step(true, embed_backward_kernel<decltype(t), b(), kAhead>, ctas_for(most), kTableThreads, 0, s, g);
         });
     });
     OP_CK(rc);
-    if (space.pieces) OP_CK(launch_step(true, vec_out ? embed_join_kernel<true> : embed_join_kernel<false>, ctas_for(op->n * across), kTableThreads, 0, s, g));
+    if (space.cuts) {
+        const int64_t threads = std::min<int64_t>(op->n, sort.count / space.piece) * ((op->cols + 3) / 4);
+        OP_CK(launch_step(true, embed_join_kernel, (unsigned)std::min<int64_t>((threads + kTableThreads - 1) / kTableThreads, kTableSms * 8), kTableThreads, 0, s, g));
+    }
     return 0;
 }
 
