@@ -26,6 +26,14 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int64_t i, int wide, i
     return id >= 0 && id < n ? id : -1;
 }
 
+// sum += v, a value of 16 bits, by one instruction (the same sum as of the value in 32 bits)
+template <class T>
+__device__ __forceinline__ void add_half(float& sum, uint16_t v) {
+    if constexpr (std::is_same_v<T, bf16>)
+        asm("add.rn.f32.bf16 %0, %1, %0;" : "+f"(sum) : "h"(v));
+    else
+        asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(sum) : "h"(v));
+}
 // A lane's columns of a warp's: BYTES side by side, or with BYTES 0 as many single elements as 16 bytes hold, 32 apart.
 template <class T, int BYTES>
 struct Lanes {
@@ -49,11 +57,11 @@ struct Lanes {
         if constexpr (sizeof(T) == 2 && kEach > 1) {
 #pragma unroll
             for (int k = 0; k < kEach; k += 2) {
-                uint32_t w;
-                memcpy(&w, v + k, 4);
-                float low, high;
-                unpack2<T>(w, low, high);
-                sum[k] += low, sum[k + 1] += high;
+                uint16_t low, high;
+                memcpy(&low, v + k, 2);
+                memcpy(&high, v + k + 1, 2);
+                add_half<T>(sum[k], low);
+                add_half<T>(sum[k + 1], high);
             }
         } else {
 #pragma unroll
@@ -134,6 +142,52 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES 
             store_sums<T, BYTES, false>(a.y, p.row * a.ldy, at, a.cols, a.y_type, sum);
     }
 }
+// Lists of up to kAhead ids: a warp takes as many lists as its lanes have room for, and of these as many at a time as have kAhead ids together.  (One id
+// each, 131072 x 1024 bf16: 147 us a list at a time.)
+template <class T, int BYTES>
+static __global__ void __launch_bounds__(kTableThreads, BYTES == 0 ? 2 : 4) embed_short_kernel(b200_embed_op a, int vec) {
+    using L = Lanes<T, BYTES>;
+    const int lane = threadIdx.x & 31, at_once = kAhead / a.slots, lists = 32 / a.slots / at_once * at_once;
+    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), (a.cols + L::kWarp - 1ll) / L::kWarp);
+    for (; p.row * lists < a.rows; p.next()) {
+        const int64_t at = L::first(p.at), first = p.row * lists;
+        const int there = (int)min((int64_t)lists, a.rows - first);
+        const int list = lane / a.slots;
+        const int id = list < there ? (int)id_at(a.ids, (first + list) * a.ldids + lane % a.slots, a.wide_ids, a.n) : -1;
+        for (int l0 = 0; l0 < there; l0 += at_once) {
+            L row[kAhead];
+            int named = 0;  // a bit each
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int r = __shfl_sync(0xffffffffu, id, (l0 * a.slots + k) & 31);
+                if (k < at_once * a.slots && r >= 0 && l0 * a.slots + k < 32) {
+                    row[k].load(static_cast<const T*>(a.table) + r * a.ldt, at, a.cols);
+                    named |= 1 << k;
+                }
+            }
+            float sum[L::kEach] = {};
+            int slot = 0, l = l0;
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                if (named >> k & 1) row[k].add(sum);
+                if (++slot == a.slots) {
+                    if (l < there && l < l0 + at_once) {
+#pragma unroll
+                        for (int i = 0; i < L::kEach; i++) sum[i] *= a.scale;
+                        if (vec)
+                            store_sums<T, BYTES, true>(a.y, (first + l) * a.ldy, at, a.cols, a.y_type, sum);
+                        else
+                            store_sums<T, BYTES, false>(a.y, (first + l) * a.ldy, at, a.cols, a.y_type, sum);
+                    }
+#pragma unroll
+                    for (int i = 0; i < L::kEach; i++) sum[i] = 0.f;
+                    slot = 0, l++;
+                }
+            }
+        }
+    }
+}
+
 
 // ---- ids sorted
 
@@ -291,31 +345,55 @@ __device__ __forceinline__ void fill_starts(int64_t i, int before, int id, int* 
         for (int64_t t = b + 1ll + lane; t <= e; t += 32) start[t] = at;
     }
 }
+constexpr int kStartsEach = 4;
 static __global__ void __launch_bounds__(kTableThreads) starts_kernel(const int2* sorted, const int* there, int n, int* start) {
     step_begin(nullptr);
-    const int64_t i = (int64_t)blockIdx.x * kTableThreads + threadIdx.x, count = __ldcg(there);
-    const int before = i == 0 ? -1 : i <= count ? __ldcg(sorted + i - 1).x : n, id = i < count ? __ldcg(sorted + i).x : n;
-    fill_starts(i, before, id, start);
+    const int64_t first = (int64_t)blockIdx.x * kTableThreads * kStartsEach + threadIdx.x, count = __ldcg(there);
+    int before[kStartsEach], id[kStartsEach];
+#pragma unroll
+    for (int k = 0; k < kStartsEach; k++) {
+        const int64_t i = first + k * kTableThreads;
+        before[k] = i == 0 ? -1 : i <= count ? __ldcg(&sorted[i - 1].x) : n, id[k] = i < count ? __ldcg(&sorted[i].x) : n;
+    }
+#pragma unroll
+    for (int k = 0; k < kStartsEach; k++) fill_starts(first + k * kTableThreads, before[k], id[k], start);
 }
 
-// Stretches of more than `piece`: `rows` (row, its first piece), `pieces` (row, where the piece begins); how many of each in counts[0] and [1].  In no order of
-// theirs: it says where a piece's sum is kept, not in which order they are joined.
+// The pieces of stretches of more than `piece`: (row, where the piece begins, the row's first piece).  counts[0]: of rows, counts[1]: of pieces.
+//  In no order of theirs: it says where a piece's sum is kept, not in which order they are joined.  done[piece][warp's columns]: at a row's first piece, its
+// seventeenth and so on, of the kGroup pieces from there on, how many are summed; at its second one how many such groups.
+constexpr int kGroup = 16;
 struct Long {
     int* counts;
-    int2 *rows, *pieces;
-    int piece;
+    int4* pieces;
+    int* done;
+    int piece, across;
 };
 __device__ __forceinline__ void list_long(const Long& l, int t, int from, int to) {  // a whole warp, a row a lane (from == to: none)
     const int lane = threadIdx.x & 31, own = to - from > l.piece ? (to - from + l.piece - 1) / l.piece : 0;
-    int first = 0;
-    if (own) {
-        first = atomicAdd(l.counts + 1, own);
-        l.rows[atomicAdd(l.counts, 1)] = make_int2(t, first);
+    const unsigned are = __ballot_sync(0xffffffffu, own > 0);
+    if (!are) return;
+    int run = own;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int u = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += u;
     }
-    for (unsigned left = __ballot_sync(0xffffffffu, own > 0); left; left &= left - 1) {
+    unsigned long long base = 0;
+    if (lane == 31) base = atomicAdd(reinterpret_cast<unsigned long long*>(l.counts), (unsigned long long)run << 32 | (unsigned)__popc(are));
+    base = __shfl_sync(0xffffffffu, base, 31);
+    const int first = (int)(base >> 32) + run - own;
+    auto list = [&](int k, int row, int begin, int at) {
+        l.pieces[at + k] = make_int4(row, begin + k * l.piece, at, 0);
+        if (k % kGroup == 0 || k == 1)
+            for (int c = 0; c < l.across; c++) l.done[(int64_t)(at + k) * l.across + c] = 0;
+    };
+    if (own <= 64)
+        for (int k = 0; k < own; k++) list(k, t, from, first);
+    for (unsigned left = __ballot_sync(0xffffffffu, own > 64); left; left &= left - 1) {  // (together)
         const int who = __ffs(left) - 1;
         const int n = __shfl_sync(0xffffffffu, own, who), at = __shfl_sync(0xffffffffu, first, who), row = __shfl_sync(0xffffffffu, t, who), begin = __shfl_sync(0xffffffffu, from, who);
-        for (int k = lane; k < n; k += 32) l.pieces[at + k] = make_int2(row, begin + k * l.piece);
+        for (int k = lane; k < n; k += 32) list(k, row, begin, at);
     }
 }
 static __global__ void __launch_bounds__(kTableThreads) list_long_kernel(const int* start, int n, Long l) {
@@ -330,10 +408,11 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
     extern __shared__ int2 pairs[];                               // [kSortOne]
     int* const count = reinterpret_cast<int*>(pairs + kSortOne);  // [32][(1 << bits) + 1]
     __shared__ int totals[256], sums[33];
+    __shared__ unsigned long long numbers;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, apart = digits + 1;
     int2 element[kOneEach];
     int digit[kOneEach], rank[kOneEach], all = (int)p.count;
-    if (threadIdx.x < 2) l.counts[threadIdx.x] = 0;
+    if (threadIdx.x == 0) numbers = 0;
 #pragma unroll
     for (int k = 0; k < kOneEach; k++) {
         const int i = (warp * kOneEach + k) * 32 + lane;
@@ -378,9 +457,13 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
         const int before = i == 0 ? -1 : i <= all ? pairs[i - 1].x : p.n, id = i < all ? pairs[i].x : p.n;
         fill_starts(i, before, id, start);
     }
-    if (all <= l.piece) return;
     __syncthreads();
-    for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads) list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0);
+    int* const counts = l.counts;
+    l.counts = reinterpret_cast<int*>(&numbers);
+    if (all > l.piece)
+        for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads) list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0);
+    __syncthreads();
+    if (threadIdx.x < 2) counts[threadIdx.x] = reinterpret_cast<const int*>(&numbers)[threadIdx.x];
 }
 
 // ---- the gradient
@@ -395,19 +478,78 @@ struct TableGrad {
     int cuts;      // there may be long stretches
     int vec;       // a row of dtable takes a lane's elements together
 };
-// Pieces of the long stretches, then rows of the table.
+template <class T, int BYTES>
+__device__ __forceinline__ void finish_row(const TableGrad& g, int64_t t, int64_t at, float (&sum)[Lanes<T, BYTES>::kEach]) {
+#pragma unroll
+    for (int k = 0; k < Lanes<T, BYTES>::kEach; k++) sum[k] *= g.a.scale;
+    if (g.vec)
+        store_sums<T, BYTES, true>(g.a.dtable, t * g.a.lddt, at, g.a.cols, g.a.dtable_type, sum);
+    else
+        store_sums<T, BYTES, false>(g.a.dtable, t * g.a.lddt, at, g.a.cols, g.a.dtable_type, sum);
+}
+// n sums, `apart` pieces from one to the next, added up: a row's, or in place of the first of them a group's.  (A call: in line it would take registers from the
+// loop that the kernel's time goes to.)
+template <class T, int BYTES>
+static __device__ __noinline__ void join_pieces(const TableGrad& g, float* parts, int n, int apart, int64_t t, int64_t at) {
+    constexpr int kEach = Lanes<T, BYTES>::kEach, kJoined = kEach > 4 ? 4 : 8;  // on their way
+    float sum[kEach] = {};
+    for (int q = 0; q < n; q += kJoined) {
+        float v[kJoined][kEach] = {};
+#pragma unroll
+        for (int i = 0; i < kJoined; i++) {
+            const float* row = parts + (int64_t)(q + i) * apart * g.ldp;
+            if (q + i >= n) continue;
+            if constexpr (BYTES != 0 && kEach >= 4) {
+#pragma unroll
+                for (int k = 0; k < kEach; k += 4)
+                    if (at < g.a.cols) {
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(row + at + k));
+                        v[i][k] = f.x, v[i][k + 1] = f.y, v[i][k + 2] = f.z, v[i][k + 3] = f.w;
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kEach; k++) {
+                    const int64_t c = at + (BYTES ? k : 32 * k);
+                    if (c < g.a.cols) v[i][k] = __ldcg(row + c);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kJoined; i++)
+#pragma unroll
+            for (int k = 0; k < kEach; k++) sum[k] += v[i][k];
+    }
+    if (t >= 0)
+        finish_row<T, BYTES>(g, t, at, sum);
+    else
+        store_sums<T, BYTES, true>(parts, 0, at, g.a.cols, B200_TYPE_F32, sum);
+}
+// Counts this warp in; whether it is the last of n.  What the others wrote before is there then.
+__device__ __forceinline__ bool last_of(int* done, int n) {
+    __threadfence();
+    __syncwarp();
+    int before = 0;
+    if ((threadIdx.x & 31) == 0) before = atomicAdd(done, 1);
+    const bool last = __shfl_sync(0xffffffffu, before, 0) == n - 1;
+    if (last) __threadfence();
+    return last;
+}
+// Pieces of the long stretches, then rows of the table.  Who finishes a stretch's last piece joins them all, in their order.
 template <class T, int BYTES, int AHEAD>
-static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES == 0 ? 2 : 4) embed_backward_kernel(TableGrad g) {
+static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES == 0 ? 2 : 3) embed_backward_kernel(const __grid_constant__ TableGrad g) {
     using L = Lanes<T, BYTES>;
     step_begin(nullptr);
     const int lane = threadIdx.x & 31;
     const int64_t pieces = g.cuts ? __ldcg(g.l.counts + 1) : 0, all = pieces + g.a.n;
-    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), (g.a.cols + L::kWarp - 1ll) / L::kWarp);
+    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), g.l.across);
     for (; p.row < all; p.next()) {
-        const int64_t at = L::first(p.at), t = p.row - pieces;
+        const int64_t at = L::first(p.at);
+        const int64_t t = p.row - pieces;
         int from, to;
-        if (t < 0) {
-            const int2 piece = __ldcg(g.l.pieces + p.row);
+        int4 piece;
+        const bool cut = t < 0;
+        if (cut) {
+            piece = __ldcg(g.l.pieces + p.row);
             from = piece.y, to = min(from + g.l.piece, __ldcg(g.start + piece.x + 1));
         } else {
             from = __ldcg(g.start + t), to = __ldcg(g.start + t + 1);
@@ -420,39 +562,21 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES 
             add_named<T, BYTES, AHEAD>(static_cast<const T*>(g.a.dy), g.a.lddy, at, g.a.cols, list, to - s >= 32 ? 0xffffffffu : (1u << (to - s)) - 1, sum);
             list = next;
         }
-        if (t < 0) {
+        if (cut) {
             store_sums<T, BYTES, true>(g.parts, p.row * g.ldp, at, g.a.cols, B200_TYPE_F32, sum);
+            const int n = (__ldcg(g.start + piece.x + 1) - __ldcg(g.start + piece.x) + g.l.piece - 1) / g.l.piece, groups = (n + kGroup - 1) / kGroup;
+            const int own = ((int)p.row - piece.z) / kGroup, of_group = min(kGroup, n - own * kGroup);
+            float* parts = g.parts + piece.z * g.ldp;
+            int* done = g.l.done + (int64_t)piece.z * g.l.across + p.at;
+            if (!last_of(done + (int64_t)own * kGroup * g.l.across, of_group)) continue;
+            if (groups > 1) {
+                join_pieces<T, BYTES>(g, parts + (int64_t)own * kGroup * g.ldp, of_group, 1, -1, at);
+                if (!last_of(done + g.l.across, groups)) continue;
+            }
+            join_pieces<T, BYTES>(g, parts, groups > 1 ? groups : n, groups > 1 ? kGroup : 1, piece.x, at);
             continue;
         }
-#pragma unroll
-        for (int k = 0; k < L::kEach; k++) sum[k] *= g.a.scale;
-        if (g.vec)
-            store_sums<T, BYTES, true>(g.a.dtable, t * g.a.lddt, at, g.a.cols, g.a.dtable_type, sum);
-        else
-            store_sums<T, BYTES, false>(g.a.dtable, t * g.a.lddt, at, g.a.cols, g.a.dtable_type, sum);
-    }
-}
-// Long stretches: a thread four columns of one.
-static __global__ void __launch_bounds__(kTableThreads) embed_join_kernel(TableGrad g) {
-    step_begin(nullptr);
-    Place p((int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads, (g.a.cols + 3) / 4);
-    const int rows = __ldcg(g.l.counts);
-    for (; p.row < rows; p.next()) {
-        const int2 row = __ldcg(g.l.rows + p.row);
-        const int n = (__ldcg(g.start + row.x + 1) - __ldcg(g.start + row.x) + g.l.piece - 1) / g.l.piece;
-        const int64_t at = p.at * 4;
-        const float* parts = g.parts + row.y * g.ldp + at;
-        float sum[4] = {};
-        for (int k = 0; k < n; k += 8) {
-            float4 v[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = k + i < n ? __ldcg(reinterpret_cast<const float4*>(parts + (k + i) * g.ldp)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int i = 0; i < 8; i++) sum[0] += v[i].x, sum[1] += v[i].y, sum[2] += v[i].z, sum[3] += v[i].w;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (at + k < g.a.cols) store_value(g.a.dtable, row.x * g.a.lddt + at + k, g.a.dtable_type, sum[k] * g.a.scale);
+        finish_row<T, BYTES>(g, t, at, sum);
     }
 }
 

@@ -69,11 +69,16 @@ Sorting sorting_of(const b200_embed_grad_op* op) {
 }
 // Where the parts of a gradient's workspace begin, in bytes.
 struct Space {
-    int64_t pairs, more_pairs, counts, start, numbers, rows, pieces, parts, all;
+    int64_t pairs, more_pairs, counts, start, numbers, done, pieces, parts, all;
     int64_t ldp;
-    int piece;
+    int piece, across;
     bool cuts;
 };
+// How many warps' columns a row has.
+int across_of(const b200_embed_grad_op* op) {
+    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
+    return (op->cols + warp - 1) / warp;
+}
 Space space_of(const b200_embed_grad_op* op) {
     Space s{};
     if (op->rows == 0) return s;
@@ -94,10 +99,11 @@ Space space_of(const b200_embed_grad_op* op) {
     s.piece = 64;
     while (s.piece < 512 && sort.count / s.piece > 8192) s.piece *= 2;
     s.cuts = sort.count > s.piece;
+    s.across = across_of(op);
     if (s.cuts) {  // (a stretch that is cut has more than `piece` ids, so their pieces are fewer than twice the whole ones)
-        const int64_t rows = std::min<int64_t>(op->n, sort.count / s.piece), pieces = sort.count / s.piece + rows;
-        s.rows = next(rows * 8);
-        s.pieces = next(pieces * 8);
+        const int64_t pieces = sort.count / s.piece + std::min<int64_t>(op->n, sort.count / s.piece);
+        s.done = next(pieces * s.across * 4);
+        s.pieces = next(pieces * 16);
         s.ldp = (op->cols + 7ll) / 8 * 8;
         s.parts = next(pieces * s.ldp * 4);
     }
@@ -134,8 +140,10 @@ int b200_op_embed(int device, void* stream, const b200_embed_op* op) {
             const int vec = together(op->y, op->ldy, op->y_type, L::kEach);
             auto go = [&](auto kernel) { kernel<<<ctas_for(warps), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, vec); };
             // (few warps: as much on its way as registers hold)
-            if (warps <= kTableSms * 8)
-                go(embed_kernel<decltype(t), b(), 2 * kAhead>);
+            if (op->slots <= kAhead && warps > kTableSms * 8)
+                go(embed_short_kernel<decltype(t), b()>);
+            else if (b() && warps <= kTableSms * 8)
+                go(embed_kernel<decltype(t), b(), b() ? 2 * kAhead : kAhead>);
             else
                 go(embed_kernel<decltype(t), b(), kAhead>);
         });
@@ -173,7 +181,7 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     int2* pairs[2] = {reinterpret_cast<int2*>(base + space.pairs), reinterpret_cast<int2*>(base + space.more_pairs)};
     int* start = reinterpret_cast<int*>(base + space.start);
     int* numbers = reinterpret_cast<int*>(base + space.numbers);
-    const Long l{numbers, reinterpret_cast<int2*>(base + space.rows), reinterpret_cast<int2*>(base + space.pieces), space.piece};
+    const Long l{numbers, reinterpret_cast<int4*>(base + space.pieces), reinterpret_cast<int*>(base + space.done), space.piece, space.across};
     SortPass p{};
     p.ids = op->ids, p.ldids = op->ldids, p.slots = (uint32_t)op->slots, p.wide = op->wide_ids, p.n = op->n;
     p.count = (uint32_t)sort.count, p.tiles = sort.tiles, p.bits = sort.bits, p.to = pairs[0];
@@ -197,7 +205,7 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
             OP_CK(launch_step(true, pass_place_kernel, sort.tiles, kSortThreads, 0, s, p));
             p.from = p.to;
         }
-        OP_CK(launch_step(true, starts_kernel, (unsigned)((sort.count + kTableThreads) / kTableThreads), kTableThreads, 0, s, p.to, p.there, op->n, start));
+        OP_CK(launch_step(true, starts_kernel, (unsigned)((sort.count + kTableThreads * kStartsEach) / (kTableThreads * kStartsEach)), kTableThreads, 0, s, p.to, p.there, op->n, start));
         OP_CK(launch_step(true, list_long_kernel, (unsigned)((op->n + kTableThreads - 1ll) / kTableThreads), kTableThreads, 0, s, start, op->n, l));
     }
     TableGrad g{*op, p.to, start, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
@@ -207,17 +215,13 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
         with_bytes(bytes, [&](auto b) {
             using L = Lanes<decltype(t), b()>;
             g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kEach);
-            const int64_t across = (op->cols + L::kWarp - 1ll) / L::kWarp, most = (op->n + (space.cuts ? 2 * sort.count / space.piece : 0)) * across;
+            const int64_t most = (op->n + (space.cuts ? 2 * sort.count / space.piece : 0)) * space.across;
             // (few warps: as much on its way as registers hold)
-            rc = most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), 2 * kAhead>, ctas_for(most), kTableThreads, 0, s, g)
-                                        : launch_step(true, embed_backward_kernel<decltype(t), b(), kAhead>, ctas_for(most), kTableThreads, 0, s, g);
+            rc = b() && most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), b() ? 2 * kAhead : kAhead>, ctas_for(most), kTableThreads, 0, s, g)
+                                               : launch_step(true, embed_backward_kernel<decltype(t), b(), kAhead>, ctas_for(most), kTableThreads, 0, s, g);
         });
     });
     OP_CK(rc);
-    if (space.cuts) {
-        const int64_t threads = std::min<int64_t>(op->n, sort.count / space.piece) * ((op->cols + 3) / 4);
-        OP_CK(launch_step(true, embed_join_kernel, (unsigned)std::min<int64_t>((threads + kTableThreads - 1) / kTableThreads, kTableSms * 8), kTableThreads, 0, s, g));
-    }
     return 0;
 }
 
