@@ -2,7 +2,7 @@
 //
 // Bound by L2's way to the SMs (16384 lists of 17 rows of 2 KB are 590 MB out of a table of 25), with few lists by latency.  A warp takes a list, or a row of the
 // table, and the columns that its lanes cover with 16 bytes each (fewer in narrow matrices; single elements 32 apart where rows do not start on 16 bytes).
-// Its lanes load 32 indices side by side and hand them round, and kAhead rows are on their way at a time.
+// Its lanes load 32 indices side by side and hand them round, and four to sixteen rows are on their way at a time.
 //
 // The gradient's sums are taken in the order of the lists, so ids are sorted first, stably, by counting digits of up to eight bits: one CTA for up to kSortOne
 // ids, else three kernels a pass.  Ids that name no row are left out by the first pass.  Then a warp adds up the rows that a table row's stretch of the
@@ -16,7 +16,25 @@
 
 namespace b200 {
 
-constexpr int kTableThreads = 256, kAhead = 8;  // rows on their way
+constexpr int kTableThreads = 256;
+// Rows on their way in a warp.  Warps that hide each other's latency count for more than rows in one: 16384 x 32 features of 1024 columns, eight rows and 32 warps of an SM 64 us,
+// four 56; their gradient, whose rows and pieces need more of their indices too, eight and 24 warps 122, eight and 32 110, four and 40 110, four and 48 113, sixteen and 16 148.
+// So many warps as fill the GPU twice over or fewer take sixteen each.
+constexpr int kEmbedAhead = 4, kGradAhead = 8, kFewAhead = 16;
+
+// A warp's place: one of up to 2^32 rows, and of `across` chunks of its columns; next() as many on as there are warps.
+struct WarpPlace {
+    uint32_t row, rows_on;
+    int at, on, across;
+    __device__ explicit WarpPlace(int across_) : across(across_) {
+        const uint32_t warps = gridDim.x * (kTableThreads / 32), own = blockIdx.x * (kTableThreads / 32) + (threadIdx.x >> 5);  // (a grid has few)
+        row = own / across, at = (int)(own % across), rows_on = warps / across, on = (int)(warps % across);
+    }
+    __device__ __forceinline__ void next() {
+        row += rows_on, at += on;
+        if (at >= across) at -= across, row++;
+    }
+};
 
 // ---- sums of rows
 
@@ -123,11 +141,11 @@ __device__ __forceinline__ void add_named(const T* rows, int64_t ld, int64_t at,
 
 // VEC: a row of y takes a lane's elements together.
 template <class T, int BYTES, int AHEAD>
-static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES == 0 ? 2 : 4) embed_kernel(b200_embed_op a, int vec) {
+static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BYTES == 0 ? 2 : 4) embed_kernel(b200_embed_op a, int vec) {
     using L = Lanes<T, BYTES>;
     const int lane = threadIdx.x & 31;
-    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), (a.cols + L::kWarp - 1ll) / L::kWarp);
-    for (; p.row < a.rows; p.next()) {
+    WarpPlace p((int)((a.cols + L::kWarp - 1ll) / L::kWarp));
+    for (; p.row < (uint32_t)a.rows; p.next()) {
         const int64_t at = L::first(p.at);
         float sum[L::kEach] = {};
         for (int s = 0; s < a.slots; s += 32) {
@@ -142,23 +160,23 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES 
             store_sums<T, BYTES, false>(a.y, p.row * a.ldy, at, a.cols, a.y_type, sum);
     }
 }
-// Lists of up to kAhead ids: a warp takes as many lists as its lanes have room for, and of these as many at a time as have kAhead ids together.  (One id
-// each, 131072 x 1024 bf16: 147 us a list at a time.)
+// Lists of up to kEmbedAhead ids: a warp takes as many lists as its lanes have room for, and of these as many at a time as have kEmbedAhead ids together.  (One
+// id each, 131072 x 1024 bf16: 67 us, a list at a time 147.)
 template <class T, int BYTES>
 static __global__ void __launch_bounds__(kTableThreads, BYTES == 0 ? 2 : 4) embed_short_kernel(b200_embed_op a, int vec) {
     using L = Lanes<T, BYTES>;
-    const int lane = threadIdx.x & 31, at_once = kAhead / a.slots, lists = 32 / a.slots / at_once * at_once;
-    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), (a.cols + L::kWarp - 1ll) / L::kWarp);
-    for (; p.row * lists < a.rows; p.next()) {
-        const int64_t at = L::first(p.at), first = p.row * lists;
+    const int lane = threadIdx.x & 31, at_once = kEmbedAhead / a.slots, lists = 32 / a.slots / at_once * at_once;
+    WarpPlace p((int)((a.cols + L::kWarp - 1ll) / L::kWarp));
+    for (; (int64_t)p.row * lists < a.rows; p.next()) {
+        const int64_t at = L::first(p.at), first = (int64_t)p.row * lists;
         const int there = (int)min((int64_t)lists, a.rows - first);
         const int list = lane / a.slots;
         const int id = list < there ? (int)id_at(a.ids, (first + list) * a.ldids + lane % a.slots, a.wide_ids, a.n) : -1;
         for (int l0 = 0; l0 < there; l0 += at_once) {
-            L row[kAhead];
+            L row[kEmbedAhead];
             int named = 0;  // a bit each
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) {
+            for (int k = 0; k < kEmbedAhead; k++) {
                 const int r = __shfl_sync(0xffffffffu, id, (l0 * a.slots + k) & 31);
                 if (k < at_once * a.slots && r >= 0 && l0 * a.slots + k < 32) {
                     row[k].load(static_cast<const T*>(a.table) + r * a.ldt, at, a.cols);
@@ -168,7 +186,7 @@ static __global__ void __launch_bounds__(kTableThreads, BYTES == 0 ? 2 : 4) embe
             float sum[L::kEach] = {};
             int slot = 0, l = l0;
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) {
+            for (int k = 0; k < kEmbedAhead; k++) {
                 if (named >> k & 1) row[k].add(sum);
                 if (++slot == a.slots) {
                     if (l < there && l < l0 + at_once) {
@@ -536,18 +554,18 @@ __device__ __forceinline__ bool last_of(int* done, int n) {
 }
 // Pieces of the long stretches, then rows of the table.  Who finishes a stretch's last piece joins them all, in their order.
 template <class T, int BYTES, int AHEAD>
-static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES == 0 ? 2 : 3) embed_backward_kernel(const __grid_constant__ TableGrad g) {
+static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BYTES == 0 ? 2 : 4) embed_backward_kernel(const __grid_constant__ TableGrad g) {
     using L = Lanes<T, BYTES>;
     step_begin(nullptr);
     const int lane = threadIdx.x & 31;
-    const int64_t pieces = g.cuts ? __ldcg(g.l.counts + 1) : 0, all = pieces + g.a.n;
-    Place p(blockIdx.x * (kTableThreads / 32ll) + (threadIdx.x >> 5), gridDim.x * (kTableThreads / 32ll), g.l.across);
+    const uint32_t pieces = g.cuts ? __ldcg(g.l.counts + 1) : 0, all = pieces + g.a.n;
+    WarpPlace p(g.l.across);
     for (; p.row < all; p.next()) {
         const int64_t at = L::first(p.at);
-        const int64_t t = p.row - pieces;
+        const int t = (int)(p.row - pieces);  // (less than 0: a piece)
         int from, to;
         int4 piece;
-        const bool cut = t < 0;
+        const bool cut = p.row < pieces;
         if (cut) {
             piece = __ldcg(g.l.pieces + p.row);
             from = piece.y, to = min(from + g.l.piece, __ldcg(g.start + piece.x + 1));
@@ -563,7 +581,7 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD > kAhead || BYTES 
             list = next;
         }
         if (cut) {
-            store_sums<T, BYTES, true>(g.parts, p.row * g.ldp, at, g.a.cols, B200_TYPE_F32, sum);
+            store_sums<T, BYTES, true>(g.parts, (int64_t)p.row * g.ldp, at, g.a.cols, B200_TYPE_F32, sum);
             const int n = (__ldcg(g.start + piece.x + 1) - __ldcg(g.start + piece.x) + g.l.piece - 1) / g.l.piece, groups = (n + kGroup - 1) / kGroup;
             const int own = ((int)p.row - piece.z) / kGroup, of_group = min(kGroup, n - own * kGroup);
             float* parts = g.parts + piece.z * g.ldp;

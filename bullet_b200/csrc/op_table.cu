@@ -140,12 +140,12 @@ int b200_op_embed(int device, void* stream, const b200_embed_op* op) {
             const int vec = together(op->y, op->ldy, op->y_type, L::kEach);
             auto go = [&](auto kernel) { kernel<<<ctas_for(warps), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, vec); };
             // (few warps: as much on its way as registers hold)
-            if (op->slots <= kAhead && warps > kTableSms * 8)
+            if (op->slots <= kEmbedAhead && warps > kTableSms * 8)
                 go(embed_short_kernel<decltype(t), b()>);
             else if (b() && warps <= kTableSms * 8)
-                go(embed_kernel<decltype(t), b(), b() ? 2 * kAhead : kAhead>);
+                go(embed_kernel<decltype(t), b(), b() ? kFewAhead : kEmbedAhead>);
             else
-                go(embed_kernel<decltype(t), b(), kAhead>);
+                go(embed_kernel<decltype(t), b(), kEmbedAhead>);
         });
     });
     OP_CK(cudaGetLastError());
@@ -217,8 +217,8 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
             g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kEach);
             const int64_t most = (op->n + (space.cuts ? 2 * sort.count / space.piece : 0)) * space.across;
             // (few warps: as much on its way as registers hold)
-            rc = b() && most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), b() ? 2 * kAhead : kAhead>, ctas_for(most), kTableThreads, 0, s, g)
-                                               : launch_step(true, embed_backward_kernel<decltype(t), b(), kAhead>, ctas_for(most), kTableThreads, 0, s, g);
+            rc = b() && most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), b() ? kFewAhead : kGradAhead>, ctas_for(most), kTableThreads, 0, s, g)
+                                               : launch_step(true, embed_backward_kernel<decltype(t), b(), kGradAhead>, ctas_for(most), kTableThreads, 0, s, g);
         });
     });
     OP_CK(rc);
