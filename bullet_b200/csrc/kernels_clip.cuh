@@ -6,7 +6,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
-#include "kernels_four.cuh"
+#include <cstring>
+
 #include "launch.cuh"
 #include "values.cuh"
 
@@ -29,50 +30,73 @@ struct ClipTotal {
     float* norm;
 };
 
-constexpr int kClipChunk = kClipThreads * 32;
-// f(values, first element, how many of them are there) for this thread's eights of a chunk, four of them
-template <class T, class F>
-__device__ __forceinline__ void chunk_eights(const ClipBatch& b, int tensor, int64_t first, F f) {
-    const T* g = static_cast<const T*>(b.g[tensor]);
-    const int64_t n = b.n[tensor];
-    const bool vec = b.vec[tensor];
-    T in[4][8];
+constexpr int kClipChunk = kClipThreads * 32;  // elements
+// 32 elements of a thread, in pieces of 16 bytes as far apart as the CTA is wide.
+template <class T>
+struct Piece {
+    static constexpr int kEach = 16 / sizeof(T), kMany = 32 / kEach;
+    T v[kMany][kEach];
+    static __device__ __forceinline__ int64_t at(int64_t chunk, int k) { return chunk * kClipChunk + (k * kClipThreads + (int)threadIdx.x) * kEach; }
+    __device__ __forceinline__ void load(const ClipBatch& b, int tensor, int64_t chunk) {
+        const T* g = static_cast<const T*>(b.g[tensor]);
+        const int64_t n = b.n[tensor];
+        const bool vec = b.vec[tensor];
+        if (vec && (chunk + 1) * kClipChunk <= n) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const int64_t at = first + (k * kClipThreads + (int)threadIdx.x) * 8;
-        if (vec && at + 8 <= n) {
+            for (int k = 0; k < kMany; k++) {
+                const uint4 w = *reinterpret_cast<const uint4*>(g + at(chunk, k));
+                memcpy(v[k], &w, 16);
+            }
+            return;
+        }
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(in[k])[i] = *(reinterpret_cast<const uint4*>(g + at) + i);
-        } else {
+        for (int k = 0; k < kMany; k++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) in[k][i] = at + i < n ? g[at + i] : from_float<T>(0.f);
+            for (int i = 0; i < kEach; i++) v[k][i] = at(chunk, k) + i < n ? g[at(chunk, k) + i] : from_float<T>(0.f);
+    }
+    __device__ __forceinline__ double squares() const {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMany; k++)
+#pragma unroll
+            for (int i = 0; i < kEach; i++) sum = fmaf(to_float(v[k][i]), to_float(v[k][i]), sum);
+        if (sum > 0x1p-90f && sum < 0x1p120f) return sum;  // (none of them was lost in the sum, or overflowed)
+        double exact = 0;
+        if (sum == 0.f) {  // (nothing but zeros, as a rule)
+            uint32_t any = 0;
+#pragma unroll
+            for (int k = 0; k < kMany; k++)
+#pragma unroll
+                for (int i = 0; i < kEach; i++) any |= __float_as_uint(to_float(v[k][i])) << 1;
+            if (!any) return exact;
+        }
+#pragma unroll
+        for (int k = 0; k < kMany; k++)
+#pragma unroll
+            for (int i = 0; i < kEach; i++) exact = fma((double)to_float(v[k][i]), (double)to_float(v[k][i]), exact);
+        return exact;
+    }
+    __device__ __forceinline__ void store(const ClipBatch& b, int tensor, int64_t chunk, float share, float then) const {
+        T* out = static_cast<T*>(b.out[tensor]);
+        const int64_t n = b.n[tensor];
+        const bool vec = b.vec[tensor] && (chunk + 1) * kClipChunk <= n;
+#pragma unroll
+        for (int k = 0; k < kMany; k++) {
+            T y[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; i++) y[i] = from_float<T>(to_float(v[k][i]) * share * then);
+            if (vec) {
+                uint4 w;
+                memcpy(&w, y, 16);
+                __stcs(reinterpret_cast<uint4*>(out + at(chunk, k)), w);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kEach; i++)
+                    if (at(chunk, k) + i < n) out[at(chunk, k) + i] = y[i];
+            }
         }
     }
-    f(in, first + (int)threadIdx.x * 8, n, vec);
-}
-template <class T>
-__device__ __forceinline__ double squares(const T (&in)[4][8]) {
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum = fmaf(to_float(in[k][i]), to_float(in[k][i]), sum);
-    if (sum > 0x1p-90f && sum < 0x1p120f) return sum;  // (none of them was lost in the sum, or overflowed)
-    double exact = 0;
-    if (sum == 0.f) {  // (nothing but zeros, as a rule)
-        uint32_t any = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) any |= __float_as_uint(to_float(in[k][i])) << 1;
-        if (!any) return exact;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) exact = fma((double)to_float(in[k][i]), (double)to_float(in[k][i]), exact);
-    return exact;
-}
+};
 template <class F>
 __device__ __forceinline__ void with_kind(int type, F f) {
     if (type == B200_TYPE_F32)
@@ -100,7 +124,9 @@ static __global__ void __launch_bounds__(kClipThreads) squares_kernel(const __gr
     for (int chunk = blockIdx.x; chunk < b.chunks; chunk += gridDim.x) {
         while (tensor + 1 < b.count && b.first[tensor + 1] <= chunk) tensor++;
         with_kind(b.type[tensor], [&](auto t) {
-            chunk_eights<decltype(t)>(b, tensor, (int64_t)(chunk - b.first[tensor]) * kClipChunk, [&](auto& in, int64_t, int64_t, bool) { sum += squares(in); });
+            Piece<decltype(t)> piece;
+            piece.load(b, tensor, chunk - b.first[tensor]);
+            sum += piece.squares();
         });
     }
     sum = cta_sum64(sum, shared);
@@ -132,21 +158,9 @@ static __global__ void __launch_bounds__(kClipThreads) clip_kernel(const __grid_
         while (b.first[tensor] > chunk) tensor--;
         if (!b.out[tensor] || (!clips && b.g[tensor] == b.out[tensor])) continue;
         with_kind(b.type[tensor], [&](auto k) {
-            using T = decltype(k);
-            chunk_eights<T>(b, tensor, (int64_t)(chunk - b.first[tensor]) * kClipChunk, [&](auto& in, int64_t first, int64_t n, bool vec) {
-                T* out = static_cast<T*>(b.out[tensor]);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int64_t at = first + q * kClipThreads * 8;
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = to_float(in[q][i]) * share * then;
-                    if (vec && at + 8 <= n)
-                        store_values<true>(out, at, n, v);
-                    else
-                        store_values<false>(out, at, n, v);
-                }
-            });
+            Piece<decltype(k)> piece;
+            piece.load(b, tensor, chunk - b.first[tensor]);
+            piece.store(b, tensor, chunk - b.first[tensor], share, then);
         });
     }
 }

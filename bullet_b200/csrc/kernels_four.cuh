@@ -7,6 +7,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cstring>
+
 #include "launch.cuh"
 #include "values.cuh"
 
@@ -65,65 +67,108 @@ __device__ __forceinline__ uint32_t four_codes_at(float (&v)[8], uint32_t scale)
     return four_codes(v);
 }
 
-// Eight elements of a row from `first` on; those at or past `cols` are 0.
-template <bool VEC, class T>
-__device__ __forceinline__ void load_eight(const T* row, int64_t first, int64_t cols, T (&v)[8]) {
-    if constexpr (VEC) {
-        if (first < cols) {
-#pragma unroll
-            for (int k = 0; k < (int)sizeof(T) / 2; k++) reinterpret_cast<uint4*>(v)[k] = __ldcs(reinterpret_cast<const uint4*>(row + first) + k);
-            return;
-        }
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = from_float<T>(0.f);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = first + k < cols ? __ldcs(row + first + k) : from_float<T>(0.f);
-    }
-}
 // A place in a matrix of `width` places a row that moves on by the same number of places each time.
 struct Place {
-    int64_t row, at, rows_on, on, width;
-    __device__ Place(int64_t first, int64_t step, int64_t width_) : row(first / width_), at(first % width_), rows_on(step / width_), on(step % width_), width(width_) {}
+    uint32_t row, at, rows_on, on, width;
+    __device__ Place(uint32_t first, uint32_t step, uint32_t width_) : row(first / width_), at(first % width_), rows_on(step / width_), on(step % width_), width(width_) {}
     __device__ __forceinline__ void next() {
         row += rows_on, at += on;
         if (at >= width) at -= width, row++;
     }
 };
 
-// Rows to codes: a thread takes eight elements, four neighbours a group, kFourAhead eights on their way.  Also the scales' bytes past the last
+// WAY: how a thread's elements of a row lie: 2, sixteen together on 32 bytes; 1, eight on 16; 0, eight anywhere.
+template <int WAY>
+constexpr int kFourEach = WAY == 2 ? 16 : 8;
+// Those from `first` on; what lies at or past `cols` is 0.
+template <int WAY, class T>
+__device__ __forceinline__ void load_elements(const T* row, int64_t first, int64_t cols, T (&v)[kFourEach<WAY>]) {
+    constexpr int kBytes = kFourEach<WAY> * sizeof(T);
+    if constexpr (WAY == 2) {
+        uint32_t w[kBytes / 4] = {};
+        if (first < cols)
+#pragma unroll
+            for (int k = 0; k < kBytes / 32; k++)
+                asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[8 * k]), "=r"(w[8 * k + 1]), "=r"(w[8 * k + 2]), "=r"(w[8 * k + 3]), "=r"(w[8 * k + 4]), "=r"(w[8 * k + 5]), "=r"(w[8 * k + 6]), "=r"(w[8 * k + 7])
+                             : "l"(reinterpret_cast<const unsigned char*>(row + first) + 32 * k));
+        memcpy(v, w, kBytes);
+    } else if constexpr (WAY == 1) {
+        uint4 w[kBytes / 16] = {};
+        if (first < cols)
+#pragma unroll
+            for (int k = 0; k < kBytes / 16; k++) w[k] = __ldcs(reinterpret_cast<const uint4*>(row + first) + k);
+        memcpy(v, w, kBytes);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kFourEach<WAY>; k++) v[k] = first + k < cols ? __ldcs(row + first + k) : from_float<T>(0.f);
+    }
+}
+// The largest magnitude of N elements, as the bits of fp32.
+template <class T, int N>
+__device__ __forceinline__ uint32_t most_of(const T (&v)[N]) {
+    uint32_t most = 0;
+    if constexpr (sizeof(T) == 2) {  // two at a time: magnitudes are in the order of their bits
+        uint32_t w[N / 2];
+        memcpy(w, v, sizeof(v));
+#pragma unroll
+        for (int k = 0; k < N / 2; k++) most = __vmaxu2(most, w[k] & 0x7fff7fffu);
+        most = max(most & 0xffffu, most >> 16);
+        const uint16_t bits = (uint16_t)most;
+        T largest;
+        memcpy(&largest, &bits, 2);
+        return __float_as_uint(to_float(largest)) & 0x7fffffffu;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) most = max(most, __float_as_uint(v[k]) & 0x7fffffffu);
+        return most;
+    }
+}
+
+// Rows to codes: a group's elements lie in two or four neighbouring threads, kFourAhead places of a thread are on their way.  Also the scales' bytes past the last
 // row and the last group (127).  HBM bound.
 constexpr int kFourAhead = 4;
-template <class T, bool VEC>
+template <class T, int WAY>
 static __global__ void __launch_bounds__(kFourThreads) pack4_rows_kernel(b200_pack4_op a, FourScales s) {
-    const int64_t rows_all = (a.rows + 127ll) / 128 * 128;  // (times 16 or more places a row: a warp's places are all there or none)
-    Place p((int64_t)blockIdx.x * kFourThreads + threadIdx.x, (int64_t)gridDim.x * kFourThreads, s.across() * 16);
+    constexpr int kEach = kFourEach<WAY>, kShare = 32 / kEach, kAhead = kEach * sizeof(T) > 32 ? kFourAhead / 2 : kFourAhead;
+    const uint32_t rows_all = (uint32_t)((a.rows + 127ll) / 128 * 128);  // (times eight or more places a row: a warp's places are all there or none)
+    Place p(blockIdx.x * kFourThreads + threadIdx.x, gridDim.x * kFourThreads, (uint32_t)s.across() * 4 * kShare);
     const T* x = static_cast<const T*>(a.x);
     uint8_t* q = static_cast<uint8_t*>(a.q);
+    const uint32_t last = (uint32_t)a.rows - 1, groups = (uint32_t)s.groups;
     while (p.row < rows_all) {
-        T in[kFourAhead][8];
+        T in[kAhead][kEach];
         Place ahead = p;
 #pragma unroll
-        for (int k = 0; k < kFourAhead; k++) {
-            load_eight<VEC>(x + min(ahead.row, (int64_t)a.rows - 1) * a.ldx, ahead.at * 8, a.cols, in[k]);
+        for (int k = 0; k < kAhead; k++) {
+            load_elements<WAY>(x + min(ahead.row, last) * a.ldx, (int64_t)ahead.at * kEach, a.cols, in[k]);
             ahead.next();
         }
 #pragma unroll
-        for (int k = 0; k < kFourAhead; k++) {
+        for (int k = 0; k < kAhead; k++) {
             if (p.row >= rows_all) return;
-            float v[8];
-            uint32_t most = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[i] = to_float(in[k][i]);
-                most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
-            }
+            uint32_t most = most_of(in[k]);
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const bool here = p.row < a.rows && p.at < 4 * s.groups;
+            if (kShare == 4) most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const uint32_t group = p.at / kShare;
+            const bool here = p.row <= last && group < groups;
             const uint32_t scale = here ? four_scale(most) : 127;
-            if (here) *reinterpret_cast<uint32_t*>(q + p.row * a.ldq + p.at * 4) = four_codes_at(v, scale);
-            if ((p.at & 3) == 0) a.scale[s.at(p.row, p.at >> 2)] = (uint8_t)scale;
+            if (here) {
+                uint32_t w[kEach / 8];
+#pragma unroll
+                for (int h = 0; h < kEach / 8; h++) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = to_float(in[k][8 * h + i]);
+                    w[h] = four_codes_at(v, scale);
+                }
+                uint8_t* to = q + p.row * a.ldq + p.at * (kEach / 2);
+                if constexpr (kEach == 16)
+                    *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+                else
+                    *reinterpret_cast<uint32_t*>(to) = w[0];
+            }
+            if (p.at % kShare == 0) a.scale[s.at(p.row, group)] = (uint8_t)scale;
             p.next();
         }
     }
@@ -181,31 +226,58 @@ __device__ __forceinline__ void store_values(T* row, int64_t first, int64_t cols
     }
 }
 
-// Codes to values, eight a thread.
-template <class T, bool VEC>
+// Codes to values: sixteen a thread where rows of values start on 32 bytes, else eight.
+template <class T, int WAY>
 static __global__ void __launch_bounds__(kFourThreads) unpack4_rows_kernel(b200_unpack4_op a, FourScales s) {
-    Place p((int64_t)blockIdx.x * kFourThreads + threadIdx.x, (int64_t)gridDim.x * kFourThreads, (a.cols + 7) / 8);
+    constexpr int kEach = kFourEach<WAY>;
+    Place p(blockIdx.x * kFourThreads + threadIdx.x, gridDim.x * kFourThreads, (uint32_t)((a.cols + kEach - 1ll) / kEach));
     const uint8_t* q = static_cast<const uint8_t*>(a.q);
-    while (p.row < a.rows) {
-        uint32_t code[kFourAhead];
+    const uint32_t rows = (uint32_t)a.rows;
+    while (p.row < rows) {
+        uint2 code[kFourAhead];
         uint8_t scale[kFourAhead];
         Place ahead = p;
 #pragma unroll
         for (int k = 0; k < kFourAhead; k++) {
-            const int64_t row = min(ahead.row, (int64_t)a.rows - 1);
-            code[k] = __ldcs(reinterpret_cast<const uint32_t*>(q + row * a.ldq + ahead.at * 4));
-            scale[k] = __ldg(a.scale + s.at(row, ahead.at >> 2));
+            const uint32_t row = min(ahead.row, rows - 1);
+            const uint8_t* from = q + row * a.ldq + ahead.at * (kEach / 2);
+            if constexpr (kEach == 16)
+                code[k] = __ldcs(reinterpret_cast<const uint2*>(from));
+            else
+                code[k].x = __ldcs(reinterpret_cast<const uint32_t*>(from));
+            scale[k] = __ldg(a.scale + s.at(row, ahead.at * kEach / 32));
             ahead.next();
         }
 #pragma unroll
         for (int k = 0; k < kFourAhead; k++) {
-            if (p.row >= a.rows) return;
-            float v[8];
-            four_values(code[k], v);
+            if (p.row >= rows) return;
             const float f = four_value(scale[k]);
+            float v[kEach / 8][8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] *= f;
-            store_values<VEC>(static_cast<T*>(a.y) + p.row * a.ldy, p.at * 8, a.cols, v);
+            for (int h = 0; h < kEach / 8; h++) {
+                four_values(h ? code[k].y : code[k].x, v[h]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[h][i] *= f;
+            }
+            T* y = static_cast<T*>(a.y) + p.row * a.ldy;
+            const int64_t first = (int64_t)p.at * kEach;
+            if constexpr (WAY == 2) {
+                uint32_t w[kEach * sizeof(T) / 4];
+#pragma unroll
+                for (int i = 0; i < kEach; i += 2) {
+                    if constexpr (sizeof(T) == 4)
+                        w[i] = __float_as_uint(v[i / 8][i % 8]), w[i + 1] = __float_as_uint(v[i / 8][i % 8 + 1]);
+                    else
+                        w[i / 2] = pack2<T>(v[i / 8][i % 8], v[i / 8][i % 8 + 1]);
+                }
+#pragma unroll
+                for (int i = 0; i < (int)(kEach * sizeof(T) / 4); i += 8)
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(y + first) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
+                                 "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                                 : "memory");
+            } else {
+                store_values<WAY == 1>(y, first, a.cols, v[0]);
+            }
             p.next();
         }
     }

@@ -23,7 +23,20 @@ int check_codes(const char* who, const char* what, const void* at, int64_t ld, i
         return fail(B200_ERR_ARG, "%s: ld of %s is %lld bytes, with rows of %lld codes", who, what, (long long)ld, (long long)n);
     return 0;
 }
-bool vectors(const void* at, int64_t ld, int cols, int type) { return cols % 8 == 0 && ((uintptr_t)at | (uintptr_t)(ld * type_bytes(type))) % 16 == 0; }
+// How elements lie in rows (kFourEach).
+int way_of(const void* at, int64_t ld, int cols, int type) {
+    const uintptr_t places = (uintptr_t)at | (uintptr_t)(ld * type_bytes(type));
+    return cols % 16 == 0 && places % 32 == 0 ? 2 : cols % 8 == 0 && places % 16 == 0 ? 1 : 0;
+}
+template <class F>
+void with_way(int way, F f) {
+    if (way == 2)
+        f(std::integral_constant<int, 2>{});
+    else if (way == 1)
+        f(std::integral_constant<int, 1>{});
+    else
+        f(std::integral_constant<int, 0>{});
+}
 // CTAs for `places` of a thread each, kFourAhead at a time
 unsigned ctas_for(int64_t places) {
     constexpr int64_t each = kFourThreads * kFourAhead;
@@ -149,8 +162,8 @@ int b200_op_pack4(int device, void* stream, const b200_pack4_op* op) {
         if (op->by_column)
             pack4_columns_kernel<T><<<column_grid((rows + 127) / 128 * 128, scales.groups), kFourThreads, 0, s>>>(*op, scales);
         else
-            with_bool(vectors(op->x, op->ldx, op->cols, op->x_type), [&](auto v) {
-                pack4_rows_kernel<T, v()><<<ctas_for((rows + 127) / 128 * 128 * scales.across() * 16), kFourThreads, 0, s>>>(*op, scales);
+            with_way(way_of(op->x, op->ldx, op->cols, op->x_type), [&](auto w) {
+                pack4_rows_kernel<T, w()><<<ctas_for((rows + 127) / 128 * 128 * scales.across() * 128 / kFourEach<w()>), kFourThreads, 0, s>>>(*op, scales);
             });
     });
     OP_CK(cudaGetLastError());
@@ -174,8 +187,8 @@ int b200_op_unpack4(int device, void* stream, const b200_unpack4_op* op) {
         if (op->by_column)
             unpack4_columns_kernel<T><<<column_grid(rows, scales.groups), kFourThreads, 0, s>>>(*op, scales);
         else
-            with_bool(vectors(op->y, op->ldy, op->cols, op->y_type), [&](auto v) {
-                unpack4_rows_kernel<T, v()><<<ctas_for(rows * ((op->cols + 7) / 8)), kFourThreads, 0, s>>>(*op, scales);
+            with_way(way_of(op->y, op->ldy, op->cols, op->y_type), [&](auto w) {
+                unpack4_rows_kernel<T, w()><<<ctas_for(rows * ((op->cols + kFourEach<w()> - 1ll) / kFourEach<w()>)), kFourThreads, 0, s>>>(*op, scales);
             });
     });
     OP_CK(cudaGetLastError());
