@@ -6,7 +6,7 @@
 //
 // The gradient's sums are taken in the order of the lists, so ids are sorted first, stably, by counting digits of up to eight bits: one CTA for up to kSortOne
 // ids, else three kernels a pass.  Ids that name no row are left out by the first pass.  Then a warp adds up the rows that a table row's stretch of the
-// sorted ids names.  Stretches of more than `piece` are listed and cut into as many, whose sums go to memory and are joined in order.
+// sorted ids names.  Stretches of more than kLongest are listed and cut into pieces, whose sums go to memory and are joined in order.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -377,18 +377,41 @@ static __global__ void __launch_bounds__(kTableThreads) starts_kernel(const int2
     for (int k = 0; k < kStartsEach; k++) fill_starts(first + k * kTableThreads, before[k], id[k], start);
 }
 
-// The pieces of stretches of more than `piece`: (row, where the piece begins, the row's first piece).  counts[0]: of rows, counts[1]: of pieces.
-//  In no order of theirs: it says where a piece's sum is kept, not in which order they are joined.  done[piece][warp's columns]: at a row's first piece, its
-// seventeenth and so on, of the kGroup pieces from there on, how many are summed; at its second one how many such groups.
-constexpr int kGroup = 16;
+// A piece of a stretch of more than kLongest: [begin, end) of the sorted ids, and of its row the first piece and how many there are.
+struct alignas(16) Piece8 {
+    int row, begin, end, first, pieces, rest[3];
+};
+__device__ __forceinline__ Piece8 load_piece(const Piece8* at) {
+    Piece8 p;
+    const int4 u = __ldcg(reinterpret_cast<const int4*>(at));
+    p.row = u.x, p.begin = u.y, p.end = u.z, p.first = u.w, p.pieces = __ldcg(&at->pieces);
+    return p;
+}
+// counts[0]: of long rows, counts[1]: of their pieces.  In no order of theirs: it says where a piece's sum is kept, not in which order they are joined.
+// A row's pieces are joined kGroup at a time, their sums kGroup at a time, and so on; done[piece][warp's columns] says how many members of a group are there: of a group of
+// level l, of kGroup^(l + 1) pieces, at the piece l behind its first one.
+constexpr int kLongest = 64, kGroup = 16;
 struct Long {
     int* counts;
-    int4* pieces;
+    Piece8* pieces;
     int* done;
     int piece, across;
 };
-__device__ __forceinline__ void list_long(const Long& l, int t, int from, int to) {  // a whole warp, a row a lane (from == to: none)
-    const int lane = threadIdx.x & 31, own = to - from > l.piece ? (to - from + l.piece - 1) / l.piece : 0;
+struct Stretch {
+    int row, begin, end, pieces, first;
+};
+__device__ __forceinline__ void list_piece(const Long& l, const Stretch& s, int k) {
+    const int begin = s.begin + k * l.piece;
+    int4* to = reinterpret_cast<int4*>(l.pieces + s.first + k);
+    to[0] = make_int4(s.row, begin, min(begin + l.piece, s.end), s.first);
+    to[1] = make_int4(s.pieces, 0, 0, 0);
+    if (k % kGroup < 8)
+        for (int c = 0; c < l.across; c++) l.done[(int64_t)(s.first + k) * l.across + c] = 0;
+}
+// A whole warp, a row a lane (from == to: none).  f(stretch), by one lane: those of more pieces than the lane lists by itself.
+template <class F>
+__device__ __forceinline__ void list_long(const Long& l, int t, int from, int to, F f) {
+    const int lane = threadIdx.x & 31, own = to - from > kLongest ? (to - from + l.piece - 1) / l.piece : 0;
     const unsigned are = __ballot_sync(0xffffffffu, own > 0);
     if (!are) return;
     int run = own;
@@ -400,24 +423,23 @@ __device__ __forceinline__ void list_long(const Long& l, int t, int from, int to
     unsigned long long base = 0;
     if (lane == 31) base = atomicAdd(reinterpret_cast<unsigned long long*>(l.counts), (unsigned long long)run << 32 | (unsigned)__popc(are));
     base = __shfl_sync(0xffffffffu, base, 31);
-    const int first = (int)(base >> 32) + run - own;
-    auto list = [&](int k, int row, int begin, int at) {
-        l.pieces[at + k] = make_int4(row, begin + k * l.piece, at, 0);
-        if (k % kGroup == 0 || k == 1)
-            for (int c = 0; c < l.across; c++) l.done[(int64_t)(at + k) * l.across + c] = 0;
-    };
-    if (own <= 64)
-        for (int k = 0; k < own; k++) list(k, t, from, first);
-    for (unsigned left = __ballot_sync(0xffffffffu, own > 64); left; left &= left - 1) {  // (together)
-        const int who = __ffs(left) - 1;
-        const int n = __shfl_sync(0xffffffffu, own, who), at = __shfl_sync(0xffffffffu, first, who), row = __shfl_sync(0xffffffffu, t, who), begin = __shfl_sync(0xffffffffu, from, who);
-        for (int k = lane; k < n; k += 32) list(k, row, begin, at);
-    }
+    const Stretch s{t, from, to, own, (int)(base >> 32) + run - own};
+    if (own > 32)
+        f(s);
+    else
+        for (int k = 0; k < own; k++) list_piece(l, s, k);
 }
 static __global__ void __launch_bounds__(kTableThreads) list_long_kernel(const int* start, int n, Long l) {
+    __shared__ Stretch many[kTableThreads];
+    __shared__ int count;
+    if (threadIdx.x == 0) count = 0;
     step_begin(nullptr);
+    __syncthreads();
     const int64_t t = (int64_t)blockIdx.x * kTableThreads + threadIdx.x;
-    list_long(l, (int)t, t < n ? __ldcg(start + t) : 0, t < n ? __ldcg(start + t + 1) : 0);
+    list_long(l, (int)t, t < n ? __ldcg(start + t) : 0, t < n ? __ldcg(start + t + 1) : 0, [&](const Stretch& s) { many[atomicAdd(&count, 1)] = s; });
+    __syncthreads();
+    for (int q = 0; q < count; q++)
+        for (int k = threadIdx.x; k < many[q].pieces; k += kTableThreads) list_piece(l, many[q], k);
 }
 
 // All passes for up to kSortOne ids, the starts and the long stretches: one CTA, the ids in shared memory between the passes.
@@ -425,12 +447,13 @@ constexpr int kOneThreads = 1024, kOneEach = 8, kSortOne = kOneThreads * kOneEac
 static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p, int passes, int* start, Long l) {
     extern __shared__ int2 pairs[];                               // [kSortOne]
     int* const count = reinterpret_cast<int*>(pairs + kSortOne);  // [32][(1 << bits) + 1]
-    __shared__ int totals[256], sums[33];
+    __shared__ int totals[256], sums[33], count_many;
     __shared__ unsigned long long numbers;
+    __shared__ Stretch many[kSortOne / kLongest];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, apart = digits + 1;
     int2 element[kOneEach];
     int digit[kOneEach], rank[kOneEach], all = (int)p.count;
-    if (threadIdx.x == 0) numbers = 0;
+    if (threadIdx.x == 0) numbers = 0, count_many = 0;
 #pragma unroll
     for (int k = 0; k < kOneEach; k++) {
         const int i = (warp * kOneEach + k) * 32 + lane;
@@ -478,9 +501,12 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
     __syncthreads();
     int* const counts = l.counts;
     l.counts = reinterpret_cast<int*>(&numbers);
-    if (all > l.piece)
-        for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads) list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0);
+    if (all > kLongest)
+        for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads)
+            list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0, [&](const Stretch& s) { many[atomicAdd(&count_many, 1)] = s; });
     __syncthreads();
+    for (int q = 0; q < count_many; q++)
+        for (int k = threadIdx.x; k < many[q].pieces; k += kOneThreads) list_piece(l, many[q], k);
     if (threadIdx.x < 2) counts[threadIdx.x] = reinterpret_cast<const int*>(&numbers)[threadIdx.x];
 }
 
@@ -552,49 +578,70 @@ __device__ __forceinline__ bool last_of(int* done, int n) {
     if (last) __threadfence();
     return last;
 }
-// Pieces of the long stretches, then rows of the table.  Who finishes a stretch's last piece joins them all, in their order.
+// The sum of stretch [from, to) of the sorted ids.
+template <class T, int BYTES, int AHEAD>
+__device__ __forceinline__ void sum_stretch(const TableGrad& g, int from, int to, int64_t at, float (&sum)[Lanes<T, BYTES>::kEach]) {
+    const int lane = threadIdx.x & 31;
+    int list = from + lane < to ? __ldcg(&g.sorted[from + lane].y) : 0;
+    for (int s = from; s < to; s += 32) {
+        const int next = s + 32 + lane < to ? __ldcg(&g.sorted[s + 32 + lane].y) : 0;
+        add_named<T, BYTES, AHEAD>(static_cast<const T*>(g.a.dy), g.a.lddy, at, g.a.cols, list, to - s >= 32 ? 0xffffffffu : (1u << (to - s)) - 1, sum);
+        list = next;
+    }
+}
+// Pieces of the long stretches, a warp each, then rows of the table.  Who finishes the last member of a group joins them, in their order.  A CTA's warps count their
+// pieces together, behind one fence.
 template <class T, int BYTES, int AHEAD>
 static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BYTES == 0 ? 2 : 4) embed_backward_kernel(const __grid_constant__ TableGrad g) {
     using L = Lanes<T, BYTES>;
+    constexpr uint32_t kWarps = kTableThreads / 32;
+    __shared__ int joins[kWarps];
     step_begin(nullptr);
-    const int lane = threadIdx.x & 31;
-    const uint32_t pieces = g.cuts ? __ldcg(g.l.counts + 1) : 0, all = pieces + g.a.n;
-    WarpPlace p(g.l.across);
-    for (; p.row < all; p.next()) {
-        const int64_t at = L::first(p.at);
-        const int t = (int)(p.row - pieces);  // (less than 0: a piece)
-        int from, to;
-        int4 piece;
-        const bool cut = p.row < pieces;
-        if (cut) {
-            piece = __ldcg(g.l.pieces + p.row);
-            from = piece.y, to = min(from + g.l.piece, __ldcg(g.start + piece.x + 1));
-        } else {
-            from = __ldcg(g.start + t), to = __ldcg(g.start + t + 1);
-            if (to - from > g.l.piece) continue;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, across = g.l.across;
+    const uint32_t items = g.cuts ? __ldcg(g.l.counts + 1) * across : 0;
+    for (uint32_t base = blockIdx.x * kWarps; base < items; base += gridDim.x * kWarps) {
+        const uint32_t item = base + warp;
+        const int64_t at = L::first(item % across);
+        if (item < items) {
+            const Piece8 piece = load_piece(g.l.pieces + item / across);
+            float sum[L::kEach] = {};
+            sum_stretch<T, BYTES, AHEAD>(g, piece.begin, piece.end, at, sum);
+            store_sums<T, BYTES, true>(g.parts, (int64_t)(item / across) * g.ldp, at, g.a.cols, B200_TYPE_F32, sum);
         }
-        float sum[L::kEach] = {};
-        int list = from + lane < to ? __ldcg(&g.sorted[from + lane].y) : 0;
-        for (int s = from; s < to; s += 32) {
-            const int next = s + 32 + lane < to ? __ldcg(&g.sorted[s + 32 + lane].y) : 0;
-            add_named<T, BYTES, AHEAD>(static_cast<const T*>(g.a.dy), g.a.lddy, at, g.a.cols, list, to - s >= 32 ? 0xffffffffu : (1u << (to - s)) - 1, sum);
-            list = next;
-        }
-        if (cut) {
-            store_sums<T, BYTES, true>(g.parts, (int64_t)p.row * g.ldp, at, g.a.cols, B200_TYPE_F32, sum);
-            const int n = (__ldcg(g.start + piece.x + 1) - __ldcg(g.start + piece.x) + g.l.piece - 1) / g.l.piece, groups = (n + kGroup - 1) / kGroup;
-            const int own = ((int)p.row - piece.z) / kGroup, of_group = min(kGroup, n - own * kGroup);
-            float* parts = g.parts + piece.z * g.ldp;
-            int* done = g.l.done + (int64_t)piece.z * g.l.across + p.at;
-            if (!last_of(done + (int64_t)own * kGroup * g.l.across, of_group)) continue;
-            if (groups > 1) {
-                join_pieces<T, BYTES>(g, parts + (int64_t)own * kGroup * g.ldp, of_group, 1, -1, at);
-                if (!last_of(done + g.l.across, groups)) continue;
+        __syncthreads();
+        if (warp == 0) {
+            __threadfence();
+            if (lane < kWarps && base + lane < items) {
+                const uint32_t row = (base + lane) / across, chunk = (base + lane) % across;
+                const Piece8 piece = load_piece(g.l.pieces + row);
+                const int group = ((int)row - piece.first) / kGroup * kGroup;
+                joins[lane] = atomicAdd(g.l.done + (int64_t)(piece.first + group) * across + chunk, 1) == min(kGroup, piece.pieces - group) - 1;
             }
-            join_pieces<T, BYTES>(g, parts, groups > 1 ? groups : n, groups > 1 ? kGroup : 1, piece.x, at);
-            continue;
         }
-        finish_row<T, BYTES>(g, t, at, sum);
+        __syncthreads();
+        if (item < items && joins[warp]) {
+            __threadfence();
+            const Piece8 piece = load_piece(g.l.pieces + item / across);
+            const int n = piece.pieces, own = (int)(item / across) - piece.first;
+            for (int apart = 1, level = 1;; apart *= kGroup, level++) {  // of the members of a group, whose first one's place takes their sum
+                const int first = own / (apart * kGroup) * (apart * kGroup);
+                const bool all = (n - 1) / apart < kGroup;
+                join_pieces<T, BYTES>(g, g.parts + (int64_t)(piece.first + first) * g.ldp, min(kGroup, (n - first + apart - 1) / apart), apart, all ? piece.row : -1, at);
+                if (all) break;
+                const int next = apart * kGroup, next_first = own / next / kGroup * kGroup * next;
+                const int members = min(kGroup, (n - next_first + next - 1) / next);
+                if (members > 1 && !last_of(g.l.done + (int64_t)(piece.first + next_first + level) * across + item % across, members)) break;
+            }
+        }
+    }
+    WarpPlace p((int)across);
+    for (; p.row < (uint32_t)g.a.n; p.next()) {
+        const int64_t at = L::first(p.at);
+        const int from = __ldcg(g.start + p.row), to = __ldcg(g.start + p.row + 1);
+        if (to - from > kLongest) continue;
+        float sum[L::kEach] = {};
+        sum_stretch<T, BYTES, AHEAD>(g, from, to, at, sum);
+        finish_row<T, BYTES>(g, p.row, at, sum);
     }
 }
 

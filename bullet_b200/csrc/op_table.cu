@@ -95,15 +95,16 @@ Space space_of(const b200_embed_grad_op* op) {
     }
     s.start = next((op->n + 1ll) * 4);
     s.numbers = next(16);
-    // Pieces short enough for a few thousand warps to share the longest stretches, and no more of them than that takes room for.
-    s.piece = 64;
-    while (s.piece < 512 && sort.count / s.piece > 8192) s.piece *= 2;
-    s.cuts = sort.count > s.piece;
+    // Pieces of 16 for few ids, whose longest stretches then have warps enough (5003 ids of 8 rows of 520: 64 27 us, 16 23), of 64 for many, as each piece costs its part of
+    // the joining (131072 ids of 8 rows of 1024: 16 159 us, 32 118, 64 90; 2^20 lists' ids of 768 rows of 256: 64 100, 512 128); more where they would take more room.
+    s.piece = 16;
+    while (s.piece < 64 ? sort.count / s.piece > 2048 : s.piece < 512 && sort.count / s.piece > 16384) s.piece *= 2;
+    s.cuts = sort.count > kLongest;
     s.across = across_of(op);
-    if (s.cuts) {  // (a stretch that is cut has more than `piece` ids, so their pieces are fewer than twice the whole ones)
-        const int64_t pieces = sort.count / s.piece + std::min<int64_t>(op->n, sort.count / s.piece);
+    if (s.cuts) {  // (whole pieces, and of each long stretch one that is none)
+        const int64_t pieces = sort.count / s.piece + std::min<int64_t>(op->n, sort.count / kLongest);
         s.done = next(pieces * s.across * 4);
-        s.pieces = next(pieces * 16);
+        s.pieces = next(pieces * (int64_t)sizeof(Piece8));
         s.ldp = (op->cols + 7ll) / 8 * 8;
         s.parts = next(pieces * s.ldp * 4);
     }
@@ -181,7 +182,7 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     int2* pairs[2] = {reinterpret_cast<int2*>(base + space.pairs), reinterpret_cast<int2*>(base + space.more_pairs)};
     int* start = reinterpret_cast<int*>(base + space.start);
     int* numbers = reinterpret_cast<int*>(base + space.numbers);
-    const Long l{numbers, reinterpret_cast<int4*>(base + space.pieces), reinterpret_cast<int*>(base + space.done), space.piece, space.across};
+    const Long l{numbers, reinterpret_cast<Piece8*>(base + space.pieces), reinterpret_cast<int*>(base + space.done), space.piece, space.across};
     SortPass p{};
     p.ids = op->ids, p.ldids = op->ldids, p.slots = (uint32_t)op->slots, p.wide = op->wide_ids, p.n = op->n;
     p.count = (uint32_t)sort.count, p.tiles = sort.tiles, p.bits = sort.bits, p.to = pairs[0];
@@ -215,7 +216,7 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
         with_bytes(bytes, [&](auto b) {
             using L = Lanes<decltype(t), b()>;
             g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kEach);
-            const int64_t most = (op->n + (space.cuts ? 2 * sort.count / space.piece : 0)) * space.across;
+            const int64_t most = (op->n + (space.cuts ? sort.count / space.piece : 0)) * space.across;
             // (few warps: as much on its way as registers hold)
             rc = b() && most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), b() ? kFewAhead : kGradAhead>, ctas_for(most), kTableThreads, 0, s, g)
                                                : launch_step(true, embed_backward_kernel<decltype(t), b(), kGradAhead>, ctas_for(most), kTableThreads, 0, s, g);

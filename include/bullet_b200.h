@@ -594,7 +594,8 @@ typedef struct b200_embed_op {
 int b200_op_embed(int device, void* stream, const b200_embed_op* op);
 
 /* Its gradient at the table: dtable[t] = scale * sum of dy[r] over all r, s with ids[r][s] == t, 0 for a row that none names.  The ids are sorted
- * and the sums taken in the order of the lists, stretches of 64 (of more than 2^19 ids: of up to 512) by themselves where there are more. */
+ * and the sums taken in the order of the lists; where a row is met more than 64 times, 16 to 512 of them by themselves (by the number of all ids), whose sums are added up
+ * sixteen at a time. */
 typedef struct b200_embed_grad_op {
     int32_t rows, slots, n, cols;
     int32_t dy_type, dtable_type;  /* B200_TYPE_F32, _BF16 or _F16 */
