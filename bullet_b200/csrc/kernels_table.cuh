@@ -223,11 +223,35 @@ struct SortPass {
     int* counts;           // [1 << bits][tiles], and behind them [1 << bits]: of a digit all
     int tiles;
 };
-// Element i of a pass, (id, list); (-1, ..) for an id that names no row.
-__device__ __forceinline__ int2 sort_element(const SortPass& p, uint32_t i) {
-    if (p.from) return __ldcg(p.from + i);
-    const uint32_t list = i / p.slots;
-    return make_int2((int)id_at(p.ids, list * p.ldids + (i - list * p.slots), p.wide, p.n), (int)list);
+// Elements first, first + apart, ... of a pass's `all`, (id, list), loaded together; (-1, ..) for an id that names no row and past the last one.
+template <int EACH>
+__device__ __forceinline__ void sort_elements(const SortPass& p, uint32_t first, uint32_t apart, uint32_t all, int2 (&element)[EACH]) {
+#pragma unroll
+    for (int k = 0; k < EACH; k++) element[k] = make_int2(-1, 0);
+    if (first >= all) return;
+    if (p.from) {
+#pragma unroll
+        for (int k = 0; k < EACH; k++) element[k] = __ldcg(p.from + min(first + k * apart, all - 1));
+    } else {
+        int64_t at[EACH], id[EACH];
+#pragma unroll
+        for (int k = 0; k < EACH; k++) {
+            const uint32_t i = min(first + k * apart, all - 1), list = p.slots == 1 ? i : i / p.slots;
+            element[k].y = (int)list, at[k] = list * p.ldids + (i - list * p.slots);
+        }
+        if (p.wide) {
+#pragma unroll
+            for (int k = 0; k < EACH; k++) id[k] = static_cast<const int64_t*>(p.ids)[at[k]];
+        } else {
+#pragma unroll
+            for (int k = 0; k < EACH; k++) id[k] = static_cast<const int32_t*>(p.ids)[at[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < EACH; k++) element[k].x = id[k] >= 0 && id[k] < p.n ? (int)id[k] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; k++)
+        if (first + k * apart >= all) element[k].x = -1;
 }
 __device__ __forceinline__ int sort_digit(const SortPass& p, int id) { return id >> p.shift & ((1 << p.bits) - 1); }
 
@@ -238,15 +262,11 @@ static __global__ void __launch_bounds__(kSortThreads) pass_count_kernel(SortPas
     count[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t first = blockIdx.x * (uint32_t)kSortTile, all = p.from ? (uint32_t)__ldcg(p.there) : p.count;
-    int id[kSortEach];
-#pragma unroll
-    for (int k = 0; k < kSortEach; k++) {
-        const uint32_t i = first + k * kSortThreads + threadIdx.x;
-        id[k] = i < all ? sort_element(p, i).x : -1;
-    }
+    int2 element[kSortEach];
+    sort_elements(p, first + threadIdx.x, kSortThreads, all, element);
 #pragma unroll
     for (int k = 0; k < kSortEach; k++)
-        if (id[k] >= 0) atomicAdd(count + sort_digit(p, id[k]), 1);
+        if (element[k].x >= 0) atomicAdd(count + sort_digit(p, element[k].x), 1);
     __syncthreads();
     if (threadIdx.x < 1 << p.bits) p.counts[(int64_t)threadIdx.x * p.tiles + blockIdx.x] = count[threadIdx.x];
 }
@@ -324,8 +344,7 @@ static __global__ void __launch_bounds__(kSortThreads) pass_place_kernel(SortPas
     const uint32_t first = blockIdx.x * (uint32_t)kSortTile + warp * 32 * kSortEach + lane, all = p.from ? (uint32_t)__ldcg(p.there) : p.count;
     int2 element[kSortEach];
     int digit[kSortEach], rank[kSortEach];
-#pragma unroll
-    for (int k = 0; k < kSortEach; k++) element[k] = first + k * 32 < all ? sort_element(p, first + k * 32) : make_int2(-1, 0);
+    sort_elements(p, first, 32, all, element);
 #pragma unroll
     for (int k = 0; k < kSortEach; k++) digit[k] = element[k].x >= 0 ? sort_digit(p, element[k].x) : -1;
     warp_ranks(digit, rank, count[warp]);
@@ -454,11 +473,7 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
     int2 element[kOneEach];
     int digit[kOneEach], rank[kOneEach], all = (int)p.count;
     if (threadIdx.x == 0) numbers = 0, count_many = 0;
-#pragma unroll
-    for (int k = 0; k < kOneEach; k++) {
-        const int i = (warp * kOneEach + k) * 32 + lane;
-        element[k] = i < all ? sort_element(p, i) : make_int2(-1, 0);
-    }
+    sort_elements(p, warp * kOneEach * 32 + lane, 32, p.count, element);
     for (int pass = 0; pass < passes; pass++, p.shift += p.bits) {
         if (pass)
 #pragma unroll
@@ -505,8 +520,8 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
         for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads)
             list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0, [&](const Stretch& s) { many[atomicAdd(&count_many, 1)] = s; });
     __syncthreads();
-    for (int q = 0; q < count_many; q++)
-        for (int k = threadIdx.x; k < many[q].pieces; k += kOneThreads) list_piece(l, many[q], k);
+    for (int q = warp; q < count_many; q += 32)
+        for (int k = lane; k < many[q].pieces; k += 32) list_piece(l, many[q], k);
     if (threadIdx.x < 2) counts[threadIdx.x] = reinterpret_cast<const int*>(&numbers)[threadIdx.x];
 }
 
