@@ -6,6 +6,10 @@
     h8 = pack8(h, act=ACT_CRELU)                                                      # all that the backward keeps of h
     dx, dw, db = dense_backward(dh, y, w, y=h8, act=ACT_CRELU)
     dx, dweight = rms_norm_backward(dx, total, rstd, weight, dtotal=dtotal)
+    h = dense(pack4(x), pack4(w, by_column=True), bias=b, act=ACT_CRELU)              # in 4 bits
+    delta = embed(table, ids)                                                         # rows by feature or bucket
+    dtable = embed_backward(ddelta, ids, len(table))
+    gradients, norm = clip_gradients(gradients, 1.0, out=gradients)
 
 Weights are [in, out], which is the networks' column-major out x in matrix.  Matrices may have any distance between rows, the
 elements of a row are consecutive.  Calls enqueue on torch's current stream of their tensors' device and do not wait; new

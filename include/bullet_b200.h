@@ -379,12 +379,12 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
  * Common to all of them:
  *   - they only enqueue on `stream` (NULL = the default stream), allocate nothing, leave the thread's current device as it
  *     was and may be captured into a graph (each once outside a capture before); memory of theirs is the caller's until the stream has passed the call;
- *   - matrices have rows of consecutive elements; `ld*` is the distance of two rows in elements, at least their length.
+ *   - matrices have rows of consecutive elements; `ld*` is the distance of two rows in elements (of codes of 4 bits, in bytes), at least their length.
  *     Any ld and any address aligned to the element will do.  Faster are, in products, rows that start on 16 bytes; over rows
  *     (norm, packing, dz) multiples of eight columns in rows that start on eight elements (fp32: 32 bytes), with a norm's
  *     weight on 32 bytes: all matrices of a call, or its rows are read element by element.  Indices are 64-bit;
  *   - no rows: nothing is done (gradients of weights become 0) and B200_OK returned;
- *   - outputs overlap neither inputs nor one another;
+ *   - outputs overlap neither inputs nor one another (b200_op_clip_gradients may write where it reads);
  *   - scratch is lent by the caller: b200_op_*_workspace says how many bytes the very operation needs that is then called
  *     (its addresses and distances count);
  *   - all sums are held in 32 bits and taken in the same order by every call of the same shape and alignment: equal inputs
