@@ -427,9 +427,27 @@ __device__ __forceinline__ void list_piece(const Long& l, const Stretch& s, int 
     if (k % kGroup < 8)
         for (int c = 0; c < l.across; c++) l.done[(int64_t)(s.first + k) * l.across + c] = 0;
 }
-// A whole warp, a row a lane (from == to: none).  f(stretch), by one lane: those of more pieces than the lane lists by itself.
-template <class F>
-__device__ __forceinline__ void list_long(const Long& l, int t, int from, int to, F f) {
+// Long stretches of more pieces than a lane lists by itself: those for a warp in front, those for all warps behind.
+template <int ROOM>
+struct ManyPieces {
+    Stretch of[ROOM];
+    int warps, all;  // how many
+    __device__ __forceinline__ void add(const Stretch& s) {
+        if (s.pieces > 256)
+            of[ROOM - 1 - atomicAdd(&all, 1)] = s;
+        else
+            of[atomicAdd(&warps, 1)] = s;
+    }
+    __device__ __forceinline__ void list(const Long& l) const {
+        for (int q = (int)threadIdx.x >> 5; q < warps; q += (int)blockDim.x >> 5)
+            for (int k = threadIdx.x & 31; k < of[q].pieces; k += 32) list_piece(l, of[q], k);
+        for (int q = 0; q < all; q++)
+            for (int k = threadIdx.x; k < of[ROOM - 1 - q].pieces; k += (int)blockDim.x) list_piece(l, of[ROOM - 1 - q], k);
+    }
+};
+// A whole warp, a row a lane (from == to: none).
+template <int ROOM>
+__device__ __forceinline__ void list_long(const Long& l, int t, int from, int to, ManyPieces<ROOM>& many) {
     const int lane = threadIdx.x & 31, own = to - from > kLongest ? (to - from + l.piece - 1) / l.piece : 0;
     const unsigned are = __ballot_sync(0xffffffffu, own > 0);
     if (!are) return;
@@ -443,22 +461,20 @@ __device__ __forceinline__ void list_long(const Long& l, int t, int from, int to
     if (lane == 31) base = atomicAdd(reinterpret_cast<unsigned long long*>(l.counts), (unsigned long long)run << 32 | (unsigned)__popc(are));
     base = __shfl_sync(0xffffffffu, base, 31);
     const Stretch s{t, from, to, own, (int)(base >> 32) + run - own};
-    if (own > 32)
-        f(s);
+    if (own > 4)
+        many.add(s);
     else
         for (int k = 0; k < own; k++) list_piece(l, s, k);
 }
 static __global__ void __launch_bounds__(kTableThreads) list_long_kernel(const int* start, int n, Long l) {
-    __shared__ Stretch many[kTableThreads];
-    __shared__ int count;
-    if (threadIdx.x == 0) count = 0;
+    __shared__ ManyPieces<kTableThreads> many;
+    if (threadIdx.x == 0) many.warps = many.all = 0;
     step_begin(nullptr);
     __syncthreads();
     const int64_t t = (int64_t)blockIdx.x * kTableThreads + threadIdx.x;
-    list_long(l, (int)t, t < n ? __ldcg(start + t) : 0, t < n ? __ldcg(start + t + 1) : 0, [&](const Stretch& s) { many[atomicAdd(&count, 1)] = s; });
+    list_long(l, (int)t, t < n ? __ldcg(start + t) : 0, t < n ? __ldcg(start + t + 1) : 0, many);
     __syncthreads();
-    for (int q = 0; q < count; q++)
-        for (int k = threadIdx.x; k < many[q].pieces; k += kTableThreads) list_piece(l, many[q], k);
+    many.list(l);
 }
 
 // All passes for up to kSortOne ids, the starts and the long stretches: one CTA, the ids in shared memory between the passes.
@@ -466,13 +482,13 @@ constexpr int kOneThreads = 1024, kOneEach = 8, kSortOne = kOneThreads * kOneEac
 static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p, int passes, int* start, Long l) {
     extern __shared__ int2 pairs[];                               // [kSortOne]
     int* const count = reinterpret_cast<int*>(pairs + kSortOne);  // [32][(1 << bits) + 1]
-    __shared__ int totals[256], sums[33], count_many;
+    __shared__ int totals[256], sums[33];
     __shared__ unsigned long long numbers;
-    __shared__ Stretch many[kSortOne / kLongest];
+    __shared__ ManyPieces<kSortOne / kLongest> many;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, apart = digits + 1;
     int2 element[kOneEach];
     int digit[kOneEach], rank[kOneEach], all = (int)p.count;
-    if (threadIdx.x == 0) numbers = 0, count_many = 0;
+    if (threadIdx.x == 0) numbers = 0, many.warps = many.all = 0;
     sort_elements(p, warp * kOneEach * 32 + lane, 32, p.count, element);
     for (int pass = 0; pass < passes; pass++, p.shift += p.bits) {
         if (pass)
@@ -517,11 +533,9 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
     int* const counts = l.counts;
     l.counts = reinterpret_cast<int*>(&numbers);
     if (all > kLongest)
-        for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads)
-            list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0, [&](const Stretch& s) { many[atomicAdd(&count_many, 1)] = s; });
+        for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads) list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0, many);
     __syncthreads();
-    for (int q = warp; q < count_many; q += 32)
-        for (int k = lane; k < many[q].pieces; k += 32) list_piece(l, many[q], k);
+    many.list(l);
     if (threadIdx.x < 2) counts[threadIdx.x] = reinterpret_cast<const int*>(&numbers)[threadIdx.x];
 }
 
