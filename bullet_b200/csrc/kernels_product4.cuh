@@ -131,6 +131,17 @@ __device__ __forceinline__ void multiply4(uint32_t sums, uint32_t a, uint32_t b,
 #undef B200_MULTIPLY4
 }
 
+// The tiles that a CTA or a pair takes, one after another, and where they lie; no division behind the first one's.
+struct TileAt {
+    uint32_t tile, row, column, step, rows_on, columns_on, across;
+    __device__ __forceinline__ TileAt(uint32_t first, uint32_t step_, uint32_t across_)
+        : tile(first), row(first / across_), column(first % across_), step(step_), rows_on(step_ / across_), columns_on(step_ % across_), across(across_) {}
+    __device__ __forceinline__ void next() {
+        tile += step, row += rows_on, column += columns_on;
+        if (column >= across) column -= across, row++;
+    }
+};
+
 template <int BN, bool PAIR, bool ADDS>
 static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
     product4_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const __grid_constant__ CUtensorMap a_scale_map,
@@ -175,14 +186,14 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
     tensor_fence_after();
     const uint32_t memory = memory_at;
 
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    const int64_t first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
+    const uint32_t tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
+    const TileAt start(blockIdx.x / kCtas, gridDim.x / kCtas, (uint32_t)p.tiles_n);
     if (warp == 0) {
         if (lane == 0) {  // fetches
             int s = 0;
             uint32_t phase = 1;  // (a new barrier's phase before is over)
-            for (int64_t tile = first; tile < tiles && !dead; tile += step) {
-                const int m0 = (int)(tile / p.tiles_n * T::kRows) + 128 * (int)rank, n0 = (int)(tile % p.tiles_n * BN);
+            for (TileAt at = start; at.tile < tiles && !dead; at.next()) {
+                const int m0 = (int)(at.row * T::kRows + 128 * rank), n0 = (int)(at.column * BN);
                 for (int kb = 0; kb < p.k_blocks; kb++) {
                     if (!wait(&empty[s], phase)) break;
                     const uint32_t a_at = smem_u32(base + s * T::kStage), b_at = a_at + T::kA;
@@ -204,7 +215,7 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
             const int whole = (int)(p.k / 256), rest = (int)((p.k % 256 + 63) / 64);  // stages, and products of the last one (past k there may be no scales)
             int s = 0;
             uint32_t phase = 0, done = 0;
-            for (int64_t tile = first; tile < tiles && !dead; tile += step, done++) {
+            for (TileAt at = start; at.tile < tiles && !dead; at.next(), done++) {
                 const uint32_t half = done & 1, sums = memory + half * T::kSumsApart;
                 bool fine = T::kShares ? done == 0 || wait(&sums_free[0], done - 1 & 1) : wait(&sums_free[half], (done >> 1 & 1) ^ 1);
                 if (!__all_sync(0xffffffffu, fine)) break;
@@ -244,29 +255,29 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
         // Where the boxes lie, in their order: of two tiles that share places the second half of the one, and the first half of the other, first; fp32, and what
         // is written element by element, 16 columns a box.
         struct Where {
-            int64_t tile;
+            TileAt at;
             uint32_t done;
             int k, h;
         };
         auto column_of = [&](uint32_t done, int k) { return (kApart * k + (T::kShares && (done & 1) == 0 ? kApart : 0)) % BN; };  // of the tile, behind c0
-        auto first_row = [&](int64_t tile) { return tile / p.tiles_n * T::kRows + 128 * rank + 32 * quarter; };
-        auto first_column = [&](const Where& w) { return w.tile % p.tiles_n * BN + c0 + column_of(w.done, w.k) + 16 * w.h; };
+        auto first_row = [&](const TileAt& at) { return (int64_t)at.row * T::kRows + 128 * rank + 32 * quarter; };
+        auto first_column = [&](const Where& w) { return (int64_t)w.at.column * BN + c0 + column_of(w.done, w.k) + 16 * w.h; };
         // ADDS and boxes: a box's residual is on its way while the box before it is filled.  (Loaded into registers, 64 bytes of a lane's row, it takes
         // twice the time: 16384 x 1024 -> 2048 37 us so, 71 in registers, 41 with one box; without a residual 24.)
-        Where next{first, 0, 0, 0};
+        Where next{start, 0, 0, 0};
         uint32_t filled = 0;  // boxes
         auto fetch_residual = [&](uint32_t number) {
             auto on = [&] {
                 next.h = wide && next.h == 0;
-                if (next.h == 0 && (next.k ^= 1) == 0) next.tile += step, next.done++;
+                if (next.h == 0 && (next.k ^= 1) == 0) next.at.next(), next.done++;
             };
-            while (next.tile < tiles && (first_row(next.tile) >= p.m || first_column(next) >= p.n)) on();
-            if (next.tile >= tiles) return;
+            while (next.at.tile < tiles && (first_row(next.at) >= p.m || first_column(next) >= p.n)) on();
+            if (next.at.tile >= tiles) return;
             if (lane == 0) {
                 bulk_wait_read<0>();
                 uint64_t* bar = &residual_in[2 * taker + (number & 1)];
                 mbar_expect_tx(bar, T::kBox);
-                load_box3(smem_u32(boxes + (number & 1) * T::kBox), &r_map, (int)first_column(next), (int)first_row(next.tile), 0, smem_u32(bar));
+                load_box3(smem_u32(boxes + (number & 1) * T::kBox), &r_map, (int)first_column(next), (int)first_row(next.at), 0, smem_u32(bar));
             }
             on();
         };
@@ -274,9 +285,9 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
         if (ahead) fetch_residual(0);
         uint32_t done = 0;
         bool fine = true;
-        for (int64_t tile = first; tile < tiles && fine; tile += step, done++) {
+        for (TileAt at = start; at.tile < tiles && fine; at.next(), done++) {
             const int half = done & 1;
-            const int64_t rows0 = first_row(tile), own0 = tile % p.tiles_n * BN + c0;
+            const int64_t rows0 = first_row(at), own0 = (int64_t)at.column * BN + c0;
             const int own = rows0 < p.m ? (int)min((int64_t)BN, p.n - own0) : 0;  // columns there are from own0 on, 0 or less: nothing here
             if (bias_at != own0) {
                 __syncwarp();
@@ -350,7 +361,7 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
         int s = 0;
         uint32_t phase = 0;
         bool fine = true;
-        for (int64_t tile = first; tile < tiles && fine && !dead; tile += step) {
+        for (TileAt at = start; at.tile < tiles && fine && !dead; at.next()) {
             for (int kb = 0; kb < p.k_blocks; kb++) {
                 // (they were fetched behind the products that last used this place, here and in tensor memory)
                 fine = __all_sync(0xffffffffu, wait(&scales_in[s], phase));

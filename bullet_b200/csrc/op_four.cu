@@ -92,6 +92,7 @@ int launch_product(const b200_dense4_op* op, ProductArgs p, cudaStream_t stream)
     using T = Tile4<BN, PAIR, ADDS>;
     p.tiles_m = (int)((p.m + T::kRows - 1) / T::kRows);
     p.tiles_n = (int)((p.n + BN - 1) / BN);
+    if ((int64_t)p.tiles_m * p.tiles_n > INT32_MAX) return fail(B200_ERR_UNSUPPORTED, "op_dense4: %lld rows, %lld out are too many", (long long)p.m, (long long)p.n);
     CUtensorMap a, b, a_scale, b_scale, d{}, r{};
     if (int rc = make_codes_map(&a, op->x, op->ldx, p.m, p.k, 128)) return rc;
     if (int rc = make_codes_map(&b, op->w, op->ldw, p.n, p.k, T::kOwnColumns)) return rc;
