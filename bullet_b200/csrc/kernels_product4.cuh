@@ -328,12 +328,14 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
                         if (lane == 0) bulk_wait_read<0>();
                         __syncwarp();
                     }
-                    if (wide || !p.boxes)
-                        box_out64<float>(row, lane, v, 16 * h, ahead);
+                    if (!p.boxes)
+                        box_out64<float>(row, lane, v, 16 * h, false);
+                    else if (wide)
+                        box_out64<float>(row, lane, v, 16 * h, ADDS);
                     else if (p.d_type == B200_TYPE_BF16)
-                        box_out64<bf16>(row, lane, v, 0, ahead);
+                        box_out64<bf16>(row, lane, v, 0, ADDS);
                     else
-                        box_out64<f16>(row, lane, v, 0, ahead);
+                        box_out64<f16>(row, lane, v, 0, ADDS);
                     if (p.boxes) {
                         fence_proxy_async();
                         __syncwarp();
