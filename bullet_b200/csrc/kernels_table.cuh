@@ -1,7 +1,8 @@
 // Rows of a table that lists of ids name: their sums per list, and the gradient, the sums of the lists' gradients per row of the table.
 //
-// Bound by L2's way to the SMs (16384 lists of 17 rows of 2 KB are 590 MB out of a table of 25), with few lists by latency.  A warp takes a list, or a row of the
-// table, and the columns that its lanes cover with 16 bytes each (fewer in narrow matrices; single elements 32 apart where rows do not start on 16 bytes).
+// Bound by L2's way to the SMs (16384 lists of 17 rows of 2 KB are 590 MB out of a table of 25, in 39 us), with few lists by latency.  A warp takes a list, or a row of
+// the table, and the columns that its lanes cover with 32 bytes each, for what a row's index and address cost: with 16, 57 us.  (Fewer in narrow matrices; single elements
+// 32 apart where rows do not start on 16 bytes; 16 in the gradient, where 32 do not leave the registers that its pieces need: 110 us where 102 had been.)
 // Its lanes load 32 indices side by side and hand them round, and four to sixteen rows are on their way at a time.
 //
 // The gradient's sums are taken in the order of the lists, so ids are sorted first, stably, by counting digits of up to eight bits: one CTA for up to kSortOne
@@ -17,8 +18,8 @@
 namespace b200 {
 
 constexpr int kTableThreads = 256;
-// Rows on their way in a warp.  Warps that hide each other's latency count for more than rows in one: 16384 x 32 features of 1024 columns, eight rows and 32 warps of an SM 64 us,
-// four 56; their gradient, whose rows and pieces need more of their indices too, eight and 24 warps 122, eight and 32 110, four and 40 110, four and 48 113, sixteen and 16 148.
+// Rows on their way in a warp.  Warps that hide each other's latency count for more than rows in one: 16384 x 32 features of 1024 columns, two rows of 32 bytes a lane and
+// 32 warps of an SM 43 us, four 39; their gradient, whose rows and pieces need more of their indices too, eight and 24 warps 122, eight and 32 110, four and 40 110, four and 48 113, sixteen and 16 148.
 // So many warps as fill the GPU twice over or fewer take sixteen each.
 constexpr int kEmbedAhead = 4, kGradAhead = 8, kFewAhead = 16;
 
@@ -52,23 +53,31 @@ __device__ __forceinline__ void add_half(float& sum, uint16_t v) {
     else
         asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(sum) : "h"(v));
 }
-// A lane's columns of a warp's: BYTES side by side, or with BYTES 0 as many single elements as 16 bytes hold, 32 apart.
+// A lane's columns of a warp's: BYTES side by side, with 32 twice 16 half a warp's columns apart, or with 0 as many single elements as 16 bytes hold, 32 apart.
 template <class T, int BYTES>
 struct Lanes {
-    static constexpr int kEach = (BYTES ? BYTES : 16) / (int)sizeof(T), kWarp = 32 * kEach;
-    static __device__ __forceinline__ int64_t first(int64_t chunk) { return chunk * kWarp + (threadIdx.x & 31) * (BYTES ? kEach : 1); }
+    static constexpr int kParts = BYTES == 32 ? 2 : 1, kBytes = BYTES == 32 || BYTES == 0 ? 16 : BYTES;  // of a part
+    static constexpr int kOf = kBytes / (int)sizeof(T), kEach = kParts * kOf, kWarp = 32 * kEach;
+    static __device__ __forceinline__ int64_t first(int64_t chunk) { return chunk * kWarp + (threadIdx.x & 31) * (BYTES ? kOf : 1); }
+    static __device__ __forceinline__ int64_t column(int64_t at, int k) { return at + (BYTES ? k / kOf * 32 * kOf + k % kOf : 32 * k); }
     T v[kEach];
     __device__ __forceinline__ void load(const T* row, int64_t at, int64_t cols) {
-        if constexpr (BYTES == 16) {
-            if (at < cols) *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(row + at));
-        } else if constexpr (BYTES == 8) {
-            if (at < cols) *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(row + at));
-        } else if constexpr (BYTES == 4) {
-            if (at < cols) *reinterpret_cast<uint32_t*>(v) = __ldg(reinterpret_cast<const uint32_t*>(row + at));
-        } else {
 #pragma unroll
-            for (int k = 0; k < kEach; k++)
-                if (at + 32 * k < cols) v[k] = __ldg(row + at + 32 * k);
+        for (int part = 0; part < kParts; part++) {
+            const T* from = row + column(at, part * kOf);
+            T* to = v + part * kOf;
+            if constexpr (BYTES == 0) {
+#pragma unroll
+                for (int k = 0; k < kEach; k++)
+                    if (column(at, k) < cols) v[k] = __ldg(row + column(at, k));
+            } else if (column(at, part * kOf) < cols) {
+                if constexpr (kBytes == 16)
+                    *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(from));
+                else if constexpr (kBytes == 8)
+                    *reinterpret_cast<uint2*>(to) = __ldg(reinterpret_cast<const uint2*>(from));
+                else
+                    *reinterpret_cast<uint32_t*>(to) = __ldg(reinterpret_cast<const uint32_t*>(from));
+            }
         }
     }
     __device__ __forceinline__ void add(float (&sum)[kEach]) const {
@@ -87,37 +96,41 @@ struct Lanes {
         }
     }
 };
-// kEach sums to a row of `type`, whose elements start where those of T did (VEC: on as many elements together).
+// kEach sums to a row of `type`, whose elements start where those of T did (VEC: on a part's elements together).
 template <class T, int BYTES, bool VEC>
 __device__ __forceinline__ void store_sums(void* y, int64_t row_at, int64_t at, int64_t cols, int type, const float (&v)[Lanes<T, BYTES>::kEach]) {
-    constexpr int kEach = Lanes<T, BYTES>::kEach;
-    if constexpr (BYTES != 0 && VEC && kEach > 1) {
-        if (at >= cols) return;
-        if (type == B200_TYPE_F32) {
-            float* to = static_cast<float*>(y) + row_at + at;
-            if constexpr (kEach >= 4) {
+    using L = Lanes<T, BYTES>;
+    constexpr int kOf = L::kOf;
 #pragma unroll
-                for (int k = 0; k < kEach; k += 4) *reinterpret_cast<float4*>(to + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+    for (int part = 0; part < L::kParts; part++) {
+        const int64_t column = L::column(at, part * kOf);
+        const int first = part * kOf;
+        if constexpr (BYTES != 0 && VEC && kOf > 1) {
+            if (column >= cols) continue;
+            if (type == B200_TYPE_F32) {
+                float* to = static_cast<float*>(y) + row_at + column;
+                if constexpr (kOf >= 4) {
+#pragma unroll
+                    for (int k = 0; k < kOf; k += 4) *reinterpret_cast<float4*>(to + k) = make_float4(v[first + k], v[first + k + 1], v[first + k + 2], v[first + k + 3]);
+                } else {
+                    *reinterpret_cast<float2*>(to) = make_float2(v[first], v[first + 1]);
+                }
             } else {
-                *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+                uint32_t w[kOf / 2];
+#pragma unroll
+                for (int k = 0; k < kOf / 2; k++) w[k] = type == B200_TYPE_BF16 ? pack2<bf16>(v[first + 2 * k], v[first + 2 * k + 1]) : pack2<f16>(v[first + 2 * k], v[first + 2 * k + 1]);
+                uint16_t* to = static_cast<uint16_t*>(y) + row_at + column;
+                if constexpr (kOf == 8)
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                else if constexpr (kOf == 4)
+                    *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+                else
+                    *reinterpret_cast<uint32_t*>(to) = w[0];
             }
         } else {
-            uint32_t w[kEach / 2];
 #pragma unroll
-            for (int k = 0; k < kEach / 2; k++) w[k] = type == B200_TYPE_BF16 ? pack2<bf16>(v[2 * k], v[2 * k + 1]) : pack2<f16>(v[2 * k], v[2 * k + 1]);
-            uint16_t* to = static_cast<uint16_t*>(y) + row_at + at;
-            if constexpr (kEach == 8)
-                *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-            else if constexpr (kEach == 4)
-                *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-            else
-                *reinterpret_cast<uint32_t*>(to) = w[0];
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < kEach; k++) {
-            const int64_t c = at + (BYTES ? k : 32 * k);
-            if (c < cols) store_value(y, row_at + c, type, v[k]);
+            for (int k = first; k < first + kOf; k++)
+                if (L::column(at, k) < cols) store_value(y, row_at + L::column(at, k), type, v[k]);
         }
     }
 }
@@ -141,7 +154,7 @@ __device__ __forceinline__ void add_named(const T* rows, int64_t ld, int64_t at,
 
 // VEC: a row of y takes a lane's elements together.
 template <class T, int BYTES, int AHEAD>
-static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BYTES == 0 ? 2 : 4) embed_kernel(b200_embed_op a, int vec) {
+static __global__ void __launch_bounds__(kTableThreads, AHEAD >= kFewAhead / 2 || BYTES == 0 ? 2 : 4) embed_kernel(b200_embed_op a, int vec) {
     using L = Lanes<T, BYTES>;
     const int lane = threadIdx.x & 31;
     WarpPlace p((int)((a.cols + L::kWarp - 1ll) / L::kWarp));
@@ -549,7 +562,7 @@ struct TableGrad {
     float* parts;  // [pieces][ldp]
     int64_t ldp;
     int cuts;      // there may be long stretches
-    int vec;       // a row of dtable takes a lane's elements together
+    int vec;       // a row of dtable takes a part's elements together
 };
 template <class T, int BYTES>
 __device__ __forceinline__ void finish_row(const TableGrad& g, int64_t t, int64_t at, float (&sum)[Lanes<T, BYTES>::kEach]) {
@@ -564,7 +577,8 @@ __device__ __forceinline__ void finish_row(const TableGrad& g, int64_t t, int64_
 // loop that the kernel's time goes to.)
 template <class T, int BYTES>
 static __device__ __noinline__ void join_pieces(const TableGrad& g, float* parts, int n, int apart, int64_t t, int64_t at) {
-    constexpr int kEach = Lanes<T, BYTES>::kEach, kJoined = kEach > 4 ? 4 : 8;  // on their way
+    using L = Lanes<T, BYTES>;
+    constexpr int kEach = L::kEach, kJoined = kEach > 4 ? 4 : 8;  // on their way
     float sum[kEach] = {};
     for (int q = 0; q < n; q += kJoined) {
         float v[kJoined][kEach] = {};
@@ -572,19 +586,17 @@ static __device__ __noinline__ void join_pieces(const TableGrad& g, float* parts
         for (int i = 0; i < kJoined; i++) {
             const float* row = parts + (int64_t)(q + i) * apart * g.ldp;
             if (q + i >= n) continue;
-            if constexpr (BYTES != 0 && kEach >= 4) {
+            if constexpr (BYTES != 0 && L::kOf >= 4) {
 #pragma unroll
                 for (int k = 0; k < kEach; k += 4)
-                    if (at < g.a.cols) {
-                        const float4 f = __ldcg(reinterpret_cast<const float4*>(row + at + k));
+                    if (L::column(at, k) < g.a.cols) {
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(row + L::column(at, k)));
                         v[i][k] = f.x, v[i][k + 1] = f.y, v[i][k + 2] = f.z, v[i][k + 3] = f.w;
                     }
             } else {
 #pragma unroll
-                for (int k = 0; k < kEach; k++) {
-                    const int64_t c = at + (BYTES ? k : 32 * k);
-                    if (c < g.a.cols) v[i][k] = __ldcg(row + c);
-                }
+                for (int k = 0; k < kEach; k++)
+                    if (L::column(at, k) < g.a.cols) v[i][k] = __ldcg(row + L::column(at, k));
             }
         }
 #pragma unroll

@@ -24,15 +24,14 @@ int check_ids(const char* who, const void* ids, int64_t ld, int rows, int slots,
     if (ld < slots || ld > INT64_MAX / 8 / (rows > 0 ? rows : 1)) return fail(B200_ERR_ARG, "%s: ld of ids is %lld, with lists of %d", who, (long long)ld, slots);
     return 0;
 }
-// How many bytes of a row of `type` a lane takes: 16 where rows start on them, fewer where the warp would have lanes to spare, 0 (single elements) where rows start anywhere.
-int bytes_of(const void* at, int64_t ld, int cols, int type) {
-    const int size = type_bytes(type);
-    for (int bytes = 16; bytes >= 4; bytes /= 2) {
-        if (bytes > 4 && cols * size <= 16 * bytes) continue;  // (half the lanes or fewer)
-        if (((uintptr_t)at | (uintptr_t)(ld * size) | (uintptr_t)((int64_t)cols * size)) % bytes == 0) return bytes;
-        if (cols * size > 128 * 4) return 0;  // (wide rows of pieces smaller than 16 bytes: elements)
-    }
-    return 0;
+// How many bytes of a row of `type` a lane takes: 32 or 16 where rows start on 16, fewer where the warp would have lanes to spare, 0 (single elements) where rows start anywhere.
+int bytes_of(const void* at, int64_t ld, int cols, int type, int most) {
+    const int64_t size = type_bytes(type), row = cols * size;
+    const auto on = [&](int bytes) { return ((uintptr_t)at | (uintptr_t)(ld * size) | (uintptr_t)row) % bytes == 0; };
+    if (row > 256 && on(16)) return most == 32 && (row + 1023) / 1024 * 1024 - row <= row / 8 ? 32 : 16;  // (an eighth of the lanes to spare at most)
+    if (row > 512) return 0;
+    if (row > 128 && on(8)) return 8;
+    return on(4) ? 4 : 0;
 }
 // Whether rows of `type` take `each` elements together.
 bool together(const void* at, int64_t ld, int type, int each) {
@@ -41,7 +40,9 @@ bool together(const void* at, int64_t ld, int type, int each) {
 }
 template <class F>
 void with_bytes(int bytes, F f) {
-    if (bytes == 16)
+    if (bytes == 32)
+        f(std::integral_constant<int, 32>{});
+    else if (bytes == 16)
         f(std::integral_constant<int, 16>{});
     else if (bytes == 8)
         f(std::integral_constant<int, 8>{});
@@ -76,7 +77,7 @@ struct Space {
 };
 // How many warps' columns a row has.
 int across_of(const b200_embed_grad_op* op) {
-    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
+    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
     return (op->cols + warp - 1) / warp;
 }
 Space space_of(const b200_embed_grad_op* op) {
@@ -133,18 +134,18 @@ int b200_op_embed(int device, void* stream, const b200_embed_op* op) {
     if (int rc = check_matrix(who, "y", op->y, op->ldy, op->rows, op->cols, op->y_type)) return rc;
     OnDevice on(device);
     OP_CK(on.status);
-    const int bytes = bytes_of(op->table, op->ldt, op->cols, op->table_type);
+    const int bytes = bytes_of(op->table, op->ldt, op->cols, op->table_type, 32);
     with_float(op->table_type, [&](auto t) {
         with_bytes(bytes, [&](auto b) {
             using L = Lanes<decltype(t), b()>;
             const int64_t warps = op->rows * ((op->cols + L::kWarp - 1ll) / L::kWarp);
-            const int vec = together(op->y, op->ldy, op->y_type, L::kEach);
+            const int vec = together(op->y, op->ldy, op->y_type, L::kOf);
             auto go = [&](auto kernel) { kernel<<<ctas_for(warps), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, vec); };
             // (few warps: as much on its way as registers hold)
             if (op->slots <= kEmbedAhead && warps > kTableSms * 8)
                 go(embed_short_kernel<decltype(t), b()>);
             else if (b() && warps <= kTableSms * 8)
-                go(embed_kernel<decltype(t), b(), b() ? kFewAhead : kEmbedAhead>);
+                go(embed_kernel<decltype(t), b(), b() == 32 ? kFewAhead / 2 : b() ? kFewAhead : kEmbedAhead>);
             else
                 go(embed_kernel<decltype(t), b(), kEmbedAhead>);
         });
@@ -210,16 +211,17 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
         OP_CK(launch_step(true, list_long_kernel, (unsigned)((op->n + kTableThreads - 1ll) / kTableThreads), kTableThreads, 0, s, start, op->n, l));
     }
     TableGrad g{*op, p.to, start, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
-    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type);
     cudaError_t rc = cudaSuccess;
     with_float(op->dy_type, [&](auto t) {
-        with_bytes(bytes, [&](auto b) {
-            using L = Lanes<decltype(t), b()>;
-            g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kEach);
-            const int64_t most = (op->n + (space.cuts ? sort.count / space.piece : 0)) * space.across;
-            // (few warps: as much on its way as registers hold)
-            rc = b() && most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), b() ? kFewAhead : kGradAhead>, ctas_for(most), kTableThreads, 0, s, g)
-                                               : launch_step(true, embed_backward_kernel<decltype(t), b(), kGradAhead>, ctas_for(most), kTableThreads, 0, s, g);
+        with_bytes(bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16), [&](auto b) {
+            if constexpr (b() != 32) {
+                using L = Lanes<decltype(t), b()>;
+                g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kOf);
+                const int64_t most = (op->n + (space.cuts ? sort.count / space.piece : 0)) * space.across;
+                // (few warps: as much on its way as registers hold)
+                rc = b() && most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), b() ? kFewAhead : kGradAhead>, ctas_for(most), kTableThreads, 0, s, g)
+                                                   : launch_step(true, embed_backward_kernel<decltype(t), b(), kGradAhead>, ctas_for(most), kTableThreads, 0, s, g);
+            }
         });
     });
     OP_CK(rc);
