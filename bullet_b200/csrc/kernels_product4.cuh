@@ -19,7 +19,7 @@
 // next is longer than one stage's products: 1050 ns a stage.)
 //
 // Measured, us: 131072 x 2048 -> 512 73 (3.8 PFLOP/s, under the power cap: 64 with codes of zeros; a tile's eight stages 2.3 us, 0.95 until the next one's begin, 3.6
-// together; HBM 42); 16384 x 1024 -> 2048 24, with a residual 37.
+// together; HBM 42); 16384 x 1024 -> 2048 22, with a residual 33.
 #pragma once
 #include "kernels_four.cuh"
 #include "product_out.cuh"
@@ -215,13 +215,15 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
             const int whole = (int)(p.k / 256), rest = (int)((p.k % 256 + 63) / 64);  // stages, and products of the last one (past k there may be no scales)
             int s = 0;
             uint32_t phase = 0, done = 0;
-            for (TileAt at = start; at.tile < tiles && !dead; at.next(), done++) {
+            bool fine = true;  // (of all lanes: they leave together)
+            for (TileAt at = start; at.tile < tiles && fine; at.next(), done++) {
                 const uint32_t half = done & 1, sums = memory + half * T::kSumsApart;
-                bool fine = T::kShares ? done == 0 || wait(&sums_free[0], done - 1 & 1) : wait(&sums_free[half], (done >> 1 & 1) ^ 1);
-                if (!__all_sync(0xffffffffu, fine)) break;
+                fine = __all_sync(0xffffffffu, T::kShares ? done == 0 || wait(&sums_free[0], done - 1 & 1) : wait(&sums_free[half], (done >> 1 & 1) ^ 1));
+                if (!fine) break;
                 tensor_fence_after();
                 for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (!__all_sync(0xffffffffu, wait(&full[s], phase))) break;
+                    fine = __all_sync(0xffffffffu, wait(&full[s], phase));
+                    if (!fine) break;
                     tensor_fence_after();
                     const uint32_t a_at = a0 + s * (T::kStage / 16), b_at = a_at + T::kA / 16, a_scales = memory + T::kScalesAt + s * T::kScaleWords, b_scales = a_scales + 8;
                     if (issues) {
@@ -263,7 +265,7 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
         auto first_row = [&](const TileAt& at) { return (int64_t)at.row * T::kRows + 128 * rank + 32 * quarter; };
         auto first_column = [&](const Where& w) { return (int64_t)w.at.column * BN + c0 + column_of(w.done, w.k) + 16 * w.h; };
         // ADDS and boxes: a box's residual is on its way while the box before it is filled.  (Loaded into registers, 64 bytes of a lane's row, it takes
-        // twice the time: 16384 x 1024 -> 2048 37 us so, 71 in registers, 41 with one box; without a residual 24.)
+        // twice the time: 16384 x 1024 -> 2048 37 us so when tried, 71 in registers, 41 with one box.)
         Where next{start, 0, 0, 0};
         uint32_t filled = 0;  // boxes
         auto fetch_residual = [&](uint32_t number) {
@@ -363,7 +365,7 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
         int s = 0;
         uint32_t phase = 0;
         bool fine = true;
-        for (TileAt at = start; at.tile < tiles && fine && !dead; at.next()) {
+        for (TileAt at = start; at.tile < tiles && fine; at.next()) {
             for (int kb = 0; kb < p.k_blocks; kb++) {
                 // (they were fetched behind the products that last used this place, here and in tensor memory)
                 fine = __all_sync(0xffffffffu, wait(&scales_in[s], phase));
