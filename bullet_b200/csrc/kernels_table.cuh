@@ -8,6 +8,8 @@
 // The gradient's sums are taken in the order of the lists, so ids are sorted first, stably, by counting digits of up to eight bits: one CTA for up to kSortOne
 // ids, else three kernels a pass.  Ids that name no row are left out by the first pass.  Then a warp adds up the rows that a table row's stretch of the
 // sorted ids names.  Stretches of more than kLongest are listed and cut into pieces, whose sums go to memory and are joined in order.
+// A table of more rows than there are ids is set to 0 first, and a warp looks at each of the sorted ids for whether a stretch begins there, so that rows without ids cost no
+// more than their zeros.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -489,10 +491,35 @@ static __global__ void __launch_bounds__(kTableThreads) list_long_kernel(const i
     __syncthreads();
     many.list(l);
 }
+// The stretch that begins at place i of `count` sorted ids, id_of(i) each, if it is long: where it ends; else i.
+template <class F>
+__device__ __forceinline__ int long_end(int i, int count, F id_of) {
+    if (i >= count - kLongest) return i;
+    const int id = id_of(i);
+    if (id_of(i + kLongest) != id || (i > 0 && id_of(i - 1) == id)) return i;
+    int in = i + kLongest, out = count;  // places in it, and behind it
+    while (out - in > 1) {
+        const int between = in + (out - in) / 2;
+        (id_of(between) == id ? in : out) = between;
+    }
+    return out;
+}
+// ... without starts: a place of the sorted ids a thread
+static __global__ void __launch_bounds__(kTableThreads) list_long_places_kernel(const int2* sorted, const int* there, Long l) {
+    __shared__ ManyPieces<kTableThreads> many;
+    if (threadIdx.x == 0) many.warps = many.all = 0;
+    step_begin(nullptr);
+    __syncthreads();
+    const int count = __ldcg(there), i = (int)(blockIdx.x * kTableThreads + threadIdx.x);
+    const int end = long_end(i, count, [&](int at) { return __ldcg(&sorted[at].x); });
+    list_long(l, end > i ? __ldcg(&sorted[i].x) : 0, i, end, many);
+    __syncthreads();
+    many.list(l);
+}
 
-// All passes for up to kSortOne ids, the starts and the long stretches: one CTA, the ids in shared memory between the passes.
+// All passes for up to kSortOne ids, the starts (unless that is NULL) and the long stretches: one CTA, the ids in shared memory between the passes.
 constexpr int kOneThreads = 1024, kOneEach = 8, kSortOne = kOneThreads * kOneEach;
-static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p, int passes, int* start, Long l) {
+static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p, int passes, int* start, int* there, Long l) {
     extern __shared__ int2 pairs[];                               // [kSortOne]
     int* const count = reinterpret_cast<int*>(pairs + kSortOne);  // [32][(1 << bits) + 1]
     __shared__ int totals[256], sums[33];
@@ -538,15 +565,22 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
         __syncthreads();
     }
     for (int i = threadIdx.x; i < all; i += kOneThreads) p.to[i] = pairs[i];
-    for (int i = threadIdx.x; i - lane <= all; i += kOneThreads) {  // (whole warps)
-        const int before = i == 0 ? -1 : i <= all ? pairs[i - 1].x : p.n, id = i < all ? pairs[i].x : p.n;
-        fill_starts(i, before, id, start);
-    }
+    if (start)
+        for (int i = threadIdx.x; i - lane <= all; i += kOneThreads) {  // (whole warps)
+            const int before = i == 0 ? -1 : i <= all ? pairs[i - 1].x : p.n, id = i < all ? pairs[i].x : p.n;
+            fill_starts(i, before, id, start);
+        }
+    if (threadIdx.x == 0) *there = all;
     __syncthreads();
     int* const counts = l.counts;
     l.counts = reinterpret_cast<int*>(&numbers);
-    if (all > kLongest)
+    if (all > kLongest && start)
         for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads) list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0, many);
+    else if (all > kLongest)
+        for (int i = threadIdx.x; i - lane < all; i += kOneThreads) {
+            const int end = long_end(i, all, [&](int at) { return pairs[at].x; });
+            list_long(l, end > i ? pairs[i].x : 0, i, end, many);
+        }
     __syncthreads();
     many.list(l);
     if (threadIdx.x < 2) counts[threadIdx.x] = reinterpret_cast<const int*>(&numbers)[threadIdx.x];
@@ -558,6 +592,7 @@ struct TableGrad {
     b200_embed_grad_op a;
     const int2* sorted;
     const int* start;
+    const int* there;  // how many sorted ids there are
     Long l;
     float* parts;  // [pieces][ldp]
     int64_t ldp;
@@ -630,9 +665,24 @@ __device__ __forceinline__ void sum_stretch(const TableGrad& g, int from, int to
         list = next;
     }
 }
+// Where the stretch that begins at place `from` ends, or more than kLongest behind it, and its row; `from` itself if none begins there.  A whole warp.
+__device__ __forceinline__ int stretch_end(const int2* sorted, int from, int count, int& row) {
+    const int lane = threadIdx.x & 31;
+    for (int to = from;; to += 31) {  // lane 0: the place before
+        const int at = to - 1 + lane, id = at >= 0 && at < count ? __ldcg(&sorted[at].x) : -1;
+        const int before = __shfl_sync(0xffffffffu, id, 0);
+        if (to == from) {
+            row = __shfl_sync(0xffffffffu, id, 1);
+            if (before == row) return from;
+        }
+        const unsigned others = __ballot_sync(0xffffffffu, lane > 0 && id != row);
+        if (others) return to + __ffs(others) - 2;
+        if (to + 31 - from > kLongest) return to + 31;
+    }
+}
 // Pieces of the long stretches, a warp each, then rows of the table.  Who finishes the last member of a group joins them, in their order.  A CTA's warps count their
-// pieces together, behind one fence.
-template <class T, int BYTES, int AHEAD>
+// pieces together, behind one fence.  PLACES: there are no starts, and rows without ids are 0 already.  (Asked while it runs, it takes registers: 102 us were 112.)
+template <class T, int BYTES, int AHEAD, bool PLACES>
 static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BYTES == 0 ? 2 : 4) embed_backward_kernel(const __grid_constant__ TableGrad g) {
     using L = Lanes<T, BYTES>;
     constexpr uint32_t kWarps = kTableThreads / 32;
@@ -676,13 +726,20 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BY
         }
     }
     WarpPlace p((int)across);
-    for (; p.row < (uint32_t)g.a.n; p.next()) {
+    const uint32_t places = PLACES ? (uint32_t)__ldcg(g.there) : (uint32_t)g.a.n;
+    for (; p.row < places; p.next()) {
         const int64_t at = L::first(p.at);
-        const int from = __ldcg(g.start + p.row), to = __ldcg(g.start + p.row + 1);
+        int t = (int)p.row, from = t, to;
+        if constexpr (PLACES) {
+            to = stretch_end(g.sorted, from, (int)places, t);
+            if (to == from) continue;
+        } else {
+            from = __ldcg(g.start + t), to = __ldcg(g.start + t + 1);
+        }
         if (to - from > kLongest) continue;
         float sum[L::kEach] = {};
         sum_stretch<T, BYTES, AHEAD>(g, from, to, at, sum);
-        finish_row<T, BYTES>(g, p.row, at, sum);
+        finish_row<T, BYTES>(g, t, at, sum);
     }
 }
 

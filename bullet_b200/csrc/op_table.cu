@@ -1,6 +1,7 @@
 // Operator-level entry points of tables whose rows are named by ids: b200_op_embed and its gradient.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "kernels_table.cuh"
 #include "op_call.h"
@@ -12,10 +13,11 @@ using namespace b200;
 
 constexpr int kTableSms = 148;
 
-int check_lists(const char* who, int rows, int slots, int n, int cols, int wide) {
+int check_lists(const char* who, int rows, int slots, int n, int cols, int wide, float scale) {
     if (rows < 0 || slots < 1 || n < 1 || cols < 1) return fail(B200_ERR_ARG, "%s: %d lists of %d, %d rows of %d", who, rows, slots, n, cols);
     if ((int64_t)rows * slots > INT32_MAX - 65536) return fail(B200_ERR_UNSUPPORTED, "%s: %d lists of %d are too many", who, rows, slots);
     if (wide != 0 && wide != 1) return fail(B200_ERR_ARG, "%s: wide_ids is %d", who, wide);
+    if (!std::isfinite(scale)) return fail(B200_ERR_ARG, "%s: scale is not finite", who);
     return 0;
 }
 int check_ids(const char* who, const void* ids, int64_t ld, int rows, int slots, int wide) {
@@ -58,6 +60,7 @@ struct Sorting {
     int64_t count;
     int passes, bits, tiles;
     bool one() const { return count <= kSortOne; }
+    bool places;  // no starts: the table has more rows than there are ids
 };
 Sorting sorting_of(const b200_embed_grad_op* op) {
     Sorting s{(int64_t)op->rows * op->slots};
@@ -66,6 +69,9 @@ Sorting sorting_of(const b200_embed_grad_op* op) {
     s.passes = (wanted + 7) / 8;
     s.bits = (wanted + s.passes - 1) / s.passes;
     s.tiles = (int)((s.count + kSortTile - 1) / kSortTile);
+    // (us without starts and with them, bf16: 65536 ids of 128 columns, 32768 rows of the table 43 and 35, 131072 58 and 60, 262144 66 and 81; 8192 ids, 8192 rows 37 and 39,
+    // 2^20 76 and 584)
+    s.places = op->n > s.count;
     return s;
 }
 // Where the parts of a gradient's workspace begin, in bytes.
@@ -94,7 +100,7 @@ Space space_of(const b200_embed_grad_op* op) {
         s.more_pairs = next(sort.passes > 1 ? sort.count * 8 : 0);
         s.counts = next((((int64_t)sort.tiles + 1) << sort.bits) * 4);
     }
-    s.start = next((op->n + 1ll) * 4);
+    if (!sort.places) s.start = next((op->n + 1ll) * 4);
     s.numbers = next(16);
     // Pieces of 16 for few ids, whose longest stretches then have warps enough (5003 ids of 8 rows of 520: 64 27 us, 16 23), of 64 for many, as each piece costs its part of
     // the joining (131072 ids of 8 rows of 1024: 16 159 us, 32 118, 64 90; 2^20 lists' ids of 768 rows of 256: 64 100, 512 128); more where they would take more room.
@@ -112,9 +118,22 @@ Space space_of(const b200_embed_grad_op* op) {
     return s;
 }
 
+// The whole gradient 0.
+int zeros(const b200_embed_grad_op* op, cudaStream_t s) {
+    const int64_t row = (int64_t)op->cols * type_bytes(op->dtable_type), apart = op->lddt * type_bytes(op->dtable_type);
+    if (apart == row || op->n == 1) {
+        OP_CK(cudaMemsetAsync(op->dtable, 0, (size_t)(row * op->n), s));
+    } else if (apart <= INT32_MAX) {
+        OP_CK(cudaMemset2DAsync(op->dtable, (size_t)apart, 0, (size_t)row, (size_t)op->n, s));
+    } else {  // (further apart than that call takes, and so few)
+        for (int64_t t = 0; t < op->n; t++) OP_CK(cudaMemsetAsync(static_cast<char*>(op->dtable) + t * apart, 0, (size_t)row, s));
+    }
+    return 0;
+}
+
 int check_embed_grad(const b200_embed_grad_op* op, const char* who) {
     if (!op) return fail(B200_ERR_ARG, "%s: null operator description", who);
-    if (int rc = check_lists(who, op->rows, op->slots, op->n, op->cols, op->wide_ids)) return rc;
+    if (int rc = check_lists(who, op->rows, op->slots, op->n, op->cols, op->wide_ids, op->scale)) return rc;
     if (!is_float(op->dy_type) || !is_float(op->dtable_type)) return fail(B200_ERR_UNSUPPORTED, "%s: types %d, %d", who, op->dy_type, op->dtable_type);
     return 0;
 }
@@ -126,7 +145,7 @@ extern "C" {
 int b200_op_embed(int device, void* stream, const b200_embed_op* op) {
     const char* who = "op_embed";
     if (!op) return fail(B200_ERR_ARG, "%s: null operator description", who);
-    if (int rc = check_lists(who, op->rows, op->slots, op->n, op->cols, op->wide_ids)) return rc;
+    if (int rc = check_lists(who, op->rows, op->slots, op->n, op->cols, op->wide_ids, op->scale)) return rc;
     if (!is_float(op->table_type) || !is_float(op->y_type)) return fail(B200_ERR_UNSUPPORTED, "%s: types %d, %d", who, op->table_type, op->y_type);
     if (op->rows == 0) return 0;
     if (int rc = check_ids(who, op->ids, op->ldids, op->rows, op->slots, op->wide_ids)) return rc;
@@ -174,14 +193,13 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     OnDevice on(device);
     OP_CK(on.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (op->rows == 0) {
-        OP_CK(cudaMemset2DAsync(op->dtable, op->lddt * type_bytes(op->dtable_type), 0, (size_t)op->cols * type_bytes(op->dtable_type), op->n, s));
-        return 0;
-    }
+    if (op->rows == 0) return zeros(op, s);
     char* base = static_cast<char*>(op->workspace);
     const Sorting sort = sorting_of(op);
+    if (sort.places)
+        if (int rc = zeros(op, s)) return rc;
     int2* pairs[2] = {reinterpret_cast<int2*>(base + space.pairs), reinterpret_cast<int2*>(base + space.more_pairs)};
-    int* start = reinterpret_cast<int*>(base + space.start);
+    int* start = sort.places ? nullptr : reinterpret_cast<int*>(base + space.start);
     int* numbers = reinterpret_cast<int*>(base + space.numbers);
     const Long l{numbers, reinterpret_cast<Piece8*>(base + space.pieces), reinterpret_cast<int*>(base + space.done), space.piece, space.across};
     SortPass p{};
@@ -194,7 +212,7 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
             OP_CK(cudaFuncSetAttribute(sort_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortOne * 8 + 32 * 257 * 4));
             if (device < 64) allowed |= (uint64_t)1 << device;
         }
-        sort_one_kernel<<<1, kOneThreads, shared, s>>>(p, sort.passes, start, l);
+        sort_one_kernel<<<1, kOneThreads, shared, s>>>(p, sort.passes, start, numbers + 2, l);
         OP_CK(cudaGetLastError());
     } else {
         p.counts = reinterpret_cast<int*>(base + space.counts);
@@ -207,20 +225,28 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
             OP_CK(launch_step(true, pass_place_kernel, sort.tiles, kSortThreads, 0, s, p));
             p.from = p.to;
         }
-        OP_CK(launch_step(true, starts_kernel, (unsigned)((sort.count + kTableThreads * kStartsEach) / (kTableThreads * kStartsEach)), kTableThreads, 0, s, p.to, p.there, op->n, start));
-        OP_CK(launch_step(true, list_long_kernel, (unsigned)((op->n + kTableThreads - 1ll) / kTableThreads), kTableThreads, 0, s, start, op->n, l));
+        if (sort.places) {
+            OP_CK(launch_step(true, list_long_places_kernel, (unsigned)((sort.count + kTableThreads - 1) / kTableThreads), kTableThreads, 0, s, p.to, p.there, l));
+        } else {
+            OP_CK(launch_step(true, starts_kernel, (unsigned)((sort.count + kTableThreads * kStartsEach) / (kTableThreads * kStartsEach)), kTableThreads, 0, s, p.to, p.there, op->n, start));
+            OP_CK(launch_step(true, list_long_kernel, (unsigned)((op->n + kTableThreads - 1ll) / kTableThreads), kTableThreads, 0, s, start, op->n, l));
+        }
     }
-    TableGrad g{*op, p.to, start, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
+    TableGrad g{*op, p.to, start, numbers + 2, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
     cudaError_t rc = cudaSuccess;
     with_float(op->dy_type, [&](auto t) {
         with_bytes(bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16), [&](auto b) {
             if constexpr (b() != 32) {
                 using L = Lanes<decltype(t), b()>;
                 g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kOf);
-                const int64_t most = (op->n + (space.cuts ? sort.count / space.piece : 0)) * space.across;
+                const int64_t most = ((sort.places ? sort.count : op->n) + (space.cuts ? sort.count / space.piece : 0)) * space.across;
+                auto go = [&](auto kernel) { rc = launch_step(true, kernel, ctas_for(most), kTableThreads, 0, s, g); };
                 // (few warps: as much on its way as registers hold)
-                rc = b() && most <= kTableSms * 16 ? launch_step(true, embed_backward_kernel<decltype(t), b(), b() ? kFewAhead : kGradAhead>, ctas_for(most), kTableThreads, 0, s, g)
-                                                   : launch_step(true, embed_backward_kernel<decltype(t), b(), kGradAhead>, ctas_for(most), kTableThreads, 0, s, g);
+                constexpr int kFew = b() ? kFewAhead : kGradAhead;
+                if (most <= kTableSms * 16)
+                    sort.places ? go(embed_backward_kernel<decltype(t), b(), kFew, true>) : go(embed_backward_kernel<decltype(t), b(), kFew, false>);
+                else
+                    sort.places ? go(embed_backward_kernel<decltype(t), b(), kGradAhead, true>) : go(embed_backward_kernel<decltype(t), b(), kGradAhead, false>);
             }
         });
     });

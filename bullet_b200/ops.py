@@ -130,7 +130,7 @@ def dense_backward(dy, x, w, y=None, act: int = ACT_NONE, dskip=None, dw_dtype=t
 
 
 def embed(table, ids, scale: float = 1.0, out_dtype=None):
-    """scale * the sum of table[ids[r][s]] over s, for every list r of `ids`: [rows, slots], or [rows] for one each, in int32 or int64.  Ids outside
+    """scale (finite) * the sum of table[ids[r][s]] over s, for every list r of `ids`: [rows, slots], or [rows] for one each, in int32 or int64.  Ids outside
     [0, len(table)), as -1, name no row and add nothing.  Sums are of 32 bits; `out_dtype`: default the table's type."""
     return _calls.embed(table, ids, scale, out_dtype)
 
@@ -148,7 +148,7 @@ def gradient_norm(gradients):
 def clip_gradients(gradients, max_norm: float, out=None):
     """([tensors], norm): the gradients times max_norm / norm where their norm together is above max_norm (and finite), else as they are.  `out`:
     where they go; may be `gradients`, or any of them, themselves, which are then written only if they change."""
-    return _calls.clip_gradients(gradients, max_norm, out)
+    return _calls.clip_gradients(gradients, float(max_norm), out)
 
 
 def gave_up(device: int) -> bool:

@@ -580,7 +580,7 @@ int b200_op_dense4(int device, void* stream, const b200_dense4_op* op);
 
 /* ---- rows of a table that lists of ids name, as embeddings of features or of an output bucket: y[r] = scale * sum over s of table[ids[r][s]], sums
  * taken in the order of the slots.  An id outside [0, n), as the -1 behind the last of a list, names no row and adds nothing.  At most 2^31 - 2^16
- * ids.  (The reference's sparse affine, crates/compiler/src/tensor/operation/sparse.rs:103-115, without its bias, in these types.) */
+ * ids; a finite scale.  (The reference's sparse affine, crates/compiler/src/tensor/operation/sparse.rs:103-115, without its bias, in these types.) */
 typedef struct b200_embed_op {
     int32_t rows, slots, n, cols;  /* lists, ids of a list, rows of the table, columns */
     int32_t table_type, y_type;    /* B200_TYPE_F32, _BF16 or _F16 */

@@ -237,3 +237,40 @@ def test_a_wait_that_gave_up_is_reported_once_by_the_next_call_in_4_bits(rows):
     with pytest.raises(_lib.B200Error, match="waited too long") as e:
         ops.dense(x, w)
     assert e.value.code == -2 and word[0] == 0 and torch.equal(ops.dense(x, w), want)
+
+
+@pytest.mark.parametrize("counts", [(1,), (64, 1, 65), (30, 31, 32, 33, 61, 62, 63, 64, 65, 66), (129, 1, 1, 3000, 2), (4097, 7), (1,) * 9000, (65,) * 130, (20000, 64, 65, 1, 300)])
+@pytest.mark.parametrize("pad,at", [(0, 0), (3, 1)])
+@pytest.mark.parametrize("places", ["first", "last", "apart"])
+def test_gradients_of_tables_with_more_rows_than_ids(counts, pad, at, places):
+    """Such tables are set to 0 first: all of their rows, nothing around them; `counts`: how often rows of the table are met."""
+    rows, cols = sum(counts), 24
+    n = 2 * rows + 100
+    named = torch.arange(len(counts)) if places == "first" else n - 1 - torch.arange(len(counts)) if places == "last" else torch.randperm(n)[:len(counts)]
+    ids = named.repeat_interleave(torch.tensor(counts))[torch.randperm(rows)].to("cuda", torch.int32)
+    dy = torch.randint(-3, 4, (rows, cols), device="cuda").to(BF16)
+    raw, d = guarded(n, cols, F32, pad, at)
+    op = _lib.CEmbedGrad(rows=rows, slots=1, n=n, cols=cols, dy_type=1, dtable_type=0, wide_ids=0, ldids=1, lddy=cols, lddt=cols + pad, ids=ids.data_ptr(), dy=dy.data_ptr(),
+                         dtable=d.data_ptr(), scale=0.5)
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().b200_op_embed_backward_workspace(ctypes.byref(op), ctypes.byref(size)))
+    space = torch.full((size.value,), 255, dtype=torch.uint8, device="cuda")
+    op.workspace, op.workspace_bytes = space.data_ptr(), size.value
+    want = torch.zeros(n, cols, dtype=torch.float64, device="cuda").index_add_(0, ids.long(), dy.double()) / 2
+    for _ in range(2):
+        call("b200_op_embed_backward", op)
+        assert torch.equal(d.double(), want) and around(raw, d, at)
+
+
+@pytest.mark.parametrize("rows", [100, 9000])
+def test_a_table_with_more_rows_than_ids_in_a_graph(rows):
+    ids, dy = torch.randint(-1, 20, (rows, 1), device="cuda", dtype=torch.int32), normal(5, rows, 40)
+    ops.embed_backward(dy, ids, 50000)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        d = ops.embed_backward(dy, ids, 50000)
+    for seed in (1, 2):
+        ids.copy_((ids * 7 + seed) % 49999)
+        dy.copy_(normal(seed, rows, 40))
+        graph.replay()
+        assert torch.equal(d, ops.embed_backward(dy, ids, 50000))

@@ -51,6 +51,7 @@ REFUSED = [
     ("b200_op_embed_backward", EMBED_GRAD, dict(dy=0), ARG), ("b200_op_embed_backward", EMBED_GRAD, dict(lddy=7), ARG), ("b200_op_embed_backward", EMBED_GRAD, dict(lddt=7), ARG),
     ("b200_op_embed_backward", EMBED_GRAD, dict(ids=A + 2), ARG), ("b200_op_embed_backward", EMBED_GRAD, dict(workspace_bytes=16), ARG),
     ("b200_op_embed_backward", EMBED_GRAD, dict(workspace=A + 8), ARG), ("b200_op_embed_backward", EMBED_GRAD, dict(wide_ids=-1), ARG),
+    ("b200_op_embed", EMBED, dict(scale=float("inf")), ARG), ("b200_op_embed_backward", EMBED_GRAD, dict(scale=float("nan")), ARG),
     ("b200_op_clip_gradients", CLIP, dict(count=-1), ARG), ("b200_op_clip_gradients", CLIP, dict(gradients=0), ARG), ("b200_op_clip_gradients", CLIP, dict(norm=0), ARG),
     ("b200_op_clip_gradients", CLIP, dict(workspace=0), ARG), ("b200_op_clip_gradients", CLIP, dict(workspace_bytes=64), ARG), ("b200_op_clip_gradients", CLIP, dict(max_norm=-1.0), ARG),
     ("b200_op_clip_gradients", CLIP, dict(max_norm=float("nan")), ARG), ("b200_op_clip_gradients", CLIP, gradients((A, A, 100, 3)), UNSUPPORTED),
@@ -112,3 +113,19 @@ def test_tensor_calls_name_what_is_wrong():
         ops.pack4(w)
     with pytest.raises(ValueError, match="requires a gradient"):
         ops.dense(p, p._replace(by_column=True), residual=w)
+    ids = torch.zeros(4, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="table: "):
+        ops.embed(x, ids)
+    with pytest.raises(ValueError, match="dy: "):
+        ops.embed_backward(x, ids, 7)
+    with pytest.raises(ValueError, match=r"gradients\[0\]: "):
+        ops.gradient_norm([x])
+    with pytest.raises(ValueError, match=r"gradients\[0\]: a tensor is wanted"):
+        ops.clip_gradients([None], 1.0)
+    with pytest.raises(ValueError, match="at least one"):
+        ops.clip_gradients([], 1.0)
+    with pytest.raises(TypeError):
+        ops.clip_gradients([x], None)
+    for call in (lambda: ops.embed(w, ids), lambda: ops.embed_backward(w, ids, 7), lambda: ops.clip_gradients([w], 1.0)):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
