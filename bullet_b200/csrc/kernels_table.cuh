@@ -743,4 +743,138 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BY
     }
 }
 
+// ---- the gradient of a table of few rows, as of output buckets: one id a list
+//
+// HBM bound (131072 x 1024 bf16, 8 rows 56 us, 4.8 TB/s; 262144 x 1024 fp32 180, 6.0), with few lists by latency (5003 x 520 7.5): nothing is sorted.  A warp takes lists one after another and the columns that its lanes cover, and keeps a sum for each of the table's
+// rows in shared memory, where each lane meets its own words alone.  A CTA's warps are added up in their order, then the CTAs' sums by few_join_kernel.
+constexpr int kFewRows = 16, kFewWarps = kTableThreads / 32;
+struct FewRows {
+    b200_embed_grad_op a;
+    float* parts;  // [chunks][across][a CTA's sums, as they lie in shared memory]
+    int lists;     // of a warp
+    int chunks, across;
+};
+template <class T, int BYTES>
+struct FewSums {
+    static constexpr int kEach = Lanes<T, BYTES>::kEach, kVec = kEach < 4 ? kEach : 4, kMany = kEach / kVec;
+    static constexpr int kRow = kEach * 32;  // words of a table row's sums
+    struct alignas(4 * kVec) Vec {
+        float v[kVec];
+    };
+    // The k-th piece of a lane's sums
+    static __device__ __forceinline__ Vec* at(float* sums, int row, int k, int lane) { return reinterpret_cast<Vec*>(sums) + (row * kMany + k) * 32 + lane; }
+    // Words 32 row kMany + ..., as at() has them, out to dtable.
+    static __device__ __forceinline__ void out(const FewRows& f, int chunk_of_columns, int vec_at, const Vec& v) {
+        const int lane = vec_at & 31, k = (vec_at >> 5) % kMany, row = (vec_at >> 5) / kMany;
+        const int64_t first = (int64_t)chunk_of_columns * Lanes<T, BYTES>::kWarp + lane * (BYTES ? kEach : 1);
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            const int64_t column = first + (BYTES ? k * kVec + i : 32 * (k * kVec + i));
+            if (column < f.a.cols) store_value(f.a.dtable, row * f.a.lddt + column, f.a.dtable_type, v.v[i] * f.a.scale);
+        }
+    }
+};
+template <class T, int BYTES>
+static __global__ void __launch_bounds__(kTableThreads, 3) few_rows_kernel(const __grid_constant__ FewRows f) {
+    using L = Lanes<T, BYTES>;
+    using S = FewSums<T, BYTES>;
+    constexpr int kAhead = 8;
+    extern __shared__ uint4 few_shared[];
+    step_begin(nullptr);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = S::kRow * f.a.n;
+    float* const all = reinterpret_cast<float*>(few_shared);
+    float* const sums = all + warp * part;
+    const uint32_t chunk = blockIdx.x / (uint32_t)f.across, columns = blockIdx.x % (uint32_t)f.across;
+    for (int k = lane; k < part; k += 32) sums[k] = 0.f;
+    __syncwarp();
+    const int64_t at = L::first(columns), first = ((int64_t)chunk * kFewWarps + warp) * f.lists, last = min(first + f.lists, (int64_t)f.a.rows);
+    const T* dy = static_cast<const T*>(f.a.dy);
+    int64_t id = first + lane < last ? id_at(f.a.ids, (first + lane) * f.a.ldids, f.a.wide_ids, f.a.n) : -1;
+    for (int64_t s = first; s < last; s += 32) {
+        const int64_t next = s + 32 + lane < last ? id_at(f.a.ids, (s + 32 + lane) * f.a.ldids, f.a.wide_ids, f.a.n) : -1;
+        for (unsigned mask = __ballot_sync(0xffffffffu, id >= 0); mask;) {
+            L row[kAhead];
+            int to[kAhead];
+            const int there = min(kAhead, __popc(mask));
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int from = __ffs(mask) - 1;  // (0 left: not used)
+                mask &= mask - 1;
+                to[k] = __shfl_sync(0xffffffffu, (int)id, from);
+                if (k < there) row[k].load(dy + (s + from) * f.a.lddy, at, f.a.cols);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                if (k >= there) continue;
+                float sum[L::kEach];
+#pragma unroll
+                for (int q = 0; q < S::kMany; q++) {
+                    const typename S::Vec v = *S::at(sums, to[k], q, lane);
+#pragma unroll
+                    for (int i = 0; i < S::kVec; i++) sum[q * S::kVec + i] = v.v[i];
+                }
+                row[k].add(sum);
+#pragma unroll
+                for (int q = 0; q < S::kMany; q++) {
+                    typename S::Vec v;
+#pragma unroll
+                    for (int i = 0; i < S::kVec; i++) v.v[i] = sum[q * S::kVec + i];
+                    *S::at(sums, to[k], q, lane) = v;
+                }
+            }
+        }
+        id = next;
+    }
+    __syncthreads();
+    using Vec = typename S::Vec;
+    const int vecs = part / S::kVec;
+    for (int k = threadIdx.x; k < vecs; k += kTableThreads) {
+        Vec sum = reinterpret_cast<const Vec*>(all)[k];
+#pragma unroll
+        for (int w = 1; w < kFewWarps; w++) {
+            const Vec v = reinterpret_cast<const Vec*>(all + w * part)[k];
+#pragma unroll
+            for (int i = 0; i < S::kVec; i++) sum.v[i] += v.v[i];
+        }
+        if (f.chunks == 1)
+            S::out(f, (int)columns, k, sum);
+        else
+            reinterpret_cast<Vec*>(f.parts + (int64_t)blockIdx.x * part)[k] = sum;
+    }
+}
+// The CTAs' sums: 32 pieces of a chunk of columns a CTA, whose warps take every eighth of the parts.
+template <class T, int BYTES>
+static __global__ void __launch_bounds__(kTableThreads) few_join_kernel(const __grid_constant__ FewRows f) {
+    using S = FewSums<T, BYTES>;
+    using Vec = typename S::Vec;
+    __shared__ Vec shared[kFewWarps][32];
+    step_begin(nullptr);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = S::kMany * f.a.n;  // (of 32 pieces)
+    const int columns = blockIdx.x / rows, at = blockIdx.x % rows * 32 + lane;
+    const float* const parts = f.parts + (int64_t)columns * S::kRow * f.a.n;
+    Vec sum{};
+#pragma unroll 8
+    for (int c = warp; c < f.chunks; c += kFewWarps) {
+        const float* from = parts + (int64_t)c * f.across * S::kRow * f.a.n + at * S::kVec;
+        Vec v;
+        if constexpr (S::kVec == 4) {
+            const float4 w = __ldcg(reinterpret_cast<const float4*>(from));
+            v.v[0] = w.x, v.v[1] = w.y, v.v[2] = w.z, v.v[3] = w.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kVec; i++) v.v[i] = __ldcg(from + i);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kVec; i++) sum.v[i] += v.v[i];
+    }
+    shared[warp][lane] = sum;
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int w = 1; w < kFewWarps; w++)
+#pragma unroll
+        for (int i = 0; i < S::kVec; i++) sum.v[i] += shared[w][lane].v[i];
+    S::out(f, columns, at, sum);
+}
+
 }  // namespace b200

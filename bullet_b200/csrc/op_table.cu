@@ -12,6 +12,7 @@ namespace {
 using namespace b200;
 
 constexpr int kTableSms = 148;
+constexpr int kFewLists = 16, kFewMost = 512;  // of a warp (5003 lists of 520 bf16 columns, 8 rows: at least 64 13 us, 32 9.0, 16 7.5)
 
 int check_lists(const char* who, int rows, int slots, int n, int cols, int wide, float scale) {
     if (rows < 0 || slots < 1 || n < 1 || cols < 1) return fail(B200_ERR_ARG, "%s: %d lists of %d, %d rows of %d", who, rows, slots, n, cols);
@@ -86,9 +87,34 @@ int across_of(const b200_embed_grad_op* op) {
     const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
     return (op->cols + warp - 1) / warp;
 }
+// Tables of few rows: how lists are cut up.  (Us, bf16, 8 rows of 1024 columns, with ids sorted and so: 1024 lists 17 and 8, 131072 86 and 56, 262144 165 and 105.)
+bool few_rows(const b200_embed_grad_op* op) { return op->n <= kFewRows && op->slots == 1; }
+struct Few {
+    int bytes, lists, chunks, across, shared;  // of a lane, as bytes_of; lists of a warp; bytes of a CTA's sums
+};
+Few few_of(const b200_embed_grad_op* op) {
+    Few f;
+    f.bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16);
+    if (f.bytes == 16 && type_bytes(op->dy_type) == 2 && op->n > 13) f.bytes = 8;  // (or an SM has room for one CTA's sums: 262144 x 1024, 16 rows 152 us instead of 210)
+    const int warp = 32 * (f.bytes ? f.bytes : 16) / type_bytes(op->dy_type);
+    f.across = (op->cols - 1) / warp + 1;
+    f.shared = kFewWarps * op->n * warp * 4;
+    // As many CTAs as run at once, or a multiple of that where warps would add up more than kFewMost lists.  (262144 x 1024 fp32: by kFewMost alone 250 us, 180.)
+    const int64_t at_once = (int64_t)kTableSms * std::max(1, std::min(3, 230000 / (f.shared + 1024))), chunks = std::max<int64_t>(1, at_once / f.across);
+    const auto over = [](int64_t all, int64_t each) { return (all + each - 1) / each; };
+    const int64_t times = over(over(op->rows, chunks * kFewWarps), kFewMost);
+    f.lists = (int)std::max<int64_t>(kFewLists, over(op->rows, chunks * times * kFewWarps));
+    f.chunks = (int)over(op->rows, (int64_t)f.lists * kFewWarps);
+    return f;
+}
 Space space_of(const b200_embed_grad_op* op) {
     Space s{};
     if (op->rows == 0) return s;
+    if (few_rows(op)) {
+        const Few f = few_of(op);
+        if (f.chunks > 1) s.all = (int64_t)f.chunks * f.across * f.shared / kFewWarps;
+        return s;
+    }
     auto next = [&](int64_t bytes) {
         const int64_t at = s.all;
         s.all += (bytes + 255) / 256 * 256;
@@ -102,8 +128,8 @@ Space space_of(const b200_embed_grad_op* op) {
     }
     if (!sort.places) s.start = next((op->n + 1ll) * 4);
     s.numbers = next(16);
-    // Pieces of 16 for few ids, whose longest stretches then have warps enough (5003 ids of 8 rows of 520: 64 27 us, 16 23), of 64 for many, as each piece costs its part of
-    // the joining (131072 ids of 8 rows of 1024: 16 159 us, 32 118, 64 90; 2^20 lists' ids of 768 rows of 256: 64 100, 512 128); more where they would take more room.
+    // Pieces of 16 for few ids, whose longest stretches then have warps enough (before tables of few rows had kernels of their own: 5003 ids of 8 rows of 520, 64 27 us, 16 23), of
+    // 64 for many, as each piece costs its part of the joining (131072 ids of 8 rows of 1024: 16 159 us, 32 118, 64 90; 2^20 lists' ids of 768 rows of 256: 64 100, 512 128); more where they would take more room.
     s.piece = 16;
     while (s.piece < 64 ? sort.count / s.piece > 2048 : s.piece < 512 && sort.count / s.piece > 16384) s.piece *= 2;
     s.cuts = sort.count > kLongest;
@@ -116,6 +142,21 @@ Space space_of(const b200_embed_grad_op* op) {
         s.parts = next(pieces * s.ldp * 4);
     }
     return s;
+}
+
+template <class T, int BYTES>
+int few_rows_gradient(const b200_embed_grad_op* op, const Few& few, cudaStream_t s) {
+    FewRows f{*op, static_cast<float*>(op->workspace), few.lists, few.chunks, few.across};
+    static std::atomic<uint64_t> allowed;  // a bit per device
+    int device = 0;
+    OP_CK(cudaGetDevice(&device));
+    if (device >= 64 || !(allowed >> device & 1)) {
+        OP_CK(cudaFuncSetAttribute(few_rows_kernel<T, BYTES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewWarps * kFewRows * FewSums<T, BYTES>::kRow * 4));
+        if (device < 64) allowed |= (uint64_t)1 << device;
+    }
+    OP_CK(launch_step(false, few_rows_kernel<T, BYTES>, (unsigned)(few.chunks * few.across), kTableThreads, (size_t)few.shared, s, f));
+    if (few.chunks > 1) OP_CK(launch_step(true, few_join_kernel<T, BYTES>, (unsigned)(few.across * op->n * FewSums<T, BYTES>::kMany), kTableThreads, 0, s, f));
+    return 0;
 }
 
 // The whole gradient 0.
@@ -194,6 +235,17 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     OP_CK(on.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (op->rows == 0) return zeros(op, s);
+    if (few_rows(op)) {
+        const Few few = few_of(op);
+        if ((int64_t)few.chunks * few.across > INT32_MAX) return fail(B200_ERR_UNSUPPORTED, "%s: %d lists, %d columns are too many", who, op->rows, op->cols);
+        int rc = 0;
+        with_float(op->dy_type, [&](auto t) {
+            with_bytes(few.bytes, [&](auto b) {
+                if constexpr (b() != 32) rc = few_rows_gradient<decltype(t), b()>(op, few, s);
+            });
+        });
+        return rc;
+    }
     char* base = static_cast<char*>(op->workspace);
     const Sorting sort = sorting_of(op);
     if (sort.places)

@@ -595,7 +595,7 @@ int b200_op_embed(int device, void* stream, const b200_embed_op* op);
 
 /* Its gradient at the table: dtable[t] = scale * sum of dy[r] over all r, s with ids[r][s] == t, 0 for a row that none names.  The ids are sorted
  * and the sums taken in the order of the lists; where a row is met more than 64 times, 16 to 512 of them by themselves (by the number of all ids), whose sums are added up
- * sixteen at a time. */
+ * sixteen at a time.  With one id a list and up to 16 rows of the table, up to 512 neighbouring lists by themselves, whose sums are added up.  Equal calls give equal bits. */
 typedef struct b200_embed_grad_op {
     int32_t rows, slots, n, cols;
     int32_t dy_type, dtable_type;  /* B200_TYPE_F32, _BF16 or _F16 */

@@ -274,3 +274,49 @@ def test_a_table_with_more_rows_than_ids_in_a_graph(rows):
         dy.copy_(normal(seed, rows, 40))
         graph.replay()
         assert torch.equal(d, ops.embed_backward(dy, ids, 50000))
+
+
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 256, 257, 5003, 200000])
+@pytest.mark.parametrize("n", [1, 2, 8, 16, 17])
+@pytest.mark.parametrize("cols,kind,out,pad,at,wide", [(520, BF16, F32, 0, 0, 0), (24, BF16, BF16, 0, 0, 1), (7, F16, F32, 3, 1, 0), (40, F32, F16, 8, 0, 0), (300, F32, F32, 3, 1, 1),
+                                                       (4, BF16, F32, 0, 0, 0), (777, BF16, F32, 5, 3, 0), (32, F32, BF16, 0, 0, 0), (96, BF16, F32, 16, 16, 0)])
+def test_gradients_of_tables_of_few_rows(rows, n, cols, kind, out, pad, at, wide):
+    """Whole numbers, whose sums are exact: one id a list, some of them none, against 64 bits; the same bits every time; what lies around is left."""
+    ids = torch.randint(-1, n + 1, (rows,), device="cuda", dtype=torch.int64 if wide else torch.int32)
+    dy = guarded(rows, cols, kind, pad, at)[1]
+    dy.copy_(torch.randint(-3, 4, (rows, cols), device="cuda"))
+    raw, d = guarded(n, cols, out, pad, at)
+    op = _lib.CEmbedGrad(rows=rows, slots=1, n=n, cols=cols, dy_type=TYPE[kind], dtable_type=TYPE[out], wide_ids=wide, ldids=1, lddy=cols + pad, lddt=cols + pad, ids=ids.data_ptr(),
+                         dy=dy.data_ptr(), dtable=d.data_ptr(), scale=0.25)
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().b200_op_embed_backward_workspace(ctypes.byref(op), ctypes.byref(size)))
+    space = torch.full((size.value + 64,), 255, dtype=torch.uint8, device="cuda")
+    op.workspace, op.workspace_bytes = space.data_ptr(), size.value
+    to = torch.where((ids >= 0) & (ids < n), ids, n).long()
+    want = (torch.zeros(n + 1, cols, dtype=torch.float64, device="cuda").index_add_(0, to, dy.double()) / 4)[:n].to(out)
+    for _ in range(2):
+        d.fill_(GUARD)
+        call("b200_op_embed_backward", op)
+        assert torch.equal(d, want) and around(raw, d, at) and bool((space[size.value:] == 255).all())
+
+
+def test_what_is_not_finite_stays_in_its_row_and_column_of_a_table_of_few_rows():
+    ids, dy = torch.arange(3000, device="cuda", dtype=torch.int32) % 9 - 1, normal(3, 3000, 40)
+    clean = ops.embed_backward(dy, ids, 8)
+    dy[90, 3], dy[91, 5], dy[92] = float("nan"), float("inf"), float("-inf")  # of ids -1, 0 and 1
+    dirty = ops.embed_backward(dy, ids, 8)
+    kept = torch.ones(8, 40, dtype=torch.bool, device="cuda")
+    kept[0, 5], kept[1] = False, False
+    assert torch.equal(clean[kept], dirty[kept]) and torch.isposinf(dirty[0, 5]) and bool(torch.isneginf(dirty[1]).all())
+
+
+def test_stretches_of_many_pieces_of_larger_tables():
+    """As test_a_stretch_of_many_pieces, of a table that is not one of few rows."""
+    rows = 16 * 16 * 16 * 64 + 64 * 300 + 70
+    ids = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    ids[64 * 300:64 * 300 + 70] = 33
+    ids[64 * 300 + 70:] = 65
+    ids = ids[torch.randperm(rows, device="cuda")]
+    dy = torch.randint(-3, 4, (rows, 8), device="cuda").to(BF16)
+    want = torch.zeros(70, 8, dtype=torch.float64, device="cuda").index_add_(0, ids.long(), dy.double())
+    assert torch.equal(ops.embed_backward(dy, ids, 70).double(), want)
