@@ -2,7 +2,7 @@
 //
 // Bound by L2's way to the SMs (16384 lists of 17 rows of 2 KB are 590 MB out of a table of 25, in 39 us), with few lists by latency.  A warp takes a list, or a row of
 // the table, and the columns that its lanes cover with 32 bytes each, for what a row's index and address cost: with 16, 57 us.  (Fewer in narrow matrices; single elements
-// 32 apart where rows do not start on 16 bytes; 16 in the gradient, where 32 do not leave the registers that its pieces need: 110 us where 102 had been.)
+// 32 apart where rows do not start on 16 bytes.)
 // Its lanes load 32 indices side by side and hand them round, and four to sixteen rows are on their way at a time.
 //
 // The gradient's sums are taken in the order of the lists, so ids are sorted first, stably, by counting digits of up to eight bits: one CTA for up to kSortOne
@@ -21,9 +21,10 @@ namespace b200 {
 
 constexpr int kTableThreads = 256;
 // Rows on their way in a warp.  Warps that hide each other's latency count for more than rows in one: 16384 x 32 features of 1024 columns, two rows of 32 bytes a lane and
-// 32 warps of an SM 43 us, four 39; their gradient, whose rows and pieces need more of their indices too, eight and 24 warps 122, eight and 32 110, four and 40 110, four and 48 113, sixteen and 16 148.
-// So many warps as fill the GPU twice over or fewer take sixteen each.
-constexpr int kEmbedAhead = 4, kGradAhead = 8, kFewAhead = 16;
+// 32 warps of an SM 43 us, four 39; their gradient, four rows and 24 warps 82, 32 (and registers spilt) 96, two rows and 32 83, six and 24 92; by 16 bytes four
+// rows and 32 warps 96, eight 102, four and 40 103.
+// So many warps as fill the GPU twice over or fewer take sixteen rows each, of 32 bytes eight.
+constexpr int kEmbedAhead = 4, kGradAhead = 4, kFewAhead = 16;
 
 // A warp's place: one of up to 2^32 rows, and of `across` chunks of its columns; next() as many on as there are warps.
 struct WarpPlace {
@@ -151,6 +152,21 @@ __device__ __forceinline__ void add_named(const T* rows, int64_t ld, int64_t at,
 #pragma unroll
         for (int k = 0; k < AHEAD; k++)
             if (k < there) row[k].add(sum);
+    }
+}
+// ... that the first `lanes` of them name: a sum's instructions count as well (the features' gradient, with four rows on their way, 110 us by masks, 96 so).
+template <class T, int BYTES, int AHEAD>
+__device__ __forceinline__ void add_first(const T* rows, int64_t ld, int64_t at, int64_t cols, int index, int lanes, float (&sum)[Lanes<T, BYTES>::kEach]) {
+    for (int j = 0; j < lanes; j += AHEAD) {
+        Lanes<T, BYTES> row[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            const int64_t r = __shfl_sync(0xffffffffu, index, j + k);  // (past the last: some lane's, and not used)
+            if (j + k < lanes) row[k].load(rows + r * ld, at, cols);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (j + k < lanes) row[k].add(sum);
     }
 }
 
@@ -613,7 +629,7 @@ __device__ __forceinline__ void finish_row(const TableGrad& g, int64_t t, int64_
 template <class T, int BYTES>
 static __device__ __noinline__ void join_pieces(const TableGrad& g, float* parts, int n, int apart, int64_t t, int64_t at) {
     using L = Lanes<T, BYTES>;
-    constexpr int kEach = L::kEach, kJoined = kEach > 4 ? 4 : 8;  // on their way
+    constexpr int kEach = L::kEach, kJoined = kEach > 8 ? 2 : kEach > 4 ? 4 : 8;  // on their way
     float sum[kEach] = {};
     for (int q = 0; q < n; q += kJoined) {
         float v[kJoined][kEach] = {};
@@ -661,7 +677,7 @@ __device__ __forceinline__ void sum_stretch(const TableGrad& g, int from, int to
     int list = from + lane < to ? __ldcg(&g.sorted[from + lane].y) : 0;
     for (int s = from; s < to; s += 32) {
         const int next = s + 32 + lane < to ? __ldcg(&g.sorted[s + 32 + lane].y) : 0;
-        add_named<T, BYTES, AHEAD>(static_cast<const T*>(g.a.dy), g.a.lddy, at, g.a.cols, list, to - s >= 32 ? 0xffffffffu : (1u << (to - s)) - 1, sum);
+        add_first<T, BYTES, AHEAD>(static_cast<const T*>(g.a.dy), g.a.lddy, at, g.a.cols, list, min(32, to - s), sum);
         list = next;
     }
 }
@@ -681,9 +697,9 @@ __device__ __forceinline__ int stretch_end(const int2* sorted, int from, int cou
     }
 }
 // Pieces of the long stretches, a warp each, then rows of the table.  Who finishes the last member of a group joins them, in their order.  A CTA's warps count their
-// pieces together, behind one fence.  PLACES: there are no starts, and rows without ids are 0 already.  (Asked while it runs, it takes registers: 102 us were 112.)
+// pieces together, behind one fence.  PLACES: there are no starts, and rows without ids are 0 already.  (Asked while it runs, it takes registers: 112 us where 102 had been.)
 template <class T, int BYTES, int AHEAD, bool PLACES>
-static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BYTES == 0 ? 2 : 4) embed_backward_kernel(const __grid_constant__ TableGrad g) {
+static __global__ void __launch_bounds__(kTableThreads, AHEAD > kGradAhead || BYTES == 0 ? 2 : BYTES == 32 ? 3 : 4) embed_backward_kernel(const __grid_constant__ TableGrad g) {
     using L = Lanes<T, BYTES>;
     constexpr uint32_t kWarps = kTableThreads / 32;
     __shared__ int joins[kWarps];

@@ -54,7 +54,9 @@ void with_bytes(int bytes, F f) {
     else
         f(std::integral_constant<int, 0>{});
 }
-unsigned ctas_for(int64_t warps) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((warps + kTableThreads / 32 - 1) / (kTableThreads / 32), kTableSms * 8)); }
+// (More than run at once, as stretches are of all lengths: by 8 an SM the features' gradient takes 81.6 us and one of 131072 ids of 12288 rows 84.8, by 12 80.5 and 81.5, by 48 83.4
+// and 78.3, but lookups longer.)
+unsigned ctas_for(int64_t warps) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((warps + kTableThreads / 32 - 1) / (kTableThreads / 32), kTableSms * 12)); }
 
 // How ids are sorted: in passes of equal digits, by whole tiles, or by one CTA.
 struct Sorting {
@@ -84,7 +86,7 @@ struct Space {
 };
 // How many warps' columns a row has.
 int across_of(const b200_embed_grad_op* op) {
-    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
+    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 32), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
     return (op->cols + warp - 1) / warp;
 }
 // Tables of few rows: how lists are cut up.  (Us, bf16, 8 rows of 1024 columns, with ids sorted and so: 1024 lists 17 and 8, 131072 86 and 56, 262144 165 and 105.)
@@ -287,19 +289,17 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     TableGrad g{*op, p.to, start, numbers + 2, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
     cudaError_t rc = cudaSuccess;
     with_float(op->dy_type, [&](auto t) {
-        with_bytes(bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16), [&](auto b) {
-            if constexpr (b() != 32) {
-                using L = Lanes<decltype(t), b()>;
-                g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kOf);
-                const int64_t most = ((sort.places ? sort.count : op->n) + (space.cuts ? sort.count / space.piece : 0)) * space.across;
-                auto go = [&](auto kernel) { rc = launch_step(true, kernel, ctas_for(most), kTableThreads, 0, s, g); };
-                // (few warps: as much on its way as registers hold)
-                constexpr int kFew = b() ? kFewAhead : kGradAhead;
-                if (most <= kTableSms * 16)
-                    sort.places ? go(embed_backward_kernel<decltype(t), b(), kFew, true>) : go(embed_backward_kernel<decltype(t), b(), kFew, false>);
-                else
-                    sort.places ? go(embed_backward_kernel<decltype(t), b(), kGradAhead, true>) : go(embed_backward_kernel<decltype(t), b(), kGradAhead, false>);
-            }
+        with_bytes(bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 32), [&](auto b) {
+            using L = Lanes<decltype(t), b()>;
+            g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kOf);
+            const int64_t most = ((sort.places ? sort.count : op->n) + (space.cuts ? sort.count / space.piece : 0)) * space.across;
+            auto go = [&](auto kernel) { rc = launch_step(true, kernel, ctas_for(most), kTableThreads, 0, s, g); };
+            // (few warps: as much on its way as registers hold)
+            constexpr int kFew = b() == 32 ? kFewAhead / 2 : b() ? kFewAhead : kGradAhead;
+            if (most <= kTableSms * 16)
+                sort.places ? go(embed_backward_kernel<decltype(t), b(), kFew, true>) : go(embed_backward_kernel<decltype(t), b(), kFew, false>);
+            else
+                sort.places ? go(embed_backward_kernel<decltype(t), b(), kGradAhead, true>) : go(embed_backward_kernel<decltype(t), b(), kGradAhead, false>);
         });
     });
     OP_CK(rc);
