@@ -87,7 +87,7 @@ struct Space {
 // How many warps' columns a row has.
 int across_of(const b200_embed_grad_op* op) {
     const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 32), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
-    return (op->cols + warp - 1) / warp;
+    return (op->cols - 1) / warp + 1;
 }
 // Tables of few rows: how lists are cut up.  (Us, bf16, 8 rows of 1024 columns, with ids sorted and so: 1024 lists 17 and 8, 131072 86 and 56, 262144 165 and 105.)
 bool few_rows(const b200_embed_grad_op* op) { return op->n <= kFewRows && op->slots == 1; }

@@ -148,7 +148,9 @@ def gradient_norm(gradients):
 def clip_gradients(gradients, max_norm: float, out=None):
     """([tensors], norm): the gradients times max_norm / norm where their norm together is above max_norm (and finite), else as they are.  `out`:
     where they go; may be `gradients`, or any of them, themselves, which are then written only if they change."""
-    return _calls.clip_gradients(gradients, float(max_norm), out)
+    if max_norm is None:
+        raise TypeError("max_norm: a number is wanted")
+    return _calls.clip_gradients(gradients, max_norm, out)
 
 
 def gave_up(device: int) -> bool:
