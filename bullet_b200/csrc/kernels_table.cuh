@@ -23,7 +23,7 @@ constexpr int kTableThreads = 256;
 // Rows on their way in a warp.  Warps that hide each other's latency count for more than rows in one: 16384 x 32 features of 1024 columns, two rows of 32 bytes a lane and
 // 32 warps of an SM 43 us, four 39; their gradient, four rows and 24 warps 82, 32 (and registers spilt) 96, two rows and 32 83, six and 24 92; by 16 bytes four
 // rows and 32 warps 96, eight 102, four and 40 103.
-// So many warps as fill the GPU twice over or fewer take sixteen rows each, of 32 bytes eight.
+// So many warps as fill the GPU twice over or fewer take sixteen rows of 16 bytes each.
 constexpr int kEmbedAhead = 4, kGradAhead = 4, kFewAhead = 16;
 
 // A warp's place: one of up to 2^32 rows, and of `across` chunks of its columns; next() as many on as there are warps.
@@ -172,7 +172,7 @@ __device__ __forceinline__ void add_first(const T* rows, int64_t ld, int64_t at,
 
 // VEC: a row of y takes a lane's elements together.
 template <class T, int BYTES, int AHEAD>
-static __global__ void __launch_bounds__(kTableThreads, AHEAD >= kFewAhead / 2 || BYTES == 0 ? 2 : 4) embed_kernel(b200_embed_op a, int vec) {
+static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BYTES == 0 ? 2 : 4) embed_kernel(b200_embed_op a, int vec) {
     using L = Lanes<T, BYTES>;
     const int lane = threadIdx.x & 31;
     WarpPlace p((int)((a.cols + L::kWarp - 1ll) / L::kWarp));
@@ -191,12 +191,12 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD >= kFewAhead / 2 |
             store_sums<T, BYTES, false>(a.y, p.row * a.ldy, at, a.cols, a.y_type, sum);
     }
 }
-// Lists of up to kEmbedAhead ids: a warp takes as many lists as its lanes have room for, and of these as many at a time as have kEmbedAhead ids together.  (One
-// id each, 131072 x 1024 bf16: 67 us, a list at a time 147.)
+// Lists of up to kEmbedAhead ids: a warp takes `lists` of them, as many as its lanes have room for or fewer, and of these as many at a time as have kEmbedAhead ids together.  (One
+// id each, 131072 x 1024 bf16: 63 us, a list at a time 147.)
 template <class T, int BYTES>
-static __global__ void __launch_bounds__(kTableThreads, BYTES == 0 ? 2 : 4) embed_short_kernel(b200_embed_op a, int vec) {
+static __global__ void __launch_bounds__(kTableThreads, BYTES == 0 ? 2 : 4) embed_short_kernel(b200_embed_op a, int lists, int vec) {
     using L = Lanes<T, BYTES>;
-    const int lane = threadIdx.x & 31, at_once = kEmbedAhead / a.slots, lists = 32 / a.slots / at_once * at_once;
+    const int lane = threadIdx.x & 31, at_once = kEmbedAhead / a.slots;
     WarpPlace p((int)((a.cols + L::kWarp - 1ll) / L::kWarp));
     for (; (int64_t)p.row * lists < a.rows; p.next()) {
         const int64_t at = L::first(p.at), first = (int64_t)p.row * lists;

@@ -36,6 +36,23 @@ int bytes_of(const void* at, int64_t ld, int cols, int type, int most) {
     if (row > 128 && on(8)) return 8;
     return on(4) ? 4 : 0;
 }
+// How many warps' columns a row has.
+int across_of(int bytes, int cols, int type) { return (cols - 1) / (32 * (bytes ? bytes : 16) / type_bytes(type)) + 1; }
+// What warps there are for `rows` of them, and the bytes of their lanes: 16 at most, and as many rows on their way as registers hold, where that makes few warps.
+struct Lines {
+    int bytes, across;
+    int64_t warps;
+    bool few;
+};
+Lines lines_of(const void* at, int64_t ld, int cols, int type, int64_t rows, int few_warps) {
+    Lines l;
+    l.bytes = bytes_of(at, ld, cols, type, 32);
+    l.few = l.bytes && rows * across_of(l.bytes, cols, type) <= few_warps;
+    if (l.few) l.bytes = std::min(l.bytes, 16);
+    l.across = across_of(l.bytes, cols, type);
+    l.warps = rows * l.across;
+    return l;
+}
 // Whether rows of `type` take `each` elements together.
 bool together(const void* at, int64_t ld, int type, int each) {
     const int64_t bytes = std::min(16, each * type_bytes(type));
@@ -81,14 +98,10 @@ Sorting sorting_of(const b200_embed_grad_op* op) {
 struct Space {
     int64_t pairs, more_pairs, counts, start, numbers, done, pieces, parts, all;
     int64_t ldp;
-    int piece, across;
+    int piece;
+    Lines lines;
     bool cuts;
 };
-// How many warps' columns a row has.
-int across_of(const b200_embed_grad_op* op) {
-    const int bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 32), warp = 32 * (bytes ? bytes : 16) / type_bytes(op->dy_type);
-    return (op->cols - 1) / warp + 1;
-}
 // Tables of few rows: how lists are cut up.  (Us, bf16, 8 rows of 1024 columns, with ids sorted and so: 1024 lists 17 and 8, 131072 86 and 56, 262144 165 and 105.)
 bool few_rows(const b200_embed_grad_op* op) { return op->n <= kFewRows && op->slots == 1; }
 struct Few {
@@ -98,9 +111,8 @@ Few few_of(const b200_embed_grad_op* op) {
     Few f;
     f.bytes = bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 16);
     if (f.bytes == 16 && type_bytes(op->dy_type) == 2 && op->n > 13) f.bytes = 8;  // (or an SM has room for one CTA's sums: 262144 x 1024, 16 rows 152 us instead of 210)
-    const int warp = 32 * (f.bytes ? f.bytes : 16) / type_bytes(op->dy_type);
-    f.across = (op->cols - 1) / warp + 1;
-    f.shared = kFewWarps * op->n * warp * 4;
+    f.across = across_of(f.bytes, op->cols, op->dy_type);
+    f.shared = kFewWarps * op->n * 32 * (f.bytes ? f.bytes : 16) / type_bytes(op->dy_type) * 4;
     // As many CTAs as run at once, or a multiple of that where warps would add up more than kFewMost lists.  (262144 x 1024 fp32: by kFewMost alone 250 us, 180.)
     const int64_t at_once = (int64_t)kTableSms * std::max(1, std::min(3, 230000 / (f.shared + 1024))), chunks = std::max<int64_t>(1, at_once / f.across);
     const auto over = [](int64_t all, int64_t each) { return (all + each - 1) / each; };
@@ -135,10 +147,10 @@ Space space_of(const b200_embed_grad_op* op) {
     s.piece = 16;
     while (s.piece < 64 ? sort.count / s.piece > 2048 : s.piece < 512 && sort.count / s.piece > 16384) s.piece *= 2;
     s.cuts = sort.count > kLongest;
-    s.across = across_of(op);
+    s.lines = lines_of(op->dy, op->lddy, op->cols, op->dy_type, (sort.places ? sort.count : op->n) + (s.cuts ? sort.count / s.piece : 0), kTableSms * 16);
     if (s.cuts) {  // (whole pieces, and of each long stretch one that is none)
         const int64_t pieces = sort.count / s.piece + std::min<int64_t>(op->n, sort.count / kLongest);
-        s.done = next(pieces * s.across * 4);
+        s.done = next(pieces * s.lines.across * 4);
         s.pieces = next(pieces * (int64_t)sizeof(Piece8));
         s.ldp = (op->cols + 7ll) / 8 * 8;
         s.parts = next(pieces * s.ldp * 4);
@@ -196,18 +208,20 @@ int b200_op_embed(int device, void* stream, const b200_embed_op* op) {
     if (int rc = check_matrix(who, "y", op->y, op->ldy, op->rows, op->cols, op->y_type)) return rc;
     OnDevice on(device);
     OP_CK(on.status);
-    const int bytes = bytes_of(op->table, op->ldt, op->cols, op->table_type, 32);
+    const Lines lines = lines_of(op->table, op->ldt, op->cols, op->table_type, op->rows, kTableSms * 8);
+    // Short lists: as many of a warp as leave an SM 32 warps, up to all that its lanes have indices of.  (5003 lists of one id, 1024 columns: 32 of a warp 14 us, four 5.3.)
+    const int at_once = std::max(1, kEmbedAhead / op->slots), most = 32 / std::min(32, op->slots) / at_once * at_once;
+    const int lists = (int)std::min<int64_t>(most, (lines.warps / (kTableSms * 32) + at_once) / at_once * at_once);
     with_float(op->table_type, [&](auto t) {
-        with_bytes(bytes, [&](auto b) {
+        with_bytes(lines.bytes, [&](auto b) {
             using L = Lanes<decltype(t), b()>;
-            const int64_t warps = op->rows * ((op->cols + L::kWarp - 1ll) / L::kWarp);
             const int vec = together(op->y, op->ldy, op->y_type, L::kOf);
-            auto go = [&](auto kernel) { kernel<<<ctas_for(warps), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, vec); };
-            // (few warps: as much on its way as registers hold)
-            if (op->slots <= kEmbedAhead && warps > kTableSms * 8)
-                go(embed_short_kernel<decltype(t), b()>);
-            else if (b() && warps <= kTableSms * 8)
-                go(embed_kernel<decltype(t), b(), b() == 32 ? kFewAhead / 2 : b() ? kFewAhead : kEmbedAhead>);
+            auto go = [&](auto kernel) { kernel<<<ctas_for(lines.warps), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, vec); };
+            constexpr int kFew = b() == 32 || b() == 0 ? kEmbedAhead : kFewAhead;
+            if (op->slots <= kEmbedAhead && !lines.few)
+                embed_short_kernel<decltype(t), b()><<<ctas_for((op->rows + lists - 1ll) / lists * lines.across), kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(*op, lists, vec);
+            else if (lines.few)
+                go(embed_kernel<decltype(t), b(), kFew>);
             else
                 go(embed_kernel<decltype(t), b(), kEmbedAhead>);
         });
@@ -255,7 +269,7 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     int2* pairs[2] = {reinterpret_cast<int2*>(base + space.pairs), reinterpret_cast<int2*>(base + space.more_pairs)};
     int* start = sort.places ? nullptr : reinterpret_cast<int*>(base + space.start);
     int* numbers = reinterpret_cast<int*>(base + space.numbers);
-    const Long l{numbers, reinterpret_cast<Piece8*>(base + space.pieces), reinterpret_cast<int*>(base + space.done), space.piece, space.across};
+    const Long l{numbers, reinterpret_cast<Piece8*>(base + space.pieces), reinterpret_cast<int*>(base + space.done), space.piece, space.lines.across};
     SortPass p{};
     p.ids = op->ids, p.ldids = op->ldids, p.slots = (uint32_t)op->slots, p.wide = op->wide_ids, p.n = op->n;
     p.count = (uint32_t)sort.count, p.tiles = sort.tiles, p.bits = sort.bits, p.to = pairs[0];
@@ -289,14 +303,12 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
     TableGrad g{*op, p.to, start, numbers + 2, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
     cudaError_t rc = cudaSuccess;
     with_float(op->dy_type, [&](auto t) {
-        with_bytes(bytes_of(op->dy, op->lddy, op->cols, op->dy_type, 32), [&](auto b) {
+        with_bytes(space.lines.bytes, [&](auto b) {
             using L = Lanes<decltype(t), b()>;
             g.vec = together(op->dtable, op->lddt, op->dtable_type, L::kOf);
-            const int64_t most = ((sort.places ? sort.count : op->n) + (space.cuts ? sort.count / space.piece : 0)) * space.across;
-            auto go = [&](auto kernel) { rc = launch_step(true, kernel, ctas_for(most), kTableThreads, 0, s, g); };
-            // (few warps: as much on its way as registers hold)
-            constexpr int kFew = b() == 32 ? kFewAhead / 2 : b() ? kFewAhead : kGradAhead;
-            if (most <= kTableSms * 16)
+            auto go = [&](auto kernel) { rc = launch_step(true, kernel, ctas_for(space.lines.warps), kTableThreads, 0, s, g); };
+            constexpr int kFew = b() == 32 || b() == 0 ? kGradAhead : kFewAhead;
+            if (space.lines.few)
                 sort.places ? go(embed_backward_kernel<decltype(t), b(), kFew, true>) : go(embed_backward_kernel<decltype(t), b(), kFew, false>);
             else
                 sort.places ? go(embed_backward_kernel<decltype(t), b(), kGradAhead, true>) : go(embed_backward_kernel<decltype(t), b(), kGradAhead, false>);
