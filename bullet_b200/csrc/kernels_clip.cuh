@@ -76,7 +76,9 @@ struct Piece {
             for (int i = 0; i < kEach; i++) exact = fma((double)to_float(v[k][i]), (double)to_float(v[k][i]), exact);
         return exact;
     }
-    __device__ __forceinline__ void store(const ClipBatch& b, int tensor, int64_t chunk, float share, float then) const {
+    // out = share(element)
+    template <class F>
+    __device__ __forceinline__ void store(const ClipBatch& b, int tensor, int64_t chunk, F share) const {
         T* out = static_cast<T*>(b.out[tensor]);
         const int64_t n = b.n[tensor];
         const bool vec = b.vec[tensor] && (chunk + 1) * kClipChunk <= n;
@@ -84,7 +86,7 @@ struct Piece {
         for (int k = 0; k < kMany; k++) {
             T y[kEach];
 #pragma unroll
-            for (int i = 0; i < kEach; i++) y[i] = from_float<T>(to_float(v[k][i]) * share * then);
+            for (int i = 0; i < kEach; i++) y[i] = from_float<T>(share(to_float(v[k][i])));
             if (vec) {
                 uint4 w;
                 memcpy(&w, y, 16);
@@ -152,7 +154,8 @@ static __global__ void __launch_bounds__(kClipThreads) clip_kernel(const __grid_
     if (threadIdx.x == 0 && blockIdx.x == 0 && t.norm) *t.norm = (float)norm;
     const bool clips = norm > t.max_norm && norm < 0x1p1023;
     const double ratio = clips ? t.max_norm / norm : 1.0;
-    const float then = ratio < 0x1p-100 ? 0x1p-100f : 1.f, share = (float)(ratio / then);  // (a share below fp32's normal numbers would lose bits)
+    const bool tiny = ratio < 0x1p-100;  // (below fp32's normal numbers a share would lose bits, or all: it stays in 64 then)
+    const float share = (float)ratio;
     int tensor = b.count - 1;
     for (int chunk = b.chunks - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
         while (b.first[tensor] > chunk) tensor--;
@@ -160,7 +163,10 @@ static __global__ void __launch_bounds__(kClipThreads) clip_kernel(const __grid_
         with_kind(b.type[tensor], [&](auto k) {
             Piece<decltype(k)> piece;
             piece.load(b, tensor, chunk - b.first[tensor]);
-            piece.store(b, tensor, chunk - b.first[tensor], share, then);
+            if (__builtin_expect(tiny, 0))
+                piece.store(b, tensor, chunk - b.first[tensor], [=](float x) { return (float)(x * ratio); });
+            else
+                piece.store(b, tensor, chunk - b.first[tensor], [=](float x) { return x * share; });
         });
     }
 }
