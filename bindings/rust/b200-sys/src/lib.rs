@@ -299,6 +299,7 @@ pub struct b200_clip_op {
     pub norm: *mut f32,
     pub workspace: *mut c_void,
     pub max_norm: f32,
+    pub max_norm_low: f32,
     pub workspace_bytes: i64,
 }
 

@@ -131,7 +131,7 @@ class CGradient(ctypes.Structure):
 class CClip(ctypes.Structure):
     """b200_clip_op"""
 
-    _fields_ = _fields("count", "", "gradients norm workspace", f32="max_norm", last="workspace_bytes")
+    _fields_ = _fields("count", "", "gradients norm workspace", f32="max_norm max_norm_low", last="workspace_bytes")
 
 
 class CSavedFormat(ctypes.Structure):

@@ -26,7 +26,7 @@ struct ClipBatch {
 struct ClipTotal {
     const double* sums;
     int n_sums;
-    float max_norm;
+    double max_norm;
     float* norm;
 };
 

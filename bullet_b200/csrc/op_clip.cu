@@ -49,6 +49,8 @@ ClipBatch batch_of(const b200_clip_op* op, int first, int last) {
     return b;
 }
 
+double limit_of(const b200_clip_op* op) { return (double)op->max_norm + op->max_norm_low; }
+
 // Whether what is written overlaps what is read or written elsewhere; a tensor may be scaled in place.
 int check_overlaps(const b200_clip_op* op, const char* who) {
     struct Range {
@@ -98,7 +100,7 @@ int b200_op_clip_gradients(int device, void* stream, const b200_clip_op* op) try
         if (((uintptr_t)t.g | (uintptr_t)t.out) % type_bytes(t.type)) return fail(B200_ERR_ARG, "%s: gradient %d is not aligned to its elements", who, k);
         writes |= t.n && t.out;
     }
-    if (writes && !(op->max_norm >= 0.f)) return fail(B200_ERR_ARG, "%s: max_norm must not be negative", who);
+    if (writes && !(limit_of(op) >= 0)) return fail(B200_ERR_ARG, "%s: max_norm must not be negative", who);
     if (int rc = check_overlaps(op, who)) return rc;
     if (int rc = check_floats(who, "norm", op->norm)) return rc;
     if (int rc = check_workspace(who, op->workspace, op->workspace_bytes, clip_bytes(op))) return rc;
@@ -106,7 +108,7 @@ int b200_op_clip_gradients(int device, void* stream, const b200_clip_op* op) try
     OP_CK(on.status);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     double* sums = static_cast<double*>(op->workspace);
-    ClipTotal total{sums, 0, op->max_norm, op->norm};
+    ClipTotal total{sums, 0, limit_of(op), op->norm};
     cudaError_t rc = cudaSuccess;
     batches(op, [&](int first, int last) {
         const ClipBatch b = batch_of(op, first, last);

@@ -13,6 +13,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
 #include <vector>
@@ -446,8 +447,10 @@ PyObject* clip_gradients(PyObject* const* a) {
     const at::Tensor norm = empty({}, at::kFloat, first);
     b200_clip_op op{};
     op.count = (int)count, op.gradients = gradients.data(), op.norm = static_cast<float*>(norm.data_ptr());
-    op.max_norm = writes ? (float)number(a[1]) : 0.f;
-    if (writes && !(op.max_norm >= 0)) refuse("max_norm: 0 or above is wanted");
+    const double max_norm = writes ? number(a[1]) : 0;
+    if (!(max_norm >= 0)) refuse("max_norm: 0 or above is wanted");
+    op.max_norm = (float)max_norm;
+    op.max_norm_low = std::isfinite(op.max_norm) ? (float)(max_norm - op.max_norm) : 0.f;
     const at::Tensor scratch = space(b200_op_clip_gradients_workspace, op, first);
     check(b200_op_clip_gradients(device_of(first), stream_of(first), &op));
     if (!writes) return Py_BuildValue("(ON)", Py_None, THPVariable_Wrap(norm));

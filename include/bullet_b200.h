@@ -611,8 +611,8 @@ typedef struct b200_embed_grad_op {
 int b200_op_embed_backward_workspace(const b200_embed_grad_op* op, int64_t* bytes);
 int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* op);
 
-/* ---- the gradients of a step together: norm = sqrt(sum of the squares of all elements), and out = share * g with share = max_norm / norm where the
- * norm is finite and above max_norm, else 1 (so a norm that is not finite changes nothing, and says so).  Squares are summed in 32 bits for 32
+/* ---- the gradients of a step together: norm = sqrt(sum of the squares of all elements), and out = share * g with share = limit / norm where the
+ * norm is finite and above the limit, else 1 (so a norm that is not finite changes nothing, and says so).  Squares are summed in 32 bits for 32
  * elements, beyond in 64; a norm past fp32 is infinity, its share is right all the same.  Elements lie side by side.  `out` may be the gradient
  * itself, which is then read and written only if it changes, or memory that overlaps no other gradient and output; NULL: counted, not written. */
 typedef struct b200_gradient {
@@ -626,7 +626,8 @@ typedef struct b200_clip_op {
     const b200_gradient* gradients; /* [count], HOST memory, read by the call */
     float* norm;                   /* out: [1] */
     void* workspace;               /* 16-byte aligned */
-    float max_norm;                /* read where anything is written; 0 or above */
+    float max_norm, max_norm_low;  /* read where anything is written: the limit is their sum, 0 or above (a number of 32 bits and 0, or both
+                                      parts of one of 64) */
     int64_t workspace_bytes;
 } b200_clip_op;
 int b200_op_clip_gradients_workspace(const b200_clip_op* op, int64_t* bytes);
