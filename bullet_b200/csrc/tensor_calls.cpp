@@ -453,6 +453,9 @@ PyObject* clip_gradients(PyObject* const* a) {
     op.max_norm_low = std::isfinite(op.max_norm) ? (float)(max_norm - op.max_norm) : 0.f;
     const at::Tensor scratch = space(b200_op_clip_gradients_workspace, op, first);
     check(b200_op_clip_gradients(device_of(first), stream_of(first), &op));
+    // (torch counts what is written in place, so that a backward which has kept such a tensor does not go on with other values; tensors of inference mode have no count)
+    for (Py_ssize_t k = 0; outs.o && k < count; k++)
+        if (!held[count + k].is_inference()) held[count + k].unsafeGetTensorImpl()->bump_version();
     if (!writes) return Py_BuildValue("(ON)", Py_None, THPVariable_Wrap(norm));
     const Reference clipped{PyList_New(count)};
     if (!clipped.o) throw Raised{};

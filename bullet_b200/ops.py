@@ -148,7 +148,8 @@ def gradient_norm(gradients):
 def clip_gradients(gradients, max_norm: float, out=None):
     """([tensors], norm): the gradients times max_norm / norm where their norm together is above max_norm (and finite), else as they are.  max_norm
     is taken in 64 bits; past fp32's numbers it is infinity.  `out`:
-    where they go; may be `gradients`, or any of them, themselves, which are then written only if they change."""
+    where they go; may be `gradients`, or any of them, themselves, which are then written only if they change.  To torch all of `out` is written in place:
+    a backward that has kept one of them raises."""
     if max_norm is None:
         raise TypeError("max_norm: a number is wanted")
     return _calls.clip_gradients(gradients, max_norm, out)
