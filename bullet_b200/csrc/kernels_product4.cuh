@@ -210,6 +210,9 @@ static __global__ void __launch_bounds__((Tile4<BN, PAIR, ADDS>::kThreads), 1)
         }
     } else if (warp == 1) {
         if (rank == 0) {  // multiplies: the whole warp keeps count, one lane issues (operands that all lanes agree on need no way into uniform registers)
+            // The pair's other CTA arrives at these barriers too, whose tensor memory the products read and write.  (The other waits are for this CTA's own copies and
+            // for what the tensor pipe leaves; at the pair's scope they take 16384 x 1024 -> 2048 26.1 us instead of 25.4, these alone nothing.)
+            const WaitsFor<PAIR> wait{&dead, p.gave_up};
             const bool issues = elected();
             const uint32_t a0 = smem_u32(base) >> 4, form = four_form(T::kRows, BN, 0), other = four_form(T::kRows, BN, 1);
             const int whole = (int)(p.k / 256), rest = (int)((p.k % 256 + 63) / 64);  // stages, and products of the last one (past k there may be no scales)
