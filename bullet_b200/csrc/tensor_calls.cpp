@@ -407,6 +407,13 @@ struct Reference {
     PyObject* o;
     ~Reference() { Py_XDECREF(o); }
 };
+// Whether the elements of two tensors of one shape lie alike (a dimension of one element lies anyhow, and so do no elements).
+bool lie_alike(Tensor a, Tensor b) {
+    if (a.sizes() != b.sizes()) return false;
+    for (int64_t k = 0; k < a.dim(); k++)
+        if (a.size(k) > 1 && a.stride(k) != b.stride(k) && a.numel()) return false;
+    return true;
+}
 // (gradients, max_norm, out) -> (outputs or None, norm); max_norm None: the norm alone; out None: new tensors
 PyObject* clip_gradients(PyObject* const* a) {
     const Reference list{PySequence_Fast(a[0], "gradients: a sequence of tensors is wanted")};
@@ -436,7 +443,7 @@ PyObject* clip_gradients(PyObject* const* a) {
         if (outs.o) {
             held.push_back(tensor(PySequence_Fast_GET_ITEM(outs.o, k), "out"));
             Tensor t = held.back();
-            if (t.scalar_type() != g.scalar_type() || t.sizes() != g.sizes() || t.strides() != g.strides() || t.device() != g.device())
+            if (t.scalar_type() != g.scalar_type() || !lie_alike(t, g) || t.device() != g.device())
                 refuse("out[" + std::to_string(k) + "]: not of its gradient's type, shape, strides and device");
         } else {
             held.push_back(at::detail::empty_strided_cuda(g.sizes(), g.strides(), g.scalar_type(), g.device()));
