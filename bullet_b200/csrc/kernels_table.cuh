@@ -289,7 +289,7 @@ __device__ __forceinline__ int sort_digit(const SortPass& p, int id) { return id
 static __global__ void __launch_bounds__(kSortThreads) pass_count_kernel(SortPass p, int* cleared) {
     __shared__ int count[256];
     step_begin(nullptr);
-    if (blockIdx.x == 0 && threadIdx.x < 2 && !p.from) cleared[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && !p.from) *cleared = 0;
     count[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t first = blockIdx.x * (uint32_t)kSortTile, all = p.from ? (uint32_t)__ldcg(p.there) : p.count;
@@ -437,12 +437,12 @@ __device__ __forceinline__ Piece8 load_piece(const Piece8* at) {
     p.row = u.x, p.begin = u.y, p.end = u.z, p.first = u.w, p.pieces = __ldcg(&at->pieces);
     return p;
 }
-// counts[0]: of long rows, counts[1]: of their pieces.  In no order of theirs: it says where a piece's sum is kept, not in which order they are joined.
+// count: of long rows' pieces.  They are listed in no order of the rows': it says where a piece's sum is kept, not in which order they are joined.
 // A row's pieces are joined kGroup at a time, their sums kGroup at a time, and so on; done[piece][warp's columns] says how many members of a group are there: of a group of
 // level l, of kGroup^(l + 1) pieces, at the piece l behind its first one.
 constexpr int kLongest = 64, kGroup = 16;
 struct Long {
-    int* counts;
+    int* count;
     Piece8* pieces;
     int* done;
     int piece, across;
@@ -480,18 +480,17 @@ struct ManyPieces {
 template <int ROOM>
 __device__ __forceinline__ void list_long(const Long& l, int t, int from, int to, ManyPieces<ROOM>& many) {
     const int lane = threadIdx.x & 31, own = to - from > kLongest ? (to - from + l.piece - 1) / l.piece : 0;
-    const unsigned are = __ballot_sync(0xffffffffu, own > 0);
-    if (!are) return;
+    if (!__any_sync(0xffffffffu, own > 0)) return;
     int run = own;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
         const int u = __shfl_up_sync(0xffffffffu, run, o);
         if (lane >= o) run += u;
     }
-    unsigned long long base = 0;
-    if (lane == 31) base = atomicAdd(reinterpret_cast<unsigned long long*>(l.counts), (unsigned long long)run << 32 | (unsigned)__popc(are));
+    int base = 0;
+    if (lane == 31) base = atomicAdd(l.count, run);
     base = __shfl_sync(0xffffffffu, base, 31);
-    const Stretch s{t, from, to, own, (int)(base >> 32) + run - own};
+    const Stretch s{t, from, to, own, base + run - own};
     if (own > 4)
         many.add(s);
     else
@@ -538,13 +537,12 @@ constexpr int kOneThreads = 1024, kOneEach = 8, kSortOne = kOneThreads * kOneEac
 static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p, int passes, int* start, int* there, Long l) {
     extern __shared__ int2 pairs[];                               // [kSortOne]
     int* const count = reinterpret_cast<int*>(pairs + kSortOne);  // [32][(1 << bits) + 1]
-    __shared__ int totals[256], sums[33];
-    __shared__ unsigned long long numbers;
+    __shared__ int totals[256], sums[33], pieces;
     __shared__ ManyPieces<kSortOne / kLongest> many;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, apart = digits + 1;
     int2 element[kOneEach];
     int digit[kOneEach], rank[kOneEach], all = (int)p.count;
-    if (threadIdx.x == 0) numbers = 0, many.warps = many.all = 0;
+    if (threadIdx.x == 0) pieces = many.warps = many.all = 0;
     sort_elements(p, warp * kOneEach * 32 + lane, 32, p.count, element);
     for (int pass = 0; pass < passes; pass++, p.shift += p.bits) {
         if (pass)
@@ -588,8 +586,8 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
         }
     if (threadIdx.x == 0) *there = all;
     __syncthreads();
-    int* const counts = l.counts;
-    l.counts = reinterpret_cast<int*>(&numbers);
+    int* const count_out = l.count;
+    l.count = &pieces;
     if (all > kLongest && start)
         for (int t = threadIdx.x; t - lane < p.n; t += kOneThreads) list_long(l, t, t < p.n ? start[t] : 0, t < p.n ? start[t + 1] : 0, many);
     else if (all > kLongest)
@@ -599,7 +597,7 @@ static __global__ void __launch_bounds__(kOneThreads) sort_one_kernel(SortPass p
         }
     __syncthreads();
     many.list(l);
-    if (threadIdx.x < 2) counts[threadIdx.x] = reinterpret_cast<const int*>(&numbers)[threadIdx.x];
+    if (threadIdx.x == 0) *count_out = pieces;
 }
 
 // ---- the gradient
@@ -705,7 +703,7 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD > kGradAhead || BY
     __shared__ int joins[kWarps];
     step_begin(nullptr);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, across = g.l.across;
-    const uint32_t items = g.cuts ? __ldcg(g.l.counts + 1) * across : 0;
+    const uint32_t items = g.cuts ? __ldcg(g.l.count) * across : 0;
     for (uint32_t base = blockIdx.x * kWarps; base < items; base += gridDim.x * kWarps) {
         const uint32_t item = base + warp;
         const int64_t at = L::first(item % across);

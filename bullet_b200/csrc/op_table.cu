@@ -280,11 +280,11 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
             OP_CK(cudaFuncSetAttribute(sort_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortOne * 8 + 32 * 257 * 4));
             if (device < 64) allowed |= (uint64_t)1 << device;
         }
-        sort_one_kernel<<<1, kOneThreads, shared, s>>>(p, sort.passes, start, numbers + 2, l);
+        sort_one_kernel<<<1, kOneThreads, shared, s>>>(p, sort.passes, start, numbers + 1, l);
         OP_CK(cudaGetLastError());
     } else {
         p.counts = reinterpret_cast<int*>(base + space.counts);
-        p.there = numbers + 2;
+        p.there = numbers + 1;
         for (int k = 0; k < sort.passes; k++) {
             p.to = pairs[k & 1];
             p.shift = k * sort.bits;
@@ -300,7 +300,7 @@ int b200_op_embed_backward(int device, void* stream, const b200_embed_grad_op* o
             OP_CK(launch_step(true, list_long_kernel, (unsigned)((op->n + kTableThreads - 1ll) / kTableThreads), kTableThreads, 0, s, start, op->n, l));
         }
     }
-    TableGrad g{*op, p.to, start, numbers + 2, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
+    TableGrad g{*op, p.to, start, numbers + 1, l, reinterpret_cast<float*>(base + space.parts), space.ldp, space.cuts, 0};
     cudaError_t rc = cudaSuccess;
     with_float(op->dy_type, [&](auto t) {
         with_bytes(space.lines.bytes, [&](auto b) {
