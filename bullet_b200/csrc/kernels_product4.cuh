@@ -18,8 +18,8 @@
 // (Scales of two stages, and an overlap of 64 columns: the way from the products that last used a place, by way of those warps, to those that use it
 // next is longer than one stage's products: 1050 ns a stage.)
 //
-// Measured, us: 131072 x 2048 -> 512 73 (3.8 PFLOP/s, under the power cap: 64 with codes of zeros; a tile's eight stages 2.3 us, 0.95 until the next one's begin, 3.6
-// together; HBM 42); 16384 x 1024 -> 2048 22, with a residual 33.
+// Measured, us: 131072 x 2048 -> 512 71 (3.9 PFLOP/s, under the power cap: 64 with codes of zeros; a tile's eight stages 2.3 us, 0.95 until the next one's begin, 3.6
+// together; HBM 42); 16384 x 1024 -> 2048 23, with SCReLU 25, with a residual 33.
 #pragma once
 #include "kernels_four.cuh"
 #include "product_out.cuh"

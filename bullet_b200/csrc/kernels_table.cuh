@@ -21,8 +21,8 @@ namespace b200 {
 
 constexpr int kTableThreads = 256;
 // Rows on their way in a warp.  Warps that hide each other's latency count for more than rows in one: 16384 x 32 features of 1024 columns, two rows of 32 bytes a lane and
-// 32 warps of an SM 43 us, four 39; their gradient, four rows and 24 warps 82, 32 (and registers spilt) 96, two rows and 32 83, six and 24 92; by 16 bytes four
-// rows and 32 warps 96, eight 102, four and 40 103.
+// 32 warps of an SM 43 us, four 39; their gradient, four rows and 24 warps (80 bytes of a thread's registers spilt) 82, 32 (and more spilt) 96, two rows and 32 83, six and
+// 24 92; by 16 bytes four rows and 32 warps 96, eight 102, four and 40 103.
 // So many warps as fill the GPU twice over or fewer take sixteen rows of 16 bytes each.
 constexpr int kEmbedAhead = 4, kGradAhead = 4, kFewAhead = 16;
 
@@ -192,7 +192,7 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD == kFewAhead || BY
     }
 }
 // Lists of up to kEmbedAhead ids: a warp takes `lists` of them, as many as its lanes have room for or fewer, and of these as many at a time as have kEmbedAhead ids together.  (One
-// id each, 131072 x 1024 bf16: 63 us, a list at a time 147.)
+// id each, 131072 x 1024 bf16: of 12288 rows 63 us, a list at a time 147; of 8 rows 51, with 41 of them what HBM takes to write y.)
 template <class T, int BYTES>
 static __global__ void __launch_bounds__(kTableThreads, BYTES == 0 ? 2 : 4) embed_short_kernel(b200_embed_op a, int lists, int vec) {
     using L = Lanes<T, BYTES>;
@@ -759,8 +759,9 @@ static __global__ void __launch_bounds__(kTableThreads, AHEAD > kGradAhead || BY
 
 // ---- the gradient of a table of few rows, as of output buckets: one id a list
 //
-// HBM bound (131072 x 1024 bf16, 8 rows 56 us, 4.8 TB/s; 262144 x 1024 fp32 180, 6.0), with few lists by latency (5003 x 520 7.5): nothing is sorted.  A warp takes lists one after another and the columns that its lanes cover, and keeps a sum for each of the table's
-// rows in shared memory, where each lane meets its own words alone.  A CTA's warps are added up in their order, then the CTAs' sums by few_join_kernel.
+// HBM bound (131072 x 1024 bf16, 8 rows 56 us, 4.8 TB/s; 262144 x 1024 fp32 180, 6.0), with few lists by latency (5003 x 520 7.7): nothing is sorted.  A warp takes lists
+// one after another and the columns that its lanes cover, and keeps a sum for each of the table's rows in shared memory, where each lane meets its own words alone.  A CTA's
+// warps are added up in their order, then the CTAs' sums by few_join_kernel.
 constexpr int kFewRows = 16, kFewWarps = kTableThreads / 32;
 struct FewRows {
     b200_embed_grad_op a;

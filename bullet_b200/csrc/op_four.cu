@@ -47,9 +47,11 @@ dim3 column_grid(int64_t columns, int64_t groups) { return dim3((unsigned)((colu
 // ---- products
 
 // Which tile: by what each way costs in ns, from the launch to the first stage, a stage (256 of k), the rest of each tile after the first; rounds of tiles
-// being whole.  Fitted to times of 16 to 131072 rows, 256 to 4096 inputs, 64 to 2048 outputs with either tile: of 75 such layers the choice is the quicker
-// one in all.  Us, 128 x 128 and 256 x 256 of a pair: 300 rows 2048 -> 1024 6.9 and 8.9, 5003 rows 1024 -> 512 7.5 and 7.9, 16384 rows 11.2 and
-// 10.3, 2048 -> 2048 44.9 and 35.6, 131072 rows 1024 -> 64 18.1 and 19.1, 2048 -> 512 94.0 and 72.9.
+// being whole.  Fitted to layers in bf16 without a residual.  With either tile, 16 to 131072 rows, 256 to 4096 inputs, 64 to 2048 outputs: of 225 such layers the choice is
+// the quicker one, or within 2 %, in 223 (the worst, 16384 rows 256 -> 1024, 16.1 us for 15.0); with a residual in 216 (22.6 for 20.5 there), of 220 with results in fp32 in 215
+// (19.7 for 17.0).  Us, 128 x 128 and 256 x 256 of a pair, in brackets with a residual: 300 rows 2048 -> 1024 8.1 and 10.1 (8.8 and 11.1), 5003 rows 10.8 and 11.2 of
+// 1024 inputs (13.5 and 14.2), 14.7 and 14.1 of 2048 (15.6 and 15.9), 16384 rows 2048 -> 2048 47.4 and 35.2 (52.8 and 42.1), 131072 rows 1024 -> 64 19.5 and 20.0 (22.1 and
+// 23.3), 2048 -> 1024 172 and 126 (202 and 159).
 struct Way {
     int columns, rows, units, start, stage, tile;
 };

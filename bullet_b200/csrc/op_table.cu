@@ -28,6 +28,8 @@ int check_ids(const char* who, const void* ids, int64_t ld, int rows, int slots,
     return 0;
 }
 // How many bytes of a row of `type` a lane takes: 32 or 16 where rows start on 16, fewer where the warp would have lanes to spare, 0 (single elements) where rows start anywhere.
+// (Us, 131072 lists of 32 ids, bf16, and their gradient by 12288 rows: rows of 64 columns by 16 bytes 156 and 390, by 8 128 and 376, by 4 122 and 354; of 128 columns 159 and
+// 393, 125 and 367, 237 and 538; of 256 columns 164 and 438, 246 and 626.)
 int bytes_of(const void* at, int64_t ld, int cols, int type, int most) {
     const int64_t size = type_bytes(type), row = cols * size;
     const auto on = [&](int bytes) { return ((uintptr_t)at | (uintptr_t)(ld * size) | (uintptr_t)row) % bytes == 0; };
@@ -71,8 +73,8 @@ void with_bytes(int bytes, F f) {
     else
         f(std::integral_constant<int, 0>{});
 }
-// (More than run at once, as stretches are of all lengths: by 8 an SM the features' gradient takes 81.6 us and one of 131072 ids of 12288 rows 84.8, by 12 80.5 and 81.5, by 48 83.4
-// and 78.3, but lookups longer.)
+// (More than run at once, as stretches are of all lengths: by 8 an SM the features' gradient takes 81.6 us and one of 131072 ids of 12288 rows 84.8, by 12 80.5 and
+// 81.5, by 48 83.4 and 78.3, but lookups longer.)
 unsigned ctas_for(int64_t warps) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((warps + kTableThreads / 32 - 1) / (kTableThreads / 32), kTableSms * 12)); }
 
 // How ids are sorted: in passes of equal digits, by whole tiles, or by one CTA.
@@ -142,8 +144,9 @@ Space space_of(const b200_embed_grad_op* op) {
     }
     if (!sort.places) s.start = next((op->n + 1ll) * 4);
     s.numbers = next(16);
-    // Pieces of 16 for few ids, whose longest stretches then have warps enough (before tables of few rows had kernels of their own: 5003 ids of 8 rows of 520, 64 27 us, 16 23), of
-    // 64 for many, as each piece costs its part of the joining (131072 ids of 8 rows of 1024: 16 159 us, 32 118, 64 90; 2^20 lists' ids of 768 rows of 256: 64 100, 512 128); more where they would take more room.
+    // Pieces of 16 for few ids, whose longest stretches then have warps enough (before tables of few rows had kernels of their own: 5003 ids of 8 rows of 520, 64 27 us,
+    // 16 23), of 64 for many, as each piece costs its part of the joining (131072 ids of 8 rows of 1024: 16 159 us, 32 118, 64 90; 2^20 lists' ids of 768 rows of 256: 64 100,
+    // 512 128); more where they would take more room.
     s.piece = 16;
     while (s.piece < 64 ? sort.count / s.piece > 2048 : s.piece < 512 && sort.count / s.piece > 16384) s.piece *= 2;
     s.cuts = sort.count > kLongest;

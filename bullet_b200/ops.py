@@ -101,8 +101,8 @@ def unpack4(packed: Packed4, dtype=torch.bfloat16):
 
 def dense(x, w, bias=None, act: int = ACT_NONE, residual=None, out_dtype=None):
     """act(x @ w + bias) + residual.  x and w: matrices of one 16-bit type, or both Packed8, or both Packed4 (w by column).  `out_dtype`: fp32 or 16
-    bits; default x's type, bf16 for codes.  The gradient of a layer on Packed4 is dense_backward's at unpack4's values.  dense_backward wants act(x @ w + bias) by itself: to train a layer that has both, call
-    without the residual, and add it behind (rms_norm does, on its way)."""
+    bits; default x's type, bf16 for codes.  The gradient of a layer on Packed4 is dense_backward's at unpack4's values.  dense_backward wants act(x @ w + bias) by
+    itself: to train a layer that has both, call without the residual, and add it behind (rms_norm does, on its way)."""
     if x.__class__ is Packed4 or w.__class__ is Packed4:
         if x.__class__ is not w.__class__:
             raise ValueError("x and w: both in 4 bits or neither")

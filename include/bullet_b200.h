@@ -387,8 +387,8 @@ int b200_op_ft_forward_noalloc(int device, void* stream, const b200_ft_op* op);
  *   - outputs overlap neither inputs nor one another (b200_op_clip_gradients may write where it reads);
  *   - scratch is lent by the caller: b200_op_*_workspace says how many bytes the very operation needs that is then called
  *     (its addresses and distances count);
- *   - all sums are held in 32 bits and taken in the same order by every call of the same shape and alignment: equal inputs
- *     give equal bits;
+ *   - all sums are held in 32 bits (b200_op_clip_gradients: in 64 beyond 32 elements) and taken in the same order by every call of the same shape and
+ *     alignment: equal inputs give equal bits;
  *   - a dense kernel that waits too long for its own copies or products gives up, which leaves its call's outputs invalid; the
  *     next call of b200_op_dense, its gradient or b200_op_dense4 with rows on the device, whoever makes it, returns B200_ERR_STATE, once, and
  *     does nothing else.  Programs that replay graphs, or that want to know whose call it was, ask b200_op_dense_gave_up;
@@ -538,7 +538,9 @@ int b200_op_dense_backward(int device, void* stream, const b200_dense_grad_op* o
 /* Activations (or weights) to 4 bits, and back.  by_column 0: rows of x become rows of codes.  by_column 1: columns do, `cols` rows of codes along
  * the rows of x, as weights [in][out] are wanted by b200_op_dense4.  The scale is the smallest power of two from 2^-126 on that brings the
  * group's largest magnitude to 6 or below (2^0 where there is none but 0); codes are the nearest, halves to the even one; a group with an
- * infinity or a NaN becomes NaN.  Values are exact in bf16 and fp32; one that would round up out of fp32 rounds down. */
+ * infinity or a NaN becomes NaN.  Values are exact in bf16 and fp32; one that would round up out of fp32 rounds down.
+ * That scale is a choice: conversions elsewhere often take 2^(floor(log2 of the largest) - 2), half of it for a largest above 1.5 times a power of two, whose codes
+ * then saturate at 6.  Codes and scales made so, any of 2^-127 to 2^127, are taken by b200_op_unpack4 and b200_op_dense4 all the same. */
 typedef struct b200_pack4_op {
     int32_t rows, cols;    /* of x */
     int32_t x_type;        /* B200_TYPE_F32, _BF16 or _F16 */
